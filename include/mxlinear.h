@@ -9,13 +9,15 @@
  *
  * Formats:  fmt 0 = E4M3 (8-bit codes), 2 = E2M3, 3 = E3M2 (FP6 packed four
  * values per three bytes, little-endian 6-bit fields: value i of a group in
- * bits [6i, 6i+6)).  Scales are E8M0 bytes (2^(s-127)), one per 32 along K.
+ * bits [6i, 6i+6)), 4 = E2M1 (FP4, two values per byte, the even column in the
+ * low half; the mxfp4 entry points and mxl_pack_weight).  Scales are E8M0 bytes (2^(s-127)), one per 32 along K.
  * rule 0 = floor_carry175 (the reference quantizer quantize_block,
  * src/vllm_mach/mxfp8/reconstruct_model.py:34-50), rule 1 = ceil_div448
  * (src/vllm_mach/mxfp6/mxfp8_mlp.py:100-105), rule 2 = rp_ue8m0 (FlashInfer's
  * mxfp8_quantize convention as src/vllm_mach/mxfp8/swiglu_quant.py:58-66 writes
  * it: amax * (1/448) rounded up onto E8M0, saturating; codes of the clamped
- * +-448 products; quantizers, dual and SwiGLU only).
+ * +-448 products; quantizers, dual and SwiGLU only).  MXFP4: rule 0 with E2M1's
+ * exponent, and rule 3 = floor (OCP MX v1.0: 2^(floor(log2 amax) - 2), saturating).
  *
  * Each declaration cites the reference interface (troycheng/vllm-mach
  * v0.4.0) it replaces.
@@ -67,6 +69,35 @@ int mxl_quantize_mxfp8_swizzled(const void* x, int64_t M, int64_t K, int64_t ldx
  * tests/native_mxfp6/test_mxfp6_sm120.py:37). */
 int mxl_quantize_mxfp6(const void* x, int64_t M, int64_t K, int64_t ldx, int fmt, void* packed, void* scales,
                        void* stream);
+
+/* MXFP4 (no counterpart in the reference, whose 4-bit path is NVFP4): bf16 x
+ * [M, K] (row stride ldx, a multiple of 8) -> E2M1 codes [M, K/2] + E8M0 scales
+ * [M, K/32], rule 0 or 3; a block with an infinity or NaN gets scale 255 (NaN) and
+ * zero codes.  x 16-byte, codes 4-byte aligned. */
+int mxl_quantize_mxfp4(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, void* codes, void* scales,
+                       void* stream);
+
+/* SwiGLU -> MXFP4: gate_up bf16 [M, 2K] -> the quantization of
+ * bf16(bf16(silu(gate)) * up), the activation of mxl_swiglu_mxfp8's rules 0 and 1. */
+int mxl_swiglu_mxfp4(const void* gate_up, int64_t M, int64_t K, int rule, void* codes, void* scales, void* stream);
+
+/* out[m, n] = sum_k A[m, k] W[n, k], MXFP4 on both sides, fp32 sums, bf16 out (row
+ * stride ldc); with a bias (bf16 [N]) the rounded sum plus the bias, rounded again.
+ * a u8 [M, K/2], sa u8 [M, K/32] row-major; w_tiled / sw_tiled from mxl_pack_weight
+ * with format 4.  a and w 16-byte, scales 4-byte aligned; the workspace holds
+ * mxl_mxfp4_gemm_workspace_bytes(M, N, K) bytes (16-byte aligned; 0: may be null). */
+int64_t mxl_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int mxl_mxfp4_gemm(const void* a, const void* sa, int64_t M, const void* w_tiled, const void* sw_tiled, int64_t N,
+                   int64_t K, const void* bias, void* out, int64_t ldc, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+
+/* mxl_grouped_gemm of MXFP4 activations and experts: routed row p of expert e
+ * (expert_offsets[e] <= p < expert_offsets[e+1]) is A[row_index[p] / row_div] . W[e]^T, or
+ * A[p] . W[e]^T where row_index is null; rows past expert_offsets[E] stay unwritten.
+ * Indices outside A and offsets past routed_rows are clamped. */
+int mxl_mxfp4_grouped_gemm(const void* a, const void* sa, int64_t a_rows, const int32_t* row_index, int row_div,
+                           const int64_t* expert_offsets, int64_t num_experts, int64_t routed_rows,
+                           const void* w_tiled, const void* sw_tiled, int64_t N, int64_t K, void* out, void* stream);
 
 /* Bytes of the swizzled scale buffer for [M, K] (mxfp8_mlp.py:122). */
 int64_t mxl_swizzled_scale_bytes(int64_t M, int64_t K);
@@ -451,6 +482,18 @@ int64_t mxl_moe_router_workspace_bytes(int64_t T, int64_t topk, int64_t E);
 int mxl_moe_router(const void* logits, int logits_bf16, int64_t T, int64_t E, int64_t topk, int renormalize,
                    float* topk_weights, int32_t* topk_ids, int32_t* sorted_routes, int64_t* expert_offsets,
                    int32_t* inverse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Routing with softmax (scoring 0) or sigmoid (1) scores s, a balance bias and groups
+ * (the role of the grouped top-k that the reference takes from vLLM's FusedMoE): choice
+ * scores c = s + bias (fp32 [E], null for none); the topk_groups best of `groups`
+ * equal groups by their largest c, or with a bias the sum of their two largest; the topk
+ * largest c among their experts, descending, ties to the lower index, NaNs last; weights
+ * s, over their sum + 1e-20 if renormalize, times factor.  Scores in binary64.
+ * E <= 1024, groups <= 64, topk <= 64; outputs and workspace as mxl_moe_router. */
+int mxl_moe_router_grouped(const void* logits, int logits_bf16, const float* bias, int64_t T, int64_t E, int64_t topk,
+                           int scoring, int64_t groups, int64_t topk_groups, int renormalize, float factor,
+                           float* topk_weights, int32_t* topk_ids, int32_t* sorted_routes, int64_t* expert_offsets,
+                           int32_t* inverse, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Weighted combine: out[t, h] = bf16(sum_k y[inverse[t*topk+k], h] * w[t, k])
  * in fp32, k ascending.  Replaces moe_reduce_out

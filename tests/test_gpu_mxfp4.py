@@ -1,0 +1,432 @@
+"""MXFP4 on the GPU against the formulas in 64 bits: quantization, SwiGLU producer, products dense and grouped,
+layers and experts."""
+import math
+
+import pytest
+import torch
+
+import mxfp4_reference as ref
+
+pytestmark = pytest.mark.gpu
+RULES = (ref.FLOOR_CARRY175, ref.FLOOR_OCP)
+
+
+def _x(g, m, k):
+    x = torch.randn(m, k, generator=g)
+    x[:, ::97] *= 20
+    return x.bfloat16()
+
+
+def _equal(got, want):
+    for x, y in zip(got, want):
+        assert x.dtype == torch.uint8 and torch.equal(x.cpu(), y)
+
+
+def _weight(pkg, g, n, k):
+    codes, scales = ref.random_operand(g, n, k)
+    return pkg.ops.pack_weight(codes.cuda(), scales.cuda(), pkg.ops.E2M1), ref.dequantize(codes, scales)
+
+
+# ------------------------------------------------------------------ quantization
+
+@pytest.mark.parametrize("rule", RULES)
+def test_quantize_every_bf16_value(pkg, dev, rule):
+    """Every bf16 value as its block's amax and, at every scale it can meet, as another value of the block: the 31
+    others lie 0 to 18 powers of two below a larger one."""
+    top = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    below = torch.arange(32, dtype=torch.int32)
+    bits = top.view(torch.int16).int() & 0xFFFF
+    e = (bits >> 7 & 255).unsqueeze(1) - (below * 19 // 32).unsqueeze(0)
+    others = torch.where(e > 0, (e << 7) | (bits.unsqueeze(1) * 37 + below * 11 & 127), 0) | (below & 1) << 15
+    x = others.to(torch.int16).view(torch.bfloat16)
+    x = torch.where((bits >> 7 & 255).unsqueeze(1) < 255, x, torch.ones_like(x))
+    x[:, 0] = top
+    _equal(pkg.ops.quantize_mxfp4(x.to(dev), rule), ref.quantize(x, rule))
+
+
+@pytest.mark.parametrize("rule", RULES)
+@pytest.mark.parametrize("m,k", [(1, 32), (3, 96), (17, 2048), (333, 2688), (64, 9216)])
+def test_quantize_shapes(pkg, dev, m, k, rule):
+    x = _x(torch.Generator().manual_seed(m * k), m, k)
+    x[m // 2, :32] = 0.0
+    _equal(pkg.ops.quantize_mxfp4(x.to(dev), rule), ref.quantize(x, rule))
+
+
+def test_quantize_borders(pkg, dev):
+    """Ties go to the even code, 1.75 2^e doubles the scale (or saturates), infinities and NaN make the block NaN,
+    signed zeros keep their sign."""
+    x = torch.zeros(6, 32)
+    x[0, :12] = torch.tensor([4.0, .25, .75, 1.25, 1.75, 2.5, 3.5, -0.25, -0.75, -2.5, -3.5, 6.0])
+    x[1, :3] = torch.tensor([6.96875, 5.0, -5.0])
+    x[2, :3] = torch.tensor([7.0, 5.0, -5.0])
+    x[3, :2] = torch.tensor([math.inf, 1.0])
+    x[4, :2] = torch.tensor([-1.0, math.nan])
+    x[5, :2] = torch.tensor([-0.0, 0.0])
+    x = x.bfloat16()
+    for rule in RULES:
+        codes, scales = pkg.ops.quantize_mxfp4(x.to(dev), rule)
+        _equal((codes, scales), ref.quantize(x, rule))
+    v = ref.dequantize(*pkg.ops.quantize_mxfp4(x.to(dev), ref.FLOOR_CARRY175))
+    assert v[0, :12].tolist() == [4, 0, 1, 1, 2, 2, 4, -0.0, -1, -2, -4, 6]
+    assert v[1, :3].tolist() == [6, 4, -4] and v[2, :3].tolist() == [8, 4, -4]
+    assert torch.isnan(v[3]).all() and torch.isnan(v[4]).all()
+    v = ref.dequantize(*pkg.ops.quantize_mxfp4(x.to(dev), ref.FLOOR_OCP))
+    assert v[2, :3].tolist() == [6, 4, -4]
+
+
+def test_quantize_strides_and_empty(pkg, dev):
+    g = torch.Generator().manual_seed(5)
+    big = _x(g, 24, 512).to(dev)
+    for x in (big[:, 64:320], big[::3, :256], big[:, 8:264], big[:, 3:259], big.t()[:, :0], big[:16].t().contiguous().t()[:, :256]):
+        if x.shape[1] == 0:
+            continue
+        _equal(pkg.ops.quantize_mxfp4(x), ref.quantize(x.contiguous()))
+    codes, scales = pkg.ops.quantize_mxfp4(big[:0])
+    assert codes.shape == (0, 256) and scales.shape == (0, 16)
+
+
+@pytest.mark.parametrize("rule", RULES)
+@pytest.mark.parametrize("m,k", [(1, 32), (5, 640), (130, 512), (1031, 2560)])
+def test_swiglu_producer(pkg, dev, m, k, rule):
+    """The quantization of the MXFP8 producer's activation, whose bits the oracle pins; against the float64
+    activation a value next to a rounding border may fall to its other side (the device's exp is a binary32 one),
+    which moves at most one value in 2^12."""
+    x = torch.randn(m, 2 * k, generator=torch.Generator().manual_seed(m + k)).bfloat16()
+    x[0, :4] = torch.tensor([100.0, -100.0, 0.0, -0.0]).bfloat16()
+    codes, scales = pkg.ops.swiglu_mxfp4(x.to(dev), rule)
+    want_codes, want_scales = ref.quantize(ref.silu_activation(x), rule)
+    assert (codes.cpu() != want_codes).double().mean() <= 2.0 ** -12
+    assert (scales.cpu() != want_scales).double().mean() <= 2.0 ** -12
+
+
+def test_swiglu_every_gate(pkg, dev, oracle_mod):
+    """Every bf16 gate against the activation with the oracle's exp: exact."""
+    gates = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16).view(-1, 32)
+    up = (torch.randn(2048, 32, generator=torch.Generator().manual_seed(1)) * 2).bfloat16()
+    x = torch.cat([gates, up], 1)
+    for rule in RULES:
+        _equal(pkg.ops.swiglu_mxfp4(x.to(dev), rule), ref.quantize(_activation(oracle_mod, x), rule))
+
+
+def _activation(oracle_mod, x):
+    """bf16(bf16(silu(g)) u) by the oracle's exp: silu(g) = g / (1 + exp(-g)) in binary32."""
+    import numpy as np
+    f = x.float().numpy()
+    g, u = f[:, : f.shape[1] // 2], f[:, f.shape[1] // 2:]
+    lib = oracle_mod.lib()
+    e = np.array([lib.mxo_exp(float(-v)) for v in g.ravel()], dtype=np.float32).reshape(g.shape)
+    with np.errstate(all="ignore"):
+        s = torch.from_numpy((g / (np.float32(1) + e)).astype(np.float32)).bfloat16().float().numpy()
+        return torch.from_numpy(s * u).bfloat16()
+
+
+# ------------------------------------------------------------------ dense products
+
+SHAPES = [(1, 16, 128), (1, 8, 256), (2, 2048, 2048), (7, 40, 384), (16, 4608, 2048), (17, 512, 640), (27, 1032, 5120),
+          (32, 100, 512), (33, 2048, 1152), (48, 264, 2688), (64, 4100, 512), (65, 128, 256), (100, 1000, 896),
+          (128, 2560, 9216), (129, 640, 128), (333, 5120, 2688), (512, 520, 1024), (777, 1030, 384)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_gemm(pkg, dev, m, n, k):
+    g = torch.Generator().manual_seed(m + n + k)
+    (w, sw), wv = _weight(pkg, g, n, k)
+    a, sa = ref.random_operand(g, m, k)
+    y = pkg.ops.mxfp4_gemm(a.to(dev), sa.to(dev), w, sw, n, k)
+    assert y.dtype == torch.bfloat16
+    ref.check_product(y, ref.dequantize(a, sa), wv)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 64, 256), (5, 100, 640), (48, 1030, 512), (300, 520, 1152), (700, 2048, 512)])
+def test_gemm_bias(pkg, dev, m, n, k):
+    g = torch.Generator().manual_seed(m + n + k)
+    (w, sw), wv = _weight(pkg, g, n, k)
+    a, sa = ref.random_operand(g, m, k)
+    bias = (torch.randn(n, generator=g) * 50).bfloat16()
+    y = pkg.ops.mxfp4_gemm(a.to(dev), sa.to(dev), w, sw, n, k, bias.to(dev))
+    ref.check_product(y, ref.dequantize(a, sa), wv, bias)
+
+
+@pytest.mark.parametrize("m", [1, 20, 64, 200])
+def test_gemm_extreme_scales(pkg, dev, m):
+    """The largest and smallest scales of either side next to each other, NaN scales only in their own rows and
+    columns, in the last K128 slice of a part super-tile too."""
+    n, k = 80, 640
+    g = torch.Generator().manual_seed(m)
+    a, sa = ref.random_operand(g, m, k)
+    wc, ws = ref.random_operand(g, n, k)
+    sa[0] = 0
+    sa[m - 1] = 200
+    ws[3] = 1
+    ws[5] = 180
+    sa[m // 2, k // 32 - 1] = 255
+    ws[7, k // 32 - 1] = 255
+    ws[n - 1, 0] = 255
+    w, sw = pkg.ops.pack_weight(wc.to(dev), ws.to(dev), pkg.ops.E2M1)
+    y = pkg.ops.mxfp4_gemm(a.to(dev), sa.to(dev), w, sw, n, k)
+    ref.check_product(y, ref.dequantize(a, sa), ref.dequantize(wc, ws))
+
+
+@pytest.mark.parametrize("m", [1, 16, 30, 64, 150, 600])
+def test_gemm_leaves_the_rest(pkg, dev, m):
+    """Rows of a wider output keep their other columns, rows behind the last stay as they were, and neither the
+    activations' neighbours nor the scales' are read into the sums: all of them hold NaN."""
+    n, k, ld = 200, 896, 256
+    g = torch.Generator().manual_seed(m)
+    (w, sw), wv = _weight(pkg, g, n, k)
+    a, sa = ref.random_operand(g, m, k)
+    codes = torch.full((m * k // 2 + 4096,), 0x77, dtype=torch.uint8, device=dev)
+    scales = torch.full((m * k // 32 + 4096,), 255, dtype=torch.uint8, device=dev)
+    codes[: m * k // 2] = a.flatten().to(dev)
+    scales[: m * k // 32] = sa.flatten().to(dev)
+    out = torch.full((m + 4, ld), 7.0, dtype=torch.bfloat16, device=dev)
+    from vllm_mach_amd import _lib
+    nbytes = _lib.query("mxl_mxfp4_gemm_workspace_bytes", m, n, k)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    _lib.call("mxl_mxfp4_gemm", codes.data_ptr(), scales.data_ptr(), m, w.data_ptr(), sw.data_ptr(), n, k, None,
+              out.data_ptr(), ld, ws.data_ptr(), nbytes, _lib.stream_handle(out.device))
+    ref.check_product(out[:m, :n], ref.dequantize(a, sa), wv)
+    assert bool((out[m:] == 7).all()) and bool((out[:, n:] == 7).all())
+
+
+def test_gemm_unaligned_and_strided_inputs(pkg, dev):
+    m, n, k = 9, 72, 256
+    g = torch.Generator().manual_seed(2)
+    (w, sw), wv = _weight(pkg, g, n, k)
+    a, sa = ref.random_operand(g, m, k)
+    wide = torch.zeros(m, 300, dtype=torch.uint8, device=dev)
+    wide[:, 5:5 + k // 2] = a.to(dev)
+    scales = sa.to(dev).t().contiguous().t()
+    ref.check_product(pkg.ops.mxfp4_gemm(wide[:, 5:5 + k // 2], scales, w, sw, n, k), ref.dequantize(a, sa), wv)
+    assert pkg.ops.mxfp4_gemm(a[:0].to(dev), sa[:0].to(dev), w, sw, n, k).shape == (0, n)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 2048), (40, 1024, 2560), (600, 512, 1024)])
+def test_gemm_is_deterministic_and_row_independent(pkg, dev, m, n, k):
+    g = torch.Generator().manual_seed(11)
+    (w, sw), _ = _weight(pkg, g, n, k)
+    a, sa = (t.to(dev) for t in ref.random_operand(g, m, k))
+    first = pkg.ops.mxfp4_gemm(a, sa, w, sw, n, k)
+    assert torch.equal(first, pkg.ops.mxfp4_gemm(a, sa, w, sw, n, k))
+
+
+# ------------------------------------------------------------------ layers
+
+def _layer(pkg, codes, scales):
+    n, k = codes.shape[0], codes.shape[1] * 2
+    method, layer = pkg.MxLinearMethod(pkg.linear.MXFP4_STATIC), torch.nn.Module()
+    method.create_weights(layer, k, [n], k, n, torch.bfloat16, device="cuda")
+    layer.weight.weight_loader(layer.weight, codes.cuda())
+    layer.weight_scale.weight_loader(layer.weight_scale, scales.cuda())
+    method.process_weights_after_loading(layer)
+    return method, layer
+
+
+@pytest.mark.parametrize("m", [1, 3, 16, 17, 40, 333])
+@pytest.mark.parametrize("n,k", [(200, 384), (2048, 2048)])
+def test_linear_layer(pkg, dev, m, n, k):
+    g = torch.Generator().manual_seed(m + n)
+    codes, scales = ref.random_operand(g, n, k)
+    method, layer = _layer(pkg, codes, scales)
+    x, bias = _x(g, m, k), torch.randn(n, generator=g).bfloat16()
+    a, w = ref.dequantize(*ref.quantize(x)), ref.dequantize(codes, scales)
+    ref.check_product(method.apply(layer, x.to(dev)), a, w)
+    ref.check_product(method.apply(layer, x.to(dev), bias.to(dev)), a, w, bias)
+    # leading dimensions, strided rows, no rows
+    y = method.apply(layer, x.to(dev).view(1, m, k))
+    assert y.shape == (1, m, n) and torch.equal(y[0], method.apply(layer, x.to(dev)))
+    wide = torch.zeros(m, k + 64, dtype=torch.bfloat16, device=dev)
+    wide[:, 8:8 + k] = x.to(dev)
+    assert torch.equal(method.apply(layer, wide[:, 8:8 + k]), y[0])
+    assert method.apply(layer, x[:0].to(dev)).shape == (0, n)
+
+
+@pytest.mark.parametrize("m", [1, 16, 64])
+def test_linear_layer_propagates_nan(pkg, dev, m):
+    g = torch.Generator().manual_seed(m)
+    codes, scales = ref.random_operand(g, 96, 512)
+    method, layer = _layer(pkg, codes, scales)
+    x = _x(g, m, 512)
+    x[m // 2, 77] = math.nan
+    y = method.apply(layer, x.to(dev))
+    bad = torch.zeros(m, dtype=torch.bool)
+    bad[m // 2] = True
+    assert torch.equal(torch.isnan(y).any(1).cpu(), bad) and torch.isnan(y[m // 2]).all()
+
+
+@pytest.mark.parametrize("m", [1, 5, 100])
+def test_swiglu_down(pkg, dev, m):
+    g = torch.Generator().manual_seed(m)
+    codes, scales = ref.random_operand(g, 264, 640)
+    method, layer = _layer(pkg, codes, scales)
+    x = torch.randn(m, 1280, generator=g).bfloat16().to(dev)
+    a, sa = pkg.ops.swiglu_mxfp4(x)
+    y = pkg.swiglu_mxfp4_down(x, layer)
+    ref.check_product(y, ref.dequantize(a, sa), ref.dequantize(codes, scales))
+    assert torch.equal(pkg.swiglu_mxfp4_down(x.view(1, m, -1), layer)[0], y)
+    assert pkg.swiglu_mxfp4_down(x[:0], layer).shape == (0, 264)
+
+
+# ------------------------------------------------------------------ experts
+
+def _experts(pkg, g, e, h, i):
+    c1, s1 = ref.random_operand(g, e * 2 * i, h)
+    c2, s2 = ref.random_operand(g, e * h, i)
+    c1, s1, c2, s2 = c1.view(e, 2 * i, -1), s1.view(e, 2 * i, -1) - 6, c2.view(e, h, -1), s2.view(e, h, -1) - 6
+    experts = pkg.Mxfp4Experts()
+    w1, w2 = experts.process_weights_after_loading(c1.cuda(), s1.cuda(), c2.cuda(), s2.cuda())
+    return experts, w1, w2, ref.dequantize(c1, s1), ref.dequantize(c2, s2)
+
+
+def _routes(g, t, e, topk, only=None):
+    pool = torch.tensor(only if only else list(range(e)))
+    return torch.stack([pool[torch.randperm(len(pool), generator=g)[:topk]] for _ in range(t)]).int()
+
+
+@pytest.mark.parametrize("t,e,topk,only", [(1, 8, 2, None), (3, 4, 1, [2]), (17, 16, 4, None), (64, 5, 2, [0, 4]),
+                                           (150, 3, 2, None), (300, 6, 3, None), (40, 33, 8, None)])
+@pytest.mark.parametrize("n,k", [(136, 384), (256, 1024)])
+def test_grouped_gemm(pkg, dev, t, e, topk, only, n, k):
+    """Experts without rows, with one, with many; gathered rows and rows in order."""
+    g = torch.Generator().manual_seed(t + e + n)
+    wc, ws = ref.random_operand(g, e * n, k)
+    wv = ref.dequantize(wc, ws).view(e, n, k)
+    w, sw = pkg.ops.pack_weight(wc.view(e, n, -1).to(dev), ws.view(e, n, -1).to(dev), pkg.ops.E2M1)
+    a, sa = ref.random_operand(g, t, k)
+    ids = _routes(g, t, e, topk, only)
+    routes, offsets, inverse = pkg.ops.moe_route(ids.to(dev), e)
+    R = t * topk
+    y = pkg.ops.mxfp4_grouped_gemm(a.to(dev), sa.to(dev), routes, topk, offsets, R, w, sw, n, k)
+    order, off = routes.cpu().long(), offsets.cpu().tolist()
+    rows = ref.dequantize(a, sa)[order // topk]
+    for x in range(e):
+        ref.check_product(y[off[x]:off[x + 1]], rows[off[x]:off[x + 1]], wv[x])
+    b, sb = a[order // topk].to(dev), sa[order // topk].to(dev)
+    assert torch.equal(y, pkg.ops.mxfp4_grouped_gemm(b, sb, None, 1, offsets, R, w, sw, n, k))
+
+
+def test_grouped_gemm_leaves_dropped_rows(pkg, dev):
+    """Routes to no expert end behind the last offset: their output rows are not written."""
+    g = torch.Generator().manual_seed(3)
+    e, n, k, t = 4, 64, 256, 50
+    wc, ws = ref.random_operand(g, e * n, k)
+    w, sw = pkg.ops.pack_weight(wc.view(e, n, -1).to(dev), ws.view(e, n, -1).to(dev), pkg.ops.E2M1)
+    a, sa = ref.random_operand(g, t, k)
+    ids = _routes(g, t, e, 2)
+    ids[::3, 1] = -1
+    routes, offsets, inverse = pkg.ops.moe_route(ids.to(dev), e)
+    kept = int(offsets[-1])
+    routes[kept:] = 1 << 30  # whatever the sort left there
+    from vllm_mach_amd import _lib
+    out = torch.full((t * 2, n), 7.0, dtype=torch.bfloat16, device=dev)
+    ad, sd = a.to(dev), sa.to(dev)
+    _lib.call("mxl_mxfp4_grouped_gemm", ad.data_ptr(), sd.data_ptr(), t, routes.data_ptr(), 2, offsets.data_ptr(), e, t * 2,
+              w.data_ptr(), sw.data_ptr(), n, k, out.data_ptr(), _lib.stream_handle(out.device))
+    assert bool((out[kept:] == 7).all()) and not bool((out[:kept] == 7).all(1).any())
+
+
+def _exact_layer(x, p, ids, w1, w2):
+    a, out = ref.dequantize(*ref.quantize(x)), torch.zeros(x.shape, dtype=torch.float64)
+    for e in range(w1.shape[0]):
+        t, slot = (ids == e).nonzero(as_tuple=True)
+        if len(t):
+            mid = (a[t] @ w1[e].t()).bfloat16()
+            act = ref.dequantize(*ref.quantize(ref.silu_activation(mid)))
+            out.index_add_(0, t, (act @ w2[e].t()).bfloat16().double() * p[t, slot].double().unsqueeze(-1))
+    return out
+
+
+@pytest.mark.parametrize("t,e,topk,h,i", [(1, 8, 2, 256, 128), (20, 16, 4, 384, 256), (200, 6, 2, 512, 384)])
+def test_experts_layer(pkg, dev, t, e, topk, h, i):
+    """The layer against the chain in 64 bits.  Its outputs are sums of bf16 values (half a step each, 2^-8) rounded
+    once more, and where a sum in fp32 rounds to another bf16 gate or up value the activation's code can move by a
+    step of E2M1, a third of its value: one in 2^10 of them at most, 3 / 2^5 / 2^5 of the norm."""
+    g = torch.Generator().manual_seed(t)
+    experts, w1, w2, v1, v2 = _experts(pkg, g, e, h, i)
+    x, ids = _x(g, t, h), _routes(g, t, e, topk)
+    p = torch.rand(t, topk, generator=g)
+    got = experts(x.to(dev), w1, w2, p.to(dev), ids.to(dev)).cpu().double()
+    want = _exact_layer(x, p, ids, v1, v2)
+    assert float((got - want).norm() / want.norm()) <= 2 * 2.0 ** -8 + 2.0 ** -10 * 3
+
+
+def test_experts_map_and_method(pkg, dev):
+    """An expert map drops the experts of other ranks; the method object runs the same layer."""
+    g = torch.Generator().manual_seed(9)
+    e, h, i, t, topk = 4, 256, 128, 12, 2
+    experts, w1, w2, v1, v2 = _experts(pkg, g, e, h, i)
+    x, ids = _x(g, t, h).to(dev), _routes(g, t, 8, topk).to(dev)
+    p = torch.rand(t, topk, generator=g).to(dev)
+    table = torch.tensor([0, -1, 1, -1, 2, -1, 3, -1], dtype=torch.int32, device=dev)
+    out = torch.empty_like(x)
+    experts.apply(out, x, w1, w2, p, ids, "silu", 8, table, None, None, None, None, None, False)
+    local = table[ids.long()]
+    want = _exact_layer(x.cpu(), p.cpu(), local.cpu(), v1, v2)
+    keep = (local >= 0).any(1).cpu()
+    assert float((out.cpu().double() - want)[keep].norm() / want.norm()) <= 2 * 2.0 ** -8 + 2.0 ** -10 * 3
+    assert bool((out.cpu()[~keep] == 0).all())
+
+
+# ------------------------------------------------------------------ a run of them together
+
+@pytest.mark.parametrize("t", [1, 16, 70])
+def test_block_router_experts_linear(pkg, dev, t):
+    """As a model's block uses them: a linear layer, the grouped router on its logits, the experts on its routes;
+    eager, and captured once and replayed on new inputs with eager work in between."""
+    g = torch.Generator().manual_seed(t)
+    e, h, i, topk = 16, 256, 128, 4
+    experts, w1, w2, v1, v2 = _experts(pkg, g, e, h, i)
+    codes, scales = ref.random_operand(g, h, h)
+    method, layer = _layer(pkg, codes, scales - 6)
+    bias = (torch.randn(e, generator=g) * 0.1).to(dev)
+    routing = pkg.GroupedRouting("sigmoid", bias, 4, 2, 2.5)
+    xs = [_x(g, t, h).to(dev) for _ in range(4)]
+    logits = [torch.randn(t, e, generator=g).to(dev) for _ in range(4)]
+
+    def block(x, z):
+        y = method.apply(layer, x)
+        out = torch.empty_like(y)
+        experts.apply_router(out, y, w1, w2, z, topk, True, routing)
+        return y, out
+
+    eager = [[v.clone() for v in block(x, z)] for x, z in zip(xs, logits)]
+    for (y, out), x, z in zip(eager, xs, logits):
+        ref.check_product(y, ref.dequantize(*ref.quantize(x)), ref.dequantize(codes, scales - 6))
+        p, ids = pkg.grouped_topk(z, topk, True, 4, 2, "sigmoid", bias, 2.5)
+        assert torch.equal(out, experts(y, w1, w2, p, ids))
+        want = _exact_layer(y.cpu(), p.cpu(), ids.cpu(), v1, v2)
+        assert float((out.cpu().double() - want).norm() / want.norm()) <= 2 * 2.0 ** -8 + 2.0 ** -10 * 3
+    stream, sx, sz = torch.cuda.Stream(), xs[0].clone(), logits[0].clone()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        block(sx, sz)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        captured = block(sx, sz)
+    for (y, out), x, z in list(zip(eager, xs, logits)) * 2:
+        sx.copy_(x)
+        sz.copy_(z)
+        graph.replay()
+        block(xs[1], logits[1])  # eager work between the replays
+        torch.cuda.synchronize()
+        assert torch.equal(captured[0], y) and torch.equal(captured[1], out)
+
+
+def test_two_streams_at_once(pkg, dev):
+    """Calls on two streams use workspaces of their own."""
+    g = torch.Generator().manual_seed(4)
+    n, k = 512, 4096
+    (w, sw), wv = _weight(pkg, g, n, k)
+    rows = [tuple(t.to(dev) for t in ref.random_operand(g, m, k)) for m in (40, 70)]
+    want = [pkg.ops.mxfp4_gemm(a, sa, w, sw, n, k) for a, sa in rows]
+    streams = [torch.cuda.Stream() for _ in rows]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for j, (s, (a, sa)) in enumerate(zip(streams, rows)):
+            with torch.cuda.stream(s):
+                got[j].append(pkg.ops.mxfp4_gemm(a, sa, w, sw, n, k))
+    torch.cuda.synchronize()
+    for j in range(2):
+        assert all(torch.equal(y, want[j]) for y in got[j])

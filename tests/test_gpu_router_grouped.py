@@ -1,0 +1,124 @@
+"""The grouped router on the GPU against its formulas in 64 bits: ids and the sort exactly, weights to one fp32
+rounding."""
+import math
+
+import pytest
+import torch
+
+import mxfp4_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _check(pkg, logits, bias, topk, sigmoid, groups, keep, renorm, factor):
+    T, E = logits.shape
+    w, ids, routes, offsets, inverse = pkg.ops.moe_router_grouped(
+        logits.cuda(), None if bias is None else bias.cuda(), topk, int(sigmoid), groups, keep, renorm, factor)
+    want, want_ids = ref.route(logits, bias, topk, sigmoid, groups, keep, renorm, factor)
+    assert ids.dtype == torch.int32 and torch.equal(ids.cpu().long(), torch.from_numpy(want_ids))
+    want = torch.from_numpy(want)
+    assert w.dtype == torch.float32 and torch.equal(torch.isnan(w.cpu()), torch.isnan(want))
+    # one rounding to fp32 (half a step, 2^-24) after sums in binary64; tiny weights round to fp32's subnormal grid
+    off = (w.cpu().double() - want).abs().nan_to_num()
+    assert bool((off <= (2.0 ** -24 + 1e-12) * want.abs().nan_to_num() + 2.0 ** -150).all())
+    flat = ids.cpu().flatten().long()
+    order = torch.sort(flat, stable=True).indices
+    assert torch.equal(routes.cpu().long(), order)
+    assert torch.equal(offsets.cpu(), torch.searchsorted(flat[order], torch.arange(E + 1)))
+    assert torch.equal(inverse.cpu().long()[order], torch.arange(T * topk))
+    two = pkg.grouped_topk(logits.cuda(), topk, renorm, groups, keep, "sigmoid" if sigmoid else "softmax",
+                           None if bias is None else bias.cuda(), factor)
+    assert torch.equal(two[0].nan_to_num(), w.nan_to_num()) and torch.equal(two[1], ids)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("T,E,topk,groups,keep", [
+    (1, 1, 1, 1, 1), (1, 256, 8, 8, 4), (5, 8, 8, 1, 1), (16, 64, 6, 8, 3), (17, 160, 6, 8, 3), (130, 256, 8, 8, 4),
+    (40, 16, 4, 16, 4), (33, 72, 2, 1, 1), (200, 512, 10, 8, 2), (9, 1000, 64, 4, 3), (3, 1024, 8, 64, 8),
+    (1, 255, 5, 3, 2), (65, 96, 1, 2, 1), (1100, 24, 3, 4, 2)])
+def test_router(pkg, dev, T, E, topk, groups, keep, biased, sigmoid):
+    g = torch.Generator().manual_seed(T * E + topk)
+    x = torch.randn(T, E, generator=g) * 2
+    bias = torch.randn(E, generator=g) * 0.1 if biased else None
+    for bf16 in (False, True):
+        _check(pkg, x.bfloat16() if bf16 else x, bias, topk, sigmoid, groups, keep, not bf16, 2.5 if biased else 1.0)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("groups,keep", [(1, 1), (4, 2)])
+def test_ties_go_to_the_lower_index(pkg, dev, groups, keep, sigmoid):
+    g = torch.Generator().manual_seed(1)
+    x = torch.randint(-1, 2, (50, 32), generator=g).float()
+    x[0] = 0.0
+    _check(pkg, x, None, 6, sigmoid, groups, keep, True, 1.0)
+    bias = torch.randint(0, 2, (32,), generator=g).float()
+    _check(pkg, x, bias, 6, sigmoid, groups, keep, True, 1.0)
+
+
+def test_scores_closer_than_an_fp32_step(pkg, dev):
+    """Sigmoid scores near 1 that are equal in fp32 and not in 64 bits are told apart."""
+    x = torch.stack([torch.linspace(18.0, 20.0, 32).flip(0), torch.linspace(30.0, 31.0, 32)])
+    _check(pkg, x, None, 8, True, 4, 2, True, 1.0)
+    _check(pkg, x, torch.full((32,), 0.5), 8, True, 4, 2, True, 1.0)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_masked_infinite_and_nan_logits(pkg, dev, sigmoid):
+    """Masked experts (-inf, the lowest finite value), infinities and NaN; a row with nothing left but masks."""
+    low = torch.finfo(torch.float32).min
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(8, 32, generator=g)
+    x[0, 5:] = -math.inf
+    x[1, 3:] = low
+    x[2] = -math.inf
+    x[3] = low
+    x[4, 7] = math.inf
+    x[5, 9] = math.nan
+    x[6] = math.nan
+    x[7, ::2] = 800.0
+    for bias in (None, torch.randn(32, generator=g) * 0.1):
+        for groups, keep in ((1, 1), (8, 3)):
+            _check(pkg, x, bias, 4, sigmoid, groups, keep, True, 1.0)
+
+
+def test_infinite_and_nan_bias(pkg, dev):
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(20, 32, generator=g)
+    bias = torch.randn(32, generator=g) * 0.1
+    bias[3], bias[9], bias[10], bias[20], bias[21] = -math.inf, math.nan, math.inf, math.inf, -math.inf
+    _check(pkg, x, bias, 5, True, 8, 4, True, 2.5)
+
+
+def test_strided_logits_and_no_tokens(pkg, dev):
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(40, 64, generator=g)
+    a = pkg.ops.moe_router_grouped(x.cuda()[::2, 8:40], None, 4, 1, 4, 2)
+    b = pkg.ops.moe_router_grouped(x[::2, 8:40].contiguous().cuda(), None, 4, 1, 4, 2)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    w, ids, routes, offsets, inverse = pkg.ops.moe_router_grouped(x[:0].cuda(), None, 4)
+    assert w.shape == (0, 4) and routes.numel() == 0 and offsets.tolist() == [0] * 65
+
+
+def test_softmax_without_groups_is_the_router(pkg, dev):
+    """The same experts as the softmax router's, and its weights to fp32's accuracy: an exp (two roundings there and
+    the division's), a sum of up to 8 terms."""
+    x = torch.randn(300, 256, generator=torch.Generator().manual_seed(6)).cuda()
+    a, b = pkg.ops.moe_router_grouped(x, None, 8), pkg.ops.moe_router(x, 8)
+    assert all(torch.equal(u, v) for u, v in zip(a[1:], b[1:]))
+    assert bool(((a[0] - b[0]).abs() <= 16 * 2.0 ** -24 * a[0]).all())
+
+
+def test_mxfp6_experts_take_the_routing(pkg, dev):
+    g = torch.Generator().manual_seed(8)
+    e, h, i, t = 8, 256, 128, 12
+    packed = lambda n, k: torch.randint(0, 256, (e, n, k * 3 // 4), generator=g, dtype=torch.uint8).cuda()  # noqa: E731
+    scales = lambda n, k: torch.full((e, n, k // 32), 118, dtype=torch.uint8).cuda()  # noqa: E731
+    experts = pkg.Mxfp6Experts(fmt=2)
+    w1, w2 = experts.process_weights_after_loading(packed(2 * i, h), scales(2 * i, h), packed(h, i), scales(h, i))
+    x, z = torch.randn(t, h, generator=g).bfloat16().cuda(), torch.randn(t, e, generator=g).cuda()
+    bias = (torch.randn(e, generator=g) * 0.1).cuda()
+    out = torch.empty_like(x)
+    experts.apply_router(out, x, w1, w2, z, 3, True, pkg.GroupedRouting("sigmoid", bias, 4, 2, 2.5))
+    p, ids = pkg.grouped_topk(z, 3, True, 4, 2, "sigmoid", bias, 2.5)
+    assert torch.equal(out, experts(x, w1, w2, p, ids))

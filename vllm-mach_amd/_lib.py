@@ -30,6 +30,11 @@ SIGNATURES = {
     "mxl_quantize_mxfp8": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P]),
     "mxl_quantize_mxfp8_swizzled": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P]),
     "mxl_quantize_mxfp6": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "mxl_quantize_mxfp4": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "mxl_swiglu_mxfp4": (_I, [_P, _I64, _I64, _I, _P, _P, _P]),
+    "mxl_mxfp4_gemm_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "mxl_mxfp4_gemm": (_I, [_P, _P, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _P]),
+    "mxl_mxfp4_grouped_gemm": (_I, [_P, _P, _I64, _P, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P]),
     "mxl_swizzled_scale_bytes": (_I64, [_I64, _I64]),
     "mxl_swizzle_scales": (_I, [_P, _I64, _I64, _P, _P]),
     "mxl_swiglu_mxfp8": (_I, [_P, _I64, _I64, _I, _I, _P, _P, _P]),
@@ -77,6 +82,8 @@ SIGNATURES = {
     "mxl_moe_reduce_add": (_I, [_P, _P, _P, _I64, _I64, _I64, _P, _P, _P]),
     "mxl_moe_router_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "mxl_moe_router": (_I, [_P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "mxl_moe_router_grouped": (_I, [_P, _I, _P, _I64, _I64, _I64, _I, _I64, _I64, _I, _F, _P, _P, _P, _P, _P, _P, _I64,
+                                    _P]),
     "mxl_gemm_plan_name": (_I, [_I64, _I64, _I64, _I, _I, _P, ctypes.c_char_p, _I64]),
     "mxl_grouped_plan_name": (_I, [_I64, _I64, _I64, _I, _I, _I, _P, ctypes.c_char_p, _I64]),
 }

@@ -1,6 +1,6 @@
 """On-disk formats of the quantized linear path, and loading them into MFMA-native layers.
 
-Three checkpoint formats reach the path (the formats the reference's loaders accept):
+Four checkpoint formats reach the path (three that the reference's loaders accept, and MXFP4):
 
 * compressed-tensors MXFP8 (``quant_method: compressed-tensors``, ``format:
   mxfp8-quantized``; src/vllm_mach/mxfp8/prepare_model.py:665-681): ``<layer>.weight``
@@ -12,6 +12,9 @@ Three checkpoint formats reach the path (the formats the reference's loaders acc
   (four 6-bit codes in three bytes, src/vllm_mach/mxfp6/dense.py:61-80) and
   ``<layer>.weight_scale`` U8 [N, K/32]; routed experts as per-expert tensors stacked
   into ``w13_weight``/``w2_weight`` (mxfp6/profile/runtime.patch:207-250);
+* Quark OCP-MX FP4 (the same config with weight ``fp4`` per_group 32 e8m0 static and input ``fp4``
+  per_group 32 e8m0 dynamic): ``<layer>.weight`` U8 [N, K/2] (the even column in a byte's low
+  half) and ``<layer>.weight_scale`` U8 [N, K/32]; routed experts as for FP6;
 * block-FP8 (``quant_method: fp8``, ``weight_block_size: [128, 128]``, dynamic
   activations): ``<layer>.weight`` F8_E4M3 [N, K] and fp32 ``<layer>.weight_scale_inv``
   (or ``weight_scale``) [ceil(N/128), K/128] (src/vllm_mach/fp8/linear.py:120-134).
@@ -35,7 +38,7 @@ import torch
 
 from . import linear as L
 from . import ops
-from .moe import Mxfp6MoEMethod
+from .moe import Mxfp4MoEMethod, Mxfp6MoEMethod, _MoEMethod
 
 _FP6_KEYS = {"fp6_e3m2": L.MXFP6_E3M2_STATIC, "fp6_e2m3": L.MXFP6_E2M3_STATIC}
 _FP6_FMT = {L.MXFP6_E3M2_STATIC: ops.E3M2, L.MXFP6_E2M3_STATIC: ops.E2M3}
@@ -100,11 +103,14 @@ def _quark_key(qc: dict, prefix: str, shards) -> Optional[str]:
     w, a = scheme.get("weight"), scheme.get("input_tensors")
     if not isinstance(w, dict) or not isinstance(a, dict):
         return None
-    ok_w = (w.get("dtype") in _FP6_KEYS and w.get("group_size") == 32 and w.get("qscheme") == "per_group"
+    fp4 = w.get("dtype") == "fp4"
+    ok_w = ((fp4 or w.get("dtype") in _FP6_KEYS) and w.get("group_size") == 32 and w.get("qscheme") == "per_group"
             and w.get("scale_format") == "e8m0" and w.get("is_dynamic") is False and w.get("symmetric") is True)
-    ok_a = (a.get("dtype") == "fp8_e4m3" and a.get("group_size") == 32 and a.get("qscheme") == "per_group"
+    ok_a = (a.get("dtype") == ("fp4" if fp4 else "fp8_e4m3") and a.get("group_size") == 32 and a.get("qscheme") == "per_group"
             and a.get("scale_format") == "e8m0" and a.get("is_dynamic") is True and a.get("symmetric") is True)
-    return _FP6_KEYS[w["dtype"]] if ok_w and ok_a else None
+    if not (ok_w and ok_a):
+        return None
+    return L.MXFP4_STATIC if fp4 else _FP6_KEYS[w["dtype"]]
 
 
 def _fp8_key(qc: dict, prefix: str, shards) -> Optional[str]:
@@ -136,10 +142,10 @@ def linear_quant_key(quant_config: Optional[dict], prefix: str,
 
 
 def moe_quant_key(quant_config: Optional[dict], prefix: str) -> Optional[str]:
-    """Quant key of the routed experts under ``prefix`` (Quark OCP-MX FP6 only: the reference's
-    W6A8 MoE admission, tests/native_mxfp6/test_moe_quant_admission_cpu.py:35-60)."""
+    """Quant key of the routed experts under ``prefix`` (Quark OCP-MX FP6, the reference's W6A8
+    MoE admission, tests/native_mxfp6/test_moe_quant_admission_cpu.py:35-60, and FP4)."""
     key = linear_quant_key(quant_config, prefix) if (quant_config or {}).get("quant_method") == "quark" else None
-    return key if key in _FP6_FMT else None
+    return key if key in _FP6_FMT or key == L.MXFP4_STATIC else None
 
 
 def quant_config_of(model_dir: Union[str, Path]) -> Optional[dict]:
@@ -267,7 +273,7 @@ def load_linear(ckpt: SafetensorsCheckpoint, prefix: str, quant_key: str,
         if len(shape) != 2:
             raise ValueError(f"{name}.weight must be two-dimensional, got {shape}")
         widths.append(shape[0])
-        ks.add(shape[1] * 4 // 3 if quant_key in _FP6_FMT else shape[1])
+        ks.add(shape[1] * 4 // 3 if quant_key in _FP6_FMT else shape[1] * 2 if quant_key == L.MXFP4_STATIC else shape[1])
         if quant_key in _FP6_FMT and shape[1] % 3:
             raise ValueError(f"{name}.weight: packed FP6 width {shape[1]} is not a multiple of 3")
     if len(ks) != 1:
@@ -294,7 +300,7 @@ def load_linear(ckpt: SafetensorsCheckpoint, prefix: str, quant_key: str,
 class QuantizedExperts(torch.nn.Module):
     """Routed experts in the tiled layout: ``forward(x, topk_weights, topk_ids)``."""
 
-    def __init__(self, method: Mxfp6MoEMethod):
+    def __init__(self, method: _MoEMethod):
         super().__init__()
         self.quant_method = method
 
@@ -307,13 +313,13 @@ def load_moe(ckpt: SafetensorsCheckpoint, prefix: str, num_experts: int, quant_k
              expert_names: tuple[str, str, str] = ("gate_proj", "up_proj", "down_proj")) -> QuantizedExperts:
     """Routed experts ``<prefix>.experts.<e>.<gate|up|down>.weight`` (+ ``.weight_scale``),
     stacked through vLLM's expert loader (gate -> w1, up -> w3, down -> w2)."""
-    if quant_key not in _FP6_FMT:
-        raise ValueError(f"routed experts load packed MXFP6 only, not {quant_key}")
+    if quant_key not in _FP6_FMT and quant_key != L.MXFP4_STATIC:
+        raise ValueError(f"routed experts load packed MXFP6 or MXFP4 only, not {quant_key}")
     gate, up, down = expert_names
     _, gshape = ckpt.info(f"{prefix}.experts.0.{gate}.weight")
     _, dshape = ckpt.info(f"{prefix}.experts.0.{down}.weight")
     inter, hidden = gshape[0], dshape[0]
-    method = Mxfp6MoEMethod(_FP6_FMT[quant_key])
+    method = Mxfp4MoEMethod() if quant_key == L.MXFP4_STATIC else Mxfp6MoEMethod(_FP6_FMT[quant_key])
     layer = QuantizedExperts(method)
     method.create_weights(layer, num_experts, hidden, inter, torch.bfloat16, device=device)
     for e in range(num_experts):

@@ -89,6 +89,20 @@ __global__ void pack_weight_kernel(const uint8_t* __restrict__ src, int64_t ld_s
   *reinterpret_cast<uint4*>(dst + tile * (CH * 1024) + c * 1024 + lane * 16) = w;
 }
 
+// The same for MXFP4: chunk j of a tile is K128 slice j, and a lane's piece the 32 columns of its
+// scale block, 16 bytes in a row of the source.
+__global__ void pack_fp4_kernel(const uint8_t* __restrict__ src, int64_t ld_src, uint8_t* __restrict__ dst, int64_t N,
+                                int64_t KT, int64_t total) {
+  const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (id >= total) return;
+  const int lane = (int)(id & 63), j = (int)(id >> 6 & 3);
+  const int64_t tile = id >> 8, nt = tile / KT, kt = tile - nt * KT;
+  const int64_t row = nt * 16 + (lane & 15), at = kt * (kTileK / 2) + 64 * j + 16 * (lane >> 4);
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (row < N && at < ld_src) v = *reinterpret_cast<const uint4*>(src + row * ld_src + at);
+  *reinterpret_cast<uint4*>(dst + id * 16) = v;
+}
+
 // One thread writes one lane's scale dword of one tile.  The source is the logical
 // [N, K/32] layout, or (swizzled) the reference's 128-row x 4-group tiles.
 __global__ void pack_scale_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst, int64_t N,
@@ -422,7 +436,7 @@ extern "C" int mxl_pack_weight_ex(const void* codes, const void* scales, int sca
 
 static int pack_common(const void* codes, const void* scales, int scale_layout, int64_t N, int64_t K, int fmt,
                        void* tiled_codes, void* tiled_scales, void* stream) {
-  MXL_CHECK_ARG(valid_wfmt(fmt), "mxl_pack_weight: unknown weight format %d", fmt);
+  MXL_CHECK_ARG(valid_wfmt(fmt) || fmt == kE2M1, "mxl_pack_weight: unknown weight format %d", fmt);
   MXL_CHECK_ARG(N > 0 && K > 0 && K % 128 == 0, "mxl_pack_weight: need N > 0 and K %% 128 == 0 (N=%lld K=%lld)",
                 (long long)N, (long long)K);
   MXL_CHECK_ARG(((uintptr_t)codes & 15) == 0 && ((uintptr_t)tiled_codes & 15) == 0,
@@ -431,8 +445,11 @@ static int pack_common(const void* codes, const void* scales, int scale_layout, 
   const int64_t NTl = (N + 15) / 16, KT = (K + kTileK - 1) / kTileK;
   const int CH = tile_chunks(fmt);
   const int64_t total = NTl * KT * CH * 64;
-  const int64_t ld = fmt == kE4M3 ? K : K * 3 / 4;
-  pack_weight_kernel<<<dim3((unsigned)((total + 255) / 256)), 256, 0, s>>>(
+  const int64_t ld = fmt == kE4M3 ? K : fmt == kE2M1 ? K / 2 : K * 3 / 4;
+  if (fmt == kE2M1)
+    pack_fp4_kernel<<<dim3((unsigned)((total + 255) / 256)), 256, 0, s>>>((const uint8_t*)codes, ld,
+                                                                         (uint8_t*)tiled_codes, N, KT, total);
+  else pack_weight_kernel<<<dim3((unsigned)((total + 255) / 256)), 256, 0, s>>>(
       (const uint8_t*)codes, ld, (uint8_t*)tiled_codes, N, K, KT, CH, fmt != kE4M3, total);
   MXL_CHECK_LAUNCH("mxl_pack_weight(codes)");
   if (scales) {

@@ -15,8 +15,10 @@ template <>
 struct FmtTraits<kE2M3> { static constexpr int CH = 6; static constexpr int RUN = 24; };
 template <>
 struct FmtTraits<kE3M2> { static constexpr int CH = 6; static constexpr int RUN = 24; };
+template <>
+struct FmtTraits<kE2M1> { static constexpr int CH = 4; static constexpr int RUN = 16; };
 
-__host__ __device__ inline int tile_chunks(int fmt) { return fmt == kE4M3 ? 8 : 6; }
+__host__ __device__ inline int tile_chunks(int fmt) { return fmt == kE4M3 ? 8 : fmt == kE2M1 ? 4 : 6; }
 
 struct GemmParams {
   const uint8_t* a;      // activation codes, row-major

@@ -19,10 +19,10 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 // element formats understood by the scaled MFMA (cbsz / blgp operand)
-enum Fmt : int { kE4M3 = 0, kE5M2 = 1, kE2M3 = 2, kE3M2 = 3 };
+enum Fmt : int { kE4M3 = 0, kE5M2 = 1, kE2M3 = 2, kE3M2 = 3, kE2M1 = 4 };
 
 // E8M0 scale rules
-enum Rule : int { kFloorCarry175 = 0, kCeilDiv448 = 1, kRpUe8m0 = 2 };
+enum Rule : int { kFloorCarry175 = 0, kCeilDiv448 = 1, kRpUe8m0 = 2, kFloorOcp = 3 };
 
 __device__ __forceinline__ uint32_t f2u(float f) { return __builtin_bit_cast(uint32_t, f); }
 __device__ __forceinline__ float u2f(uint32_t u) { return __builtin_bit_cast(float, u); }

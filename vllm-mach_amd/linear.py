@@ -29,6 +29,8 @@ MXFP8_STATIC = "mxfp8_e4m3_static"
 MXFP6_E3M2_STATIC = "mxfp6_e3m2_static"
 MXFP6_E2M3_STATIC = "mxfp6_e2m3_static"
 FP8_BLOCK128 = "fp8_e4m3_block128"
+MXFP4_STATIC = "mxfp4_e2m1_static"
+MXFP4_DYNAMIC = "mxfp4_e2m1_dynamic"
 
 _FP6_FORMAT = {MXFP6_E3M2_STATIC: ops.E3M2, MXFP6_E2M3_STATIC: ops.E2M3}
 
@@ -280,11 +282,59 @@ class BlockFp8LinearKernel(_Kernel):
         return y if bias is inner else y + bias
 
 
+class Mxfp4LinearKernel(_Kernel):
+    """W4A4 MXFP4: packed E2M1 weights u8 [N, K/2] (the even column in a byte's low half) with E8M0
+    scales [N, K/32]; bf16 activations quantized to MXFP4 on the fly (rule floor_carry175); bf16 out.
+
+    No counterpart in the reference (its 4-bit path is NVFP4); the surface is the other kernels'.
+    """
+
+    act_rule = ops.FLOOR_CARRY175
+
+    @classmethod
+    def can_implement(cls, config: MxLinearLayerConfig) -> tuple[bool, Optional[str]]:
+        if config.weight_quant_key != MXFP4_STATIC:
+            return False, "requires static MXFP4 (E2M1) weights"
+        if config.activation_quant_key != MXFP4_DYNAMIC:
+            return False, "requires dynamic MXFP4 activations"
+        return True, None
+
+    def process_weights_after_loading(self, layer: torch.nn.Module) -> None:
+        weight = layer.weight.data
+        if weight.dtype != torch.uint8 or weight.ndim != 2:
+            raise ValueError("MXFP4 requires packed uint8 weights [N, K/2]")
+        n, k = weight.shape[0], weight.shape[1] * 2
+        if n <= 0 or n % 8 or k <= 0 or k % 128:
+            raise ValueError(f"MXFP4 requires N % 8 == 0 and K % 128 == 0; got N={n}, K={k}")
+        scale = layer.weight_scale.data
+        if scale.dtype != torch.uint8 or tuple(scale.shape) != (n, k // 32):
+            raise ValueError("MXFP4 requires uint8 E8M0 scales shaped [N, K/32]")
+        tiled, tiled_s = ops.pack_weight(weight.contiguous(), scale.contiguous(), ops.E2M1)
+        _replace(layer, "weight", tiled)
+        _replace(layer, "weight_scale", tiled_s)
+        layer.mxl_shape = (n, k)
+        layer.mxl_format = ops.E2M1
+        layer.mxl_kernel = self
+
+    def apply_weights(self, layer: torch.nn.Module, x: torch.Tensor,
+                      bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+        n, k = layer.mxl_shape
+        if x.dtype != torch.bfloat16 or x.shape[-1] != k:
+            raise ValueError("MXFP4 requires BF16 activations with matching K")
+        if x.numel() == 0:
+            return x.new_empty((*x.shape[:-1], n))
+        inner = _epilogue_bias(bias, x, n)
+        y = ops.mxfp4_gemm_from_float(_flatten(x, k), layer.weight, layer.weight_scale, n, self.act_rule, inner)
+        y = y.reshape(*x.shape[:-1], n)
+        return y if bias is inner else y + bias
+
+
 _KERNELS = {
     MXFP8_STATIC: Mxfp8LinearKernel,
     MXFP6_E3M2_STATIC: Mxfp6LinearKernel,
     MXFP6_E2M3_STATIC: Mxfp6LinearKernel,
     FP8_BLOCK128: BlockFp8LinearKernel,
+    MXFP4_STATIC: Mxfp4LinearKernel,
 }
 
 
@@ -292,7 +342,7 @@ class MxLinearMethod:
     """``LinearMethodBase``-shaped method for one of the quantized linear schemes.
 
     ``create_weights`` registers the checkpoint-format parameters (the layouts of
-    compressed-tensors MXFP8, Quark OCP-MX packed FP6 and block-FP8 ``weight_scale_inv``);
+    compressed-tensors MXFP8, Quark OCP-MX packed FP6 and FP4, and block-FP8 ``weight_scale_inv``);
     ``process_weights_after_loading`` repacks them to the MFMA-tiled layout;
     ``apply`` runs the layer.
     """
@@ -300,7 +350,7 @@ class MxLinearMethod:
     def __init__(self, weight_quant_key: str = MXFP8_STATIC):
         if weight_quant_key not in _KERNELS:
             raise ValueError(f"unknown weight quant key {weight_quant_key!r}")
-        act = FP8_BLOCK128 if weight_quant_key == FP8_BLOCK128 else MXFP8_DYNAMIC
+        act = {FP8_BLOCK128: FP8_BLOCK128, MXFP4_STATIC: MXFP4_DYNAMIC}.get(weight_quant_key, MXFP8_DYNAMIC)
         self.config = MxLinearLayerConfig(weight_quant_key, act)
         self.kernel = _KERNELS[weight_quant_key](self.config)
 
@@ -326,8 +376,8 @@ class MxLinearMethod:
             w = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=device)
             s = torch.empty((n, k // 32), dtype=torch.uint8, device=device)
             names = ("weight", "weight_scale")
-        elif key in _FP6_FORMAT:
-            w = torch.empty((n, k * 3 // 4), dtype=torch.uint8, device=device)
+        elif key in _FP6_FORMAT or key == MXFP4_STATIC:
+            w = torch.empty((n, k // 2 if key == MXFP4_STATIC else k * 3 // 4), dtype=torch.uint8, device=device)
             s = torch.empty((n, k // 32), dtype=torch.uint8, device=device)
             names = ("weight", "weight_scale")
         else:
@@ -368,15 +418,27 @@ def swiglu_mxfp8_down(gate_up: torch.Tensor, down: torch.nn.Module) -> torch.Ten
     return ops.swiglu_mx_down(gate_up, down.weight, down.weight_scale, n, down.mxl_format)
 
 
+def swiglu_mxfp4_down(gate_up: torch.Tensor, down: torch.nn.Module) -> torch.Tensor:
+    """Fused SwiGLU -> MXFP4 -> down projection for a layer prepared by ``Mxfp4LinearKernel``."""
+    if getattr(down, "mxl_format", None) != ops.E2M1:
+        raise ValueError("the down projection is not an MXFP4 layer")
+    n, k = down.mxl_shape
+    if gate_up.shape[-1] != 2 * k:
+        raise ValueError("gate_up width must be twice the down projection's K")
+    y = ops.swiglu_mxfp4_down(_flatten(gate_up, 2 * k), down.weight, down.weight_scale, n)
+    return y.reshape(*gate_up.shape[:-1], n)
+
+
 # registration: the reference prepends its kernels to vLLM's per-platform candidate
 # lists (src/vllm_mach/mxfp6/dense.py:244-275, dense_mxfp8.py:165-174)
-POSSIBLE_KERNELS: dict[str, list[type]] = {"mxfp8": [], "mxfp6": [], "fp8_block": []}
+POSSIBLE_KERNELS: dict[str, list[type]] = {"mxfp8": [], "mxfp6": [], "fp8_block": [],
+                                              "mxfp4": []}
 
 
 def register_kernels(registry: Optional[dict] = None) -> dict:
     registry = POSSIBLE_KERNELS if registry is None else registry
     for name, cls in (("mxfp8", Mxfp8LinearKernel), ("mxfp6", Mxfp6LinearKernel),
-                      ("fp8_block", BlockFp8LinearKernel)):
+                      ("fp8_block", BlockFp8LinearKernel), ("mxfp4", Mxfp4LinearKernel)):
         lst = registry.setdefault(name, [])
         while cls in lst:
             lst.remove(cls)

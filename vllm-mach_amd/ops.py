@@ -26,9 +26,10 @@ import torch
 from . import _lib
 from ._lib import call, ptr, query, stream_handle
 
-E4M3, E2M3, E3M2 = 0, 2, 3
-FLOOR_CARRY175, CEIL_DIV448, RP_UE8M0 = 0, 1, 2
-FORMATS = {"e4m3": E4M3, "e2m3": E2M3, "e3m2": E3M2}
+E4M3, E2M3, E3M2, E2M1 = 0, 2, 3, 4
+FLOOR_CARRY175, CEIL_DIV448, RP_UE8M0, FLOOR_OCP = 0, 1, 2, 3
+SOFTMAX, SIGMOID = 0, 1  # router scores
+FORMATS = {"e4m3": E4M3, "e2m3": E2M3, "e3m2": E3M2, "e2m1": E2M1}
 
 _ws_lock = threading.RLock()
 
@@ -385,10 +386,15 @@ def pack_weight(codes: torch.Tensor, scales: Optional[torch.Tensor], fmt: int) -
     """Logical checkpoint layout -> MFMA-tiled layout (load time, replaces ``pack_scales``,
     src/vllm_mach/mxfp6/dense_mxfp8.py:150-151 and dense.py:185-188).
 
-    codes: E4M3 [N, K] (fmt 0) or packed FP6 u8 [N, 3K/4]; scales: E8M0 u8 [N, K/32] or None.
+    codes: E4M3 [N, K] (fmt 0), packed FP6 u8 [N, 3K/4] or packed E2M1 u8 [N, K/2] (fmt 4, the even
+    column in a byte's low half); scales: E8M0 u8 [N, K/32] or None.
     Batched [E, N, ...] inputs are packed per expert into one contiguous buffer.
     """
     _check_cuda(codes, scales)
+    if codes.ndim == 3 and codes.shape[1] % 16 == 0 and (scales is None or scales.ndim == 3):
+        # (n-tiles of 16 rows do not span experts: the experts' layouts back to back are one of E N rows)
+        w, s = pack_weight(codes.flatten(0, 1), None if scales is None else scales.flatten(0, 1), fmt)
+        return w.view(codes.shape[0], -1), None if s is None else s.view(codes.shape[0], -1)
     if codes.ndim == 3:
         parts = [pack_weight(codes[e], None if scales is None else scales[e], fmt) for e in range(codes.shape[0])]
         w = torch.stack([p[0] for p in parts])
@@ -396,7 +402,7 @@ def pack_weight(codes: torch.Tensor, scales: Optional[torch.Tensor], fmt: int) -
         return w, s
     c = _u8(codes).contiguous()
     N = c.shape[0]
-    K = c.shape[1] if fmt == E4M3 else c.shape[1] * 4 // 3
+    K = c.shape[1] if fmt == E4M3 else c.shape[1] * 2 if fmt == E2M1 else c.shape[1] * 4 // 3
     tiled = torch.empty(query("mxl_tiled_weight_bytes", N, K, fmt), dtype=torch.uint8, device=c.device)
     tiled_s = None
     if scales is not None:
@@ -736,6 +742,198 @@ def block_fp8_from_float(x: torch.Tensor, w: torch.Tensor, sb: torch.Tensor, n: 
     return torch.ops.mach_amd.block_fp8_gemm(q, s, w, sb, n, x.shape[1], bias)
 
 
+# ------------------------------------------------------------------ MXFP4
+
+def _on(device: torch.device):
+    """The device of a call's tensors as the current one (a no-op where it is)."""
+    return contextlib.nullcontext() if _device_index(device) == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    _check_cuda(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+def _rows16(x: torch.Tensor) -> torch.Tensor:
+    """x as rows of unit column stride that start on 16 bytes (a copy where they do not)."""
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < x.shape[1] or x.data_ptr() % 16:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
+    return x
+
+
+def _aligned(t: torch.Tensor, nbytes: int) -> torch.Tensor:
+    """t contiguous and starting on ``nbytes`` bytes."""
+    if not t.is_contiguous() or t.data_ptr() % nbytes:
+        return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+    return t
+
+
+@torch.library.custom_op("mach_amd::quantize_mxfp4", mutates_args=())
+def quantize_mxfp4(x: torch.Tensor, rule: int = FLOOR_CARRY175) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 [M, K] -> (packed E2M1 codes u8 [M, K/2], E8M0 scales u8 [M, K/32]), K % 32 == 0.
+
+    Two codes per byte, the even column in the low half.  A block's scale is 2^(floor(log2 amax) - 2),
+    doubled from 1.75 times a power of two on (``FLOOR_CARRY175``: no value rounds past 6) or not
+    (``FLOOR_OCP``, OCP MX v1.0: values past 6 saturate); codes round to nearest even.  A block with an
+    infinity or NaN gets the NaN scale (255) and zero codes.
+    """
+    _check_cuda(x)
+    if x.dtype != torch.bfloat16 or x.ndim != 2 or x.shape[1] == 0 or x.shape[1] % 32:
+        raise ValueError("quantize_mxfp4 needs a 2-D bf16 tensor with K > 0 and K % 32 == 0")
+    if rule not in (FLOOR_CARRY175, FLOOR_OCP):
+        raise ValueError(f"quantize_mxfp4: unknown rule {rule}")
+    x = _rows16(x)
+    M, K = x.shape
+    codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((M, K // 32), dtype=torch.uint8, device=x.device)
+    if M:
+        with _on(x.device):
+            call("mxl_quantize_mxfp4", ptr(x), M, K, x.stride(0), rule, ptr(codes), ptr(scales),
+                 stream_handle(x.device))
+    _count("quantize_mxfp4")
+    return codes, scales
+
+
+@quantize_mxfp4.register_fake
+def _(x, rule=FLOOR_CARRY175):
+    return (x.new_empty((x.shape[0], x.shape[1] // 2), dtype=torch.uint8),
+            x.new_empty((x.shape[0], x.shape[1] // 32), dtype=torch.uint8))
+
+
+@torch.library.custom_op("mach_amd::swiglu_mxfp4", mutates_args=())
+def swiglu_mxfp4(gate_up: torch.Tensor, rule: int = FLOOR_CARRY175) -> tuple[torch.Tensor, torch.Tensor]:
+    """SwiGLU -> MXFP4: gate_up bf16 [M, 2K] -> (codes u8 [M, K/2], scales u8 [M, K/32]) of
+    bf16(bf16(silu(gate)) * up), the activation of ``swiglu_mxfp8``, quantized as ``quantize_mxfp4`` does."""
+    _check_cuda(gate_up)
+    if gate_up.dtype != torch.bfloat16 or gate_up.ndim != 2 or gate_up.shape[1] == 0 or gate_up.shape[1] % 64:
+        raise ValueError("swiglu_mxfp4 needs bf16 [M, 2K] with K > 0 and K % 32 == 0")
+    if rule not in (FLOOR_CARRY175, FLOOR_OCP):
+        raise ValueError(f"swiglu_mxfp4: unknown rule {rule}")
+    gate_up = _aligned(gate_up, 16)
+    M, K = gate_up.shape[0], gate_up.shape[1] // 2
+    codes = torch.empty((M, K // 2), dtype=torch.uint8, device=gate_up.device)
+    scales = torch.empty((M, K // 32), dtype=torch.uint8, device=gate_up.device)
+    if M:
+        with _on(gate_up.device):
+            call("mxl_swiglu_mxfp4", ptr(gate_up), M, K, rule, ptr(codes), ptr(scales), stream_handle(gate_up.device))
+    _count("swiglu_mxfp4")
+    return codes, scales
+
+
+@swiglu_mxfp4.register_fake
+def _(gate_up, rule=FLOOR_CARRY175):
+    M, K = gate_up.shape[0], gate_up.shape[1] // 2
+    return (gate_up.new_empty((M, K // 2), dtype=torch.uint8), gate_up.new_empty((M, K // 32), dtype=torch.uint8))
+
+
+def _fp4_weight(what: str, w: torch.Tensor, sw: torch.Tensor, n: int, k: int, experts: int = 1):
+    """The tiled weight's tensors, of the size that (n, k) asks for."""
+    if n <= 0 or k <= 0 or k % 128:
+        raise ValueError(f"{what} needs N > 0 and K > 0, K % 128 == 0 (N={n}, K={k})")
+    if w.dtype != torch.uint8 or w.numel() != experts * query("mxl_tiled_weight_bytes", n, k, E2M1):
+        raise ValueError(f"{what}: the weight is not {experts} x [{n}, {k}] E2M1 in the tiled layout (pack_weight)")
+    if sw.dtype != torch.uint8 or sw.numel() != experts * query("mxl_tiled_scale_bytes", n, k):
+        raise ValueError(f"{what}: the scales are not {experts} x [{n}, {k}] in the tiled layout (pack_weight)")
+    return _aligned(w, 16), _aligned(sw, 16)
+
+
+def _fp4_rows(what: str, a: torch.Tensor, sa: torch.Tensor, k: int):
+    if a.dtype != torch.uint8 or a.ndim != 2 or a.shape[1] != k // 2:
+        raise ValueError(f"{what}: activation codes must be u8 [M, K/2] (K={k}), got {a.dtype} {tuple(a.shape)}")
+    if sa.dtype != torch.uint8 or tuple(sa.shape) != (a.shape[0], k // 32):
+        raise ValueError(f"{what}: activation scales must be u8 [M, K/32] = [{a.shape[0]}, {k // 32}]")
+    return _aligned(a, 16), _aligned(sa, 16)
+
+
+def _fp4_bias(what: str, bias: Optional[torch.Tensor], n: int) -> Optional[torch.Tensor]:
+    if bias is None:
+        return None
+    if bias.dtype != torch.bfloat16 or tuple(bias.shape) != (n,):
+        raise ValueError(f"{what}: bias must be bf16 [{n}]")
+    return bias.contiguous()
+
+
+@torch.library.custom_op("mach_amd::mxfp4_gemm", mutates_args=())
+def mxfp4_gemm(a: torch.Tensor, sa: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, k: int,
+               bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Product of MXFP4 activations and weights: y = A W^T (+ bias), fp32 sums, bf16 [M, N].
+
+    a, sa: ``quantize_mxfp4``'s codes u8 [M, K/2] and scales u8 [M, K/32]; w, sw: the weight in the tiled
+    layout (``pack_weight`` with ``E2M1``).  A bias is added to the rounded sum, and rounded again.
+    """
+    _same_device("mxfp4_gemm", a, sa, w, sw, bias)
+    w, sw = _fp4_weight("mxfp4_gemm", w, sw, n, k)
+    a, sa = _fp4_rows("mxfp4_gemm", a, sa, k)
+    bias = _fp4_bias("mxfp4_gemm", bias, n)
+    M = a.shape[0]
+    out = torch.empty((M, n), dtype=torch.bfloat16, device=a.device)
+    if M:
+        with _on(a.device):
+            nbytes = query("mxl_mxfp4_gemm_workspace_bytes", M, n, k)
+            ws = workspace(a.device, nbytes)
+            call("mxl_mxfp4_gemm", ptr(a), ptr(sa), M, ptr(w), ptr(sw), n, k, ptr(bias), ptr(out), n, ptr(ws), nbytes,
+                 stream_handle(a.device))
+    _count("mxfp4_gemm")
+    return out
+
+
+@mxfp4_gemm.register_fake
+def _(a, sa, w, sw, n, k, bias=None):
+    return a.new_empty((a.shape[0], n), dtype=torch.bfloat16)
+
+
+def mxfp4_gemm_from_float(x: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, rule: int = FLOOR_CARRY175,
+                          bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bf16 rows x [M, K] quantized to MXFP4 and multiplied with an MXFP4 weight."""
+    a, sa = torch.ops.mach_amd.quantize_mxfp4(x, rule)
+    return torch.ops.mach_amd.mxfp4_gemm(a, sa, w, sw, n, x.shape[1], bias)
+
+
+def swiglu_mxfp4_down(gate_up: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int,
+                      rule: int = FLOOR_CARRY175) -> torch.Tensor:
+    """SwiGLU -> MXFP4, then the down projection with an MXFP4 weight (``swiglu_mx_down`` in 4 bits)."""
+    a, sa = torch.ops.mach_amd.swiglu_mxfp4(gate_up, rule)
+    return torch.ops.mach_amd.mxfp4_gemm(a, sa, w, sw, n, gate_up.shape[1] // 2, None)
+
+
+@torch.library.custom_op("mach_amd::mxfp4_grouped_gemm", mutates_args=())
+def mxfp4_grouped_gemm(a: torch.Tensor, sa: torch.Tensor, row_index: Optional[torch.Tensor], row_div: int,
+                       expert_offsets: torch.Tensor, routed_rows: int, w: torch.Tensor, sw: torch.Tensor, n: int,
+                       k: int) -> torch.Tensor:
+    """``grouped_gemm`` of MXFP4 activations and experts: output row p (sorted order) of expert e
+    (expert_offsets[e] <= p < expert_offsets[e+1]) is A[row_index[p] // row_div] . W[e]^T, or A[p] . W[e]^T
+    without row_index.  Rows past expert_offsets[E] are left unwritten."""
+    _same_device("mxfp4_grouped_gemm", a, sa, row_index, expert_offsets, w, sw)
+    if expert_offsets.dtype != torch.int64 or expert_offsets.ndim != 1 or expert_offsets.numel() < 2:
+        raise ValueError("mxfp4_grouped_gemm: expert_offsets must be i64 [E + 1]")
+    E = expert_offsets.numel() - 1
+    w, sw = _fp4_weight("mxfp4_grouped_gemm", w, sw, n, k, E)
+    a, sa = _fp4_rows("mxfp4_grouped_gemm", a, sa, k)
+    if row_index is not None and (row_index.dtype != torch.int32 or row_index.ndim != 1
+                                  or row_index.numel() < routed_rows):
+        raise ValueError("mxfp4_grouped_gemm: row_index must be i32 with an entry per routed row")
+    if routed_rows < 0 or row_div < 1 or (row_index is None and a.shape[0] < routed_rows):
+        raise ValueError("mxfp4_grouped_gemm: need row_div >= 1 and, without row_index, an activation row per routed row")
+    if routed_rows and not a.shape[0]:
+        raise ValueError("mxfp4_grouped_gemm: no activation rows")
+    row_index = row_index.contiguous() if row_index is not None else None
+    offsets = expert_offsets.contiguous()
+    out = torch.empty((routed_rows, n), dtype=torch.bfloat16, device=a.device)
+    if routed_rows:
+        with _on(a.device):
+            call("mxl_mxfp4_grouped_gemm", ptr(a), ptr(sa), a.shape[0], ptr(row_index), row_div, ptr(offsets), E,
+                 routed_rows, ptr(w), ptr(sw), n, k, ptr(out), stream_handle(a.device))
+    _count("mxfp4_grouped_gemm")
+    return out
+
+
+@mxfp4_grouped_gemm.register_fake
+def _(a, sa, row_index, row_div, expert_offsets, routed_rows, w, sw, n, k):
+    return a.new_empty((routed_rows, n), dtype=torch.bfloat16)
+
+
 # ---------------------------------------------------------------------- MoE
 
 @torch.library.custom_op("mach_amd::moe_route", mutates_args=())
@@ -801,6 +999,61 @@ def moe_router(router_logits: torch.Tensor, top_k: int, renormalize: bool = True
 
 @moe_router.register_fake
 def _(router_logits, top_k, renormalize=True):
+    T, E = router_logits.shape
+    R = T * top_k
+    return (router_logits.new_empty((T, top_k), dtype=torch.float32),
+            router_logits.new_empty((T, top_k), dtype=torch.int32),
+            router_logits.new_empty((R,), dtype=torch.int32),
+            router_logits.new_empty((E + 1,), dtype=torch.int64),
+            router_logits.new_empty((R,), dtype=torch.int32))
+
+
+@torch.library.custom_op("mach_amd::moe_router_grouped", mutates_args=())
+def moe_router_grouped(router_logits: torch.Tensor, bias: Optional[torch.Tensor], top_k: int, scoring: int = SOFTMAX,
+                       num_groups: int = 1, topk_groups: int = 1, renormalize: bool = True, factor: float = 1.0
+                       ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``moe_router`` with softmax or sigmoid scores, a balance bias and groups of experts.
+
+    Scores s of the logits [T, E] (fp32 or bf16) are ``SOFTMAX`` over the experts or ``SIGMOID``; the choice
+    scores are c = s + bias (fp32 [E] or None).  Of ``num_groups`` equal groups of consecutive experts the
+    ``topk_groups`` best are kept, by their largest c or with a bias the sum of their two largest; the
+    ``top_k`` largest c among the kept groups' experts are chosen, in descending order.  Ties go to the lower
+    index, and a NaN ranks below every other score.  Weights are s (not c), divided by their sum + 1e-20 with
+    ``renormalize``, times ``factor``.  Scores are held in 64 bits.  Returns moe_router's five tensors.
+    """
+    _same_device("moe_router_grouped", router_logits, bias)
+    if router_logits.ndim != 2 or router_logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("moe_router_grouped needs fp32 or bf16 logits [T, E]")
+    logits = router_logits.contiguous()
+    T, E = logits.shape
+    if bias is not None:
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (E,):
+            raise ValueError(f"moe_router_grouped: bias must be fp32 [{E}]")
+        bias = bias.contiguous()
+    if scoring not in (SOFTMAX, SIGMOID):
+        raise ValueError(f"moe_router_grouped: unknown scoring {scoring}")
+    if num_groups < 1 or E < 1 or E % num_groups or not 1 <= topk_groups <= num_groups:
+        raise ValueError(f"moe_router_grouped: {topk_groups} of {num_groups} groups of {E} experts")
+    if not 1 <= top_k <= topk_groups * (E // num_groups):
+        raise ValueError(f"moe_router_grouped: top_k {top_k} of {topk_groups * (E // num_groups)} experts")
+    dev = logits.device
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    sorted_routes = torch.empty(T * top_k, dtype=torch.int32, device=dev)
+    offsets = torch.empty(E + 1, dtype=torch.int64, device=dev)
+    inverse = torch.empty(T * top_k, dtype=torch.int32, device=dev)
+    with _on(dev):
+        nbytes = query("mxl_moe_router_workspace_bytes", T, top_k, E)
+        buf = workspace(dev, nbytes, "route")
+        call("mxl_moe_router_grouped", ptr(logits), int(logits.dtype == torch.bfloat16), ptr(bias), T, E, top_k, scoring,
+             num_groups, topk_groups, int(renormalize), float(factor), ptr(weights), ptr(ids), ptr(sorted_routes),
+             ptr(offsets), ptr(inverse), ptr(buf), nbytes, stream_handle(dev))
+    _count("moe_router_grouped")
+    return weights, ids, sorted_routes, offsets, inverse
+
+
+@moe_router_grouped.register_fake
+def _(router_logits, bias, top_k, scoring=SOFTMAX, num_groups=1, topk_groups=1, renormalize=True, factor=1.0):
     T, E = router_logits.shape
     R = T * top_k
     return (router_logits.new_empty((T, top_k), dtype=torch.float32),
