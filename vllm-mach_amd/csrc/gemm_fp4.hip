@@ -81,6 +81,22 @@ static int check_operands(const char* who, const void* a, const void* sa, const 
   return MXL_OK;
 }
 
+// A stage of the 2 x 2-wave tiles is 128 bytes of a row, whatever its format, and takes two MFMAs of a K128
+// slice of MXFP4 the time of one of 8-bit activations: the time model of K / 2 bytes holds.
+static WideConfig fp4_tiles_config(int64_t M, int64_t N, int64_t K) {
+  const int64_t KT = (K + kTileK - 1) / kTileK;
+  WideConfig c = wide_tiles_config(M, N, (K / 2 + 127) / 128 * 128, false);
+  c.kt_per_split = 2 * c.kt_per_split < KT ? 2 * c.kt_per_split : KT;  // super-tiles of half the stages
+  c.S = (int)((KT + c.kt_per_split - 1) / c.kt_per_split);
+  if (c.dp_tiles > 0) {
+    c.kt2 = 2 * c.kt2 < KT ? 2 * c.kt2 : KT;
+    c.S2 = (int)((KT + c.kt2 - 1) / c.kt2);
+  }
+  return c;
+}
+
+static bool fp4_tiles_eligible(int64_t M, int64_t N, int64_t K) { return wide_tiles_eligible(M, N, K / 2, false); }
+
 static GemmParams fp4_params(const void* a, const void* sa, const void* w, const void* sw, int64_t N, int64_t K,
                              void* out, int64_t ldc) {
   GemmParams p{};
@@ -90,7 +106,10 @@ static GemmParams fp4_params(const void* a, const void* sa, const void* w, const
   return p;
 }
 
-extern "C" int64_t mxl_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
+extern "C" int64_t mxl_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 16 || N <= 0 || K <= 0 || K % 128 || !fp4_tiles_eligible(M, N, K)) return 0;
+  return wide_workspace_bytes(fp4_tiles_config(M, N, K), M, N);
+}
 
 extern "C" int mxl_mxfp4_gemm(const void* a, const void* sa, int64_t M, const void* w_tiled, const void* sw_tiled,
                               int64_t N, int64_t K, const void* bias, void* out, int64_t ldc, void* workspace,
@@ -103,6 +122,21 @@ extern "C" int mxl_mxfp4_gemm(const void* a, const void* sa, int64_t M, const vo
   GemmParams p = fp4_params(a, sa, w_tiled, sw_tiled, N, K, out, ldc);
   p.M = p.a_rows = M;
   p.bias = (const uint16_t*)bias;
+  if (M > 16 && fp4_tiles_eligible(M, N, K)) {
+    const WideConfig c = fp4_tiles_config(M, N, K);
+    const int64_t need = wide_workspace_bytes(c, M, N);
+    MXL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+                  "%s: needs a 16-byte aligned workspace of %lld bytes (have %lld)", who, (long long)need,
+                  (long long)workspace_bytes);
+    p.S = c.S;
+    p.partial = (float*)workspace;
+    const hipError_t e = launch_gemm_wide(kE2M1, false, c, p, 0, (hipStream_t)stream);
+    if (e != hipSuccess) {
+      set_error("%s: launch failed: %s", who, hipGetErrorString(e));
+      return MXL_EHIP;
+    }
+    return MXL_OK;
+  }
   fp4_gemm_kernel<<<dim3((unsigned)((N + 63) / 64), (unsigned)((M + 15) / 16)), 256, 0, (hipStream_t)stream>>>(p);
   MXL_CHECK_LAUNCH(who);
   return MXL_OK;
@@ -122,6 +156,17 @@ extern "C" int mxl_mxfp4_grouped_gemm(const void* a, const void* sa, int64_t a_r
   p.M = routed_rows; p.a_rows = a_rows; p.row_index = row_index; p.row_div = row_div; p.expert_offsets = expert_offsets;
   p.w_expert_stride = mxl_tiled_weight_bytes(N, K, kE2M1);
   p.sw_expert_stride = mxl_tiled_scale_bytes(N, K);
+  if (routed_rows >= 16 * num_experts && num_experts <= kWideGroupedMaxExperts && a_rows > 0 &&
+      fp4_tiles_eligible(a_rows, N, K)) {
+    WideConfig c{2, 1, p.KT};
+    c.MT = routed_rows >= 48 * num_experts ? 8 : 4;
+    const hipError_t e = launch_gemm_wide(kE2M1, false, c, p, num_experts, (hipStream_t)stream);
+    if (e != hipSuccess) {
+      set_error("%s: launch failed: %s", who, hipGetErrorString(e));
+      return MXL_EHIP;
+    }
+    return MXL_OK;
+  }
   fp4_grouped_kernel<<<dim3((unsigned)((N + 63) / 64), (unsigned)num_experts), 256, 0, (hipStream_t)stream>>>(p);
   MXL_CHECK_LAUNCH(who);
   return MXL_OK;

@@ -1,5 +1,7 @@
 // One output tile of the 2 x 2-wave GEMM on gfx950 (MX and block-FP8 weights): the device
 // body of the dense kernels of gemm_tile.hip and the grouped ones of gemm_tile_grouped.hip.
+// A stage is 128 bytes of an activation row: K128 of 8-bit activations, or K256 of MXFP4 ones
+// (E2M1 weights take E2M1 activations), whose two K128 slices are an MFMA each, at half the time.
 //
 // What bounds it.  At 128 x 128 tiles per workgroup every K128 stage moves as many LDS
 // bytes as the LDS serves in the time of its MFMAs, so the wide kernel (gemm_wide.hip)
@@ -70,6 +72,7 @@ __device__ __forceinline__ int tile_swz(int r) { return ((r >> 1) ^ ((r & 1) << 
 template <int J>
 struct Slice { static constexpr int value = J; };
 
+typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v6i __attribute__((ext_vector_type(6)));
 template <int FMT>
 struct TileB { typedef v8i type; };
@@ -77,6 +80,14 @@ template <>
 struct TileB<kE2M3> { typedef v6i type; };
 template <>
 struct TileB<kE3M2> { typedef v6i type; };
+// MXFP4, weights and activations alike: a lane's operands of the stage's two slices
+struct TileFp4 { v4i half[2]; };
+template <>
+struct TileB<kE2M1> { typedef TileFp4 type; };
+template <int FMT>
+struct TileA { typedef v8i type; };
+template <>
+struct TileA<kE2M1> { typedef TileFp4 type; };
 
 // c += W A^T for one 16 x 16 tile over a K128 slice, J the slice's byte of the packed E8M0
 // operands.  Written as assembly so that the accumulator is updated in place: with 256
@@ -99,9 +110,13 @@ __device__ __forceinline__ void tile_mfma(v4f& c, const typename TileB<FMT>::typ
   if constexpr (FMT == kE4M3) { MXL_TILE_MFMA_J(""); }
   else if constexpr (FMT == kE2M3) { MXL_TILE_MFMA_J(" cbsz:2"); }
   else { MXL_TILE_MFMA_J(" cbsz:3"); }
+}
+template <int J>
+__device__ __forceinline__ void tile_mfma_fp4(v4f& c, const v4i& w, const v4i& a, uint32_t sw, uint32_t sa) {
+  MXL_TILE_MFMA_J(" cbsz:4 blgp:4");
+}
 #undef MXL_TILE_MFMA_J
 #undef MXL_TILE_MFMA
-}
 
 // An accumulator's values, read where they are used (left to the compiler, all of them are
 // copied to vector registers at the end of the loop, more than there are)
@@ -155,6 +170,8 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   using S = TileShape<MTW, NTW>;
   using L = TileLds<MTW, NTW, BLOCK>;
   constexpr int MH = MTW / 2, NH = NTW / 2, CH = FmtTraits<FMT>::CH;
+  constexpr bool FP4 = FMT == kE2M1;
+  constexpr int SPT = FP4 ? 2 : 4;  // stages of a 512-wide super-tile
   // A stage's copies take the slots of the stage DEPTH before it in the order those fall free.
   // At an odd depth that stage reads its B units in the other order, so the B unit this stage
   // needs first is copied second, and the barrier that hands it over waits for CB copies more.
@@ -165,9 +182,10 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   const int r = lane & 15, q = lane >> 4;
 
   // stage and tile indices in 32 bits (the host bounds the operands below 4 GiB)
-  const int T = (int)(p.K / 128), KT = (int)p.KT, ntiles = (int)((p.N + 15) / 16), kb = w.kb, ke = w.ke;
-  // stages 4 kb .. te - 1; an odd count runs one more (end), whose weights (past K) are zero
-  const int te = 4 * ke < T ? 4 * ke : T, end = (te + 1) & ~1;
+  const int slices = (int)(p.K / 128), T = FP4 ? (slices + 1) / 2 : slices;  // K128 slices, stages
+  const int KT = (int)p.KT, ntiles = (int)((p.N + 15) / 16), kb = w.kb, ke = w.ke;
+  // stages SPT kb .. te - 1; an odd count runs one more (end), whose weights (past K) are zero
+  const int te = SPT * ke < T ? SPT * ke : T, end = (te + 1) & ~1;
   const int nt_base = w.nb * (S::BN / 16);
 
   // copy sources.  A unit h: chunk c = CA wv + u holds rows 8 (c % 2) .. + 7 of the unit's
@@ -181,6 +199,9 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       const int row = a_row(w.row0 + ((e / MH) * MTW + h * MH + e % MH) * 16 + cr);
       a_off[h][u] = (uint32_t)row * (uint32_t)p.lda + 16 * ((lane & 7) ^ tile_swz(cr));
     }
+  // MXFP4: the last of an odd number of slices is half a stage, whose other half is the next row's first
+  // bytes (the weights there are zero, and E2M1 has no NaN) or, past the last row, its last 16 again
+  const uint32_t a_last = FP4 ? (uint32_t)(p.a_rows * p.lda - 16) : 0;
   // B unit h: chunk c = CB wv + u is chunk c % 2 of the unit's n-tile e = c / 2
   const uint8_t* b_src[2][(S::CB + 1) / 2];
 #pragma unroll
@@ -198,11 +219,13 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   // copies of stage tt into the slot at `slot`
   auto copy_a = [&](int h, int u, int tt, int slot) {
     const int tc = tt < te ? tt : te - 1;  // an odd count's last stage: a valid one again
-    tile_copy16(p.a + (uint32_t)tc * 128, a_off[h][u], lds_a + slot + h * S::AU + u * 1024);
+    uint32_t off = a_off[h][u];
+    if constexpr (FP4) off = __builtin_elementwise_min(off, a_last - (uint32_t)tc * 128);
+    tile_copy16(p.a + (uint32_t)tc * 128, off, lds_a + slot + h * S::AU + u * 1024);
   };
   auto copy_b = [&](int h, int u, int tt, int slot) {
-    const int j = tt & 3, c0 = FMT == kE4M3 ? 2 * j : (3 * j) >> 1;
-    tile_copy16(b_src[h][u >> 1] + (uint32_t)((tt >> 2) * CH + c0 + (u & 1)) * 1024, lane16,
+    const int j = tt & (SPT - 1), c0 = FMT == kE4M3 || FP4 ? 2 * j : (3 * j) >> 1;
+    tile_copy16(b_src[h][u >> 1] + (uint32_t)((tt >> (FP4 ? 1 : 2)) * CH + c0 + (u & 1)) * 1024, lane16,
                 lds_b + slot + h * S::BU + u * 1024);
   };
   // MX: scales of super-tile kt, 64 rows (16 bytes each) and four n-tiles per wave (where the
@@ -210,7 +233,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   // with the row.  Swizzled scales, and rows shorter than a window: dword by dword, 16 rows a
   // copy, clamped to the last slice.  Block-FP8: the four groups' fp32 scales of the rows, one
   // group per wave.
-  const bool dwords = !BLOCK && (p.sa_swz || p.K < kTileK);
+  const bool dwords = !BLOCK && ((!FP4 && p.sa_swz) || p.K < kTileK);  // (MXFP4 scales are logical)
   const uint32_t srow = (uint32_t)(p.K / 32);
   const int swa = wv % (S::BM / 64), swb = wv % (S::BN / 64);
   uint32_t sa_off[BLOCK ? S::BM / 64 : 1];
@@ -225,7 +248,8 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   const uint32_t sb_off = (uint32_t)snt * (uint32_t)KT * 256 + 16 * (lane & 15);
   const uint32_t lds_sa = tile_lds(lds + L::SA) + (BLOCK ? wv * S::BM * 4 : 64 * swa * 16);
   const uint32_t lds_sb = tile_lds(lds + L::SB) + 4 * swb * 256;
-  auto copy_scales = [&](int kt) {
+  // (FIRST: of the range's first super-tile; MXFP4's others belong to rows of a window and more)
+  auto copy_scales = [&](int kt, auto FIRST) {
     const int st = kt & 1;
     const int kc = kt < ke ? kt : ke - 1;
     if constexpr (BLOCK) {
@@ -235,13 +259,13 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
         tile_copy4(static_cast<const uint8_t*>(p.sa) + (int64_t)g * p.M * 4, sa_off[c],
                    lds_sa + st * (S::BM * 16) + 256 * c);
     } else {
-      if (dwords) {
-        const int slice = 4 * kc + (lane & 3) < T ? 4 * kc + (lane & 3) : T - 1;
+      if (dwords && (!FP4 || decltype(FIRST)::value)) {
+        const int slice = 4 * kc + (lane & 3) < slices ? 4 * kc + (lane & 3) : slices - 1;
 #pragma unroll
         for (int u = 0; u < S::BM / 64; ++u) {
-          const int c = wv + 4 * u;
+          const int c = wv + 4 * u, row = a_row(w.row0 + 16 * c + (lane >> 2));
           tile_copy4(static_cast<const uint8_t*>(p.sa),
-                     (uint32_t)(sa_row_offset(p, a_row(w.row0 + 16 * c + (lane >> 2))) + slice * (int)p.sa_ss),
+                     FP4 ? (uint32_t)row * srow + 4 * slice : (uint32_t)(sa_row_offset(p, row) + slice * (int)p.sa_ss),
                      tile_lds(lds + L::SA) + st * (S::BM * 16) + 256 * c);
         }
       } else {
@@ -251,7 +275,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       tile_copy16(w.sw + (uint32_t)kc * 256, sb_off, lds_sb + st * (S::BN * 16));
     }
   };
-  const int tb = 4 * kb;
+  const int tb = SPT * kb;
   if constexpr (BLOCK) {
     // the weight block scales of the split's stages, one LDS row per 128 columns (read in the
     // loop from global memory they would be compiler-counted loads, whose waits drain the copies)
@@ -271,7 +295,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   for (int i = 0; i < MTW; ++i)
 #pragma unroll
     for (int n = 0; n < NTW; ++n) acc[i][n] = v4f{0.f, 0.f, 0.f, 0.f};
-  v8i a[2][MH];
+  typename TileA<FMT>::type a[2][MH];
   typename TileB<FMT>::type b[2][NH];
   uint32_t sa[MTW], sb[NTW];         // MX: packed E8M0 bytes of the super-tile's slices
   float fa[BLOCK ? MTW : 1][4], fb[4];  // block-FP8: the super-tile's activation and weight scales
@@ -283,14 +307,20 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   const int rb = wn * NH * 2048 + lane * 16;
   auto read_a = [&](int h, int i, int half, int slot) {  // K 16 q .. (half 0) or 64 + 16 q .. (half 1)
     const uint8_t* src = lds + L::RING + slot + (half ? ra_hi : ra_lo) + h * S::AU + i * 2048;
-    const uint4 v = *reinterpret_cast<const uint4*>(src);
-    a[h][i][4 * half] = (int)v.x; a[h][i][4 * half + 1] = (int)v.y;
-    a[h][i][4 * half + 2] = (int)v.z; a[h][i][4 * half + 3] = (int)v.w;
+    if constexpr (FP4) {  // (slice 0 or 1 of the stage, K 32 q .. of it)
+      a[h][i].half[half] = *reinterpret_cast<const v4i*>(src);
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(src);
+      a[h][i][4 * half] = (int)v.x; a[h][i][4 * half + 1] = (int)v.y;
+      a[h][i][4 * half + 2] = (int)v.z; a[h][i][4 * half + 3] = (int)v.w;
+    }
   };
   auto read_b = [&](int h, int n, int half, int slot, int odd) {  // odd: the parity of the stage's slice
     const uint8_t* src = lds + L::RING + 2 * S::AU + slot + rb + h * S::BU + n * 2048;
     auto& x = b[h][n];
-    if constexpr (FMT == kE4M3) {
+    if constexpr (FP4) {
+      x.half[half] = *reinterpret_cast<const v4i*>(src + 1024 * half);
+    } else if constexpr (FMT == kE4M3) {
       const uint4 v = *reinterpret_cast<const uint4*>(src + 1024 * half);
       x[4 * half] = (int)v.x; x[4 * half + 1] = (int)v.y; x[4 * half + 2] = (int)v.z; x[4 * half + 3] = (int)v.w;
     } else if (!odd) {  // even slice: the first chunk and 8 bytes of the second
@@ -336,7 +366,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       }
     } else {
       // a part super-tile's window ends with the row: its first byte moves to byte 0
-      const int shift = 4 * kt + 4 <= T || dwords ? 0 : 8 * (4 * kt + 4 - T);
+      const int shift = 4 * kt + 4 <= slices || dwords ? 0 : 8 * (4 * kt + 4 - slices);
 #pragma unroll
       for (int i = 0; i < MTW; ++i) {
         const uint4 x = *reinterpret_cast<const uint4*>(lds + L::SA + st * (S::BM * 16) + ((wm * MTW + i) * 16 + r) * 16);
@@ -372,12 +402,30 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
     };
     auto quad = [&](auto QI, auto&& between) {
       constexpr int s = decltype(QI)::value, ah = s >> 1, bh = s == 0 || s == 3 ? x : y;
+      if constexpr (FP4) {  // the first slice's Q MFMAs, then the second's: a share after every two
+        auto slice = [&](auto H) {
+          constexpr int hf = decltype(H)::value;
+#pragma unroll
+          for (int i = 0; i < MH; ++i)
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+              tile_mfma_fp4<2 * st + hf>(acc[ah * MH + i][bh * NH + n], b[bh][n].half[hf], a[ah][i].half[hf],
+                                        sb[bh * NH + n], sa[ah * MH + i]);
+              const int m = hf * Q + i * NH + n;
+              if (m & 1) between(m >> 1);
+            }
+        };
+        slice(Slice<0>{});
+        slice(Slice<1>{});
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < MH; ++i)
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
           const int k = i * NH + n, g = s * Q + k;
-          if constexpr (BLOCK) {
+          if constexpr (FP4) {
+          } else if constexpr (BLOCK) {
             const v4f z = {0.f, 0.f, 0.f, 0.f};
             raw[g % 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[bh][n], a[ah][i], z, kE4M3, kE4M3, 0, 127, 0,
                                                                           127);
@@ -422,6 +470,12 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       }
     };
     tile_wait<S::HALF * (left && 2 * left - 2 < full ? 2 * left - 2 : full)>();
+    if constexpr (FP4 && st == 0) {
+      // every wave has read this super-tile's scales: their slot takes those of the one after the next.  (A
+      // super-tile is two stages, which a copy into the other slot one ahead could outlast: seven half-stages of
+      // copies follow it before the wait ahead of its read, which leaves at most six in flight.)
+      if ((tt >> 1) + 2 < ke) copy_scales((tt >> 1) + 2, Slice<0>{});
+    }
     quad(Slice<0>{}, [&](int k) { reads_b(k, y, cur, st); copies_a(k, 0); });
     quad(Slice<1>{}, [&](int k) { reads_a(k, 1, cur); copies_b(k, x); });
     if constexpr (left != 1) tile_wait<S::HALF * (ahead ? full : 2 * left - 3) - ODD>();
@@ -433,7 +487,8 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
     }
   };
 
-  copy_scales(kb);
+  copy_scales(kb, Slice<1>{});
+  if (FP4 && kb + 1 < ke) copy_scales(kb + 1, Slice<0>{});
   const int count = end - tb;  // stages: an even number
 #pragma unroll
   for (int k = 0; k < DEPTH; ++k) {  // units in the order the loop copies them
@@ -458,9 +513,9 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   // two stages per iteration, byte pairs 0, 1 then 2, 3 of the packed scales
   int cur = 0;  // the slot of the pair's first stage
   auto pair = [&](auto LEFT, int pr) {  // LEFT: the stages left at the pair's first, 0 for many
-    const int kt = pr >> 1;
-    if ((pr & 1) == 0) {
-      if (kt + 1 < ke) copy_scales(kt + 1);
+    const int kt = FP4 ? pr : pr >> 1;
+    if (FP4 || (pr & 1) == 0) {
+      if (!FP4 && kt + 1 < ke) copy_scales(kt + 1, Slice<0>{});
       read_scales(kt);  // landed: the copies of the stages before this one were issued after them
     } else if constexpr (BLOCK) {
 #pragma unroll
@@ -497,7 +552,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
     cur = two;
   };
   const int last = end >> 1;  // pairs 2 kb .. last - 1; the copies end in the final one or two
-  int pr = 2 * kb;
+  int pr = FP4 ? kb : 2 * kb;
   for (; pr + (DEPTH > 2 ? 2 : 1) < last; ++pr) pair(Slice<0>{}, pr);
   if (DEPTH > 2 && pr + 1 < last) pair(Slice<4>{}, pr++);
   pair(Slice<2>{}, pr);

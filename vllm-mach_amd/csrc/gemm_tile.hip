@@ -92,6 +92,7 @@ hipError_t launch_wide_tiles(int fmt, bool block, const WideConfig& c, const Gem
   if (fmt == kE4M3) return launch_tiles_fmt<kE4M3, false>(c, p, g, grid, s);
   if (fmt == kE2M3) return launch_tiles_fmt<kE2M3, false>(c, p, g, grid, s);
   if (fmt == kE3M2) return launch_tiles_fmt<kE3M2, false>(c, p, g, grid, s);
+  if (fmt == kE2M1) return launch_tiles_fmt<kE2M1, false>(c, p, g, grid, s);
   return hipErrorInvalidValue;
 }
 

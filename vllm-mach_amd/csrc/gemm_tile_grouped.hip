@@ -38,7 +38,11 @@ struct WideKernel<FMT, MT, NT, false, true, 1> {
     int pre[EPT + 1], row[EPT + 1];
     pre[0] = 0;
 #pragma unroll
-    for (int j = 0; j <= EPT; ++j) row[j] = (int)p.expert_offsets[e0 + j < E ? e0 + j : E];  // none past E
+    for (int j = 0; j <= EPT; ++j) {
+      const int64_t off = p.expert_offsets[e0 + j < E ? e0 + j : E];  // none past E
+      row[j] = (int)off;
+      if (FMT == kE2M1) row[j] = off < 0 ? 0 : off < p.M ? (int)off : (int)p.M;
+    }
 #pragma unroll
     for (int j = 0; j < EPT; ++j) pre[j + 1] = pre[j] + (row[j + 1] - row[j] + BM - 1) / BM;
     int sum = pre[EPT];
@@ -69,7 +73,9 @@ struct WideKernel<FMT, MT, NT, false, true, 1> {
     // activation row of thread t's row of the tile (past the expert's last: that one)
     auto gather = [&](const int4& x) -> int {
       const int r = x.y + t < x.z ? x.y + t : x.z - 1;
-      return t >= BM ? 0 : p.row_index ? p.row_index[r] / p.row_div : r;
+      const int at = t >= BM ? 0 : p.row_index ? p.row_index[r] / p.row_div : r;
+      if (FMT == kE2M1) return at < 0 ? 0 : at < (int)p.a_rows ? at : (int)p.a_rows - 1;
+      return at;
     };
     auto tile_of = [&](int slot) -> int4 {
       const int4 x = sh_tile[slot];
@@ -130,6 +136,7 @@ hipError_t launch_wide_grouped(int fmt, const WideConfig& c, const GemmParams& p
   if (fmt == kE4M3) return launch_grouped_fmt<kE4M3>(c, p, g, grid, s);
   if (fmt == kE2M3) return launch_grouped_fmt<kE2M3>(c, p, g, grid, s);
   if (fmt == kE3M2) return launch_grouped_fmt<kE3M2>(c, p, g, grid, s);
+  if (fmt == kE2M1) return launch_grouped_fmt<kE2M1>(c, p, g, grid, s);
   return hipErrorInvalidValue;
 }
 
