@@ -91,6 +91,49 @@ int mxl_mxfp4_gemm(const void* a, const void* sa, int64_t M, const void* w_tiled
                    int64_t K, const void* bias, void* out, int64_t ldc, void* workspace, int64_t workspace_bytes,
                    void* stream);
 
+/* mxl_quantize_mxfp4 then mxl_mxfp4_gemm in one launch: bf16 x [M, K] (row stride ldx, 16-byte
+ * aligned) of few rows, quantized inside the product (the same bits).  Shapes:
+ * mxl_mxfp4_quant_gemm_supported (up to 16 rows, fewer of a long K or a wide N), else
+ * MXL_EUNSUPPORTED. */
+int mxl_mxfp4_quant_gemm_supported(int64_t M, int64_t N, int64_t K);
+int mxl_mxfp4_quant_gemm(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, const void* w_tiled,
+                         const void* sw_tiled, int64_t N, const void* bias, void* out, int64_t ldc, void* stream);
+
+/* An expert layer's first half in one launch, for few rows an expert: quantized rows of
+ * bf16 x [a_rows, K] (gathered as mxl_mxfp4_grouped_gemm does), the gate/up product with
+ * W13[e] [2 I, K], and mxl_swiglu_mxfp4 of its rounded result: codes [routed_rows, I/2] and
+ * scales [routed_rows, I/32] of the routed rows.  Shapes: mxl_mxfp4_grouped_swiglu_supported
+ * (fewer than 8 rows an expert, I % 32 == 0), else MXL_EUNSUPPORTED. */
+int mxl_mxfp4_grouped_swiglu_supported(int64_t routed_rows, int64_t num_experts, int64_t I, int64_t K);
+int mxl_mxfp4_grouped_swiglu(const void* x, int64_t a_rows, int64_t ldx, const int32_t* row_index, int row_div,
+                             const int64_t* expert_offsets, int64_t num_experts, int64_t routed_rows,
+                             const void* w_tiled, const void* sw_tiled, int64_t I, int64_t K, int rule, void* codes,
+                             void* scales, void* stream);
+
+/* An MXFP4 linear layer in one call: bf16 x [M, K] (row stride ldx) quantized, or with
+ * swiglu gate/up rows [M, 2K] (ldx = 2 K) through mxl_swiglu_mxfp4, then the product --
+ * one launch where mxl_mxfp4_quant_gemm runs, else two and the join of a K split.  The
+ * workspace, 256-byte aligned, holds mxl_mxfp4_linear_workspace_bytes. */
+int64_t mxl_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int swiglu);
+int mxl_mxfp4_linear(const void* x, int64_t M, int64_t K, int64_t ldx, int swiglu, int rule, const void* w_tiled,
+                     const void* sw_tiled, int64_t N, const void* bias, void* out, int64_t ldc, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* A layer of MXFP4 experts in one call: routes sorted by mxl_moe_route from topk_ids i32
+ * [T, topk] (or given: sorted_routes, expert_offsets, inverse), the gate/up product of the
+ * quantized rows of x [T, H] (row stride ldx) with w13 [E][2I, H], SwiGLU -> MXFP4, the
+ * product with w2 [E][H, I], and the combine with fp32 topk_weights [T, topk] into out bf16
+ * [T, H].  fuse: mxl_mxfp4_grouped_swiglu where it runs (four launches from the ids).
+ * H, I multiples of 128; the workspace, 256-byte aligned, holds
+ * mxl_mxfp4_experts_workspace_bytes (sorted: the routes are given). */
+int64_t mxl_mxfp4_experts_workspace_bytes(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int sorted,
+                                          int fuse);
+int mxl_mxfp4_experts(const void* x, int64_t T, int64_t ldx, const int32_t* topk_ids, const float* topk_weights,
+                      int64_t topk, const int32_t* sorted_routes, const int64_t* expert_offsets, const int32_t* inverse,
+                      int64_t E, int64_t H, int64_t I, const void* w13, const void* sw13, const void* w2,
+                      const void* sw2, int rule, int fuse, void* out, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
 /* mxl_grouped_gemm of MXFP4 activations and experts: routed row p of expert e
  * (expert_offsets[e] <= p < expert_offsets[e+1]) is A[row_index[p] / row_div] . W[e]^T, or
  * A[p] . W[e]^T where row_index is null; rows past expert_offsets[E] stay unwritten.

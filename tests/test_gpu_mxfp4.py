@@ -201,6 +201,51 @@ def test_gemm_unaligned_and_strided_inputs(pkg, dev):
     assert pkg.ops.mxfp4_gemm(a[:0].to(dev), sa[:0].to(dev), w, sw, n, k).shape == (0, n)
 
 
+@pytest.mark.parametrize("rule", RULES)
+@pytest.mark.parametrize("m", [1, 2, 7, 16, 17, 40, 130])
+@pytest.mark.parametrize("n,k", [(16, 128), (72, 896), (4608, 2048), (1030, 5120), (2560, 9216), (104, 16384)])
+def test_linear_is_quantizer_and_product(pkg, dev, m, n, k, rule):
+    """The layer in one call (one launch for few rows) against its parts.  Sums may be joined in another order; of
+    their roundings at most one in 2^7 falls to its other side, by a step."""
+    g = torch.Generator().manual_seed(m + n + k)
+    (w, sw), wv = _weight(pkg, g, n, k)
+    x, bias = _x(g, m, k).to(dev), torch.randn(n, generator=g).bfloat16().to(dev)
+    a, sa = pkg.ops.quantize_mxfp4(x, rule)
+    for b in (None, bias):
+        y, z = pkg.ops.mxfp4_linear(x, w, sw, n, rule, b), pkg.ops.mxfp4_gemm(a, sa, w, sw, n, k, b)
+        ref.check_product(y, ref.dequantize(a, sa), wv, b)
+        assert float((y != z).double().mean()) <= 2.0 ** -7
+    assert torch.equal(torch.ops.mach_amd.mxfp4_linear(x, w, sw, n, rule, bias), y)
+
+
+def test_operators_under_transforms(pkg, dev):
+    """The short way of eager calls is not taken where something looks on: gradients, tracing, compile-time fakes."""
+    g = torch.Generator().manual_seed(1)
+    (w, sw), _ = _weight(pkg, g, 64, 256)
+    x = _x(g, 5, 256).to(dev)
+    y = pkg.ops.mxfp4_linear(x, w, sw, 64)
+    lin = lambda v: pkg.ops.mxfp4_linear(v, w, sw, 64)  # noqa: E731
+    assert torch.equal(lin(x.clone().requires_grad_()).detach(), y)
+    with torch.no_grad():
+        assert torch.equal(lin(x.clone().requires_grad_()), y)
+    z = _x(g, 5, 256).to(dev)
+    traced = torch.jit.trace(lin, (x,), check_trace=False)
+    assert torch.equal(traced(z), lin(z))
+    from torch.fx.experimental.proxy_tensor import make_fx
+    assert torch.equal(make_fx(lin)(x)(z), lin(z))
+    with torch.inference_mode():
+        assert torch.equal(lin(x), y)
+
+
+@pytest.mark.parametrize("m,n,k", [(16, 40, 20480), (1, 24, 21504), (12, 1000, 17408)])
+def test_gemm_past_lds(pkg, dev, m, n, k):
+    """Few rows of a K that does not fit in LDS."""
+    g = torch.Generator().manual_seed(m + n + k)
+    (w, sw), wv = _weight(pkg, g, n, k)
+    a, sa = ref.random_operand(g, m, k)
+    ref.check_product(pkg.ops.mxfp4_gemm(a.to(dev), sa.to(dev), w, sw, n, k), ref.dequantize(a, sa), wv)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 2048, 2048), (40, 1024, 2560), (600, 512, 1024)])
 def test_gemm_is_deterministic_and_row_independent(pkg, dev, m, n, k):
     g = torch.Generator().manual_seed(11)
@@ -305,6 +350,39 @@ def test_grouped_gemm(pkg, dev, t, e, topk, only, n, k):
     assert torch.equal(y, pkg.ops.mxfp4_grouped_gemm(b, sb, None, 1, offsets, R, w, sw, n, k))
 
 
+def test_grouped_gemm_of_many_experts(pkg, dev):
+    """More than 1024 experts with many rows each, and as many with few."""
+    g = torch.Generator().manual_seed(12)
+    e, n, k = 1030, 24, 128
+    wc, ws = ref.random_operand(g, e * n, k)
+    wv = ref.dequantize(wc, ws).view(e, n, k)
+    w, sw = pkg.ops.pack_weight(wc.view(e, n, -1).to(dev), ws.view(e, n, -1).to(dev), pkg.ops.E2M1)
+    for t in (17 * e, 40):
+        ids = torch.randint(0, e, (t, 1), generator=g).int()
+        a, sa = ref.random_operand(g, t, k)
+        routes, offsets, _ = pkg.ops.moe_route(ids.to(dev), e)
+        y = pkg.ops.mxfp4_grouped_gemm(a.to(dev), sa.to(dev), routes, 1, offsets, t, w, sw, n, k)
+        rows, of = ref.dequantize(a, sa)[routes.cpu().long()], ids[routes.cpu().long(), 0].long()
+        want = torch.cat([(r.unsqueeze(1) @ wv[o].transpose(1, 2)).squeeze(1) for r, o in zip(rows.split(4096), of.split(4096))])
+        assert float((y.cpu().double() - want).abs().max() / want.abs().max()) <= 2.0 ** -8
+        assert float((y.cpu().double() - want).norm() / want.norm()) <= 2.0 ** -8
+
+
+def test_gemm_past_four_gib(pkg, dev):
+    """Activation codes past 4 GiB: rows on both sides of the borders and the last ones."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB")
+    n, k = 8, 128
+    m = (1 << 32) // (k // 2) + 1000
+    g = torch.Generator().manual_seed(13)
+    (w, sw), wv = _weight(pkg, g, n, k)
+    a = torch.randint(0, 256, (m, k // 2), dtype=torch.uint8, device=dev)
+    sa = torch.randint(124, 131, (m, k // 32), dtype=torch.uint8, device=dev)
+    y = pkg.ops.mxfp4_gemm(a, sa, w, sw, n, k)
+    at = torch.cat([torch.arange(0, 300), torch.arange(m // 2, m // 2 + 300), torch.arange(m - 1600, m)]).to(dev)
+    ref.check_product(y[at], ref.dequantize(a[at], sa[at]), wv)
+
+
 def test_grouped_gemm_leaves_dropped_rows(pkg, dev):
     """Routes to no expert end behind the last offset: their output rows are not written."""
     g = torch.Generator().manual_seed(3)
@@ -325,6 +403,31 @@ def test_grouped_gemm_leaves_dropped_rows(pkg, dev):
     assert bool((out[kept:] == 7).all()) and not bool((out[:kept] == 7).all(1).any())
 
 
+@pytest.mark.parametrize("rule", RULES)
+@pytest.mark.parametrize("t,e,topk,only", [(1, 8, 2, None), (2, 40, 3, None), (17, 16, 4, None), (17, 5, 2, [0, 4]),
+                                           (32, 33, 8, None), (60, 70, 2, [3, 69])])
+@pytest.mark.parametrize("i,k", [(128, 384), (160, 1024), (32, 5120)])
+def test_grouped_swiglu_is_the_separate_launches(pkg, dev, t, e, topk, only, i, k, rule):
+    """Quantization, gate/up product and SwiGLU producer in one launch.  The two ways may add a K sum's parts in
+    another order, so a bf16 gate or up next to a border may fall to its other side and move a code: at most one in
+    2^9 codes and scales; decoded, both stand within that of each other."""
+    assert pkg.ops.mxfp4_grouped_swiglu_supported(t * topk, e, i, k)
+    g = torch.Generator().manual_seed(t + e + i)
+    wc, ws = ref.random_operand(g, e * 2 * i, k)
+    w, sw = pkg.ops.pack_weight(wc.view(e, 2 * i, -1).to(dev), (ws - 6).view(e, 2 * i, -1).to(dev), pkg.ops.E2M1)
+    x = _x(g, t, k).to(dev)
+    routes, offsets, _ = pkg.ops.moe_route(_routes(g, t, e, topk, only).to(dev), e)
+    R = t * topk
+    codes, scales = pkg.ops.mxfp4_grouped_swiglu(x, routes, topk, offsets, R, w, sw, i, rule)
+    a, sa = pkg.ops.quantize_mxfp4(x, rule)
+    gate_up = pkg.ops.mxfp4_grouped_gemm(a, sa, routes, topk, offsets, R, w, sw, 2 * i, k)
+    want = pkg.ops.swiglu_mxfp4(gate_up, rule)
+    for u, v in zip((codes, scales), want):
+        assert u.shape == v.shape and float((u != v).double().mean()) <= 2.0 ** -9
+    u, v = ref.dequantize(codes, scales), ref.dequantize(*want)
+    assert float((u - v).norm() / v.norm()) <= 2.0 ** -4
+
+
 def _exact_layer(x, p, ids, w1, w2):
     a, out = ref.dequantize(*ref.quantize(x)), torch.zeros(x.shape, dtype=torch.float64)
     for e in range(w1.shape[0]):
@@ -336,13 +439,16 @@ def _exact_layer(x, p, ids, w1, w2):
     return out
 
 
-@pytest.mark.parametrize("t,e,topk,h,i", [(1, 8, 2, 256, 128), (20, 16, 4, 384, 256), (200, 6, 2, 512, 384)])
-def test_experts_layer(pkg, dev, t, e, topk, h, i):
+@pytest.mark.parametrize("fuse", [True, False])
+@pytest.mark.parametrize("t,e,topk,h,i", [(1, 8, 2, 256, 128), (20, 16, 4, 384, 256), (200, 6, 2, 512, 384),
+                                          (2, 300, 8, 256, 128), (600, 16, 4, 1152, 640)])
+def test_experts_layer(pkg, dev, t, e, topk, h, i, fuse):
     """The layer against the chain in 64 bits.  Its outputs are sums of bf16 values (half a step each, 2^-8) rounded
     once more, and where a sum in fp32 rounds to another bf16 gate or up value the activation's code can move by a
     step of E2M1, a third of its value: one in 2^10 of them at most, 3 / 2^5 / 2^5 of the norm."""
     g = torch.Generator().manual_seed(t)
     experts, w1, w2, v1, v2 = _experts(pkg, g, e, h, i)
+    experts.fuse = fuse
     x, ids = _x(g, t, h), _routes(g, t, e, topk)
     p = torch.rand(t, topk, generator=g)
     got = experts(x.to(dev), w1, w2, p.to(dev), ids.to(dev)).cpu().double()

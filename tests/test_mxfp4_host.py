@@ -48,6 +48,24 @@ def test_tiled_sizes(c):
     ("mxl_mxfp4_grouped_gemm", (16, 16, 4, None, 0, 16, 2, 4, 16, 16, 16, 128, 16, None), "row_div"),
     ("mxl_mxfp4_grouped_gemm", (16, 16, 4, None, 1, 16, 2, -4, 16, 16, 16, 128, 16, None), "row counts"),
     ("mxl_mxfp4_grouped_gemm", (16, 16, 4, None, 1, 16, 2, 4, 16, 16, 16, 96, 16, None), "K % 128"),
+    ("mxl_mxfp4_quant_gemm", (16, 4, 256, 256, 1, 16, 16, 16, None, 16, 16, None), "unknown rule"),
+    ("mxl_mxfp4_quant_gemm", (16, 4, 256, 248, 0, 16, 16, 16, None, 16, 16, None), "ldx"),
+    ("mxl_mxfp4_quant_gemm", (16, 4, 256, 256, 0, 16, 16, 16, None, 16, 8, None), "ldc"),
+    ("mxl_mxfp4_quant_gemm", (16, 40, 256, 256, 0, 16, 16, 16, None, 16, 16, None), "one launch"),
+    ("mxl_mxfp4_quant_gemm", (8, 4, 256, 256, 0, 16, 16, 16, None, 16, 16, None), "aligned"),
+    ("mxl_mxfp4_linear", (16, 40, 256, 256, 0, 0, 16, 16, 16, None, 16, 16, None, 0, None), "workspace"),
+    ("mxl_mxfp4_linear", (16, 40, 256, 512, 0, 0, 16, 16, 16, None, 17, 16, 256, 1 << 20, None), "misaligned"),
+    ("mxl_mxfp4_linear", (16, 40, 256, 256, 1, 0, 16, 16, 16, None, 16, 16, 256, 1 << 20, None), "2 K"),
+    ("mxl_mxfp4_linear", (16, 40, 1 << 23, 1 << 23, 0, 0, 16, 16, 16, None, 16, 16, 256, 1 << 20, None), "0 < K"),
+    ("mxl_mxfp4_gemm", (16, 16, 600, 16, 16, 16, 16384, None, 16, 16, None, 0, None), "workspace"),
+    ("mxl_mxfp4_experts", (16, 4, 256, None, 16, 2, None, None, None, 4, 256, 128, 16, 16, 16, 16, 0, 1, 16, 256, 1 << 30, None), "ids"),
+    ("mxl_mxfp4_experts", (16, 4, 256, 16, 16, 2, None, None, None, 4, 256, 100, 16, 16, 16, 16, 0, 1, 16, 256, 1 << 30, None), "by 128"),
+    ("mxl_mxfp4_experts", (16, 4, 256, 16, 16, 2, None, None, None, 4, 256, 128, 16, 16, 16, 16, 0, 1, 16, None, 0, None), "workspace"),
+    ("mxl_mxfp4_experts", (16, 4, 256, 16, 16, 0, None, None, None, 4, 256, 128, 16, 16, 16, 16, 0, 1, 16, 256, 1 << 30, None), "topk"),
+    ("mxl_mxfp4_grouped_swiglu", (16, 4, 256, None, 1, 16, 2, 4, 16, 16, 48, 256, 0, 16, 16, None), "I % 32"),
+    ("mxl_mxfp4_grouped_swiglu", (16, 4, 256, None, 1, 16, 2, 40, 16, 16, 64, 256, 0, 16, 16, None), "one launch"),
+    ("mxl_mxfp4_grouped_swiglu", (16, 4, 256, None, 1, 16, 2, 4, 16, 16, 64, 256, 0, 18, 16, None), "aligned"),
+    ("mxl_mxfp4_grouped_swiglu", (16, 0, 256, None, 1, 16, 2, 4, 16, 16, 64, 256, 0, 16, 16, None), "no activation"),
     ("mxl_mx_gemm", (16, 16, 1, 16, 16, 16, 128, 4, None, 16, 16, None, 0, None), "unknown weight format"),
     ("mxl_moe_router_grouped", (16, 0, None, 4, 1025, 8, 0, 1, 1, 1, 1.0, 16, 16, 16, 16, 16, 16, 1 << 20, None), "E <="),
     ("mxl_moe_router_grouped", (16, 0, None, 4, 64, 8, 0, 5, 1, 1, 1.0, 16, 16, 16, 16, 16, 16, 1 << 20, None), "groups"),
@@ -95,6 +113,8 @@ def test_fakes_keep_shapes(pkg):
         y = torch.ops.mach_amd.mxfp4_gemm(a, sa, w, sw, 24, 256)
         assert y.shape == (5, 24) and y.dtype == torch.bfloat16
         off = torch.empty(3, dtype=torch.int64)
+        assert torch.ops.mach_amd.mxfp4_linear(x, w, sw, 24).shape == (5, 24)
+        assert pkg.ops.mxfp4_linear(x, w, sw, 24, 0, None, True).shape == (5, 24)
         assert torch.ops.mach_amd.mxfp4_grouped_gemm(a, sa, None, 1, off, 5, w, sw, 24, 256).shape == (5, 24)
         out = torch.ops.mach_amd.moe_router_grouped(torch.empty(5, 16), None, 4)
         assert [tuple(t.shape) for t in out] == [(5, 4), (5, 4), (20,), (17,), (20,)]

@@ -34,6 +34,15 @@ SIGNATURES = {
     "mxl_swiglu_mxfp4": (_I, [_P, _I64, _I64, _I, _P, _P, _P]),
     "mxl_mxfp4_gemm_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "mxl_mxfp4_gemm": (_I, [_P, _P, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _P]),
+    "mxl_mxfp4_quant_gemm_supported": (_I, [_I64, _I64, _I64]),
+    "mxl_mxfp4_quant_gemm": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _I64, _P, _P, _I64, _P]),
+    "mxl_mxfp4_grouped_swiglu_supported": (_I, [_I64, _I64, _I64, _I64]),
+    "mxl_mxfp4_grouped_swiglu": (_I, [_P, _I64, _I64, _P, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _I, _P, _P, _P]),
+    "mxl_mxfp4_linear_workspace_bytes": (_I64, [_I64, _I64, _I64, _I]),
+    "mxl_mxfp4_linear": (_I, [_P, _I64, _I64, _I64, _I, _I, _P, _P, _I64, _P, _P, _I64, _P, _I64, _P]),
+    "mxl_mxfp4_experts_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I, _I]),
+    "mxl_mxfp4_experts": (_I, [_P, _I64, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I, _I, _P, _P,
+                               _I64, _P]),
     "mxl_mxfp4_grouped_gemm": (_I, [_P, _P, _I64, _P, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P]),
     "mxl_swizzled_scale_bytes": (_I64, [_I64, _I64]),
     "mxl_swizzle_scales": (_I, [_P, _I64, _I64, _P, _P]),

@@ -13,14 +13,15 @@
 
 namespace mxl {
 
-// The E8M0 code of a block from the bf16 magnitude bits of its amax (a NaN's above infinity's).
-// bf16 keeps seven mantissa bits: +32 (a quarter) carries into the exponent from 1.75 on.
-template <int RULE>
-__device__ __forceinline__ uint32_t scale_e2m1(uint32_t amax) {
-  static_assert(RULE == kFloorCarry175 || RULE == kFloorOcp, "MXFP4 rules");
-  const uint32_t e = (amax + (RULE == kFloorCarry175 ? 32u : 0u)) >> 7;
+// The E8M0 code of a block from the bf16 magnitude bits of its amax (a NaN's above infinity's).  carry: 32
+// (floor_carry175) or 0 (floor): bf16 keeps seven mantissa bits, so +32, a quarter, carries into the exponent from
+// 1.75 on.
+__device__ __forceinline__ uint32_t scale_e2m1(uint32_t amax, uint32_t carry) {
+  const uint32_t e = (amax + carry) >> 7;
   return amax >= 0x7F80u ? 255u : e > 2u ? e - 2u : 0u;
 }
+inline bool fp4_rule(int rule) { return rule == kFloorCarry175 || rule == kFloorOcp; }
+inline uint32_t fp4_carry(int rule) { return rule == kFloorCarry175 ? 32u : 0u; }
 
 // Eight raw bf16 values (four pairs) -> eight E2M1 codes divided by 2^(s - 127), one dword:
 // v_cvt_scalef32_pk_fp4_bf16 divides by the power of two that its scale operand's exponent field
@@ -38,12 +39,11 @@ __device__ __forceinline__ uint32_t codes_e2m1(const uint32_t* d, uint32_t s) {
 
 // A block of 32 held by four consecutive lanes, eight values each: its E8M0 code (in every lane) and
 // the lane's codes.
-template <int RULE>
-__device__ __forceinline__ uint32_t quant_e2m1_x4(const uint32_t* d, uint32_t& codes) {
+__device__ __forceinline__ uint32_t quant_e2m1_x4(const uint32_t* d, uint32_t carry, uint32_t& codes) {
   uint32_t amax = amax_bf16_bits<4, false>(d);
   amax = __builtin_elementwise_max(amax, (uint32_t)__shfl_xor((int)amax, 1, 4));
   amax = __builtin_elementwise_max(amax, (uint32_t)__shfl_xor((int)amax, 2, 4));
-  const uint32_t s = scale_e2m1<RULE>(amax);
+  const uint32_t s = scale_e2m1(amax, carry);
   codes = codes_e2m1(d, s);
   return s;
 }

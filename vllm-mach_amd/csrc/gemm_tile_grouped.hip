@@ -127,7 +127,8 @@ static hipError_t launch_grouped_fmt(const WideConfig& c, const GemmParams& p, c
                                      hipStream_t s) {
   if (c.NT != 2) return hipErrorInvalidValue;
   if (c.MT == 8) return launch_grouped_tile<FMT, 8, 2>(p, g, grid, s);
-  if (c.MT == 4) return launch_grouped_tile<FMT, 4, 2>(p, g, grid, s);
+  if constexpr (FMT != kE2M1)
+    if (c.MT == 4) return launch_grouped_tile<FMT, 4, 2>(p, g, grid, s);
   return hipErrorInvalidValue;
 }
 

@@ -10,10 +10,9 @@
 
 namespace mxl {
 
-template <int RULE>
 __global__ __launch_bounds__(256) void quant_mxfp4_kernel(const uint16_t* __restrict__ x, int64_t ldx,
                                                           uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                          uint32_t blocks_per_row, uint32_t blocks) {
+                                                          uint32_t blocks_per_row, uint32_t blocks, uint32_t carry) {
   // (32-bit lane indices: the host bounds the block count; lanes past the end shadow the last block)
   const uint32_t t = blockIdx.x * blockDim.x + threadIdx.x, sub = t & 3;
   const bool live = t / 4 < blocks;
@@ -21,17 +20,16 @@ __global__ __launch_bounds__(256) void quant_mxfp4_kernel(const uint16_t* __rest
   const uint4 v = *reinterpret_cast<const uint4*>(x + (int64_t)row * ldx + blk * 32 + sub * 8);
   const uint32_t d[4] = {v.x, v.y, v.z, v.w};
   uint32_t c;
-  const uint32_t s = quant_e2m1_x4<RULE>(d, c);
+  const uint32_t s = quant_e2m1_x4(d, carry, c);
   if (!live) return;
   reinterpret_cast<uint32_t*>(codes)[(int64_t)id * 4 + sub] = c;
   if (sub == 0) scales[id] = (uint8_t)s;
 }
 
 // v = bf16(bf16(silu(g)) u) of the MXFP8 producer (rules 0 and 1 there), then the quantization.
-template <int RULE>
 __global__ __launch_bounds__(256) void swiglu_mxfp4_kernel(const uint16_t* __restrict__ gate_up,
                                                            uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                           uint32_t blocks_per_row, uint32_t blocks) {
+                                                           uint32_t blocks_per_row, uint32_t blocks, uint32_t carry) {
   const uint32_t t = blockIdx.x * blockDim.x + threadIdx.x, sub = t & 3;
   const bool live = t / 4 < blocks;
   const uint32_t id = live ? t / 4 : blocks - 1, row = id / blocks_per_row, blk = id - row * blocks_per_row;
@@ -44,7 +42,7 @@ __global__ __launch_bounds__(256) void swiglu_mxfp4_kernel(const uint16_t* __res
 #pragma unroll
   for (int i = 0; i < 4; ++i) d[i] = cvt_pk_bf16(v[2 * i], v[2 * i + 1]);  // (bf16 values already)
   uint32_t c;
-  const uint32_t s = quant_e2m1_x4<RULE>(d, c);
+  const uint32_t s = quant_e2m1_x4(d, carry, c);
   if (!live) return;
   reinterpret_cast<uint32_t*>(codes)[(int64_t)id * 4 + sub] = c;
   if (sub == 0) scales[id] = (uint8_t)s;
@@ -57,7 +55,7 @@ using namespace mxl;
 static int check_quant(const char* who, const void* in, int64_t M, int64_t K, int rule, const void* codes) {
   MXL_CHECK_ARG(M >= 0 && K > 0 && K % 32 == 0, "%s: need M >= 0, K > 0, K %% 32 == 0 (M=%lld K=%lld)", who,
                 (long long)M, (long long)K);
-  MXL_CHECK_ARG(rule == kFloorCarry175 || rule == kFloorOcp, "%s: unknown rule %d", who, rule);
+  MXL_CHECK_ARG(fp4_rule(rule), "%s: unknown rule %d", who, rule);
   MXL_CHECK_ARG(((uintptr_t)in & 15) == 0 && ((uintptr_t)codes & 3) == 0,
                 "%s: the input must be 16-byte aligned, the codes 4-byte aligned", who);
   // lanes are indexed in 32 bits
@@ -76,10 +74,8 @@ extern "C" int mxl_quantize_mxfp4(const void* x, int64_t M, int64_t K, int64_t l
   const dim3 grid((unsigned)((blocks * 4 + 255) / 256));
   hipStream_t s = (hipStream_t)stream;
   const uint32_t per = (uint32_t)(K / 32), n = (uint32_t)blocks;
-  if (rule == kFloorCarry175)
-    quant_mxfp4_kernel<kFloorCarry175><<<grid, 256, 0, s>>>((const uint16_t*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, per, n);
-  else
-    quant_mxfp4_kernel<kFloorOcp><<<grid, 256, 0, s>>>((const uint16_t*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, per, n);
+  quant_mxfp4_kernel<<<grid, 256, 0, s>>>((const uint16_t*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, per, n,
+                                          fp4_carry(rule));
   MXL_CHECK_LAUNCH("mxl_quantize_mxfp4");
   return MXL_OK;
 }
@@ -93,10 +89,8 @@ extern "C" int mxl_swiglu_mxfp4(const void* gate_up, int64_t M, int64_t K, int r
   const dim3 grid((unsigned)((blocks * 4 + 255) / 256));
   hipStream_t s = (hipStream_t)stream;
   const uint32_t per = (uint32_t)(K / 32), n = (uint32_t)blocks;
-  if (rule == kFloorCarry175)
-    swiglu_mxfp4_kernel<kFloorCarry175><<<grid, 256, 0, s>>>((const uint16_t*)gate_up, (uint8_t*)codes, (uint8_t*)scales, per, n);
-  else
-    swiglu_mxfp4_kernel<kFloorOcp><<<grid, 256, 0, s>>>((const uint16_t*)gate_up, (uint8_t*)codes, (uint8_t*)scales, per, n);
+  swiglu_mxfp4_kernel<<<grid, 256, 0, s>>>((const uint16_t*)gate_up, (uint8_t*)codes, (uint8_t*)scales, per, n,
+                                           fp4_carry(rule));
   MXL_CHECK_LAUNCH("mxl_swiglu_mxfp4");
   return MXL_OK;
 }

@@ -324,7 +324,7 @@ class Mxfp4LinearKernel(_Kernel):
         if x.numel() == 0:
             return x.new_empty((*x.shape[:-1], n))
         inner = _epilogue_bias(bias, x, n)
-        y = ops.mxfp4_gemm_from_float(_flatten(x, k), layer.weight, layer.weight_scale, n, self.act_rule, inner)
+        y = ops.mxfp4_linear(_flatten(x, k), layer.weight, layer.weight_scale, n, self.act_rule, inner)
         y = y.reshape(*x.shape[:-1], n)
         return y if bias is inner else y + bias
 
@@ -425,7 +425,7 @@ def swiglu_mxfp4_down(gate_up: torch.Tensor, down: torch.nn.Module) -> torch.Ten
     n, k = down.mxl_shape
     if gate_up.shape[-1] != 2 * k:
         raise ValueError("gate_up width must be twice the down projection's K")
-    y = ops.swiglu_mxfp4_down(_flatten(gate_up, 2 * k), down.weight, down.weight_scale, n)
+    y = ops.mxfp4_linear(_flatten(gate_up, 2 * k), down.weight, down.weight_scale, n, ops.FLOOR_CARRY175, None, True)
     return y.reshape(*gate_up.shape[:-1], n)
 
 

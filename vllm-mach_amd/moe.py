@@ -52,8 +52,8 @@ class GroupedRouting:
     def route(self, router_logits: torch.Tensor, top_k: int, renormalize: bool):
         if self.scoring not in _SCORING:
             raise ValueError(f"unknown scoring {self.scoring!r} ({' or '.join(_SCORING)})")
-        return torch.ops.mach_amd.moe_router_grouped(router_logits, self.bias, top_k, _SCORING[self.scoring],
-                                                     self.num_groups, self.topk_groups, renormalize, self.factor)
+        return ops.moe_router_grouped(router_logits, self.bias, top_k, _SCORING[self.scoring], self.num_groups,
+                                      self.topk_groups, renormalize, self.factor)
 
 
 _SCORING = {"softmax": ops.SOFTMAX, "sigmoid": ops.SIGMOID}
@@ -99,11 +99,13 @@ class _Experts:
         if expert_map is None and global_num_experts != E:
             raise ValueError("global and local expert counts require an expert_map")
         ids = topk_ids if expert_map is None else expert_map[topk_ids.long()]
-        topk = ids.shape[1]
         if T == 0:
             return
-        sorted_routes, offsets, inverse = torch.ops.mach_amd.moe_route(ids, E)
-        self._experts(output, hidden_states, w1, w2, topk_weights, topk, sorted_routes, offsets, inverse)
+        self._experts_of_ids(output, hidden_states, w1, w2, topk_weights, ids)
+
+    def _experts_of_ids(self, output, hidden_states, w1, w2, topk_weights, ids):
+        sorted_routes, offsets, inverse = torch.ops.mach_amd.moe_route(ids, self.shapes[0])
+        self._experts(output, hidden_states, w1, w2, topk_weights, ids.shape[1], sorted_routes, offsets, inverse)
 
     def apply_router(self, output: torch.Tensor, hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor,
                      router_logits: torch.Tensor, top_k: int, renormalize: bool = True,
@@ -220,8 +222,8 @@ class Mxfp4Experts(_Experts):
     """Routed experts over packed MXFP4 weights, activations quantized to MXFP4 (W4A4).
 
     Checkpoint layout (Quark OCP-MX): w13 u8 [E, 2I, H/2] + E8M0 [E, 2I, H/32] (gate rows [0, I), up
-    rows [I, 2I)); w2 u8 [E, H, I/2] + E8M0 [E, H, I/32].  The hidden states are quantized once, the
-    routed gate/up rows inside the SwiGLU producer.
+    rows [I, 2I)); w2 u8 [E, H, I/2] + E8M0 [E, H, I/32].  With few rows an expert the layer is four
+    launches: route, w13 with the quantization ahead of it and the SwiGLU producer behind it, w2, combine.
     """
 
     name = "MXFP4"
@@ -231,6 +233,7 @@ class Mxfp4Experts(_Experts):
         if rule not in (ops.FLOOR_CARRY175, ops.FLOOR_OCP):
             raise ValueError(f"unknown MXFP4 scale rule {rule}")
         self.rule = rule
+        self.fuse = True  # the first half in one launch where it runs (False: separate launches)
         self.w1_scale: Optional[torch.Tensor] = None
         self.w2_scale: Optional[torch.Tensor] = None
 
@@ -250,14 +253,15 @@ class Mxfp4Experts(_Experts):
         return w1_t, w2_t
 
     def _experts(self, output, hidden_states, w1, w2, topk_weights, topk, sorted_routes, offsets, inverse):
-        _, H, I = self.shapes
-        routes = hidden_states.shape[0] * topk
-        a, sa = torch.ops.mach_amd.quantize_mxfp4(hidden_states, self.rule)
-        gate_up = torch.ops.mach_amd.mxfp4_grouped_gemm(a, sa, sorted_routes, topk, offsets, routes, w1, self.w1_scale,
-                                                        2 * I, H)
-        a2, sa2 = torch.ops.mach_amd.swiglu_mxfp4(gate_up, self.rule)
-        y = torch.ops.mach_amd.mxfp4_grouped_gemm(a2, sa2, None, 1, offsets, routes, w2, self.w2_scale, H, I)
-        torch.ops.mach_amd.moe_reduce(output, y, topk_weights, inverse)
+        self._layer(output, hidden_states, w1, w2, topk_weights, None, sorted_routes, offsets, inverse)
+
+    def _experts_of_ids(self, output, hidden_states, w1, w2, topk_weights, ids):
+        self._layer(output, hidden_states, w1, w2, topk_weights, ids)
+
+    def _layer(self, output, x, w1, w2, weights, ids, routes=None, offsets=None, inverse=None):
+        E, _, I = self.shapes
+        ops.mxfp4_experts(output, x, ids, weights, routes, offsets, inverse, w1, self.w1_scale, w2, self.w2_scale, E, I,
+                          self.rule, self.fuse)
 
 
 _MOE_PARAMS = ("w13_weight", "w13_weight_scale", "w2_weight", "w2_weight_scale")

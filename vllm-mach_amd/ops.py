@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import threading
 from typing import Optional
 
@@ -743,24 +744,67 @@ def block_fp8_from_float(x: torch.Tensor, w: torch.Tensor, sb: torch.Tensor, n: 
 
 
 # ------------------------------------------------------------------ MXFP4
+#
+# Eager calls of these operators skip torch's dispatcher, whose wrappers take 6 us a call (a layer of one call 36
+# -> 12 us with its two launches): ``ops.<name>`` runs the operator's function itself where nothing looks on --
+# plain tensors without gradients, no tracing, no transform, no dispatch mode -- and ``torch.ops.mach_amd.<name>``
+# otherwise.  Scratch memory is a tensor of the call, so graphs and streams never share it.
+
+def _plain(args) -> bool:
+    """Whether nothing but the operator itself has to see the call."""
+    if (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._get_tracing_state() is not None
+            or torch._C._functorch.peek_interpreter_stack() is not None or torch._C._is_torch_function_mode_enabled()):
+        return False
+    grad = torch.is_grad_enabled()
+    for t in args:
+        if isinstance(t, torch.Tensor) and (type(t) not in (torch.Tensor, torch.nn.Parameter) or (grad and t.requires_grad)
+                                            or not t.is_cuda):
+            return False
+    return not torch.autograd.forward_ad._current_level >= 0
+
+
+def _operator(name: str, mutates_args=()):
+    """``torch.library.custom_op`` whose Python name takes the short way above."""
+    def wrap(fn):
+        op = torch.library.custom_op(f"mach_amd::{name}", mutates_args=mutates_args)(fn)
+
+        @functools.wraps(fn)
+        def call_op(*args, **kwargs):
+            return fn(*args, **kwargs) if _plain(args) and _plain(kwargs.values()) else op(*args, **kwargs)
+
+        call_op.register_fake = op.register_fake
+        return call_op
+    return wrap
+
 
 def _on(device: torch.device):
     """The device of a call's tensors as the current one (a no-op where it is)."""
-    return contextlib.nullcontext() if _device_index(device) == torch.cuda.current_device() else torch.cuda.device(device)
+    return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_NOTHING = contextlib.nullcontext()
 
 
 def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     _check_cuda(first, *others)
+    device = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
 
 
 def _rows16(x: torch.Tensor) -> torch.Tensor:
-    """x as rows of unit column stride that start on 16 bytes (a copy where they do not)."""
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < x.shape[1] or x.data_ptr() % 16:
+    """x as rows of unit column stride that start on 16 bytes (a copy where they do not, and of rows further apart
+    than the kernels' offsets reach)."""
+    m, k = x.shape
+    ld = x.stride(0) if m > 1 else k
+    if (x.stride(1) != 1 and k > 1) or ld % 8 or ld < k or x.data_ptr() % 16 or (m - 1) * ld + k >= 1 << 31:
         return torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
     return x
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
 def _aligned(t: torch.Tensor, nbytes: int) -> torch.Tensor:
@@ -770,7 +814,16 @@ def _aligned(t: torch.Tensor, nbytes: int) -> torch.Tensor:
     return t
 
 
-@torch.library.custom_op("mach_amd::quantize_mxfp4", mutates_args=())
+def _scratch(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _fp4_rule(what: str, rule: int) -> None:
+    if rule not in (FLOOR_CARRY175, FLOOR_OCP):
+        raise ValueError(f"{what}: unknown rule {rule}")
+
+
+@_operator("quantize_mxfp4")
 def quantize_mxfp4(x: torch.Tensor, rule: int = FLOOR_CARRY175) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16 [M, K] -> (packed E2M1 codes u8 [M, K/2], E8M0 scales u8 [M, K/32]), K % 32 == 0.
 
@@ -782,15 +835,14 @@ def quantize_mxfp4(x: torch.Tensor, rule: int = FLOOR_CARRY175) -> tuple[torch.T
     _check_cuda(x)
     if x.dtype != torch.bfloat16 or x.ndim != 2 or x.shape[1] == 0 or x.shape[1] % 32:
         raise ValueError("quantize_mxfp4 needs a 2-D bf16 tensor with K > 0 and K % 32 == 0")
-    if rule not in (FLOOR_CARRY175, FLOOR_OCP):
-        raise ValueError(f"quantize_mxfp4: unknown rule {rule}")
+    _fp4_rule("quantize_mxfp4", rule)
     x = _rows16(x)
     M, K = x.shape
     codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
     scales = torch.empty((M, K // 32), dtype=torch.uint8, device=x.device)
     if M:
         with _on(x.device):
-            call("mxl_quantize_mxfp4", ptr(x), M, K, x.stride(0), rule, ptr(codes), ptr(scales),
+            call("mxl_quantize_mxfp4", ptr(x), M, K, _row_stride(x), rule, ptr(codes), ptr(scales),
                  stream_handle(x.device))
     _count("quantize_mxfp4")
     return codes, scales
@@ -802,15 +854,13 @@ def _(x, rule=FLOOR_CARRY175):
             x.new_empty((x.shape[0], x.shape[1] // 32), dtype=torch.uint8))
 
 
-@torch.library.custom_op("mach_amd::swiglu_mxfp4", mutates_args=())
+@_operator("swiglu_mxfp4")
 def swiglu_mxfp4(gate_up: torch.Tensor, rule: int = FLOOR_CARRY175) -> tuple[torch.Tensor, torch.Tensor]:
     """SwiGLU -> MXFP4: gate_up bf16 [M, 2K] -> (codes u8 [M, K/2], scales u8 [M, K/32]) of
     bf16(bf16(silu(gate)) * up), the activation of ``swiglu_mxfp8``, quantized as ``quantize_mxfp4`` does."""
     _check_cuda(gate_up)
-    if gate_up.dtype != torch.bfloat16 or gate_up.ndim != 2 or gate_up.shape[1] == 0 or gate_up.shape[1] % 64:
-        raise ValueError("swiglu_mxfp4 needs bf16 [M, 2K] with K > 0 and K % 32 == 0")
-    if rule not in (FLOOR_CARRY175, FLOOR_OCP):
-        raise ValueError(f"swiglu_mxfp4: unknown rule {rule}")
+    _fp4_gate_up("swiglu_mxfp4", gate_up)
+    _fp4_rule("swiglu_mxfp4", rule)
     gate_up = _aligned(gate_up, 16)
     M, K = gate_up.shape[0], gate_up.shape[1] // 2
     codes = torch.empty((M, K // 2), dtype=torch.uint8, device=gate_up.device)
@@ -828,13 +878,19 @@ def _(gate_up, rule=FLOOR_CARRY175):
     return (gate_up.new_empty((M, K // 2), dtype=torch.uint8), gate_up.new_empty((M, K // 32), dtype=torch.uint8))
 
 
+def _fp4_gate_up(what: str, gate_up: torch.Tensor) -> None:
+    if gate_up.dtype != torch.bfloat16 or gate_up.ndim != 2 or gate_up.shape[1] == 0 or gate_up.shape[1] % 64:
+        raise ValueError(f"{what} needs bf16 [M, 2K] with K > 0 and K % 32 == 0")
+
+
 def _fp4_weight(what: str, w: torch.Tensor, sw: torch.Tensor, n: int, k: int, experts: int = 1):
     """The tiled weight's tensors, of the size that (n, k) asks for."""
     if n <= 0 or k <= 0 or k % 128:
         raise ValueError(f"{what} needs N > 0 and K > 0, K % 128 == 0 (N={n}, K={k})")
-    if w.dtype != torch.uint8 or w.numel() != experts * query("mxl_tiled_weight_bytes", n, k, E2M1):
+    tiles = experts * ((n + 15) // 16) * ((k + 511) // 512)  # of 16 x 512
+    if w.dtype != torch.uint8 or w.numel() != tiles * 4096:
         raise ValueError(f"{what}: the weight is not {experts} x [{n}, {k}] E2M1 in the tiled layout (pack_weight)")
-    if sw.dtype != torch.uint8 or sw.numel() != experts * query("mxl_tiled_scale_bytes", n, k):
+    if sw.dtype != torch.uint8 or sw.numel() != tiles * 256:
         raise ValueError(f"{what}: the scales are not {experts} x [{n}, {k}] in the tiled layout (pack_weight)")
     return _aligned(w, 16), _aligned(sw, 16)
 
@@ -855,7 +911,7 @@ def _fp4_bias(what: str, bias: Optional[torch.Tensor], n: int) -> Optional[torch
     return bias.contiguous()
 
 
-@torch.library.custom_op("mach_amd::mxfp4_gemm", mutates_args=())
+@_operator("mxfp4_gemm")
 def mxfp4_gemm(a: torch.Tensor, sa: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, k: int,
                bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Product of MXFP4 activations and weights: y = A W^T (+ bias), fp32 sums, bf16 [M, N].
@@ -872,7 +928,7 @@ def mxfp4_gemm(a: torch.Tensor, sa: torch.Tensor, w: torch.Tensor, sw: torch.Ten
     if M:
         with _on(a.device):
             nbytes = query("mxl_mxfp4_gemm_workspace_bytes", M, n, k)
-            ws = workspace(a.device, nbytes)
+            ws = _scratch(nbytes, a.device)
             call("mxl_mxfp4_gemm", ptr(a), ptr(sa), M, ptr(w), ptr(sw), n, k, ptr(bias), ptr(out), n, ptr(ws), nbytes,
                  stream_handle(a.device))
     _count("mxfp4_gemm")
@@ -884,21 +940,54 @@ def _(a, sa, w, sw, n, k, bias=None):
     return a.new_empty((a.shape[0], n), dtype=torch.bfloat16)
 
 
-def mxfp4_gemm_from_float(x: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, rule: int = FLOOR_CARRY175,
-                          bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """bf16 rows x [M, K] quantized to MXFP4 and multiplied with an MXFP4 weight."""
-    a, sa = torch.ops.mach_amd.quantize_mxfp4(x, rule)
-    return torch.ops.mach_amd.mxfp4_gemm(a, sa, w, sw, n, x.shape[1], bias)
+@_operator("mxfp4_linear")
+def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, rule: int = FLOOR_CARRY175,
+                 bias: Optional[torch.Tensor] = None, swiglu: bool = False) -> torch.Tensor:
+    """bf16 rows x [M, K] quantized to MXFP4 (``quantize_mxfp4``) and multiplied with an MXFP4 weight
+    (``mxfp4_gemm``), the bits of the two; with ``swiglu`` gate/up rows [M, 2K] through ``swiglu_mxfp4``.
+    One launch for few rows, else two."""
+    _same_device("mxfp4_linear", x, w, sw, bias)
+    if swiglu:
+        _fp4_gate_up("mxfp4_linear", x)
+    elif x.dtype != torch.bfloat16 or x.ndim != 2:
+        raise ValueError("mxfp4_linear needs bf16 [M, K]")
+    _fp4_rule("mxfp4_linear", rule)
+    M, K = x.shape[0], x.shape[1] // 2 if swiglu else x.shape[1]
+    w, sw = _fp4_weight("mxfp4_linear", w, sw, n, K)
+    bias = _fp4_bias("mxfp4_linear", bias, n)
+    out = torch.empty((M, n), dtype=torch.bfloat16, device=x.device)
+    if M:
+        x = _aligned(x, 16) if swiglu else _rows16(x)
+        with _on(x.device):
+            nbytes = query("mxl_mxfp4_linear_workspace_bytes", M, n, K, int(swiglu))
+            ws = _scratch(nbytes, x.device)
+            call("mxl_mxfp4_linear", ptr(x), M, K, _row_stride(x), int(swiglu), rule, ptr(w), ptr(sw), n, ptr(bias),
+                 ptr(out), n, ptr(ws), nbytes, stream_handle(x.device))
+    _count("mxfp4_linear")
+    return out
 
 
-def swiglu_mxfp4_down(gate_up: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int,
-                      rule: int = FLOOR_CARRY175) -> torch.Tensor:
-    """SwiGLU -> MXFP4, then the down projection with an MXFP4 weight (``swiglu_mx_down`` in 4 bits)."""
-    a, sa = torch.ops.mach_amd.swiglu_mxfp4(gate_up, rule)
-    return torch.ops.mach_amd.mxfp4_gemm(a, sa, w, sw, n, gate_up.shape[1] // 2, None)
+@mxfp4_linear.register_fake
+def _(x, w, sw, n, rule=FLOOR_CARRY175, bias=None, swiglu=False):
+    return x.new_empty((x.shape[0], n), dtype=torch.bfloat16)
 
 
-@torch.library.custom_op("mach_amd::mxfp4_grouped_gemm", mutates_args=())
+def _fp4_groups(what: str, rows: int, row_index: Optional[torch.Tensor], row_div: int, expert_offsets: torch.Tensor,
+                routed_rows: int):
+    """Checks of the grouped operators; (row_index, expert_offsets) contiguous."""
+    if expert_offsets.dtype != torch.int64 or expert_offsets.ndim != 1 or expert_offsets.numel() < 2:
+        raise ValueError(f"{what}: expert_offsets must be i64 [E + 1]")
+    if row_index is not None and (row_index.dtype != torch.int32 or row_index.ndim != 1
+                                  or row_index.numel() < routed_rows):
+        raise ValueError(f"{what}: row_index must be i32 with an entry per routed row")
+    if routed_rows < 0 or row_div < 1 or (row_index is None and rows < routed_rows):
+        raise ValueError(f"{what}: need row_div >= 1 and, without row_index, an activation row per routed row")
+    if routed_rows and not rows:
+        raise ValueError(f"{what}: no activation rows")
+    return row_index.contiguous() if row_index is not None else None, expert_offsets.contiguous()
+
+
+@_operator("mxfp4_grouped_gemm")
 def mxfp4_grouped_gemm(a: torch.Tensor, sa: torch.Tensor, row_index: Optional[torch.Tensor], row_div: int,
                        expert_offsets: torch.Tensor, routed_rows: int, w: torch.Tensor, sw: torch.Tensor, n: int,
                        k: int) -> torch.Tensor:
@@ -906,20 +995,10 @@ def mxfp4_grouped_gemm(a: torch.Tensor, sa: torch.Tensor, row_index: Optional[to
     (expert_offsets[e] <= p < expert_offsets[e+1]) is A[row_index[p] // row_div] . W[e]^T, or A[p] . W[e]^T
     without row_index.  Rows past expert_offsets[E] are left unwritten."""
     _same_device("mxfp4_grouped_gemm", a, sa, row_index, expert_offsets, w, sw)
-    if expert_offsets.dtype != torch.int64 or expert_offsets.ndim != 1 or expert_offsets.numel() < 2:
-        raise ValueError("mxfp4_grouped_gemm: expert_offsets must be i64 [E + 1]")
-    E = expert_offsets.numel() - 1
+    row_index, offsets = _fp4_groups("mxfp4_grouped_gemm", a.shape[0], row_index, row_div, expert_offsets, routed_rows)
+    E = offsets.numel() - 1
     w, sw = _fp4_weight("mxfp4_grouped_gemm", w, sw, n, k, E)
     a, sa = _fp4_rows("mxfp4_grouped_gemm", a, sa, k)
-    if row_index is not None and (row_index.dtype != torch.int32 or row_index.ndim != 1
-                                  or row_index.numel() < routed_rows):
-        raise ValueError("mxfp4_grouped_gemm: row_index must be i32 with an entry per routed row")
-    if routed_rows < 0 or row_div < 1 or (row_index is None and a.shape[0] < routed_rows):
-        raise ValueError("mxfp4_grouped_gemm: need row_div >= 1 and, without row_index, an activation row per routed row")
-    if routed_rows and not a.shape[0]:
-        raise ValueError("mxfp4_grouped_gemm: no activation rows")
-    row_index = row_index.contiguous() if row_index is not None else None
-    offsets = expert_offsets.contiguous()
     out = torch.empty((routed_rows, n), dtype=torch.bfloat16, device=a.device)
     if routed_rows:
         with _on(a.device):
@@ -932,6 +1011,101 @@ def mxfp4_grouped_gemm(a: torch.Tensor, sa: torch.Tensor, row_index: Optional[to
 @mxfp4_grouped_gemm.register_fake
 def _(a, sa, row_index, row_div, expert_offsets, routed_rows, w, sw, n, k):
     return a.new_empty((routed_rows, n), dtype=torch.bfloat16)
+
+
+def mxfp4_grouped_swiglu_supported(routed_rows: int, num_experts: int, i: int, k: int) -> bool:
+    """Whether ``mxfp4_grouped_swiglu`` runs this shape (few rows an expert)."""
+    return bool(query("mxl_mxfp4_grouped_swiglu_supported", routed_rows, num_experts, i, k))
+
+
+@_operator("mxfp4_grouped_swiglu")
+def mxfp4_grouped_swiglu(x: torch.Tensor, row_index: Optional[torch.Tensor], row_div: int, expert_offsets: torch.Tensor,
+                         routed_rows: int, w: torch.Tensor, sw: torch.Tensor, i: int, rule: int = FLOOR_CARRY175
+                         ) -> tuple[torch.Tensor, torch.Tensor]:
+    """An expert layer's first half in one launch: ``quantize_mxfp4`` of the gathered bf16 rows x [T, K],
+    ``mxfp4_grouped_gemm`` with the gate/up weights [E, 2 I, K] and ``swiglu_mxfp4`` of its rows -> (codes u8
+    [routed_rows, I/2], scales u8 [routed_rows, I/32]).  Rows past expert_offsets[E] are left unwritten."""
+    _same_device("mxfp4_grouped_swiglu", x, row_index, expert_offsets, w, sw)
+    if x.dtype != torch.bfloat16 or x.ndim != 2:
+        raise ValueError("mxfp4_grouped_swiglu needs bf16 rows [T, K]")
+    if i <= 0 or i % 32:
+        raise ValueError(f"mxfp4_grouped_swiglu needs I > 0 and I % 32 == 0 (I={i})")
+    _fp4_rule("mxfp4_grouped_swiglu", rule)
+    row_index, offsets = _fp4_groups("mxfp4_grouped_swiglu", x.shape[0], row_index, row_div, expert_offsets, routed_rows)
+    E, k = offsets.numel() - 1, x.shape[1]
+    w, sw = _fp4_weight("mxfp4_grouped_swiglu", w, sw, 2 * i, k, E)
+    x = _rows16(x)
+    codes = torch.empty((routed_rows, i // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((routed_rows, i // 32), dtype=torch.uint8, device=x.device)
+    if routed_rows:
+        with _on(x.device):
+            if not mxfp4_grouped_swiglu_supported(routed_rows, E, i, k):
+                raise ValueError(f"mxfp4_grouped_swiglu runs few rows an expert (rows={routed_rows}, E={E}, I={i}, K={k})")
+            call("mxl_mxfp4_grouped_swiglu", ptr(x), x.shape[0], _row_stride(x), ptr(row_index), row_div, ptr(offsets), E,
+                 routed_rows, ptr(w), ptr(sw), i, k, rule, ptr(codes), ptr(scales), stream_handle(x.device))
+    _count("mxfp4_grouped_swiglu")
+    return codes, scales
+
+
+@mxfp4_grouped_swiglu.register_fake
+def _(x, row_index, row_div, expert_offsets, routed_rows, w, sw, i, rule=FLOOR_CARRY175):
+    return x.new_empty((routed_rows, i // 2), dtype=torch.uint8), x.new_empty((routed_rows, i // 32), dtype=torch.uint8)
+
+
+@_operator("mxfp4_experts", mutates_args=("output",))
+def mxfp4_experts(output: torch.Tensor, x: torch.Tensor, topk_ids: Optional[torch.Tensor], topk_weights: torch.Tensor,
+                  sorted_routes: Optional[torch.Tensor], expert_offsets: Optional[torch.Tensor],
+                  inverse: Optional[torch.Tensor], w13: torch.Tensor, sw13: torch.Tensor, w2: torch.Tensor,
+                  sw2: torch.Tensor, e: int, i: int, rule: int = FLOOR_CARRY175, fuse: bool = True) -> None:
+    """A layer of MXFP4 experts on bf16 x [T, H], into ``output`` (contiguous bf16 [T, H]): the routes of ``topk_ids`` i32 [T, k] sorted (``moe_route``; or
+    given sorted, as ``moe_route`` and the routers return them), the gate/up product of the quantized rows with
+    w13 [e, 2 i, H], ``swiglu_mxfp4``, the product with w2 [e, H, i] and ``moe_reduce`` with the fp32 weights
+    [T, k].  ``fuse``: the first half as ``mxfp4_grouped_swiglu`` where that runs."""
+    _same_device("mxfp4_experts", x, output, topk_ids, topk_weights, sorted_routes, expert_offsets, inverse, w13, sw13, w2, sw2)
+    if x.dtype != torch.bfloat16 or x.ndim != 2:
+        raise ValueError("mxfp4_experts needs bf16 x [T, H]")
+    T, H = x.shape
+    if topk_weights.ndim != 2 or topk_weights.shape[0] != T or not topk_weights.shape[1]:
+        raise ValueError(f"mxfp4_experts: topk_weights must be [{T}, k]")
+    if output.dtype != torch.bfloat16 or output.shape != x.shape or not output.is_contiguous():
+        raise ValueError(f"mxfp4_experts: output must be contiguous bf16 [{T}, {H}]")
+    topk = topk_weights.shape[1]
+    if e < 1 or i <= 0 or i % 128 or H <= 0 or H % 128:
+        raise ValueError(f"mxfp4_experts needs experts, and H and I divisible by 128 (E={e}, H={H}, I={i})")
+    _fp4_rule("mxfp4_experts", rule)
+    given = sorted_routes is not None
+    if given:
+        for name, t, n, dtype in (("sorted_routes", sorted_routes, T * topk, torch.int32),
+                                  ("expert_offsets", expert_offsets, e + 1, torch.int64),
+                                  ("inverse", inverse, T * topk, torch.int32)):
+            if t is None or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+                raise ValueError(f"mxfp4_experts: {name} must be contiguous {dtype} of {n} values")
+    elif topk_ids is None or tuple(topk_ids.shape) != (T, topk):
+        raise ValueError(f"mxfp4_experts: topk_ids must be [{T}, {topk}]")
+    w13, sw13 = _fp4_weight("mxfp4_experts", w13, sw13, 2 * i, H, e)
+    w2, sw2 = _fp4_weight("mxfp4_experts", w2, sw2, H, i, e)
+    out = output if output.data_ptr() % 16 == 0 else torch.empty((T, H), dtype=torch.bfloat16, device=x.device)
+    if T:
+        x = _rows16(x)
+        weights = topk_weights.to(torch.float32).contiguous()
+        ids = None if given else topk_ids.to(torch.int32).contiguous()
+        with _on(x.device):
+            nbytes = query("mxl_mxfp4_experts_workspace_bytes", T, topk, e, H, i, int(given), int(fuse))
+            ws = _scratch(nbytes, x.device)
+            call("mxl_mxfp4_experts", ptr(x), T, _row_stride(x), ptr(ids), ptr(weights), topk, ptr(sorted_routes),
+                 ptr(expert_offsets), ptr(inverse), e, H, i, ptr(w13), ptr(sw13), ptr(w2), ptr(sw2), rule, int(fuse),
+                 ptr(out), ptr(ws), nbytes, stream_handle(x.device))
+        if out is not output:
+            output.copy_(out)
+        elif not output.is_inference():
+            torch.autograd.graph.increment_version(output)
+    _count("mxfp4_experts")
+
+
+@mxfp4_experts.register_fake
+def _(output, x, topk_ids, topk_weights, sorted_routes, expert_offsets, inverse, w13, sw13, w2, sw2, e, i,
+      rule=FLOOR_CARRY175, fuse=True):
+    return None
 
 
 # ---------------------------------------------------------------------- MoE
@@ -1008,7 +1182,7 @@ def _(router_logits, top_k, renormalize=True):
             router_logits.new_empty((R,), dtype=torch.int32))
 
 
-@torch.library.custom_op("mach_amd::moe_router_grouped", mutates_args=())
+@_operator("moe_router_grouped")
 def moe_router_grouped(router_logits: torch.Tensor, bias: Optional[torch.Tensor], top_k: int, scoring: int = SOFTMAX,
                        num_groups: int = 1, topk_groups: int = 1, renormalize: bool = True, factor: float = 1.0
                        ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -1044,7 +1218,7 @@ def moe_router_grouped(router_logits: torch.Tensor, bias: Optional[torch.Tensor]
     inverse = torch.empty(T * top_k, dtype=torch.int32, device=dev)
     with _on(dev):
         nbytes = query("mxl_moe_router_workspace_bytes", T, top_k, E)
-        buf = workspace(dev, nbytes, "route")
+        buf = _scratch(nbytes, dev)
         call("mxl_moe_router_grouped", ptr(logits), int(logits.dtype == torch.bfloat16), ptr(bias), T, E, top_k, scoring,
              num_groups, topk_groups, int(renormalize), float(factor), ptr(weights), ptr(ids), ptr(sorted_routes),
              ptr(offsets), ptr(inverse), ptr(buf), nbytes, stream_handle(dev))
