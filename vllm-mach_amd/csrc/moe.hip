@@ -15,29 +15,9 @@
 //
 // Combine: out[t, h] = bf16(sum_k y[inverse[t*topk + k], h] * w[t, k]),
 // each product rounded to binary32 and added in ascending k from zero.
-#include "mx_common.h"
+#include "moe_sort.h"
 
 namespace mxl {
-
-constexpr int kChunk = 1024;
-
-// Routes of the same key in the earlier lanes of this wavefront (the rank of the lane's
-// route among its expert's routes in the wavefront); key = the expert id, or E for a
-// route whose expert is outside [0, E).  The lanes holding the same key are found one key
-// bit at a time with a ballot -- a bit's ballot, or its complement where the lane's bit
-// is 0, keeps the lanes that agree on it -- bit_width(E) ballots (9 for 256 experts)
-// instead of 64 lane-by-lane comparisons; only wavefront-uniform control flow, so every
-// lane takes part in every ballot.
-__device__ __forceinline__ int same_expert_rank(int key, int E, int lane) {
-  const int bits = 32 - __builtin_clz((unsigned)E);
-  uint64_t same = ~0ull;
-  for (int b = 0; b < bits; ++b) {
-    const bool bit = (key >> b) & 1;
-    const uint64_t on = __ballot(bit);
-    same &= bit ? on : ~on;
-  }
-  return __popcll(same & ((1ull << lane) - 1ull));
-}
 
 __global__ __launch_bounds__(kChunk) void route_hist_kernel(const int32_t* __restrict__ ids, int64_t R, int E,
                                                            int32_t* __restrict__ chunk_counts) {
@@ -54,18 +34,49 @@ __global__ __launch_bounds__(kChunk) void route_hist_kernel(const int32_t* __res
   for (int e = threadIdx.x; e < E; e += blockDim.x) chunk_counts[c * E + e] = hist[e];
 }
 
-// One workgroup: chunk bases per expert (in place) and expert offsets.
+// One workgroup: chunk bases per expert (in place) and expert offsets.  P threads share an expert's chunks (as
+// many as the workgroup has), each first adding up its own, sixteen loads at a time, then handing out its bases
+// from the sum of those before it (131072 routes of 256 experts, 128 chunks: 29 us with one thread an expert and
+// load after load).
+__device__ __host__ inline int route_scan_parts(int E) { return E < 1024 ? 1024 / E : 1; }
 __global__ __launch_bounds__(1024) void route_scan_kernel(int32_t* __restrict__ chunk_counts, int64_t C, int E,
                                                          int64_t* __restrict__ expert_offsets) {
-  extern __shared__ int64_t tot[];  // [2][E]
-  for (int e = threadIdx.x; e < E; e += blockDim.x) {
-    int64_t run = 0;
-    for (int64_t c = 0; c < C; ++c) {
-      const int32_t v = chunk_counts[c * E + e];
-      chunk_counts[c * E + e] = (int32_t)run;
-      run += v;
+  constexpr int B = 16;
+  extern __shared__ int64_t tot[];  // [2][E], then the parts' sums i32 [P][E]
+  const int P = route_scan_parts(E);
+  int32_t* const part = reinterpret_cast<int32_t*>(tot + 2 * E);
+  const int64_t per = (C + P - 1) / P;
+  for (int i = threadIdx.x; i < P * E; i += blockDim.x) {
+    const int e = i % E;
+    const int64_t c0 = i / E * per, c1 = c0 + per < C ? c0 + per : C;
+    int32_t sum = 0;
+    for (int64_t c = c0; c < c1; c += B) {
+      int32_t v[B];
+#pragma unroll
+      for (int k = 0; k < B; ++k) v[k] = c + k < c1 ? chunk_counts[(c + k) * E + e] : 0;
+#pragma unroll
+      for (int k = 0; k < B; ++k) sum += v[k];
     }
-    tot[e] = run;
+    part[i] = sum;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < P * E; i += blockDim.x) {
+    const int e = i % E;
+    const int64_t c0 = i / E * per, c1 = c0 + per < C ? c0 + per : C;
+    int32_t run = 0;
+    for (int k = 0; k < i / E; ++k) run += part[k * E + e];
+    for (int64_t c = c0; c < c1; c += B) {
+      int32_t v[B];
+#pragma unroll
+      for (int k = 0; k < B; ++k) v[k] = c + k < c1 ? chunk_counts[(c + k) * E + e] : 0;
+#pragma unroll
+      for (int k = 0; k < B; ++k)
+        if (c + k < c1) {
+          chunk_counts[(c + k) * E + e] = run;
+          run += v[k];
+        }
+    }
+    if (i / E == P - 1) tot[e] = run;
   }
   __syncthreads();
   // inclusive Hillis-Steele scan over E values (ping-pong buffers)
@@ -171,63 +182,6 @@ __global__ __launch_bounds__(kChunk) void route_count_scan_kernel(const int32_t*
   if (t == 0) expert_offsets[0] = 0;
 }
 
-// All routes in one chunk (R <= 1024, E <= 1024): the three passes in one
-// workgroup -- per-wavefront expert counts in LDS, per-expert totals scanned into
-// the offsets, then the same rank and scatter -- so a decode-sized step pays one
-// launch.  The result is the multi-chunk path's (chunk base 0).
-constexpr int kSingleMaxExperts = 1024;
-// Largest expert count any route schedule launches: the scatter's (kChunk / 64) * E
-// ints of LDS must fit gfx950's 160 KiB per workgroup.
-constexpr int kRouteMaxExperts = 160 * 1024 / ((kChunk / 64) * (int)sizeof(int32_t));
-static_assert(kRouteMaxExperts == 2560, "the documented expert limit");
-
-// The single-chunk sort for route t (expert e, -1 if none): per-wavefront expert counts in
-// LDS, per-expert totals scanned into the offsets, then the rank and scatter.  Called by
-// every thread of a 1024-thread workgroup (t = threadIdx.x).
-__device__ __forceinline__ void single_chunk_sort(int32_t e, int64_t R, int E, int64_t* __restrict__ expert_offsets,
-                                                  int32_t* __restrict__ sorted_routes,
-                                                  int32_t* __restrict__ inverse, int32_t* whist,
-                                                  int32_t (*tot)[kSingleMaxExperts]) {
-  constexpr int W = kChunk / 64;
-  const int t = threadIdx.x, w = t >> 6, lane = t & 63;
-  for (int i = t; i < W * E; i += kChunk) whist[i] = 0;
-  const bool valid = e >= 0 && e < E;
-  const int rank = same_expert_rank(valid ? e : E, E, lane);
-  __syncthreads();
-  if (valid) atomicAdd(&whist[w * E + e], 1);
-  __syncthreads();
-  for (int x = t; x < E; x += kChunk) {  // per-wavefront bases and the expert's total
-    int32_t run = 0;
-    for (int v = 0; v < W; ++v) {
-      const int32_t n = whist[v * E + x];
-      whist[v * E + x] = run;
-      run += n;
-    }
-    tot[0][x] = run;
-  }
-  __syncthreads();
-  int src = 0;  // inclusive scan of the totals (ping-pong)
-  for (int d = 1; d < E; d <<= 1) {
-    for (int x = t; x < E; x += kChunk) {
-      int32_t v = tot[src][x];
-      if (x >= d) v += tot[src][x - d];
-      tot[1 - src][x] = v;
-    }
-    __syncthreads();
-    src = 1 - src;
-  }
-  for (int x = t; x < E; x += kChunk) expert_offsets[x + 1] = tot[src][x];
-  if (t == 0) expert_offsets[0] = 0;
-  if (t >= R) return;
-  if (!valid) {
-    inverse[t] = -1;
-    return;
-  }
-  const int32_t pos = (e > 0 ? tot[src][e - 1] : 0) + whist[w * E + e] + rank;
-  sorted_routes[pos] = t;
-  inverse[t] = pos;
-}
-
 __global__ __launch_bounds__(kChunk) void route_single_kernel(const int32_t* __restrict__ ids, int64_t R, int E,
                                                              int64_t* __restrict__ expert_offsets,
                                                              int32_t* __restrict__ sorted_routes,
@@ -331,32 +285,7 @@ __global__ __launch_bounds__(kChunk) void route_sort_kernel(const int32_t* __res
 constexpr int kRouterSlots = kSingleMaxExperts / 64;  // logits per lane: E <= 1024
 constexpr int kRouterMaxTopk = 64;
 
-// Binary32 as an unsigned key in value order (-0 read as +0, so equal values tie; NaNs
-// order outside the finite values by sign).
-__device__ __forceinline__ uint32_t order_key(float x) {
-  uint32_t u = f2u(x);
-  if (u == 0x80000000u) u = 0u;
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
 __device__ __forceinline__ float key_value(uint32_t k) { return u2f((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k); }
-
-// The wavefront's largest value, in every lane: an inclusive maximum along the lanes (rows of
-// 16, then across rows), read from lane 63.  Lanes without a source keep 0.
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#define MXL_DPP_MAX(CTRL_, ROWS_)                                                              \
-  {                                                                                            \
-    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL_, ROWS_, 0xf, false); \
-    v = o > v ? o : v;                                                                         \
-  }
-  MXL_DPP_MAX(0x111, 0xf)  // row_shr:1, 2, 4, 8
-  MXL_DPP_MAX(0x112, 0xf)
-  MXL_DPP_MAX(0x114, 0xf)
-  MXL_DPP_MAX(0x118, 0xf)
-  MXL_DPP_MAX(0x142, 0xa)  // row_bcast:15 into rows 1 and 3
-  MXL_DPP_MAX(0x143, 0xc)  // row_bcast:31 into rows 2 and 3
-#undef MXL_DPP_MAX
-  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-}
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -539,7 +468,8 @@ extern "C" int mxl_moe_route(const int32_t* topk_ids, int64_t T, int64_t topk, i
       route_hist_kernel<<<dim3((unsigned)C), kChunk, E * sizeof(int32_t), s>>>(topk_ids, R, (int)E, counts);
       MXL_CHECK_LAUNCH("mxl_moe_route(hist)");
     }
-    route_scan_kernel<<<1, 1024, 2 * E * sizeof(int64_t), s>>>(counts, C, (int)E, expert_offsets);
+    route_scan_kernel<<<1, 1024, 2 * E * sizeof(int64_t) + route_scan_parts((int)E) * E * sizeof(int32_t), s>>>(
+          counts, C, (int)E, expert_offsets);
     MXL_CHECK_LAUNCH("mxl_moe_route(scan)");
   }
   if (C > 0) {
