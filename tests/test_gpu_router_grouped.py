@@ -64,6 +64,41 @@ def test_scores_closer_than_an_fp32_step(pkg, dev):
 
 
 @pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("groups,keep", [(1, 1), (8, 3)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_calls_closer_than_binary32(pkg, dev, biased, groups, keep, sigmoid):
+    """Scores that binary32 cannot order, in the middle of the choice, at its end and between groups: logits a few
+    steps of fp32 apart, with biases that make up for them."""
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(400, 64, generator=g)
+    steps = torch.randint(0, 4, (400, 64), generator=g).float() * 2.0 ** -22
+    x = (x * 4).round() / 4 + steps
+    bias = (torch.randn(64, generator=g) * 8).round() / 64 + torch.randint(0, 3, (64,), generator=g) * 2.0 ** -26 if biased else None
+    _check(pkg, x, bias, 6, sigmoid, groups, keep, True, 1.0)
+    _check(pkg, x * 30, bias, 6, sigmoid, groups, keep, False, 1.0)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("E,groups,keep", [(32, 4, 2), (60, 5, 3), (256, 8, 4), (640, 1, 1)])
+def test_zeros_of_both_signs_and_tiny_logits_tie(pkg, dev, E, groups, keep, sigmoid):
+    """Logits whose exponentials are equal in 64 bits: -0 and 0, subnormals, and (sigmoid) those far above 37."""
+    g = torch.Generator().manual_seed(5)
+    pool = torch.tensor([0.0, -0.0, 1e-40, -1e-40, 1e-30] + ([100.0, 101.0] if sigmoid else []))
+    x = pool[torch.randint(0, len(pool), (70, E), generator=g)]
+    _check(pkg, x, None, 6, sigmoid, groups, keep, True, 1.0)
+    _check(pkg, x.bfloat16(), None, 6, sigmoid, groups, keep, True, 1.0)
+    _check(pkg, x, torch.zeros(E), 6, sigmoid, groups, keep, True, 1.0)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_large_biases(pkg, dev, sigmoid):
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(64, 96, generator=g)
+    for scale in (1e3, 1e6, 1e30):
+        _check(pkg, x, torch.randn(96, generator=g) * scale, 7, sigmoid, 4, 2, True, 1.0)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
 def test_masked_infinite_and_nan_logits(pkg, dev, sigmoid):
     """Masked experts (-inf, the lowest finite value), infinities and NaN; a row with nothing left but masks."""
     low = torch.finfo(torch.float32).min
