@@ -29,6 +29,9 @@
 // sides, the choice is the true one; for a token with a closer call (or an infinity or NaN), one in some hundred, the
 // whole wavefront makes it in binary64 (choose_exact: 64-bit keys, compared by their halves).
 // The weights are of binary64 scores of the k chosen, one a lane.
+//
+// 16384 tokens of 256 experts, 8 of 128 in 4 of 8 groups: 19 us (31.3 with every score in binary64 and a token per
+// wavefront, 27 with the binary32 choice alone, 26 with four tokens to a wavefront that all made a close one's choice).
 #include "moe_sort.h"
 
 namespace mxl {
