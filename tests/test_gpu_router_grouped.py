@@ -36,7 +36,8 @@ def _check(pkg, logits, bias, topk, sigmoid, groups, keep, renorm, factor):
 @pytest.mark.parametrize("T,E,topk,groups,keep", [
     (1, 1, 1, 1, 1), (1, 256, 8, 8, 4), (5, 8, 8, 1, 1), (16, 64, 6, 8, 3), (17, 160, 6, 8, 3), (130, 256, 8, 8, 4),
     (40, 16, 4, 16, 4), (33, 72, 2, 1, 1), (200, 512, 10, 8, 2), (9, 1000, 64, 4, 3), (3, 1024, 8, 64, 8),
-    (1, 255, 5, 3, 2), (65, 96, 1, 2, 1), (1100, 24, 3, 4, 2)])
+    (1, 255, 5, 3, 2), (65, 96, 1, 2, 1), (1100, 24, 3, 4, 2), (2049, 256, 8, 8, 4), (2500, 160, 6, 8, 3),
+    (2301, 100, 4, 5, 2)])
 def test_router(pkg, dev, T, E, topk, groups, keep, biased, sigmoid):
     g = torch.Generator().manual_seed(T * E + topk)
     x = torch.randn(T, E, generator=g) * 2
@@ -66,25 +67,27 @@ def test_scores_closer_than_an_fp32_step(pkg, dev):
 @pytest.mark.parametrize("sigmoid", [False, True])
 @pytest.mark.parametrize("groups,keep", [(1, 1), (8, 3)])
 @pytest.mark.parametrize("biased", [False, True])
-def test_calls_closer_than_binary32(pkg, dev, biased, groups, keep, sigmoid):
+@pytest.mark.parametrize("T,E", [(400, 64), (400, 96), (2200, 96)])
+def test_calls_closer_than_binary32(pkg, dev, T, E, biased, groups, keep, sigmoid):
     """Scores that binary32 cannot order, in the middle of the choice, at its end and between groups: logits a few
     steps of fp32 apart, with biases that make up for them."""
     g = torch.Generator().manual_seed(7)
-    x = torch.randn(400, 64, generator=g)
-    steps = torch.randint(0, 4, (400, 64), generator=g).float() * 2.0 ** -22
+    x = torch.randn(T, E, generator=g)
+    steps = torch.randint(0, 4, (T, E), generator=g).float() * 2.0 ** -22
     x = (x * 4).round() / 4 + steps
-    bias = (torch.randn(64, generator=g) * 8).round() / 64 + torch.randint(0, 3, (64,), generator=g) * 2.0 ** -26 if biased else None
+    bias = (torch.randn(E, generator=g) * 8).round() / 64 + torch.randint(0, 3, (E,), generator=g) * 2.0 ** -26 if biased else None
     _check(pkg, x, bias, 6, sigmoid, groups, keep, True, 1.0)
     _check(pkg, x * 30, bias, 6, sigmoid, groups, keep, False, 1.0)
 
 
 @pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("T", [70, 2100])
 @pytest.mark.parametrize("E,groups,keep", [(32, 4, 2), (60, 5, 3), (256, 8, 4), (640, 1, 1)])
-def test_zeros_of_both_signs_and_tiny_logits_tie(pkg, dev, E, groups, keep, sigmoid):
+def test_zeros_of_both_signs_and_tiny_logits_tie(pkg, dev, E, groups, keep, T, sigmoid):
     """Logits whose exponentials are equal in 64 bits: -0 and 0, subnormals, and (sigmoid) those far above 37."""
     g = torch.Generator().manual_seed(5)
     pool = torch.tensor([0.0, -0.0, 1e-40, -1e-40, 1e-30] + ([100.0, 101.0] if sigmoid else []))
-    x = pool[torch.randint(0, len(pool), (70, E), generator=g)]
+    x = pool[torch.randint(0, len(pool), (T, E), generator=g)]
     _check(pkg, x, None, 6, sigmoid, groups, keep, True, 1.0)
     _check(pkg, x.bfloat16(), None, 6, sigmoid, groups, keep, True, 1.0)
     _check(pkg, x, torch.zeros(E), 6, sigmoid, groups, keep, True, 1.0)

@@ -10,7 +10,8 @@
 // whole number, and two sigmoid scores a rounding of exp apart must not decide it.  NaN choice scores rank
 // below every other.
 //
-// LPT lanes per token: 16, four tokens to a wavefront, or 64 (more than 16 choices, groups or experts to a lane).
+// LPT lanes per token: 16, four tokens to a wavefront, or 64 (few tokens; more than 16 choices, groups or experts to a
+// lane).
 // Each group has 2^lpg_log of them (the most that fit), each lane successive experts of its group, so that a group's
 // two largest c come from lpg_log exchanges of all groups at once and the lowest lane is the lowest index.
 //
@@ -453,14 +454,19 @@ static void launch_grouped_slots(GroupedRouting& g, int64_t* offsets, int32_t* s
                                  hipStream_t s) {
   g.deal = deal_groups(g, 16);
   g.deal64 = deal_groups(g, 64);
-  if (g.topk <= 16 && g.groups <= 16 && g.deal.per <= 16) {  // (then four experts a lane of 64 at most)
+  // A wavefront per token where tokens are few, its walk over four experts a lane being the shorter (256 experts,
+  // routing and sort in us, 64 lanes against 16: 10.7 to 11.6 at 17 tokens, 14.3 to 17.1 at 512, 18.4 to 18.5 at 2000,
+  // 37.6 to 29.7 at 16384; 9.3 to 9.0 at 8, 10.6 to 9.3 at 16, which share a CU; 64 experts 10.4 to 9.6 at 512).
+  const bool few = g.deal.per > 4 && g.T <= (offsets ? 8 : 2048);
+  if (!few && g.topk <= 16 && g.groups <= 16 && g.deal.per <= 16) {  // (then four experts a lane of 64 at most)
     if (g.deal.per <= 4) launch_grouped<BF16, 16, 4>(g, offsets, sorted_routes, inverse, s);
     else if (g.deal.per <= 8) launch_grouped<BF16, 16, 8>(g, offsets, sorted_routes, inverse, s);
     else launch_grouped<BF16, 16, 16>(g, offsets, sorted_routes, inverse, s);
     return;
   }
   g.deal = g.deal64;
-  if (g.deal.per <= 8) launch_grouped<BF16, 64, 8>(g, offsets, sorted_routes, inverse, s);
+  if (g.deal.per <= 4) launch_grouped<BF16, 64, 4>(g, offsets, sorted_routes, inverse, s);
+  else if (g.deal.per <= 8) launch_grouped<BF16, 64, 8>(g, offsets, sorted_routes, inverse, s);
   else launch_grouped<BF16, 64, 32>(g, offsets, sorted_routes, inverse, s);
 }
 

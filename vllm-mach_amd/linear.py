@@ -324,8 +324,10 @@ class Mxfp4LinearKernel(_Kernel):
         if x.numel() == 0:
             return x.new_empty((*x.shape[:-1], n))
         inner = _epilogue_bias(bias, x, n)
-        y = ops.mxfp4_linear(_flatten(x, k), layer.weight, layer.weight_scale, n, self.act_rule, inner)
-        y = y.reshape(*x.shape[:-1], n)
+        rows = x.ndim == 2  # (views are 1 us each of an eager call)
+        y = ops.mxfp4_linear(x if rows else _flatten(x, k), layer.weight, layer.weight_scale, n, self.act_rule, inner)
+        if not rows:
+            y = y.reshape(*x.shape[:-1], n)
         return y if bias is inner else y + bias
 
 
@@ -425,8 +427,10 @@ def swiglu_mxfp4_down(gate_up: torch.Tensor, down: torch.nn.Module) -> torch.Ten
     n, k = down.mxl_shape
     if gate_up.shape[-1] != 2 * k:
         raise ValueError("gate_up width must be twice the down projection's K")
-    y = ops.mxfp4_linear(_flatten(gate_up, 2 * k), down.weight, down.weight_scale, n, ops.FLOOR_CARRY175, None, True)
-    return y.reshape(*gate_up.shape[:-1], n)
+    rows = gate_up.ndim == 2
+    x = gate_up if rows else _flatten(gate_up, 2 * k)
+    y = ops.mxfp4_linear(x, down.weight, down.weight_scale, n, ops.FLOOR_CARRY175, None, True)
+    return y if rows else y.reshape(*gate_up.shape[:-1], n)
 
 
 # registration: the reference prepends its kernels to vLLM's per-platform candidate
