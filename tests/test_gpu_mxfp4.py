@@ -456,6 +456,33 @@ def test_experts_layer(pkg, dev, t, e, topk, h, i, fuse):
     assert float((got - want).norm() / want.norm()) <= 2 * 2.0 ** -8 + 2.0 ** -10 * 3
 
 
+@pytest.mark.parametrize("rule", RULES)
+@pytest.mark.parametrize("t,e,topk,h,i", [(300, 6, 2, 640, 128), (700, 16, 4, 1152, 640), (130, 3, 1, 128, 256),
+                                          (900, 5, 3, 2048, 384), (1500, 64, 2, 512, 512)])
+def test_swiglu_in_the_tiles_is_the_separate_launches(pkg, dev, t, e, topk, h, i, rule):
+    """Many rows an expert: the producer in the epilogue of the gate/up product against a launch of its own, bit for
+    bit, with ordinary gates, rows of zeros, gates past the table's both ends and NaN, one expert with most of the
+    rows, one with none and some ids of no expert."""
+    g = torch.Generator().manual_seed(t + i)
+    experts, w1, w2, _, _ = _experts(pkg, g, e, h, i)
+    experts.rule = rule
+    x = _x(g, t, h)
+    x[3::50] = 0.0
+    x[4::50] *= 2.0 ** 20
+    x[5::50] *= 2.0 ** -30
+    x[6, 7] = math.nan
+    x[8, 9] = math.inf
+    ids = torch.where(torch.rand(t, topk, generator=g) < 0.5, e - 1, torch.randint(0, e - 1, (t, topk), generator=g)).int()
+    ids[ids == 0] = -1 if e > 4 else 1
+    p = torch.rand(t, topk, generator=g).to(dev)
+    args = (x.to(dev), w1, w2, p, ids.to(dev))
+    one = experts(*args)
+    experts.fuse = False
+    two = experts(*args)
+    assert torch.equal(one.view(torch.int16), two.view(torch.int16))
+    assert bool(one[6].isnan().all()) and not bool(one[10].isnan().any())
+
+
 def test_experts_map_and_method(pkg, dev):
     """An expert map drops the experts of other ranks; the method object runs the same layer."""
     g = torch.Generator().manual_seed(9)

@@ -57,6 +57,11 @@ struct GemmParams {
   const uint16_t* fsrc = nullptr;
   int64_t fsrc_ld = 0;
   uint32_t* fsync = nullptr;
+  // Grouped MXFP4 gate/up product with the SwiGLU producer in its epilogue: codes [routed rows, N / 4], scales
+  // [routed rows, N / 64] of N = 2 I, and the scale rule (fp4_carry).
+  uint8_t* mid_codes = nullptr;
+  uint8_t* mid_scales = nullptr;
+  uint32_t mid_carry = 0;
 };
 
 // Output element formats (mxl_gemm_options.out_dtype).

@@ -557,6 +557,32 @@ extern "C" int mxl_mxfp4_grouped_gemm(const void* a, const void* sa, int64_t a_r
   return MXL_OK;
 }
 
+// Whether the gate/up product of an experts call (I % 128 == 0) runs in the tiles, whose epilogue then is the SwiGLU
+// producer.
+static bool fp4_swiglu_tiles(int64_t T, int64_t routed_rows, int64_t num_experts, int64_t I, int64_t K) {
+  Fp4StreamPlan pl;
+  return num_experts <= kWideGroupedMaxExperts &&
+         !fp4_grouped_streams(routed_rows, num_experts, 2 * I, K, false, pl) &&
+         fp4_tiles_eligible(std::max(T, routed_rows), 2 * I, K);
+}
+
+// Its launch: codes a / sa of T rows, MXFP4 SwiGLU codes [routed rows, I / 2] and scales [routed rows, I / 32] out.
+static int fp4_swiglu_tiles_launch(const char* who, const void* a, const void* sa, int64_t T, const int32_t* row_index,
+                                   int row_div, const int64_t* expert_offsets, int64_t num_experts, int64_t routed_rows,
+                                   const void* w_tiled, const void* sw_tiled, int64_t I, int64_t K, int rule, void* codes,
+                                   void* scales, hipStream_t s) {
+  const int rc = check_operands(who, a, sa, w_tiled, sw_tiled, 2 * I, K, nullptr);
+  if (rc != MXL_OK) return rc;
+  GemmParams p = fp4_params(a, sa, w_tiled, sw_tiled, 2 * I, K, nullptr, 2 * I);
+  p.M = routed_rows; p.a_rows = T; p.row_index = row_index; p.row_div = row_div; p.expert_offsets = expert_offsets;
+  p.w_expert_stride = mxl_tiled_weight_bytes(2 * I, K, kE2M1);
+  p.sw_expert_stride = mxl_tiled_scale_bytes(2 * I, K);
+  p.mid_codes = (uint8_t*)codes; p.mid_scales = (uint8_t*)scales; p.mid_carry = fp4_carry(rule);
+  WideConfig c{2, 1, p.KT};
+  c.MT = 8;
+  return launch_status(launch_gemm_wide(kE2M1, false, c, p, num_experts, s), who);
+}
+
 // ------------------------------------------------------------------ layers in one call
 
 extern "C" int mxl_quantize_mxfp4(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, void* codes, void* scales,
@@ -601,7 +627,7 @@ LinearScratch linear_scratch(uint8_t* base, int64_t M, int64_t N, int64_t K) {
 struct ExpertScratch {
   void *routes, *offsets, *inverse, *sort, *codes, *scales, *gate_up, *codes2, *scales2, *y;
   int64_t sort_bytes, bytes;
-  bool fused;
+  bool fused, tiles;  // the SwiGLU producer in the gate/up product's launch: with the quantizer, or behind it
 };
 ExpertScratch expert_scratch(uint8_t* base, int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, bool sorted,
                              bool fuse) {
@@ -610,6 +636,7 @@ ExpertScratch expert_scratch(uint8_t* base, int64_t T, int64_t topk, int64_t E, 
   ExpertScratch x{};
   x.sort_bytes = sorted ? 0 : mxl_moe_route_workspace_bytes(T, topk, E);
   x.fused = fuse && mxl_mxfp4_grouped_swiglu_supported(R, E, I, H);
+  x.tiles = fuse && !x.fused && fp4_swiglu_tiles(T, R, E, I, H);
   if (!sorted) {
     x.routes = p.take(R * 4);
     x.offsets = p.take((E + 1) * 8);
@@ -619,7 +646,7 @@ ExpertScratch expert_scratch(uint8_t* base, int64_t T, int64_t topk, int64_t E, 
   if (!x.fused) {
     x.codes = p.take(T * (H / 2));
     x.scales = p.take(T * (H / 32));
-    x.gate_up = p.take(R * 2 * I * 2);
+    if (!x.tiles) x.gate_up = p.take(R * 2 * I * 2);
   }
   x.codes2 = p.take(R * (I / 2));
   x.scales2 = p.take(R * (I / 32));
@@ -694,9 +721,11 @@ extern "C" int mxl_mxfp4_experts(const void* x, int64_t T, int64_t ldx, const in
   } else {
     st = mxl_quantize_mxfp4(x, T, H, ldx, rule, s.codes, s.scales, stream);
     if (st == MXL_OK)
-      st = mxl_mxfp4_grouped_gemm(s.codes, s.scales, T, sorted_routes, (int)topk, expert_offsets, E, R, w13, sw13, 2 * I,
-                                  H, s.gate_up, stream);
-    if (st == MXL_OK) st = mxl_swiglu_mxfp4(s.gate_up, R, I, rule, s.codes2, s.scales2, stream);
+      st = s.tiles ? fp4_swiglu_tiles_launch(who, s.codes, s.scales, T, sorted_routes, (int)topk, expert_offsets, E, R, w13,
+                                             sw13, I, H, rule, s.codes2, s.scales2, (hipStream_t)stream)
+                   : mxl_mxfp4_grouped_gemm(s.codes, s.scales, T, sorted_routes, (int)topk, expert_offsets, E, R, w13, sw13,
+                                            2 * I, H, s.gate_up, stream);
+    if (st == MXL_OK && !s.tiles) st = mxl_swiglu_mxfp4(s.gate_up, R, I, rule, s.codes2, s.scales2, stream);
   }
   if (st == MXL_OK)
     st = mxl_mxfp4_grouped_gemm(s.codes2, s.scales2, R, nullptr, 1, expert_offsets, E, R, w2, sw2, H, I, s.y, stream);

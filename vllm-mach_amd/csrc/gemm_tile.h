@@ -37,6 +37,7 @@
 // sums share one activation scale.
 #pragma once
 
+#include "fp4.h"
 #include "gemm_wide.h"
 
 // the copies set M0 (the LDS base of a global->LDS load) themselves
@@ -163,8 +164,10 @@ struct TileLds {
   static constexpr int bytes(int depth) { return RING + depth * STAGE; }
 };
 
-// a_row(row): the activation row of output row `row` (rows past the last: any valid one)
-template <int FMT, int MTW, int NTW, bool BLOCK, int DEPTH, class Row>
+// a_row(row): the activation row of output row `row` (rows past the last: any valid one).  SWIGLU (MXFP4, N = 2 I, I %
+// 64 == 0, W = gate rows then up rows): half of a wave's n-tiles are gate columns, half the up columns of the same 32, and the
+// epilogue writes their SwiGLU as MXFP4 (p.mid_codes, p.mid_scales) instead of the product.
+template <int FMT, int MTW, int NTW, bool BLOCK, int DEPTH, bool SWIGLU = false, class Row>
 __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w, uint8_t* lds, Row&& a_row) {
   static_assert(!BLOCK || FMT == kE4M3, "block-FP8 weights are E4M3");
   using S = TileShape<MTW, NTW>;
@@ -172,6 +175,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   constexpr int MH = MTW / 2, NH = NTW / 2, CH = FmtTraits<FMT>::CH;
   constexpr bool FP4 = FMT == kE2M1;
   constexpr int SPT = FP4 ? 2 : 4;  // stages of a 512-wide super-tile
+  static_assert(!SWIGLU || (FP4 && NH == 2), "a wave's gate columns are a block of 32");
   // A stage's copies take the slots of the stage DEPTH before it in the order those fall free.
   // At an odd depth that stage reads its B units in the other order, so the B unit this stage
   // needs first is copied second, and the barrier that hands it over waits for CB copies more.
@@ -186,7 +190,16 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   const int KT = (int)p.KT, ntiles = (int)((p.N + 15) / 16), kb = w.kb, ke = w.ke;
   // stages SPT kb .. te - 1; an odd count runs one more (end), whose weights (past K) are zero
   const int te = SPT * ke < T ? SPT * ke : T, end = (te + 1) & ~1;
-  const int nt_base = w.nb * (S::BN / 16);
+  const int nt_base = w.nb * (S::BN / (SWIGLU ? 32 : 16)), up = ntiles / 2;
+  // n-tile k of half h of wave column c
+  auto n_tile = [&](int c, int h, int k) -> int {
+    if constexpr (SWIGLU) {
+      return nt_base + c * NH + k + h * up;
+    } else {
+      const int nt = nt_base + c * NTW + h * NH + k;
+      return nt < ntiles ? nt : ntiles - 1;
+    }
+  };
 
   // copy sources.  A unit h: chunk c = CA wv + u holds rows 8 (c % 2) .. + 7 of the unit's
   // m-tile e = c / 2 (wave row e / MH, its m-tile h MH + e % MH); rows past M re-read the last
@@ -209,8 +222,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
 #pragma unroll
     for (int u = 0; u < S::CB; u += 2) {
       const int e = (S::CB * wv + u) >> 1;
-      int nt = nt_base + (e / NH) * NTW + h * NH + e % NH;
-      nt = nt < ntiles ? nt : ntiles - 1;
+      const int nt = n_tile(e / NH, h, e % NH);
       b_src[h][u / 2] = w.w + (int64_t)nt * KT * (CH * 1024) + (S::CB == 1 ? (wv & 1) * 1024 : 0);
     }
   const uint32_t lane16 = (uint32_t)lane * 16;
@@ -243,8 +255,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   } else {
     sa_off[0] = (uint32_t)a_row(w.row0 + 64 * swa + lane) * srow;
   }
-  int snt = nt_base + 4 * swb + (lane >> 4);
-  snt = snt < ntiles ? snt : ntiles - 1;
+  const int sc = 4 * swb + (lane >> 4), snt = n_tile(sc / NTW, sc % NTW / NH, sc % NH);
   const uint32_t sb_off = (uint32_t)snt * (uint32_t)KT * 256 + 16 * (lane & 15);
   const uint32_t lds_sa = tile_lds(lds + L::SA) + (BLOCK ? wv * S::BM * 4 : 64 * swa * 16);
   const uint32_t lds_sb = tile_lds(lds + L::SB) + 4 * swb * 256;
@@ -563,6 +574,69 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   };
   if constexpr (!BLOCK) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // the last MFMAs' results
   // lane (q, r): columns 4 q .. 4 q + 3 of row r of every 16 x 16 tile
+  if constexpr (SWIGLU) {
+    // Against a launch of its own (us, 777 tokens top 6 of 48 experts of 1280 x 1920: product and producer 24.0 + 5.2,
+    // here 22.9; 2048 top 8 of 256 of 1024 x 2048: 66 + 9.2, here 69.5).
+    // The activations of bf16 gates come from the 16 KiB table (silu_math.h), staged where the ring was (arithmetic for
+    // gates outside it): exp and a division take 30 instructions of each of a lane's values.
+    const uint16_t* const tab = reinterpret_cast<const uint16_t*>(lds + L::RING);
+    static_assert(kSiluEntries * 2 == 16 * 1024 && 2 * L::STAGE >= 16 * 1024, "four copies a wave, within the ring");
+    tile_wait<0>();
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      tile_copy16(reinterpret_cast<const uint8_t*>(kSiluAct) + (4 * wv + u) * 1024, lane16,
+                  tile_lds(lds + L::RING) + (4 * wv + u) * 1024);
+    tile_wait<0>();
+    auto pack = [](float x, float y) -> uint32_t {
+      uint32_t d = cvt_pk_bf16(x, y);
+      d = x != x ? (d & 0xFFFF0000u) | 0x7FC0u : d;
+      return y != y ? (d & 0x0000FFFFu) | 0x7FC00000u : d;
+    };
+    const int blk = w.nb * (NTW / 2) + wn, blocks = up / 2;
+#pragma unroll
+    for (int i = 0; i < MTW; ++i) {
+      uint32_t gd[4], ud[4], d[4];  // pairs: columns 4 q .. + 3 of the block's first 16, then of the others
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const v4f g = values(i, n), u = values(i, NH + n);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          gd[2 * n + e] = pack(g[2 * e], g[2 * e + 1]);
+          ud[2 * n + e] = pack(u[2 * e], u[2 * e + 1]);
+        }
+      }
+      if (__builtin_amdgcn_ballot_w64(!silu_in_table(uint4{gd[0], gd[1], gd[2], gd[3]})) == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t o = silu_offsets(gd[e]) + ((gd[e] >> 3) & 0x10001000u);
+          const float a0 = u2f((uint32_t)tab[o & 0xFFFFu] << 16), a1 = u2f((uint32_t)tab[o >> 16] << 16);
+          d[e] = cvt_pk_bf16(a0 * u2f(ud[e] << 16), a1 * u2f(ud[e] & 0xFFFF0000u));
+        }
+      } else {
+        float g[8], u[8], v[8];
+        bf16x8_to_f32(uint4{gd[0], gd[1], gd[2], gd[3]}, g);
+        bf16x8_to_f32(uint4{ud[0], ud[1], ud[2], ud[3]}, u);
+        swiglu8<kFloorCarry175>(g, u, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = cvt_pk_bf16(v[2 * e], v[2 * e + 1]);
+      }
+      uint32_t amax = amax_bf16_bits<4, false>(d);
+      amax = __builtin_elementwise_max(amax, (uint32_t)__shfl_xor((int)amax, 16, 64));
+      amax = __builtin_elementwise_max(amax, (uint32_t)__shfl_xor((int)amax, 32, 64));
+      const uint32_t s = scale_e2m1(amax, p.mid_carry), c = codes_e2m1(d, s);
+      // lanes q and q ^ 1 make eight columns of the first half and eight of the second
+      const uint32_t other = (uint32_t)__shfl_xor((int)c, 16, 64);
+      const uint32_t word = q & 1 ? other >> 16 | (c & 0xFFFF0000u) : (c & 0xFFFFu) | other << 16;
+      const int row = w.row0 + (wm * MTW + i) * 16 + r;
+      if (row < w.row_hi) {
+        const int64_t at = (int64_t)row * blocks + blk;
+        reinterpret_cast<uint32_t*>(p.mid_codes)[at * 4 + (q & 1) * 2 + (q >> 1)] = word;
+        if (q == 0) p.mid_scales[at] = (uint8_t)s;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return;
+  }
   if (w.part) {
 #pragma unroll
     for (int i = 0; i < MTW; ++i)

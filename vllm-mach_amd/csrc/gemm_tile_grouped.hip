@@ -21,8 +21,9 @@ struct GroupedDepth {
   static constexpr int value = MT == 8 ? 2 : 3;
 };
 
-template <int FMT, int MT, int NT>
-struct WideKernel<FMT, MT, NT, false, true, 1> {
+// (WM = 2: with the SwiGLU producer in the epilogue, MXFP4)
+template <int FMT, int MT, int NT, int WM>
+struct WideKernel<FMT, MT, NT, false, true, WM> {
   static __device__ __forceinline__ void run(const GemmParams& p, const WideGrid& g) {
     constexpr int BM = 16 * MT, EPT = (int)kWideGroupedMaxExperts / 256;  // experts per thread
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -103,8 +104,8 @@ struct WideKernel<FMT, MT, NT, false, true, 1> {
                        static_cast<const uint8_t*>(p.sw) + x.x * p.sw_expert_stride, nullptr};
       const int* const rows = sh_row[buf];
       auto a_row = [&](int r) -> int { return rows[r - x.y]; };
-      if (MT == 8 && x.z - x.y <= 64) tile_gemm<FMT, 2, 2 * NT, false, GroupedDepth<4>::value>(p, w, lds, a_row);
-      else tile_gemm<FMT, MT / 2, 2 * NT, false, GroupedDepth<MT>::value>(p, w, lds, a_row);
+      if (MT == 8 && x.z - x.y <= 64) tile_gemm<FMT, 2, 2 * NT, false, GroupedDepth<4>::value, WM == 2>(p, w, lds, a_row);
+      else tile_gemm<FMT, MT / 2, 2 * NT, false, GroupedDepth<MT>::value, WM == 2>(p, w, lds, a_row);
       buf ^= 1;
       if (t < BM) sh_row[buf][t] = ahead;
       x = y;
@@ -112,13 +113,13 @@ struct WideKernel<FMT, MT, NT, false, true, 1> {
   }
 };
 
-template <int FMT, int MT, int NT>
+template <int FMT, int MT, int NT, int WM = 1>
 static hipError_t launch_grouped_tile(const GemmParams& p, const WideGrid& g, int64_t grid, hipStream_t s) {
   constexpr int whole = TileLds<MT / 2, 2 * NT, false>::bytes(GroupedDepth<MT>::value);
   constexpr int half = TileLds<2, 2 * NT, false>::bytes(GroupedDepth<4>::value);
   constexpr int bytes = whole > half ? whole : half;
   static_assert(2 * (bytes + 1088) <= 160 * 1024, "two workgroups per CU");
-  hipLaunchKernelGGL((gemm_wide_kernel<FMT, MT, NT, false, true, 1>), dim3((unsigned)grid), dim3(256), bytes, s, p, g);
+  hipLaunchKernelGGL((gemm_wide_kernel<FMT, MT, NT, false, true, WM>), dim3((unsigned)grid), dim3(256), bytes, s, p, g);
   return hipGetLastError();
 }
 
@@ -137,6 +138,8 @@ hipError_t launch_wide_grouped(int fmt, const WideConfig& c, const GemmParams& p
   if (fmt == kE4M3) return launch_grouped_fmt<kE4M3>(c, p, g, grid, s);
   if (fmt == kE2M3) return launch_grouped_fmt<kE2M3>(c, p, g, grid, s);
   if (fmt == kE3M2) return launch_grouped_fmt<kE3M2>(c, p, g, grid, s);
+  if (fmt == kE2M1 && p.mid_codes)
+    return c.NT == 2 && c.MT == 8 ? launch_grouped_tile<kE2M1, 8, 2, 2>(p, g, grid, s) : hipErrorInvalidValue;
   if (fmt == kE2M1) return launch_grouped_fmt<kE2M1>(c, p, g, grid, s);
   return hipErrorInvalidValue;
 }
