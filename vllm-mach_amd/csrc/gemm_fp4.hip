@@ -54,25 +54,48 @@ __global__ __launch_bounds__(64 * kFp4StreamWaves) void fp4_stream_kernel(GemmPa
   const int ntiles = (int)((p.N + 15) / 16);
   int64_t lo = 0, hi = p.M;
   int e = blockIdx.y;
+  auto within = [&](int64_t row) -> int { return row < 0 ? 0 : row < p.M ? (int)row : (int)p.M; };
   if (g.E) {
-    if (g.by_rank) {  // the blockIdx.y-th expert with rows
+    if (g.by_rank) {  // the blockIdx.y-th expert with rows: four experts a lane, whose offsets load together
       int left = blockIdx.y, found = -1;
-      for (int e0 = 0; e0 < g.E && found < 0; e0 += 64) {
-        const int x = e0 + lane;
-        const uint64_t some = __ballot(x < g.E && p.expert_offsets[x + 1 < g.E ? x + 1 : g.E] > p.expert_offsets[x < g.E ? x : g.E]);
-        const int n = __popcll(some);
+      for (int e0 = 0; e0 < g.E && found < 0; e0 += 256) {
+        const int x = e0 + 4 * lane;
+        int64_t off[5];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) off[j] = p.expert_offsets[x + j < g.E ? x + j : g.E];
+        uint32_t some = 0;
+        int before = 0, n = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool is = off[j + 1] > off[j];
+          const uint64_t all = __ballot(is);
+          some |= is ? 1u << j : 0u;
+          before += __popcll(all & ((1ull << lane) - 1));
+          n += __popcll(all);
+        }
         if (left < n) {
-          uint64_t m = some;
-          for (int i = 0; i < left; ++i) m &= m - 1;
-          found = e0 + __builtin_ctzll(m);
+          int k = left - before;
+          const int who = __builtin_ctzll(__ballot(k >= 0 && k < __popc(some)));
+          for (; k > 0 && some; --k) some &= some - 1;
+          const int j = __builtin_ctz(some | 8u);
+          int64_t first = off[0], end = off[1];
+#pragma unroll
+          for (int i = 1; i < 4; ++i) {
+            first = j == i ? off[i] : first;
+            end = j == i ? off[i + 1] : end;
+          }
+          found = __builtin_amdgcn_readlane(x + j, who);
+          lo = __builtin_amdgcn_readlane(within(first), who);
+          hi = __builtin_amdgcn_readlane(within(end), who);
         }
         left -= n;
       }
       if (found < 0) return;
       e = found;
+    } else {
+      lo = within(p.expert_offsets[e]);
+      hi = within(p.expert_offsets[e + 1]);
     }
-    lo = p.expert_offsets[e] > 0 ? p.expert_offsets[e] : 0;
-    hi = p.expert_offsets[e + 1] < p.M ? p.expert_offsets[e + 1] : p.M;
     if (lo >= hi) return;
   }
   // n-tile: SWIGLU's second half of the waves holds up
