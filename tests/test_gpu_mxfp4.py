@@ -137,7 +137,8 @@ def test_gemm(pkg, dev, m, n, k):
     ref.check_product(y, ref.dequantize(a, sa), wv)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 64, 256), (5, 100, 640), (48, 1030, 512), (300, 520, 1152), (700, 2048, 512)])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 256), (5, 100, 640), (48, 1030, 512), (300, 520, 1152), (700, 2048, 512),
+                                   (40, 100, 640), (200, 1028, 1152), (1000, 36, 384), (33, 24, 128)])
 def test_gemm_bias(pkg, dev, m, n, k):
     g = torch.Generator().manual_seed(m + n + k)
     (w, sw), wv = _weight(pkg, g, n, k)
@@ -563,3 +564,67 @@ def test_two_streams_at_once(pkg, dev):
     torch.cuda.synchronize()
     for j in range(2):
         assert all(torch.equal(y, want[j]) for y in got[j])
+
+
+def test_graphs_of_one_layer_replayed_together(pkg, dev):
+    """Graphs of the same layers captured on two streams share no scratch: replayed at once, again and again, with
+    eager work between, each gives its own input's result."""
+    g = torch.Generator().manual_seed(3)
+    e, h, i, topk = 12, 640, 256, 3
+    experts, w1, w2, _, _ = _experts(pkg, g, e, h, i)
+    codes, scales = ref.random_operand(g, 520, h)
+    method, layer = _layer(pkg, codes, scales - 6)
+    sets = []
+    for t in (400, 9, 150):
+        x, z = _x(g, t, h).to(dev), torch.randn(t, e, generator=g).to(dev)
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+        def run(x=x, z=z):
+            w, ids, routes, offsets, inverse = pkg.ops.moe_router_grouped(z, None, topk, pkg.ops.SIGMOID, 4, 2, True, 1.5)
+            return method.apply(layer, x), experts(x, w1, w2, w, ids)
+
+        want = [v.clone() for v in run()]
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            run()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            out = run()
+        sets.append((stream, graph, out, want, run))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for _, _, out, _, _ in sets:
+            for v in out:
+                v.zero_()
+        torch.cuda.synchronize()
+        for stream, graph, _, _, _ in sets:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = sets[1][4]()
+        torch.cuda.synchronize()
+        for _, _, out, want, _ in sets:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert all(torch.equal(a, b) for a, b in zip(eager, sets[1][3]))
+
+
+def test_warmup_runs_the_layers(pkg, dev):
+    """``warmup`` finds prepared MXFP4 layers and experts and runs each; they keep no workspace to reserve."""
+    g = torch.Generator().manual_seed(4)
+    codes, scales = ref.random_operand(g, 264, 384)
+    _, layer = _layer(pkg, codes, scales)
+    c1, s1 = ref.random_operand(g, 4 * 256, 256)
+    c2, s2 = ref.random_operand(g, 4 * 256, 128)
+    method, moe = pkg.Mxfp4MoEMethod(), torch.nn.Module()
+    method.create_weights(moe, 4, 256, 128, torch.bfloat16)
+    for name, v in (("w13_weight", c1.view(4, 256, -1)), ("w13_weight_scale", s1.view(4, 256, -1)),
+                    ("w2_weight", c2.view(4, 256, -1)), ("w2_weight_scale", s2.view(4, 256, -1))):
+        getattr(moe, name).data = v.to(dev)
+    method.process_weights_after_loading(moe)
+    before = pkg.ops.inspect()
+    done = pkg.warmup.warmup([layer, moe], (1, 16, 200))
+    assert [k[0] for k in done["dense"]] == ["Mxfp4LinearKernel"] and len(done["moe"]) == 1
+    assert {1, 16, 64, 128, 200} == set(done["sizes"])
+    after = pkg.ops.inspect()
+    for op in ("mxfp4_linear", "mxfp4_experts"):
+        assert after["counts"][op] - before["counts"].get(op, 0) == 5
+    assert after["workspaces"] == before["workspaces"]

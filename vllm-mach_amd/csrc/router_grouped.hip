@@ -434,13 +434,20 @@ __global__ __launch_bounds__(kChunk) void router_grouped_single_kernel(GroupedRo
   single_chunk_sort(t < R ? sids[t] : -1, R, g.E, offsets, sorted_routes, inverse, whist, tot);
 }
 
-// The routing launch: routing alone, or (offsets set) with the sort.
+// The routing launch, with the sort (offsets set, and a lane's experts few enough for the registers of a workgroup of
+// 1024) or alone; whether it sorted.
 template <bool BF16, int LPT, int NS>
-static void launch_grouped(const GroupedRouting& g, int64_t* offsets, int32_t* sorted_routes, int32_t* inverse,
+static bool launch_grouped(const GroupedRouting& g, int64_t* offsets, int32_t* sorted_routes, int32_t* inverse,
                            hipStream_t s) {
   constexpr int kTokens = 256 / LPT;
-  if (offsets) router_grouped_single_kernel<BF16, LPT, NS><<<1, kChunk, 0, s>>>(g, offsets, sorted_routes, inverse);
-  else router_grouped_kernel<BF16, LPT, NS><<<dim3((unsigned)((g.T + kTokens - 1) / kTokens)), 256, 0, s>>>(g);
+  if constexpr (NS <= 16) {
+    if (offsets) {
+      router_grouped_single_kernel<BF16, LPT, NS><<<1, kChunk, 0, s>>>(g, offsets, sorted_routes, inverse);
+      return true;
+    }
+  }
+  router_grouped_kernel<BF16, LPT, NS><<<dim3((unsigned)((g.T + kTokens - 1) / kTokens)), 256, 0, s>>>(g);
+  return false;
 }
 // The lanes of a group and the experts of a lane, of LPT lanes for a token.
 static GroupedRouting::Deal deal_groups(const GroupedRouting& g, int LPT) {
@@ -450,7 +457,7 @@ static GroupedRouting::Deal deal_groups(const GroupedRouting& g, int LPT) {
   return d;
 }
 template <bool BF16>
-static void launch_grouped_slots(GroupedRouting& g, int64_t* offsets, int32_t* sorted_routes, int32_t* inverse,
+static bool launch_grouped_slots(GroupedRouting& g, int64_t* offsets, int32_t* sorted_routes, int32_t* inverse,
                                  hipStream_t s) {
   g.deal = deal_groups(g, 16);
   g.deal64 = deal_groups(g, 64);
@@ -459,15 +466,14 @@ static void launch_grouped_slots(GroupedRouting& g, int64_t* offsets, int32_t* s
   // 37.6 to 29.7 at 16384; 9.3 to 9.0 at 8, 10.6 to 9.3 at 16, which share a CU; 64 experts 10.4 to 9.6 at 512).
   const bool few = g.deal.per > 4 && g.T <= (offsets ? 8 : 2048);
   if (!few && g.topk <= 16 && g.groups <= 16 && g.deal.per <= 16) {  // (then four experts a lane of 64 at most)
-    if (g.deal.per <= 4) launch_grouped<BF16, 16, 4>(g, offsets, sorted_routes, inverse, s);
-    else if (g.deal.per <= 8) launch_grouped<BF16, 16, 8>(g, offsets, sorted_routes, inverse, s);
-    else launch_grouped<BF16, 16, 16>(g, offsets, sorted_routes, inverse, s);
-    return;
+    if (g.deal.per <= 4) return launch_grouped<BF16, 16, 4>(g, offsets, sorted_routes, inverse, s);
+    if (g.deal.per <= 8) return launch_grouped<BF16, 16, 8>(g, offsets, sorted_routes, inverse, s);
+    return launch_grouped<BF16, 16, 16>(g, offsets, sorted_routes, inverse, s);
   }
   g.deal = g.deal64;
-  if (g.deal.per <= 4) launch_grouped<BF16, 64, 4>(g, offsets, sorted_routes, inverse, s);
-  else if (g.deal.per <= 8) launch_grouped<BF16, 64, 8>(g, offsets, sorted_routes, inverse, s);
-  else launch_grouped<BF16, 64, 32>(g, offsets, sorted_routes, inverse, s);
+  if (g.deal.per <= 4) return launch_grouped<BF16, 64, 4>(g, offsets, sorted_routes, inverse, s);
+  if (g.deal.per <= 8) return launch_grouped<BF16, 64, 8>(g, offsets, sorted_routes, inverse, s);
+  return launch_grouped<BF16, 64, 32>(g, offsets, sorted_routes, inverse, s);
 }
 
 }  // namespace mxl
@@ -506,11 +512,11 @@ extern "C" int mxl_moe_router_grouped(const void* logits, int logits_bf16, const
                      renormalize != 0, 0, {}, {}, (double)factor, topk_weights, topk_ids};
     const uintptr_t logits_at = (uintptr_t)logits, bias_at = (uintptr_t)bias;
     g.quads = g.size % 4 == 0 && logits_at % (logits_bf16 ? 8 : 16) == 0 && bias_at % 16 == 0;
-    const bool single = T <= kGroupedSingleTokens && T * topk <= kChunk;
-    if (logits_bf16) launch_grouped_slots<true>(g, single ? expert_offsets : nullptr, sorted_routes, inverse, s);
-    else launch_grouped_slots<false>(g, single ? expert_offsets : nullptr, sorted_routes, inverse, s);
+    int64_t* const offsets = T <= kGroupedSingleTokens && T * topk <= kChunk ? expert_offsets : nullptr;
+    const bool sorted = logits_bf16 ? launch_grouped_slots<true>(g, offsets, sorted_routes, inverse, s)
+                                    : launch_grouped_slots<false>(g, offsets, sorted_routes, inverse, s);
     MXL_CHECK_LAUNCH(who);
-    if (single) return MXL_OK;
+    if (sorted) return MXL_OK;
   }
   return mxl_moe_route(topk_ids, T, topk, E, sorted_routes, expert_offsets, inverse, workspace, workspace_bytes, stream);
 }

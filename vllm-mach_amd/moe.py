@@ -223,7 +223,8 @@ class Mxfp4Experts(_Experts):
 
     Checkpoint layout (Quark OCP-MX): w13 u8 [E, 2I, H/2] + E8M0 [E, 2I, H/32] (gate rows [0, I), up
     rows [I, 2I)); w2 u8 [E, H, I/2] + E8M0 [E, H, I/32].  With few rows an expert the layer is four
-    launches: route, w13 with the quantization ahead of it and the SwiGLU producer behind it, w2, combine.
+    launches: route, w13 with the quantization ahead of it and the SwiGLU producer behind it, w2, combine;
+    with many the quantization is one of its own.
     """
 
     name = "MXFP4"
@@ -233,7 +234,7 @@ class Mxfp4Experts(_Experts):
         if rule not in (ops.FLOOR_CARRY175, ops.FLOOR_OCP):
             raise ValueError(f"unknown MXFP4 scale rule {rule}")
         self.rule = rule
-        self.fuse = True  # the first half in one launch where it runs (False: separate launches)
+        self.fuse = True  # producers in the gate/up product's launch where it takes them (False: separate launches)
         self.w1_scale: Optional[torch.Tensor] = None
         self.w2_scale: Optional[torch.Tensor] = None
 

@@ -1057,10 +1057,11 @@ def mxfp4_experts(output: torch.Tensor, x: torch.Tensor, topk_ids: Optional[torc
                   sorted_routes: Optional[torch.Tensor], expert_offsets: Optional[torch.Tensor],
                   inverse: Optional[torch.Tensor], w13: torch.Tensor, sw13: torch.Tensor, w2: torch.Tensor,
                   sw2: torch.Tensor, e: int, i: int, rule: int = FLOOR_CARRY175, fuse: bool = True) -> None:
-    """A layer of MXFP4 experts on bf16 x [T, H], into ``output`` (contiguous bf16 [T, H]): the routes of ``topk_ids`` i32 [T, k] sorted (``moe_route``; or
-    given sorted, as ``moe_route`` and the routers return them), the gate/up product of the quantized rows with
-    w13 [e, 2 i, H], ``swiglu_mxfp4``, the product with w2 [e, H, i] and ``moe_reduce`` with the fp32 weights
-    [T, k].  ``fuse``: the first half as ``mxfp4_grouped_swiglu`` where that runs."""
+    """A layer of MXFP4 experts on bf16 x [T, H], into ``output`` (contiguous bf16 [T, H]): the routes of ``topk_ids``
+    i32 [T, k] sorted (``moe_route``; or given sorted, as ``moe_route`` and the routers return them), the gate/up
+    product of the quantized rows with w13 [e, 2 i, H], ``swiglu_mxfp4``, the product with w2 [e, H, i] and
+    ``moe_reduce`` with the fp32 weights [T, k].  ``fuse``: the SwiGLU producer in the gate/up product's launch, with
+    few rows an expert the quantization too (the same bits as separate launches)."""
     _same_device("mxfp4_experts", x, output, topk_ids, topk_weights, sorted_routes, expert_offsets, inverse, w13, sw13, w2, sw2)
     if x.dtype != torch.bfloat16 or x.ndim != 2:
         raise ValueError("mxfp4_experts needs bf16 x [T, H]")

@@ -12,7 +12,7 @@ runs each distinct problem at each size (zeros in, no host sync per call) and le
 current stream's workspaces at the planned maxima; ``warmup(model, sizes, stream=True)``
 gives the current (capture) stream workspaces of the planned sizes without running
 anything.  Layers are found by what ``process_weights_after_loading`` left on them:
-``mxl_kernel`` (dense kernels of ``linear``) and ``mxl_experts`` (``moe.Mxfp6MoEMethod``).
+``mxl_kernel`` (dense kernels of ``linear``) and ``mxl_experts`` (``moe.Mxfp6MoEMethod``, ``moe.Mxfp4MoEMethod``).
 """
 from __future__ import annotations
 
