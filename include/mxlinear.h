@@ -124,8 +124,8 @@ int mxl_mxfp4_linear(const void* x, int64_t M, int64_t K, int64_t ldx, int swigl
  * quantized rows of x [T, H] (row stride ldx) with w13 [E][2I, H], SwiGLU -> MXFP4, the
  * product with w2 [E][H, I], and the combine with fp32 topk_weights [T, topk] into out bf16
  * [T, H].  fuse: the SwiGLU producer in the gate/up product's launch, with few rows an expert
- * the quantization too (mxl_mxfp4_grouped_swiglu; four launches from the ids, else five):
- * the bits are those of separate launches.
+ * the quantization too (mxl_mxfp4_grouped_swiglu; four launches from the ids, without the
+ * sort three up to 32 routes, else five): the bits are those of separate launches.
  * H, I multiples of 128; the workspace, 256-byte aligned, holds
  * mxl_mxfp4_experts_workspace_bytes (sorted: the routes are given). */
 int64_t mxl_mxfp4_experts_workspace_bytes(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int sorted,

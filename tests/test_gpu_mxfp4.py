@@ -484,6 +484,35 @@ def test_swiglu_in_the_tiles_is_the_separate_launches(pkg, dev, t, e, topk, h, i
     assert bool(one[6].isnan().all()) and not bool(one[10].isnan().any())
 
 
+@pytest.mark.parametrize("t,e,topk,h,i", [(1, 256, 8, 2048, 512), (2, 6, 2, 128, 128), (4, 4, 4, 640, 384),
+                                          (16, 8, 1, 256, 128), (5, 300, 3, 1152, 256), (32, 9, 1, 384, 256),
+                                          (1, 1, 1, 128, 128)])
+def test_few_routes_unsorted(pkg, dev, t, e, topk, h, i):
+    """Up to 32 routes run as they come: the bits of the sorted launches, with an expert twice in a token, ids of no
+    expert, a token with nothing but those, strided rows and a NaN row."""
+    g = torch.Generator().manual_seed(t + e)
+    experts, w1, w2, v1, v2 = _experts(pkg, g, e, h, i)
+    wide = _x(g, t, 2 * h).to(dev)
+    x, p = wide[:, 8:8 + h], torch.rand(t, topk, generator=g).to(dev)
+    ids = torch.randint(0, e, (t, topk), generator=g).int()
+    if t > 3:
+        ids[0] = -1
+        ids[1, 0] = e
+        ids[2] = ids[2, 0]
+        wide[3, 10] = math.nan
+    ids = ids.to(dev)
+    got = experts(x, w1, w2, p, ids)
+    experts.fuse = False
+    want = experts(x, w1, w2, p, ids)
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+    if t > 3:
+        assert bool((got[0] == 0).all())
+        assert bool(got[3].isnan().all()) == bool(((ids[3] >= 0) & (ids[3] < e)).any())
+    if t < 4:
+        exact = _exact_layer(x.cpu(), p.cpu(), ids.cpu(), v1, v2)
+        assert float((got.cpu().double() - exact).norm() / exact.norm()) <= 2 * 2.0 ** -8 + 2.0 ** -10 * 3
+
+
 def test_experts_map_and_method(pkg, dev):
     """An expert map drops the experts of other ranks; the method object runs the same layer."""
     g = torch.Generator().manual_seed(9)

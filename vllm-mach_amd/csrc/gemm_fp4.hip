@@ -33,9 +33,14 @@ __device__ __forceinline__ v4f mfma_fp4(const uint4& w, const uint4& a, v4f c, u
 // weights are read once whatever its rows.  SWIGLU (an expert's gate/up product): the workgroup's n-tiles are two
 // of gate and the same two of up, and the epilogue quantizes the 32 columns' bf16(bf16(silu(g)) u) in place of
 // storing gate and up.
+int moe_reduce_by_route(const char* who, const void* routed_output, const float* topk_weights, const int32_t* topk_ids,
+                        int64_t T, int64_t topk, int64_t E, int64_t H, void* out, void* stream);  // (moe.hip)
+
+// kRoutes: a few routes as they come, their experts in row_index and route r's activation row r / row_div: no sort.
+enum Fp4Unit : int { kExperts = 0, kHitExperts = 1, kRoutes = 2 };
 struct Fp4Stream {
   int WN, WK;
-  int E, by_rank;         // grouped: experts (0: dense); blockIdx.y counts the experts with rows
+  int E, unit;            // grouped: experts (0: dense), and what blockIdx.y counts (Fp4Unit)
   const uint16_t* x;      // PROD 1: bf16 rows, stride ldx
   int64_t ldx;
   uint32_t carry;         // the scale rule of PROD 1 and SWIGLU
@@ -56,7 +61,12 @@ __global__ __launch_bounds__(64 * kFp4StreamWaves) void fp4_stream_kernel(GemmPa
   int e = blockIdx.y;
   auto within = [&](int64_t row) -> int { return row < 0 ? 0 : row < p.M ? (int)row : (int)p.M; };
   if (g.E) {
-    if (g.by_rank) {  // the blockIdx.y-th expert with rows: four experts a lane, whose offsets load together
+    if (g.unit == kRoutes) {
+      e = p.row_index[blockIdx.y];
+      if (e < 0 || e >= g.E) return;
+      lo = blockIdx.y;
+      hi = lo + 1;
+    } else if (g.unit == kHitExperts) {  // the blockIdx.y-th expert with rows: four experts a lane, whose offsets load together
       int left = blockIdx.y, found = -1;
       for (int e0 = 0; e0 < g.E && found < 0; e0 += 256) {
         const int x = e0 + 4 * lane;
@@ -140,7 +150,7 @@ __global__ __launch_bounds__(64 * kFp4StreamWaves) void fp4_stream_kernel(GemmPa
         rr[u] = at - b[u] * rows;
         int ar = (int)row0 + rr[u];  // (32-bit offsets: the host bounds the operands below 4 GiB)
         if (g.E) {
-          if (p.row_index) ar = p.row_index[ar] / p.row_div;
+          if (p.row_index) ar = (g.unit == kRoutes ? ar : p.row_index[ar]) / p.row_div;
           ar = ar < 0 ? 0 : ar < (int)p.a_rows ? ar : (int)p.a_rows - 1;
         }
         if constexpr (PROD == 0) {
@@ -539,7 +549,7 @@ extern "C" int mxl_mxfp4_grouped_swiglu(const void* x, int64_t a_rows, int64_t l
   p.sw_expert_stride = mxl_tiled_scale_bytes(2 * I, K);
   Fp4Stream g{};
   g.E = (int)num_experts;
-  g.by_rank = routed_rows < num_experts;
+  g.unit = routed_rows < num_experts ? kHitExperts : kExperts;
   g.x = (const uint16_t*)x;
   g.ldx = ldx;
   g.carry = fp4_carry(rule);
@@ -565,7 +575,7 @@ extern "C" int mxl_mxfp4_grouped_gemm(const void* a, const void* sa, int64_t a_r
   if (fp4_grouped_streams(routed_rows, num_experts, N, K, false, pl)) {
     Fp4Stream g{};
     g.E = (int)num_experts;
-    g.by_rank = routed_rows < num_experts;
+    g.unit = routed_rows < num_experts ? kHitExperts : kExperts;
     return launch_status(launch_fp4_stream<0, false>(pl, p, g, std::min(routed_rows, num_experts), (hipStream_t)stream), who);
   }
   if (num_experts <= kWideGroupedMaxExperts && fp4_tiles_eligible(std::max(a_rows, routed_rows), N, K)) {
@@ -578,6 +588,47 @@ extern "C" int mxl_mxfp4_grouped_gemm(const void* a, const void* sa, int64_t a_r
   fp4_grouped_kernel<<<dim3((unsigned)((N + 63) / 64), (unsigned)num_experts), 256, 0, (hipStream_t)stream>>>(p);
   MXL_CHECK_LAUNCH(who);
   return MXL_OK;
+}
+
+// Routes that an experts call of few tokens runs unsorted, each a unit of its own: the sort's launch costs
+// more than weights that some share, which come from L2 the second time (256 experts, top 8, K = 2048, I = 512, graph-
+// timed, us, unsorted | sorted: one token 14.5 | 18.9, four 21.4 | 26.2, four of the same experts 16.9 | 19.4, eight of
+// the same 23.0 | 20.0).
+constexpr int64_t kFp4DirectRoutes = 32;
+static bool fp4_direct(int64_t routes, int64_t E, int64_t H, int64_t I) {
+  Fp4StreamPlan pl;
+  return routes <= kFp4DirectRoutes && E <= 0x7FFFFFFF && fp4_grouped_streams(routes, E, 2 * I, H, true, pl) &&
+         fp4_grouped_streams(routes, E, H, I, false, pl);
+}
+
+// Both products of the unsorted routes: x bf16 [T, H] through w13 and the SwiGLU producer to codes and scales [routes,
+// I], then through w2 to y [routes, H].
+static hipError_t fp4_direct_launch(const void* x, int64_t T, int64_t ldx, const int32_t* ids, int64_t topk, int64_t E,
+                                    int64_t H, int64_t I, const void* w13, const void* sw13, const void* w2,
+                                    const void* sw2, int rule, void* codes, void* scales, void* y, hipStream_t s) {
+  const int64_t routes = T * topk;
+  Fp4StreamPlan pl;
+  Fp4Stream g{};
+  g.E = (int)E;
+  g.unit = kRoutes;
+  GemmParams p = fp4_params(nullptr, nullptr, w13, sw13, 2 * I, H, nullptr, 2 * I);
+  p.M = routes; p.a_rows = T; p.row_index = ids; p.row_div = (int)topk;
+  p.w_expert_stride = mxl_tiled_weight_bytes(2 * I, H, kE2M1);
+  p.sw_expert_stride = mxl_tiled_scale_bytes(2 * I, H);
+  g.x = (const uint16_t*)x;
+  g.ldx = ldx;
+  g.carry = fp4_carry(rule);
+  g.codes = (uint8_t*)codes;
+  g.scales = (uint8_t*)scales;
+  if (!fp4_stream_plan(2 * I, H, routes, true, pl)) return hipErrorInvalidValue;
+  const hipError_t e = launch_fp4_stream<1, true>(pl, p, g, routes, s);
+  if (e != hipSuccess) return e;
+  GemmParams q = fp4_params(codes, scales, w2, sw2, H, I, y, H);
+  q.M = q.a_rows = routes; q.row_index = ids; q.row_div = 1;
+  q.w_expert_stride = mxl_tiled_weight_bytes(H, I, kE2M1);
+  q.sw_expert_stride = mxl_tiled_scale_bytes(H, I);
+  if (!fp4_stream_plan(H, I, routes, false, pl)) return hipErrorInvalidValue;
+  return launch_fp4_stream<0, false>(pl, q, g, routes, s);
 }
 
 // Whether the gate/up product of an experts call (I % 128 == 0) runs in the tiles, whose epilogue then is the SwiGLU
@@ -650,6 +701,7 @@ LinearScratch linear_scratch(uint8_t* base, int64_t M, int64_t N, int64_t K) {
 struct ExpertScratch {
   void *routes, *offsets, *inverse, *sort, *codes, *scales, *gate_up, *codes2, *scales2, *y;
   int64_t sort_bytes, bytes;
+  bool direct;        // the routes unsorted
   bool fused, tiles;  // the SwiGLU producer in the gate/up product's launch: with the quantizer, or behind it
 };
 ExpertScratch expert_scratch(uint8_t* base, int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, bool sorted,
@@ -657,6 +709,8 @@ ExpertScratch expert_scratch(uint8_t* base, int64_t T, int64_t topk, int64_t E, 
   const int64_t R = T * topk;
   Pieces p{base};
   ExpertScratch x{};
+  x.direct = fuse && !sorted && fp4_direct(R, E, H, I);
+  sorted |= x.direct;  // (no sort)
   x.sort_bytes = sorted ? 0 : mxl_moe_route_workspace_bytes(T, topk, E);
   x.fused = fuse && mxl_mxfp4_grouped_swiglu_supported(R, E, I, H);
   x.tiles = fuse && !x.fused && fp4_swiglu_tiles(T, R, E, I, H);
@@ -730,6 +784,16 @@ extern "C" int mxl_mxfp4_experts(const void* x, int64_t T, int64_t ldx, const in
                 (long long)workspace_bytes);
   ExpertScratch s = expert_scratch((uint8_t*)workspace, T, topk, E, H, I, sorted, fuse != 0);
   int st = MXL_OK;
+  if (s.direct) {
+    MXL_CHECK_ARG(ldx >= H && ldx % 8 == 0 && fp4_rule(rule) && (((uintptr_t)x | (uintptr_t)w13 | (uintptr_t)w2) & 15) == 0 &&
+                      (((uintptr_t)sw13 | (uintptr_t)sw2) & 3) == 0 && H <= kFp4MaxK && I <= kFp4MaxK,
+                  "%s: bad stride, rule, alignment or size (ldx=%lld rule=%d H=%lld I=%lld)", who, (long long)ldx, rule,
+                  (long long)H, (long long)I);
+    MXL_CHECK_ARG(T < (int64_t(1) << 31) / ldx, "%s: the rows span more than 4 GiB", who);
+    st = launch_status(fp4_direct_launch(x, T, ldx, topk_ids, topk, E, H, I, w13, sw13, w2, sw2, rule, s.codes2, s.scales2,
+                                         s.y, (hipStream_t)stream), who);
+    return st != MXL_OK ? st : moe_reduce_by_route(who, s.y, topk_weights, topk_ids, T, topk, E, H, out, stream);
+  }
   if (!sorted) {
     st = mxl_moe_route(topk_ids, T, topk, E, (int32_t*)s.routes, (int64_t*)s.offsets, (int32_t*)s.inverse, s.sort,
                        s.sort_bytes, stream);

@@ -387,10 +387,12 @@ __global__ __launch_bounds__(256) void router_kernel(const void* __restrict__ lo
 
 // One thread: 8 consecutive hidden columns of one token, its routes four at a time, whose places, then rows, load
 // together (64 tokens of 8 routes, H = 2048: 4.0 us, 6.2 route after route; one token 2.9, 4.1; 777 of 6, H = 1920, 5.4, 6.6).
+// ids (or null): the rows lie in the order of their routes, and count where the id is one of the E experts
 // addend (bf16 [T, H] or null): added to the fp32 sum after the routes, before the one rounding
 __global__ __launch_bounds__(256) void moe_reduce_kernel(const uint16_t* __restrict__ y,
                                                          const float* __restrict__ topk_weights,
-                                                         const int32_t* __restrict__ inverse, int64_t T, int topk,
+                                                         const int32_t* __restrict__ inverse,
+                                                         const int32_t* __restrict__ ids, int E, int64_t T, int topk,
                                                          int64_t H, const uint16_t* __restrict__ addend,
                                                          uint16_t* __restrict__ out) {
   const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -408,7 +410,9 @@ __global__ __launch_bounds__(256) void moe_reduce_kernel(const uint16_t* __restr
 #pragma unroll
     for (int b = 0; b < B; ++b) {
       const int64_t at = t * topk + (k0 + b < topk ? k0 + b : topk - 1);
-      p[b] = k0 + b < topk ? inverse[at] : -1;
+      p[b] = (ids ? ids : inverse)[at];
+      if (ids) p[b] = p[b] >= 0 && p[b] < E ? (int32_t)at : -1;
+      p[b] = k0 + b < topk ? p[b] : -1;
       wk[b] = topk_weights[at];
     }
 #pragma unroll
@@ -541,8 +545,8 @@ extern "C" int mxl_moe_router(const void* logits, int logits_bf16, int64_t T, in
 }
 
 static int moe_reduce_common(const char* who, const void* routed_output, const float* topk_weights,
-                             const int32_t* inverse, int64_t T, int64_t topk, int64_t H, const void* addend, void* out,
-                             void* stream) {
+                             const int32_t* inverse, const int32_t* ids, int64_t E, int64_t T, int64_t topk, int64_t H,
+                             const void* addend, void* out, void* stream) {
   MXL_CHECK_ARG(T >= 0 && topk > 0 && H > 0 && H % 8 == 0, "%s: need H %% 8 == 0 (H=%lld)", who, (long long)H);
   MXL_CHECK_ARG(((uintptr_t)routed_output & 15) == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)addend & 15) == 0,
                 "%s: misaligned", who);
@@ -551,20 +555,30 @@ static int moe_reduce_common(const char* who, const void* routed_output, const f
   // (few rows: single wavefronts, over more CUs)
   const int threads = n < 256 * (int64_t)cu_count() ? 64 : 256;
   moe_reduce_kernel<<<dim3((unsigned)((n + threads - 1) / threads)), threads, 0, (hipStream_t)stream>>>(
-      (const uint16_t*)routed_output, topk_weights, inverse, T, (int)topk, H, (const uint16_t*)addend,
+      (const uint16_t*)routed_output, topk_weights, inverse, ids, (int)E, T, (int)topk, H, (const uint16_t*)addend,
       (uint16_t*)out);
   MXL_CHECK_LAUNCH(who);
   return MXL_OK;
 }
 
+// mxl_moe_reduce of routed rows in the order of their routes (row t topk + k) instead of sorted by expert: those whose
+// id is one of the E experts.
+namespace mxl {
+int moe_reduce_by_route(const char* who, const void* routed_output, const float* topk_weights, const int32_t* topk_ids,
+                        int64_t T, int64_t topk, int64_t E, int64_t H, void* out, void* stream) {
+  return moe_reduce_common(who, routed_output, topk_weights, nullptr, topk_ids, E, T, topk, H, nullptr, out, stream);
+}
+}  // namespace mxl
+
 extern "C" int mxl_moe_reduce(const void* routed_output, const float* topk_weights, const int32_t* inverse, int64_t T,
                               int64_t topk, int64_t H, void* out, void* stream) {
-  return moe_reduce_common("mxl_moe_reduce", routed_output, topk_weights, inverse, T, topk, H, nullptr, out, stream);
+  return moe_reduce_common("mxl_moe_reduce", routed_output, topk_weights, inverse, nullptr, 0, T, topk, H, nullptr, out,
+                           stream);
 }
 
 extern "C" int mxl_moe_reduce_add(const void* routed_output, const float* topk_weights, const int32_t* inverse,
                                   int64_t T, int64_t topk, int64_t H, const void* addend, void* out, void* stream) {
   MXL_CHECK_ARG(addend != nullptr, "mxl_moe_reduce_add: no addend");
-  return moe_reduce_common("mxl_moe_reduce_add", routed_output, topk_weights, inverse, T, topk, H, addend, out,
-                           stream);
+  return moe_reduce_common("mxl_moe_reduce_add", routed_output, topk_weights, inverse, nullptr, 0, T, topk, H, addend,
+                           out, stream);
 }

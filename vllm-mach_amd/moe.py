@@ -224,7 +224,7 @@ class Mxfp4Experts(_Experts):
     Checkpoint layout (Quark OCP-MX): w13 u8 [E, 2I, H/2] + E8M0 [E, 2I, H/32] (gate rows [0, I), up
     rows [I, 2I)); w2 u8 [E, H, I/2] + E8M0 [E, H, I/32].  With few rows an expert the layer is four
     launches: route, w13 with the quantization ahead of it and the SwiGLU producer behind it, w2, combine;
-    with many the quantization is one of its own.
+    up to 32 routes run unsorted, and with many rows the quantization is a launch of its own.
     """
 
     name = "MXFP4"
