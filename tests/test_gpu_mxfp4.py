@@ -657,3 +657,17 @@ def test_warmup_runs_the_layers(pkg, dev):
     for op in ("mxfp4_linear", "mxfp4_experts"):
         assert after["counts"][op] - before["counts"].get(op, 0) == 5
     assert after["workspaces"] == before["workspaces"]
+
+
+def test_gemm_of_codes_past_4_gib(pkg, dev):
+    """Rows whose codes pass 32-bit offsets: those around the border and the last against the 64-bit product."""
+    g = torch.Generator().manual_seed(6)
+    m, n, k = (1 << 20) + 777, 40, 8192
+    (w, sw), wv = _weight(pkg, g, n, k)
+    border = (1 << 32) // (k // 2)
+    rows = torch.cat([torch.arange(40), torch.arange(border - 300, border + 300), torch.arange(m - 40, m)])
+    codes, scales = ref.random_operand(g, len(rows), k)
+    a, sa = torch.zeros(m, k // 2, dtype=torch.uint8, device=dev), torch.full((m, k // 32), 127, dtype=torch.uint8, device=dev)
+    a[rows.to(dev)], sa[rows.to(dev)] = codes.to(dev), scales.to(dev)
+    y = pkg.ops.mxfp4_gemm(a, sa, w, sw, n, k)
+    ref.check_product(y[rows.to(dev)], ref.dequantize(codes, scales), wv)

@@ -160,3 +160,29 @@ def test_mxfp6_experts_take_the_routing(pkg, dev):
     experts.apply_router(out, x, w1, w2, z, 3, True, pkg.GroupedRouting("sigmoid", bias, 4, 2, 2.5))
     p, ids = pkg.grouped_topk(z, 3, True, 4, 2, "sigmoid", bias, 2.5)
     assert torch.equal(out, experts(x, w1, w2, p, ids))
+
+
+@pytest.mark.parametrize("T,E,groups", [(20, 256, 8), (3000, 64, 4), (7, 512, 1)])
+def test_operands_off_their_alignment(pkg, dev, T, E, groups):
+    """Logits and a bias that start one element behind an aligned address."""
+    g = torch.Generator().manual_seed(T)
+    x, bias = torch.randn(T * E + 1, generator=g).cuda(), (torch.randn(E + 1, generator=g) * 0.1).cuda()
+    for cast in (torch.float32, torch.bfloat16):
+        xs = x.to(cast)
+        off, aligned = xs[1:].view(T, E), xs[1:].view(T, E).clone()
+        a = pkg.ops.moe_router_grouped(off, bias[1:], 4, 1, groups, 1, True, 1.0)
+        b = pkg.ops.moe_router_grouped(aligned, bias[1:].clone(), 4, 1, groups, 1, True, 1.0)
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+        _check(pkg, off.cpu(), bias[1:].cpu(), 4, True, groups, 1, True, 1.0)
+
+
+def test_a_token_routes_alike_in_any_batch(pkg, dev):
+    """The choices of a token do not depend on the tokens beside it, nor on which of the layouts their number takes."""
+    g = torch.Generator().manual_seed(2)
+    x, bias = torch.randn(5000, 192, generator=g).cuda(), (torch.randn(192, generator=g) * 0.1).cuda()
+    whole = pkg.ops.moe_router_grouped(x, bias, 6, 1, 8, 3, True, 2.0)
+    for lo, hi in ((0, 1), (5, 21), (100, 1100), (4990, 5000)):
+        part = pkg.ops.moe_router_grouped(x[lo:hi], bias, 6, 1, 8, 3, True, 2.0)
+        assert torch.equal(part[1], whole[1][lo:hi])
+        # (binary64 sums in another order, then one rounding to fp32)
+        assert bool(((part[0] - whole[0][lo:hi]).abs() <= 2.0 ** -23 * whole[0][lo:hi]).all())
