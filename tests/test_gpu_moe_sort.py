@@ -7,7 +7,8 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("T,topk,E", [
     (0, 2, 2000), (3, 1, 2560), (40000, 1, 1), (34000, 1, 3), (5000, 8, 17), (16384, 8, 256), (131072, 1, 256),
-    (50000, 8, 1024), (9000, 8, 1025), (20001, 5, 2560), (600000, 1, 40), (7000, 8, 256)])
+    (50000, 8, 1024), (9000, 8, 1025), (20001, 5, 2560), (600000, 1, 40), (7000, 8, 256), (5120, 8, 256),
+    (6144, 8, 60), (6145, 8, 256), (4096, 8, 1000), (4097, 8, 1000), (16384, 8, 64)])
 def test_sort_of_many_chunks(pkg, dev, T, topk, E):
     g = torch.Generator().manual_seed(T + E)
     ids = torch.randint(0, E, (T, topk), generator=g, dtype=torch.int32)

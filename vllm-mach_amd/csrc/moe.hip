@@ -6,12 +6,11 @@
 //   sorted_routes[pos]     route at each sorted position
 //   inverse[r]             sorted position of each route (-1 if dropped)
 // Three passes over 1024-route chunks: per-chunk histograms (LDS atomics,
-// order free), one workgroup scanning chunks and experts (the two in one
-// workgroup when the histograms fit in LDS), then a pass that
-// ranks each route inside its chunk (a ballot match of the expert id's bits inside the
+// order free), a scan over the chunks, 16 experts a workgroup, then a pass that adds up the
+// experts' totals, ranks each route inside its chunk (a ballot match of the expert id's bits inside the
 // wavefront plus an LDS prefix over the chunk's 16 wavefronts) and scatters.  A single chunk
-// (decode-sized steps) runs all three in one workgroup; up to 32 chunks run them in one launch
-// that counts in every workgroup.
+// (decode-sized steps) runs all three in one workgroup; up to 40 chunks (32 past 256
+// experts) run them in one launch that counts in every workgroup.
 //
 // Combine: out[t, h] = bf16(sum_k y[inverse[t*topk + k], h] * w[t, k]),
 // each product rounded to binary32 and added in ascending k from zero.
@@ -148,39 +147,6 @@ __global__ __launch_bounds__(kChunk) void route_scatter_kernel(const int32_t* __
   inverse[r] = pos;
 }
 
-// Count and scan in one workgroup when the per-chunk histograms fit in LDS
-// (C x E <= kCountScanMaxEntries, E <= 1024): the chunk histograms of route_hist_kernel
-// (route ids loaded eight at a time, LDS atomics), then per expert their sums in chunk
-// order -- the values route_scan_kernel writes, in one launch instead of two.
-constexpr int kCountScanMaxEntries = 14336;
-__global__ __launch_bounds__(kChunk) void route_count_scan_kernel(const int32_t* __restrict__ ids, int64_t R,
-                                                                  int64_t C, int E,
-                                                                  int32_t* __restrict__ chunk_sums) {
-  extern __shared__ int32_t hist[];  // [C][E]
-  const int t = threadIdx.x;
-  for (int64_t i = t; i < C * E; i += kChunk) hist[i] = 0;
-  __syncthreads();
-  for (int64_t c0 = 0; c0 < C; c0 += 8) {
-    int32_t e[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int64_t r = (c0 + k) * kChunk + t;
-      e[k] = (c0 + k < C && r < R) ? ids[r] : -1;
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (e[k] >= 0 && e[k] < E) atomicAdd(&hist[(c0 + k) * E + e[k]], 1);
-  }
-  __syncthreads();
-  for (int x = t; x < E; x += kChunk) {
-    int32_t run = 0;
-    for (int64_t c = 0; c < C; ++c) {
-      run += hist[c * E + x];
-      chunk_sums[c * E + x] = run;
-    }
-  }
-}
-
 __global__ __launch_bounds__(kChunk) void route_single_kernel(const int32_t* __restrict__ ids, int64_t R, int E,
                                                              int64_t* __restrict__ expert_offsets,
                                                              int32_t* __restrict__ sorted_routes,
@@ -191,13 +157,14 @@ __global__ __launch_bounds__(kChunk) void route_single_kernel(const int32_t* __r
   single_chunk_sort(t < R ? ids[t] : -1, R, E, expert_offsets, sorted_routes, inverse, whist, tot);
 }
 
-// 2 .. kSortMaxChunks chunks in one launch (E <= 1024): every workgroup counts all routes for
+// 2 .. sort_max_chunks chunks in one launch (E <= 1024): every workgroup counts all routes for
 // itself, those of the chunks before its own apart from the rest (one LDS atomic per route and
 // workgroup), scans the totals into the offsets, which workgroup 0 writes, and ranks and
 // scatters its chunk as route_scatter_kernel does.  Repeating the counts costs less than the
-// launches that share them (16384 routes of 256 experts: 6.7 us against 9.2 for
-// route_count_scan_kernel and route_scatter_kernel), up to 32 chunks, where a thread counts 32.
-constexpr int kSortMaxChunks = 32;
+// three launches that share them up to 40 chunks, where a thread counts 40 (256 experts, us: 16
+// chunks 6.9, 40 9.6, 48 10.5, 128 20.4, against 10.0 at 49 and 11.0 at 128; 1024 experts 33
+// chunks 11.6 against 11.0, so 32).
+constexpr int sort_max_chunks(int64_t E) { return E <= 256 ? 40 : 32; }
 __global__ __launch_bounds__(kChunk) void route_sort_kernel(const int32_t* __restrict__ ids, int64_t R, int C, int E,
                                                            int64_t* __restrict__ expert_offsets,
                                                            int32_t* __restrict__ sorted_routes,
@@ -470,17 +437,14 @@ extern "C" int mxl_moe_route(const int32_t* topk_ids, int64_t T, int64_t topk, i
     MXL_CHECK_LAUNCH("mxl_moe_route(single)");
     return MXL_OK;
   }
-  if (C > 1 && C <= kSortMaxChunks && E <= kSingleMaxExperts) {
+  if (C > 1 && C <= sort_max_chunks(E) && E <= kSingleMaxExperts) {
     route_sort_kernel<<<dim3((unsigned)C), kChunk, (kChunk / 64 + 4) * E * sizeof(int32_t), s>>>(
         topk_ids, R, (int)C, (int)E, expert_offsets, sorted_routes, inverse);
     MXL_CHECK_LAUNCH("mxl_moe_route(sort)");
     return MXL_OK;
   }
   int32_t* counts = (int32_t*)workspace;
-  if (C > 0 && C * E <= kCountScanMaxEntries && E <= 1024) {
-    route_count_scan_kernel<<<1, kChunk, C * E * sizeof(int32_t), s>>>(topk_ids, R, C, (int)E, counts);
-    MXL_CHECK_LAUNCH("mxl_moe_route(count_scan)");
-  } else if (C > 0) {
+  if (C > 0) {
     route_hist_kernel<<<dim3((unsigned)C), kChunk, E * sizeof(int32_t), s>>>(topk_ids, R, (int)E, counts);
     MXL_CHECK_LAUNCH("mxl_moe_route(hist)");
     route_scan_kernel<<<dim3((unsigned)((E + kScanExperts - 1) / kScanExperts)), 1024, 0, s>>>(counts, C, (int)E);
