@@ -786,10 +786,11 @@ _NOTHING = contextlib.nullcontext()
 
 
 def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    _check_cuda(first, *others)
+    _check_cuda(first)
     device = first.device
     for t in others:
         if t is not None and t.device != device:
+            _check_cuda(t)
             raise ValueError(f"{what}: tensors on {device} and {t.device}")
 
 
@@ -814,8 +815,10 @@ def _aligned(t: torch.Tensor, nbytes: int) -> torch.Tensor:
     return t
 
 
-def _scratch(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _scratch(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    """Scratch on the device of ``like`` (new_empty spares torch.empty's parsing of a type and a device)."""
+    size = like.element_size()
+    return like.new_empty((nbytes + size - 1) // size) if nbytes else None
 
 
 def _fp4_rule(what: str, rule: int) -> None:
@@ -928,7 +931,7 @@ def mxfp4_gemm(a: torch.Tensor, sa: torch.Tensor, w: torch.Tensor, sw: torch.Ten
     if M:
         with _on(a.device):
             nbytes = query("mxl_mxfp4_gemm_workspace_bytes", M, n, k)
-            ws = _scratch(nbytes, a.device)
+            ws = _scratch(nbytes, w)
             call("mxl_mxfp4_gemm", ptr(a), ptr(sa), M, ptr(w), ptr(sw), n, k, ptr(bias), ptr(out), n, ptr(ws), nbytes,
                  stream_handle(a.device))
     _count("mxfp4_gemm")
@@ -955,12 +958,12 @@ def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, rul
     M, K = x.shape[0], x.shape[1] // 2 if swiglu else x.shape[1]
     w, sw = _fp4_weight("mxfp4_linear", w, sw, n, K)
     bias = _fp4_bias("mxfp4_linear", bias, n)
-    out = torch.empty((M, n), dtype=torch.bfloat16, device=x.device)
+    out = x.new_empty((M, n))
     if M:
         x = _aligned(x, 16) if swiglu else _rows16(x)
         with _on(x.device):
             nbytes = query("mxl_mxfp4_linear_workspace_bytes", M, n, K, int(swiglu))
-            ws = _scratch(nbytes, x.device)
+            ws = _scratch(nbytes, w)
             call("mxl_mxfp4_linear", ptr(x), M, K, _row_stride(x), int(swiglu), rule, ptr(w), ptr(sw), n, ptr(bias),
                  ptr(out), n, ptr(ws), nbytes, stream_handle(x.device))
     _count("mxfp4_linear")
@@ -1092,7 +1095,7 @@ def mxfp4_experts(output: torch.Tensor, x: torch.Tensor, topk_ids: Optional[torc
         ids = None if given else topk_ids.to(torch.int32).contiguous()
         with _on(x.device):
             nbytes = query("mxl_mxfp4_experts_workspace_bytes", T, topk, e, H, i, int(given), int(fuse))
-            ws = _scratch(nbytes, x.device)
+            ws = _scratch(nbytes, w13)
             call("mxl_mxfp4_experts", ptr(x), T, _row_stride(x), ptr(ids), ptr(weights), topk, ptr(sorted_routes),
                  ptr(expert_offsets), ptr(inverse), e, H, i, ptr(w13), ptr(sw13), ptr(w2), ptr(sw2), rule, int(fuse),
                  ptr(out), ptr(ws), nbytes, stream_handle(x.device))
@@ -1212,14 +1215,14 @@ def moe_router_grouped(router_logits: torch.Tensor, bias: Optional[torch.Tensor]
     if not 1 <= top_k <= topk_groups * (E // num_groups):
         raise ValueError(f"moe_router_grouped: top_k {top_k} of {topk_groups * (E // num_groups)} experts")
     dev = logits.device
-    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
     sorted_routes = torch.empty(T * top_k, dtype=torch.int32, device=dev)
+    inverse, ids = sorted_routes.new_empty(T * top_k), sorted_routes.new_empty((T, top_k))
+    fp32 = logits if logits.dtype == torch.float32 else bias
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev) if fp32 is None else fp32.new_empty((T, top_k))
     offsets = torch.empty(E + 1, dtype=torch.int64, device=dev)
-    inverse = torch.empty_like(sorted_routes)
     with _on(dev):
         nbytes = query("mxl_moe_router_workspace_bytes", T, top_k, E)
-        buf = _scratch(nbytes, dev)
+        buf = _scratch(nbytes, inverse)
         call("mxl_moe_router_grouped", ptr(logits), int(logits.dtype == torch.bfloat16), ptr(bias), T, E, top_k, scoring,
              num_groups, topk_groups, int(renormalize), float(factor), ptr(weights), ptr(ids), ptr(sorted_routes),
              ptr(offsets), ptr(inverse), ptr(buf), nbytes, stream_handle(dev))
