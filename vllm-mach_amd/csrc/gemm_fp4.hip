@@ -12,6 +12,9 @@
 
 namespace mxl {
 
+int moe_reduce_by_route(const char* who, const void* routed_output, const float* topk_weights, const int32_t* topk_ids,
+                        int64_t T, int64_t topk, int64_t E, int64_t H, void* out, void* stream);  // (moe.hip)
+
 // c += W A^T over a K128 slice whose scales are byte J of sw and byte JA of sa.
 template <int J, int JA>
 __device__ __forceinline__ v4f mfma_fp4(const uint4& w, const uint4& a, v4f c, uint32_t sw, uint32_t sa) {
@@ -33,9 +36,9 @@ __device__ __forceinline__ v4f mfma_fp4(const uint4& w, const uint4& a, v4f c, u
 // weights are read once whatever its rows.  SWIGLU (an expert's gate/up product): the workgroup's n-tiles are two
 // of gate and the same two of up, and the epilogue quantizes the 32 columns' bf16(bf16(silu(g)) u) in place of
 // storing gate and up.
-int moe_reduce_by_route(const char* who, const void* routed_output, const float* topk_weights, const int32_t* topk_ids,
-                        int64_t T, int64_t topk, int64_t E, int64_t H, void* out, void* stream);  // (moe.hip)
-
+// Cold weights: 1 x 2048 x 2048 3.9 us; w13 and w2 of 64 tokens, top 8 of 256 experts (K = 2048, I = 512) 50 and 24 us,
+// 5 TB/s of weights, the rate of a large copy.
+//
 // kRoutes: a few routes as they come, their experts in row_index and route r's activation row r / row_div: no sort.
 enum Fp4Unit : int { kExperts = 0, kHitExperts = 1, kRoutes = 2 };
 struct Fp4Stream {
