@@ -82,7 +82,7 @@ int mxl_quantize_mxfp4(const void* x, int64_t M, int64_t K, int64_t ldx, int rul
 int mxl_swiglu_mxfp4(const void* gate_up, int64_t M, int64_t K, int rule, void* codes, void* scales, void* stream);
 
 /* out[m, n] = sum_k A[m, k] W[n, k], MXFP4 on both sides, fp32 sums, bf16 out (row
- * stride ldc); with a bias (bf16 [N]) the rounded sum plus the bias, rounded again.
+ * stride ldc); a bias (bf16 [N]) joins the fp32 sum, which is rounded once.
  * a u8 [M, K/2], sa u8 [M, K/32] row-major; w_tiled / sw_tiled from mxl_pack_weight
  * with format 4.  a and w 16-byte, scales 4-byte aligned; the workspace holds
  * mxl_mxfp4_gemm_workspace_bytes(M, N, K) bytes (16-byte aligned; 0: may be null). */

@@ -671,3 +671,31 @@ def test_gemm_of_codes_past_4_gib(pkg, dev):
     a[rows.to(dev)], sa[rows.to(dev)] = codes.to(dev), scales.to(dev)
     y = pkg.ops.mxfp4_gemm(a, sa, w, sw, n, k)
     ref.check_product(y[rows.to(dev)], ref.dequantize(codes, scales), wv)
+
+
+# ------------------------------------------------------------------ one rounding with a bias
+
+# by kernel: few rows in one wave and in several over K, tiles with 16- and 8-byte stores and through LDS, a K split
+BIASED = [(5, 100, 640), (1, 2048, 2048), (200, 1032, 1152), (200, 1028, 1152), (48, 1030, 512), (17, 256, 8192),
+          (40, 130, 8192)]
+
+
+@pytest.mark.parametrize("m,n,k", BIASED)
+def test_bias_joins_the_sum_ahead_of_the_rounding(pkg, dev, m, n, k):
+    """A bias next to minus the sums of row 0, whose outputs are what is left of them: an output is off by half a
+    step of its own value, not of the sum's, besides fp32's K products (K 2^-23 of their magnitudes) and sum (2^-24)."""
+    g = torch.Generator().manual_seed(m + n + k)
+    (w, sw), wv = _weight(pkg, g, n, k)
+    x = _x(g, m, k)
+    a, sa = ref.quantize(x)
+    av, wv = ref.dequantize(a, sa).cuda(), wv.cuda()
+    sums, most = av @ wv.t(), av.abs() @ wv.abs().t()
+    bias = (-sums[0]).bfloat16()
+    want = sums + bias.double()
+    room = 2.0 ** -8 * want.abs() + (k * 2.0 ** -23 * most + 2.0 ** -24 * want.abs()) * (1 + 2.0 ** -8)
+    split = pkg.ops.query("mxl_mxfp4_gemm_workspace_bytes", m, n, k) > 0
+    assert split == (k == 8192)
+    for y in (pkg.ops.mxfp4_gemm(a.to(dev), sa.to(dev), w, sw, n, k, bias),
+              pkg.ops.mxfp4_linear(x.to(dev), w, sw, n, ref.FLOOR_CARRY175, bias)):
+        off = (y.double() - want).abs()
+        assert bool((off <= room).all()), float((off / room).max())

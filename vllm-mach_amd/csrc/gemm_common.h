@@ -87,6 +87,10 @@ __device__ __forceinline__ uint16_t out_bits(float v, float alpha, int f16, bool
   const uint16_t h = f32_to_f16(y);
   return has_bias ? f32_to_f16(f16_to_f32(h) + bf16_to_f32(bias)) : h;
 }
+// MXFP4: a bias joins the fp32 sum ahead of the one rounding (bf16, no scaling).
+__device__ __forceinline__ uint16_t out_bits_fp4(float v, const uint16_t* bias, int64_t col) {
+  return f32_to_bf16(bias ? v + bf16_to_f32(bias[col]) : v);
+}
 __device__ __forceinline__ uint16_t out_bits(const GemmParams& p, float v, int64_t col) {
   return out_bits(v, p.alpha, p.out_f16, p.bias != nullptr, p.bias ? p.bias[col] : (uint16_t)0);
 }

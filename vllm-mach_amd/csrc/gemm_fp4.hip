@@ -255,7 +255,7 @@ __global__ __launch_bounds__(64 * kFp4StreamWaves) void fp4_stream_kernel(GemmPa
       if (r < rows) {
         uint16_t h[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = out_bits(p, v[i], col + i < p.N ? col + i : 0);
+        for (int i = 0; i < 4; ++i) h[i] = out_bits_fp4(v[i], p.bias, col + i < p.N ? col + i : 0);
         uint16_t* dst = p.out + (row0 + r) * p.ldc + col;
         if (col + 4 <= p.N && p.ldc % 4 == 0 && ((uintptr_t)p.out & 7) == 0) {
           *reinterpret_cast<uint2*>(dst) = uint2{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
@@ -361,7 +361,7 @@ __device__ __forceinline__ void fp4_tile(const GemmParams& p, const uint8_t* w, 
   const int64_t col = nt * 16 + 4 * q;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (col + e < p.N) p.out[row * p.ldc + col + e] = out_bits(p, acc[e], col + e);
+    if (col + e < p.N) p.out[row * p.ldc + col + e] = out_bits_fp4(acc[e], p.bias, col + e);
 }
 
 __global__ __launch_bounds__(256) void fp4_grouped_kernel(GemmParams p) {

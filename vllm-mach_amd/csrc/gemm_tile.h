@@ -664,7 +664,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       return y != y ? (d & 0x0000FFFFu) | 0x7FC00000u : d;
     };
     // BIAS: one is added to the rounded output (MXFP8 2048 x 18432 x 2560 135 us with a pass of its
-    // own, 104 here, 222 through the LDS below).  WIDE (MXFP4, rows of whole 16-byte pieces): of two n-tiles side
+    // own, 104 here, 222 through the LDS below), to MXFP4's sums ahead of the rounding.  WIDE (MXFP4, rows of whole 16-byte pieces): of two n-tiles side
     // by side every other 16 lanes change places, after which a lane holds eight consecutive columns of one
     // of them: half the stores, of 64 bytes of a row each (4096 x 17408 x 5120 206 -> 198 us).
     auto store = [&](auto BIAS, auto WIDE) {
@@ -688,10 +688,17 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
           u2 h;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            h[e] = pack(v[2 * e], v[2 * e + 1]);
-            if constexpr (decltype(BIAS)::value)
-              h[e] = pack(u2f(h[e] << 16) + u2f(bias[n][e] << 16),
-                          u2f(h[e] & 0xFFFF0000u) + u2f(bias[n][e] & 0xFFFF0000u));
+            float lo = v[2 * e], hi = v[2 * e + 1];
+            if constexpr (decltype(BIAS)::value) {
+              if constexpr (!FP4) {
+                h[e] = pack(lo, hi);
+                lo = u2f(h[e] << 16);
+                hi = u2f(h[e] & 0xFFFF0000u);
+              }
+              lo = lo + u2f(bias[n][e] << 16);
+              hi = hi + u2f(bias[n][e] & 0xFFFF0000u);
+            }
+            h[e] = pack(lo, hi);
           }
           if constexpr (!wide) {
             const uint32_t off = c0 + 16 * n < (int)p.N ? (uint32_t)((r0 + 16 * i) * ld + c0 + 16 * n) * 2 : 0xFFFFFFF0u;
@@ -739,7 +746,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       for (int c = lane; c < 16 * TW; c += 64) {
         const int64_t row = w.row0 + (wm * MTW + i) * 16 + c / TW, col = (int64_t)w.nb * S::BN + wn * TW + c % TW;
         const float v = stage_out[c];
-        if (row < w.row_hi && col < p.N) p.out[row * p.ldc + col] = out_bits(p, v, col);
+        if (row < w.row_hi && col < p.N) p.out[row * p.ldc + col] = FP4 ? out_bits_fp4(v, p.bias, col) : out_bits(p, v, col);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }

@@ -601,7 +601,7 @@ __global__ __launch_bounds__(256) void wide_tile_reduce_kernel(const float* __re
                                                                uint16_t* __restrict__ out, int64_t M, int64_t N,
                                                                int64_t ldc, WideGrid g, int64_t tile0,
                                                                int64_t tiles, int S, int BM, int TW, int cols4,
-                                                               float alpha, int f16) {
+                                                               float alpha, int f16, int fp4) {
   const int64_t per_tile = (int64_t)BM * TW / 4;  // float4 items of a tile block
   const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (id >= tiles * per_tile) return;
@@ -632,8 +632,10 @@ __global__ __launch_bounds__(256) void wide_tile_reduce_kernel(const float* __re
   if (cols4) {
     uint16_t h[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      h[e] = out_bits(a4[e], alpha, f16, b, b ? bias[col + e < N ? col + e : N - 1] : (uint16_t)0);
+    for (int e = 0; e < 4; ++e) {
+      const int64_t at = col + e < N ? col + e : N - 1;
+      h[e] = fp4 ? out_bits_fp4(a4[e], bias, at) : out_bits(a4[e], alpha, f16, b, b ? bias[at] : (uint16_t)0);
+    }
     uint16_t* dst = out + row0 * ldc + col;
     if (col + 4 <= N && ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
       *reinterpret_cast<uint2*>(dst) = uint2{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
@@ -948,7 +950,7 @@ hipError_t launch_gemm_wide(int fmt, bool block, const WideConfig& c, const Gemm
     const int64_t items = tiles * bm * tw / 4;
     wide_tile_reduce_kernel<<<dim3((unsigned)((items + 255) / 256)), 256, 0, s>>>(
         p.partial, p.bias, p.out, p.M, p.N, p.ldc, g, tile0, tiles, S, (int)bm, (int)tw, c.WM == 2, p.alpha,
-        p.out_f16);
+        p.out_f16, fmt == kE2M1);
     return hipGetLastError();
   };
   if (c.dp_tiles <= 0 || c.dp_tiles >= g.tiles) {

@@ -920,7 +920,7 @@ def mxfp4_gemm(a: torch.Tensor, sa: torch.Tensor, w: torch.Tensor, sw: torch.Ten
     """Product of MXFP4 activations and weights: y = A W^T (+ bias), fp32 sums, bf16 [M, N].
 
     a, sa: ``quantize_mxfp4``'s codes u8 [M, K/2] and scales u8 [M, K/32]; w, sw: the weight in the tiled
-    layout (``pack_weight`` with ``E2M1``).  A bias is added to the rounded sum, and rounded again.
+    layout (``pack_weight`` with ``E2M1``).  A bias is added to the fp32 sum, which is rounded once.
     """
     _same_device("mxfp4_gemm", a, sa, w, sw, bias)
     w, sw = _fp4_weight("mxfp4_gemm", w, sw, n, k)
