@@ -228,3 +228,11 @@ def test_checkpoint_shapes(pkg, tmp_path, monkeypatch):
     assert experts.mxl_experts.shapes == (2, 256, 128) and [p[2] for p in packed] == [4, 4, 4]
     assert torch.equal(packed[1][0][1, 128:], tensors["m.experts.1.up_proj.weight"])
     assert torch.equal(packed[2][1][0], tensors["m.experts.0.down_proj.weight_scale"])
+
+
+@pytest.mark.parametrize("n,match", [(32768, "workspace"), (32769, "too large"), (40000, "too large")])
+def test_weights_past_the_scale_offsets_are_refused(c, n, match):
+    """The tiles index a weight's scales (256 bytes for 16 x 512 of it) in 32 bits: the largest K and the N at which
+    they end, admitted as far as the missing workspace, and the next."""
+    with pytest.raises(c.MxlError, match=match):
+        c.call("mxl_mxfp4_gemm", 16, 16, 128, 16, 16, n, 1 << 22, None, 16, n, None, 0, None)

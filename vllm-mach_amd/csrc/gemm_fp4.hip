@@ -413,7 +413,11 @@ static WideConfig fp4_tiles_config(int64_t M, int64_t N, int64_t K) {
   return c;
 }
 
-static bool fp4_tiles_eligible(int64_t M, int64_t N, int64_t K) { return wide_tiles_eligible(M, N, K / 2, false); }
+// (the codes' offsets are those of K / 2 bytes a row; a weight's scales, 256 bytes a super-tile of 512 columns, are
+// indexed in 32 bits)
+static bool fp4_tiles_eligible(int64_t M, int64_t N, int64_t K) {
+  return wide_tiles_eligible(M, N, K / 2, false) && ((N + 15) / 16) * ((K + kTileK - 1) / kTileK) <= (int64_t(1) << 24);
+}
 
 static GemmParams fp4_params(const void* a, const void* sa, const void* w, const void* sw, int64_t N, int64_t K,
                              void* out, int64_t ldc) {
