@@ -699,3 +699,36 @@ def test_bias_joins_the_sum_ahead_of_the_rounding(pkg, dev, m, n, k):
               pkg.ops.mxfp4_linear(x.to(dev), w, sw, n, ref.FLOOR_CARRY175, bias)):
         off = (y.double() - want).abs()
         assert bool((off <= room).all()), float((off / room).max())
+
+
+# ------------------------------------------------------------------ rows far apart, large operands
+
+def _need(gib):
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GiB")
+
+
+@pytest.mark.parametrize("rows,gib", [((1 << 26) + 999, 6), ((1 << 30) + 999, 72)])
+@pytest.mark.parametrize("routed", [20, 9000])
+def test_grouped_gemm_of_rows_past_32_bit_offsets(pkg, dev, rows, gib, routed):
+    """Activations past 4 GiB, and past 2^32 pieces of 16 bytes, gathered from both sides of the border: few routed
+    rows an expert and many."""
+    _need(gib)
+    e, n, k = 4, 72, 128
+    g = torch.Generator().manual_seed(routed)
+    wc, ws = ref.random_operand(g, e * n, k)
+    wv = ref.dequantize(wc, ws).view(e, n, k)
+    w, sw = pkg.ops.pack_weight(wc.view(e, n, -1).to(dev), ws.view(e, n, -1).to(dev), pkg.ops.E2M1)
+    border = 1 << (rows.bit_length() - 1)
+    at = torch.cat([torch.arange(999), torch.arange(border - 999, border + 999)])
+    codes, scales = ref.random_operand(g, len(at), k)
+    a = torch.empty(rows, k // 2, dtype=torch.uint8, device=dev)
+    sa = torch.empty(rows, k // 32, dtype=torch.uint8, device=dev)
+    a[at.to(dev)], sa[at.to(dev)] = codes.to(dev), scales.to(dev)
+    pick = torch.randint(0, len(at), (routed,), generator=g)
+    offsets = torch.arange(e + 1) * routed // e
+    y = pkg.ops.mxfp4_grouped_gemm(a, sa, at[pick].int().to(dev), 1, offsets.to(dev), routed, w, sw, n, k)
+    values = ref.dequantize(codes, scales)[pick]
+    for x in range(e):
+        lo, hi = offsets[x], offsets[x + 1]
+        ref.check_product(y[lo:hi], values[lo:hi], wv[x])

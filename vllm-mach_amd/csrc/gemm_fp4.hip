@@ -151,7 +151,7 @@ __global__ __launch_bounds__(64 * kFp4StreamWaves) void fp4_stream_kernel(GemmPa
         at = at < items ? at : items - 1;  // (past the end: the last again)
         b[u] = rows > 1 ? (int)__umulhi((uint32_t)at, inv) : at;
         rr[u] = at - b[u] * rows;
-        int ar = (int)row0 + rr[u];  // (32-bit offsets: the host bounds the operands below 4 GiB)
+        int ar = (int)row0 + rr[u];  // (32-bit offsets, of codes in pieces of 16 bytes: the host admits no rows past them)
         if (g.E) {
           if (p.row_index) ar = (g.unit == kRoutes ? ar : p.row_index[ar]) / p.row_div;
           ar = ar < 0 ? 0 : ar < (int)p.a_rows ? ar : (int)p.a_rows - 1;
@@ -579,7 +579,8 @@ extern "C" int mxl_mxfp4_grouped_gemm(const void* a, const void* sa, int64_t a_r
   p.w_expert_stride = mxl_tiled_weight_bytes(N, K, kE2M1);
   p.sw_expert_stride = mxl_tiled_scale_bytes(N, K);
   Fp4StreamPlan pl;
-  if (fp4_grouped_streams(routed_rows, num_experts, N, K, false, pl)) {
+  // (the streaming kernel numbers the 16-byte pieces of A in 32 bits)
+  if (a_rows <= (int64_t(1) << 32) / (K / 32) && fp4_grouped_streams(routed_rows, num_experts, N, K, false, pl)) {
     Fp4Stream g{};
     g.E = (int)num_experts;
     g.unit = routed_rows < num_experts ? kHitExperts : kExperts;
