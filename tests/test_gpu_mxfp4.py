@@ -732,3 +732,28 @@ def test_grouped_gemm_of_rows_past_32_bit_offsets(pkg, dev, rows, gib, routed):
     for x in range(e):
         lo, hi = offsets[x], offsets[x + 1]
         ref.check_product(y[lo:hi], values[lo:hi], wv[x])
+
+
+# ------------------------------------------------------------------ the routes sorted and as they come
+
+@pytest.mark.parametrize("t,e,topk,h,i", [(16, 8, 2, 2048, 128), (8, 3, 2, 1024, 1024), (16, 5, 2, 2048, 512),
+                                          (4, 8, 8, 5120, 128), (1, 8, 4, 2048, 512)])
+def test_experts_of_a_router_and_of_its_ids_give_the_same_bits(pkg, dev, t, e, topk, h, i):
+    """``apply_router`` (sorted routes) against ``apply`` of the same ids (up to 32 routes as they come), where the order
+    of a K sum shows: half of K cancels the other's large values, which cost the rest of the sum its low bits."""
+    g = torch.Generator().manual_seed(t + e + h)
+    c1, s1 = ref.random_operand(g, e * 2 * i, h)
+    c2, s2 = ref.random_operand(g, e * h, i)
+    c1, s1, c2, s2 = c1.view(e, 2 * i, -1), s1.view(e, 2 * i, -1) - 8, c2.view(e, h, -1), s2.view(e, h, -1) - 6
+    half = h // 2  # 32 columns in the middle: the weights of the first 32
+    c1[..., half // 2:half // 2 + 16], s1[..., half // 32] = c1[..., :16], s1[..., 0]
+    experts = pkg.Mxfp4Experts()
+    w1, w2 = experts.process_weights_after_loading(c1.to(dev), s1.to(dev), c2.to(dev), s2.to(dev))
+    x = _x(g, t, h)
+    x[:, :32] *= 2.0 ** 18
+    x[:, half:half + 32] = -x[:, :32]
+    x, z = x.to(dev), torch.randn(t, e, generator=g).to(dev)
+    p, ids = pkg.select_experts(z, topk)
+    one, two = experts(x, w1, w2, p, ids), torch.empty_like(x)
+    experts.apply_router(two, x, w1, w2, z, topk)
+    assert bool(one.isfinite().all()) and torch.equal(one, two)

@@ -610,7 +610,8 @@ static bool fp4_direct(int64_t routes, int64_t E, int64_t H, int64_t I) {
 }
 
 // Both products of the unsorted routes: x bf16 [T, H] through w13 and the SwiGLU producer to codes and scales [routes,
-// I], then through w2 to y [routes, H].
+// I], then through w2 to y [routes, H].  The plans are those of the sorted routes' units, min(routes, E): K is split over
+// the same waves, so a layer has the same bits from ids and from a router's sorted routes.
 static hipError_t fp4_direct_launch(const void* x, int64_t T, int64_t ldx, const int32_t* ids, int64_t topk, int64_t E,
                                     int64_t H, int64_t I, const void* w13, const void* sw13, const void* w2,
                                     const void* sw2, int rule, void* codes, void* scales, void* y, hipStream_t s) {
@@ -628,14 +629,14 @@ static hipError_t fp4_direct_launch(const void* x, int64_t T, int64_t ldx, const
   g.carry = fp4_carry(rule);
   g.codes = (uint8_t*)codes;
   g.scales = (uint8_t*)scales;
-  if (!fp4_stream_plan(2 * I, H, routes, true, pl)) return hipErrorInvalidValue;
+  if (!fp4_stream_plan(2 * I, H, std::min(routes, E), true, pl)) return hipErrorInvalidValue;
   const hipError_t e = launch_fp4_stream<1, true>(pl, p, g, routes, s);
   if (e != hipSuccess) return e;
   GemmParams q = fp4_params(codes, scales, w2, sw2, H, I, y, H);
   q.M = q.a_rows = routes; q.row_index = ids; q.row_div = 1;
   q.w_expert_stride = mxl_tiled_weight_bytes(H, I, kE2M1);
   q.sw_expert_stride = mxl_tiled_scale_bytes(H, I);
-  if (!fp4_stream_plan(H, I, routes, false, pl)) return hipErrorInvalidValue;
+  if (!fp4_stream_plan(H, I, std::min(routes, E), false, pl)) return hipErrorInvalidValue;
   return launch_fp4_stream<0, false>(pl, q, g, routes, s);
 }
 
