@@ -92,9 +92,9 @@ int mxl_mxfp4_gemm(const void* a, const void* sa, int64_t M, const void* w_tiled
                    void* stream);
 
 /* mxl_quantize_mxfp4 then mxl_mxfp4_gemm in one launch: bf16 x [M, K] (row stride ldx, 16-byte
- * aligned) of few rows, quantized inside the product (the same bits).  Shapes:
- * mxl_mxfp4_quant_gemm_supported (up to 16 rows, fewer of a long K or a wide N), else
- * MXL_EUNSUPPORTED. */
+ * aligned, ((M - 1) ldx + K) 2 bytes at most 4 GiB) of few rows, quantized inside the product (the
+ * same bits).  Shapes: mxl_mxfp4_quant_gemm_supported (up to 16 rows, fewer of a long K or a
+ * wide N), else MXL_EUNSUPPORTED. */
 int mxl_mxfp4_quant_gemm_supported(int64_t M, int64_t N, int64_t K);
 int mxl_mxfp4_quant_gemm(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, const void* w_tiled,
                          const void* sw_tiled, int64_t N, const void* bias, void* out, int64_t ldc, void* stream);
@@ -102,8 +102,9 @@ int mxl_mxfp4_quant_gemm(const void* x, int64_t M, int64_t K, int64_t ldx, int r
 /* An expert layer's first half in one launch, for few rows an expert: quantized rows of
  * bf16 x [a_rows, K] (gathered as mxl_mxfp4_grouped_gemm does), the gate/up product with
  * W13[e] [2 I, K], and mxl_swiglu_mxfp4 of its rounded result: codes [routed_rows, I/2] and
- * scales [routed_rows, I/32] of the routed rows.  Shapes: mxl_mxfp4_grouped_swiglu_supported
- * (fewer than 8 rows an expert, I % 32 == 0), else MXL_EUNSUPPORTED. */
+ * scales [routed_rows, I/32] of the routed rows.  x spans at most 4 GiB.  Shapes:
+ * mxl_mxfp4_grouped_swiglu_supported (fewer than 8 rows an expert, I % 32 == 0), else
+ * MXL_EUNSUPPORTED. */
 int mxl_mxfp4_grouped_swiglu_supported(int64_t routed_rows, int64_t num_experts, int64_t I, int64_t K);
 int mxl_mxfp4_grouped_swiglu(const void* x, int64_t a_rows, int64_t ldx, const int32_t* row_index, int row_div,
                              const int64_t* expert_offsets, int64_t num_experts, int64_t routed_rows,

@@ -757,3 +757,27 @@ def test_experts_of_a_router_and_of_its_ids_give_the_same_bits(pkg, dev, t, e, t
     one, two = experts(x, w1, w2, p, ids), torch.empty_like(x)
     experts.apply_router(two, x, w1, w2, z, topk)
     assert bool(one.isfinite().all()) and torch.equal(one, two)
+
+
+@pytest.mark.parametrize("m,k", [(16, 2048), (64, 2048), (5, 512)])
+@pytest.mark.parametrize("beyond", [-8, 0, 8])
+def test_rows_up_to_four_gib_apart(pkg, dev, m, k, beyond):
+    """Rows that end within 2^31 values of the first (32-bit byte offsets), by a hair or by a row's, and rows further
+    apart: the layer and the experts give what they give for the same rows side by side."""
+    _need(16)
+    g = torch.Generator().manual_seed(m + k)
+    ld = ((1 << 31) - k) // (m - 1) // 8 * 8 + beyond
+    x = torch.empty((m - 1) * ld + k, dtype=torch.bfloat16, device=dev).as_strided((m, k), (ld, 1))
+    near = _x(g, m, k).to(dev)
+    x.copy_(near)
+    (w, sw), _ = _weight(pkg, g, 72, k)
+    assert torch.equal(pkg.ops.mxfp4_linear(x, w, sw, 72), pkg.ops.mxfp4_linear(near, w, sw, 72))
+    _equal(pkg.ops.quantize_mxfp4(x), ref.quantize(near))
+    e, topk = 40, 2
+    experts, w1, w2, _, _ = _experts(pkg, g, e, k, 128)
+    ids, p = _routes(g, m, e, topk).to(dev), torch.rand(m, topk, generator=g).to(dev)
+    assert torch.equal(experts(x, w1, w2, p, ids), experts(near, w1, w2, p, ids))
+    routes, offsets, _ = pkg.ops.moe_route(ids, e)
+    one, two = (pkg.ops.mxfp4_grouped_swiglu(v, routes, topk, offsets, m * topk, w1, experts.w1_scale, 128)
+                for v in (x, near))
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])

@@ -236,3 +236,16 @@ def test_weights_past_the_scale_offsets_are_refused(c, n, match):
     they end, admitted as far as the missing workspace, and the next."""
     with pytest.raises(c.MxlError, match=match):
         c.call("mxl_mxfp4_gemm", 16, 16, 128, 16, 16, n, 1 << 22, None, 16, n, None, 0, None)
+
+
+@pytest.mark.parametrize("name,head,tail", [
+    ("mxl_mxfp4_quant_gemm", (16, 16, 2048), (0, 16, 16, 16, None, 16, 16, None)),
+    ("mxl_mxfp4_linear", (16, 16, 2048), (0, 0, 16, 16, 16, None, 16, 16, None, 0, None)),
+    ("mxl_mxfp4_experts", (16, 16), (16, 16, 2, None, None, None, 8, 2048, 128, 16, 16, 16, 16, 0, 1, 16, 256, 1 << 30, None)),
+    ("mxl_mxfp4_grouped_swiglu", (16, 16), (None, 1, 16, 8, 16, 16, 16, 128, 2048, 0, 16, 16, None))])
+def test_rows_past_32_bit_offsets_are_refused(c, name, head, tail):
+    """16 rows of 2048 whose last ends 2^31 values behind the first's start are the furthest that one launch takes."""
+    ld = ((1 << 31) - 2048) // 15
+    assert 15 * ld + 2048 == 1 << 31 and ld % 8 == 0
+    with pytest.raises(c.MxlError, match="span more than 4 GiB"):
+        c.call(name, *head, ld + 8, *tail)

@@ -399,6 +399,11 @@ static int check_operands(const char* who, const void* a, const void* sa, const 
   return MXL_OK;
 }
 
+// Whether bf16 rows [rows, K] of stride ldx lie within the 32-bit byte offsets of the streaming kernel's producer.
+static bool fp4_rows_reach(int64_t rows, int64_t ldx, int64_t K) {
+  return rows <= 1 || rows - 1 <= ((int64_t(1) << 31) - K) / ldx;
+}
+
 // A stage of the 2 x 2-wave tiles is 128 bytes of a row, whatever its format, and takes two MFMAs of a K128
 // slice of MXFP4 the time of one of 8-bit activations: the time model of K / 2 bytes holds.
 static WideConfig fp4_tiles_config(int64_t M, int64_t N, int64_t K) {
@@ -501,7 +506,7 @@ extern "C" int mxl_mxfp4_quant_gemm(const void* x, int64_t M, int64_t K, int64_t
   MXL_CHECK_ARG(ldx >= K && ldx % 8 == 0, "%s: ldx must be >= K and a multiple of 8", who);
   MXL_CHECK_ARG(fp4_rule(rule), "%s: unknown rule %d", who, rule);
   if (M == 0) return MXL_OK;
-  MXL_CHECK_ARG(M * ldx < (int64_t(1) << 31), "%s: the rows span more than 4 GiB", who);
+  MXL_CHECK_ARG(fp4_rows_reach(M, ldx, K), "%s: the rows span more than 4 GiB", who);
   Fp4StreamPlan pl;
   if (!fp4_dense_streams(M, N, K, true, pl)) {
     set_error("%s: %lld rows of K = %lld do not run in one launch", who, (long long)M, (long long)K);
@@ -542,7 +547,7 @@ extern "C" int mxl_mxfp4_grouped_swiglu(const void* x, int64_t a_rows, int64_t l
   MXL_CHECK_ARG(ldx >= K && ldx % 8 == 0, "%s: ldx must be >= K and a multiple of 8", who);
   MXL_CHECK_ARG(fp4_rule(rule), "%s: unknown rule %d", who, rule);
   MXL_CHECK_ARG(((uintptr_t)codes & 3) == 0, "%s: the codes must be 4-byte aligned", who);
-  MXL_CHECK_ARG(a_rows < (int64_t(1) << 31) / ldx, "%s: the rows span more than 4 GiB", who);
+  MXL_CHECK_ARG(fp4_rows_reach(a_rows, ldx, K), "%s: the rows span more than 4 GiB", who);
   if (routed_rows == 0) return MXL_OK;
   Fp4StreamPlan pl;
   if (!fp4_grouped_streams(routed_rows, num_experts, 2 * I, K, true, pl)) {
@@ -798,7 +803,7 @@ extern "C" int mxl_mxfp4_experts(const void* x, int64_t T, int64_t ldx, const in
                       (((uintptr_t)sw13 | (uintptr_t)sw2) & 3) == 0 && H <= kFp4MaxK && I <= kFp4MaxK,
                   "%s: bad stride, rule, alignment or size (ldx=%lld rule=%d H=%lld I=%lld)", who, (long long)ldx, rule,
                   (long long)H, (long long)I);
-    MXL_CHECK_ARG(T < (int64_t(1) << 31) / ldx, "%s: the rows span more than 4 GiB", who);
+    MXL_CHECK_ARG(fp4_rows_reach(T, ldx, H), "%s: the rows span more than 4 GiB", who);
     st = launch_status(fp4_direct_launch(x, T, ldx, topk_ids, topk, E, H, I, w13, sw13, w2, sw2, rule, s.codes2, s.scales2,
                                          s.y, (hipStream_t)stream), who);
     return st != MXL_OK ? st : moe_reduce_by_route(who, s.y, topk_weights, topk_ids, T, topk, E, H, out, stream);

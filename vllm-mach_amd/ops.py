@@ -799,7 +799,7 @@ def _rows16(x: torch.Tensor) -> torch.Tensor:
     than the kernels' offsets reach)."""
     m, k = x.shape
     ld = x.stride(0) if m > 1 else k
-    if (x.stride(1) != 1 and k > 1) or ld % 8 or ld < k or x.data_ptr() % 16 or (m - 1) * ld + k >= 1 << 31:
+    if (x.stride(1) != 1 and k > 1) or ld % 8 or ld < k or x.data_ptr() % 16 or (m - 1) * ld + k > 1 << 31:
         return torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
     return x
 
@@ -1027,7 +1027,8 @@ def mxfp4_grouped_swiglu(x: torch.Tensor, row_index: Optional[torch.Tensor], row
                          ) -> tuple[torch.Tensor, torch.Tensor]:
     """An expert layer's first half in one launch: ``quantize_mxfp4`` of the gathered bf16 rows x [T, K],
     ``mxfp4_grouped_gemm`` with the gate/up weights [E, 2 I, K] and ``swiglu_mxfp4`` of its rows -> (codes u8
-    [routed_rows, I/2], scales u8 [routed_rows, I/32]).  Rows past expert_offsets[E] are left unwritten."""
+    [routed_rows, I/2], scales u8 [routed_rows, I/32]).  x is at most 4 GiB.  Rows past expert_offsets[E] are left
+    unwritten."""
     _same_device("mxfp4_grouped_swiglu", x, row_index, expert_offsets, w, sw)
     if x.dtype != torch.bfloat16 or x.ndim != 2:
         raise ValueError("mxfp4_grouped_swiglu needs bf16 rows [T, K]")
