@@ -249,3 +249,14 @@ def test_rows_past_32_bit_offsets_are_refused(c, name, head, tail):
     assert 15 * ld + 2048 == 1 << 31 and ld % 8 == 0
     with pytest.raises(c.MxlError, match="span more than 4 GiB"):
         c.call(name, *head, ld + 8, *tail)
+
+
+def test_only_rows_with_gaps_are_brought_together(pkg):
+    """Contiguous rows are never copied for their size; rows with gaps only for a kernel of 32-bit offsets."""
+    big = torch.empty((1 << 20) + 8, 4096, dtype=torch.bfloat16, device="meta")
+    assert pkg.ops._rows16(big) is big and pkg.ops._rows16(big, True) is big
+    ld = ((1 << 31) - 2048) // 15
+    for step, copied in ((0, False), (8, True)):
+        x = torch.empty(1 << 32, dtype=torch.bfloat16, device="meta").as_strided((16, 2048), (ld + step, 1))
+        assert pkg.ops._rows16(x) is x
+        assert (pkg.ops._rows16(x, True) is not x) == copied

@@ -726,7 +726,7 @@ ExpertScratch expert_scratch(uint8_t* base, int64_t T, int64_t topk, int64_t E, 
   x.direct = fuse && !sorted && fp4_direct(R, E, H, I);
   sorted |= x.direct;  // (no sort)
   x.sort_bytes = sorted ? 0 : mxl_moe_route_workspace_bytes(T, topk, E);
-  x.fused = fuse && mxl_mxfp4_grouped_swiglu_supported(R, E, I, H);
+  x.fused = fuse && T <= (int64_t(1) << 31) / H && mxl_mxfp4_grouped_swiglu_supported(R, E, I, H);  // (32-bit offsets)
   x.tiles = fuse && !x.fused && fp4_swiglu_tiles(T, R, E, I, H);
   if (!sorted) {
     x.routes = p.take(R * 4);

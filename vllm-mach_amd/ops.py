@@ -794,12 +794,14 @@ def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]
             raise ValueError(f"{what}: tensors on {device} and {t.device}")
 
 
-def _rows16(x: torch.Tensor) -> torch.Tensor:
-    """x as rows of unit column stride that start on 16 bytes (a copy where they do not, and of rows further apart
-    than the kernels' offsets reach)."""
+def _rows16(x: torch.Tensor, near: bool = False) -> torch.Tensor:
+    """x as rows of unit column stride that start on 16 bytes; a copy where they do not, and (``near``: for the kernels
+    that quantize under a product, whose byte offsets have 32 bits) where gaps between them spread them over more than
+    4 GiB."""
     m, k = x.shape
     ld = x.stride(0) if m > 1 else k
-    if (x.stride(1) != 1 and k > 1) or ld % 8 or ld < k or x.data_ptr() % 16 or (m - 1) * ld + k > 1 << 31:
+    if ((x.stride(1) != 1 and k > 1) or ld % 8 or ld < k or x.data_ptr() % 16
+            or (near and ld != k and (m - 1) * ld + k > 1 << 31)):
         return torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
     return x
 
@@ -960,7 +962,7 @@ def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, rul
     bias = _fp4_bias("mxfp4_linear", bias, n)
     out = x.new_empty((M, n))
     if M:
-        x = _aligned(x, 16) if swiglu else _rows16(x)
+        x = _aligned(x, 16) if swiglu else _rows16(x, M <= 16)  # (more rows are quantized by themselves)
         with _on(x.device):
             nbytes = query("mxl_mxfp4_linear_workspace_bytes", M, n, K, int(swiglu))
             ws = _scratch(nbytes, w)
@@ -1038,7 +1040,7 @@ def mxfp4_grouped_swiglu(x: torch.Tensor, row_index: Optional[torch.Tensor], row
     row_index, offsets = _fp4_groups("mxfp4_grouped_swiglu", x.shape[0], row_index, row_div, expert_offsets, routed_rows)
     E, k = offsets.numel() - 1, x.shape[1]
     w, sw = _fp4_weight("mxfp4_grouped_swiglu", w, sw, 2 * i, k, E)
-    x = _rows16(x)
+    x = _rows16(x, True)
     codes = torch.empty((routed_rows, i // 2), dtype=torch.uint8, device=x.device)
     scales = torch.empty((routed_rows, i // 32), dtype=torch.uint8, device=x.device)
     if routed_rows:
@@ -1091,7 +1093,7 @@ def mxfp4_experts(output: torch.Tensor, x: torch.Tensor, topk_ids: Optional[torc
     w2, sw2 = _fp4_weight("mxfp4_experts", w2, sw2, H, i, e)
     out = output if output.data_ptr() % 16 == 0 else torch.empty((T, H), dtype=torch.bfloat16, device=x.device)
     if T:
-        x = _rows16(x)
+        x = _rows16(x, True)
         weights = topk_weights.to(torch.float32).contiguous()
         ids = None if given else topk_ids.to(torch.int32).contiguous()
         with _on(x.device):
