@@ -781,3 +781,21 @@ def test_rows_up_to_four_gib_apart(pkg, dev, m, k, beyond):
     one, two = (pkg.ops.mxfp4_grouped_swiglu(v, routes, topk, offsets, m * topk, w1, experts.w1_scale, 128)
                 for v in (x, near))
     assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
+def test_pack_experts_past_64_gib(pkg, dev):
+    """Experts whose tiled codes together pass 2^32 pieces of 16 bytes: the first, one in the middle, those on both
+    sides of the border and the last against each packed by itself."""
+    n, k = 8192, 8192
+    e = (1 << 36) // (n * k // 2) + 2
+    _need(145)
+    codes = torch.empty(e, n, k // 2, dtype=torch.uint8, device=dev)
+    scales = torch.empty(e, n, k // 32, dtype=torch.uint8, device=dev)
+    at = [0, e // 2 - 2, e // 2 - 1, e // 2, e - 3, e - 2, e - 1]
+    for x in at:
+        codes[x].random_(0, 256)
+        scales[x].random_(0, 255)
+    w, sw = pkg.ops.pack_weight(codes, scales, pkg.ops.E2M1)
+    for x in at:
+        one, s = pkg.ops.pack_weight(codes[x], scales[x], pkg.ops.E2M1)
+        assert torch.equal(w[x], one) and torch.equal(sw[x], s)

@@ -39,6 +39,7 @@
 // cannot fill 256 CUs, S workgroups split K further and write fp32 partials
 // that a second kernel sums in split order: both orders are fixed, so every
 // result is deterministic.
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 #include <string>
@@ -444,14 +445,21 @@ static int pack_common(const void* codes, const void* scales, int scale_layout, 
   hipStream_t s = (hipStream_t)stream;
   const int64_t NTl = (N + 15) / 16, KT = (K + kTileK - 1) / kTileK;
   const int CH = tile_chunks(fmt);
-  const int64_t total = NTl * KT * CH * 64;
   const int64_t ld = fmt == kE4M3 ? K : fmt == kE2M1 ? K / 2 : K * 3 / 4;
-  if (fmt == kE2M1)
-    pack_fp4_kernel<<<dim3((unsigned)((total + 255) / 256)), 256, 0, s>>>((const uint8_t*)codes, ld,
-                                                                         (uint8_t*)tiled_codes, N, KT, total);
-  else pack_weight_kernel<<<dim3((unsigned)((total + 255) / 256)), 256, 0, s>>>(
-      (const uint8_t*)codes, ld, (uint8_t*)tiled_codes, N, K, KT, CH, fmt != kE4M3, total);
-  MXL_CHECK_LAUNCH("mxl_pack_weight(codes)");
+  // n-tiles of a launch: a launch has fewer than 2^32 threads, a thread for 16 bytes (many experts' weights side by side
+  // pass that at 64 GiB; the scales, a thread for 4 bytes of 17 or more, stay below it)
+  const int64_t pieces = KT * CH * 64, most = std::max<int64_t>((int64_t(1) << 31) / pieces, 1);
+  MXL_CHECK_ARG(pieces < (int64_t(1) << 32) && NTl * KT * 64 < (int64_t(1) << 32), "mxl_pack_weight: too large (N=%lld K=%lld)",
+                (long long)N, (long long)K);
+  for (int64_t nt = 0; nt < NTl; nt += most) {
+    const int64_t total = std::min(most, NTl - nt) * pieces, rows = N - nt * 16;
+    const uint8_t* const src = (const uint8_t*)codes + nt * 16 * ld;
+    uint8_t* const dst = (uint8_t*)tiled_codes + nt * pieces * 16;
+    const dim3 grid((unsigned)((total + 255) / 256));
+    if (fmt == kE2M1) pack_fp4_kernel<<<grid, 256, 0, s>>>(src, ld, dst, rows, KT, total);
+    else pack_weight_kernel<<<grid, 256, 0, s>>>(src, ld, dst, rows, K, KT, CH, fmt != kE4M3, total);
+    MXL_CHECK_LAUNCH("mxl_pack_weight(codes)");
+  }
   if (scales) {
     const int64_t ts = NTl * KT * 64;
     pack_scale_kernel<<<dim3((unsigned)((ts + 255) / 256)), 256, 0, s>>>(
