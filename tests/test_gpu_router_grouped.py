@@ -186,3 +186,20 @@ def test_a_token_routes_alike_in_any_batch(pkg, dev):
         assert torch.equal(part[1], whole[1][lo:hi])
         # (binary64 sums in another order, then one rounding to fp32)
         assert bool(((part[0] - whole[0][lo:hi]).abs() <= 2.0 ** -23 * whole[0][lo:hi]).all())
+
+
+@pytest.mark.parametrize("T", [1, 40, 3000])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_group_scores_past_the_largest_fp32(pkg, dev, T, sigmoid):
+    """Biases whose sum of two passes the largest fp32 value, in every group: the groups' order is that of the sums."""
+    g = torch.Generator().manual_seed(T)
+    top = torch.finfo(torch.float32).max
+    # groups of two, of which the second has the larger sum (-1.03 of `top`) and not the larger value
+    bias = torch.tensor([-.3, -.75, -.31, -.72, -.4, -.7, -.33, -.73]) * top
+    for keep, topk in ((1, 1), (1, 2), (2, 1), (3, 3)):
+        _check(pkg, torch.randn(T, 8, generator=g), bias, topk, sigmoid, 4, keep, True, 1.0)
+    share = torch.tensor([[.9, .7, .69, .6], [.85, .84, .2, .19], [.95, .94, .93, .92], [1.0, .81, .99, .8]])
+    for sign in (-1.0, 1.0):
+        bias = (share * top * sign).flatten()
+        for keep, topk in ((1, 4), (2, 5), (3, 12)):
+            _check(pkg, torch.randn(T, 16, generator=g), bias, topk, sigmoid, 4, keep, True, 1.0)

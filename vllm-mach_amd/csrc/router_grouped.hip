@@ -319,6 +319,7 @@ struct GroupedToken {
       if (LPT > 16 && deal.lpg_log > 4) merge(__shfl_xor(a1, 16, 64), __shfl_xor(a2, 16, 64));
       const bool two = g.bias && g.size > 1;
       const float mine = two ? a1 + a2 : a1;
+      close |= grp < g.groups && __builtin_fabsf(mine) == __builtin_inff();  // (past the largest binary32: not in order)
       // (sums of two have twice the error, on both sides; the group of the larger magnitudes finds a close call)
       const float scale = two ? 0.25f : 1.0f, mag = 2 * (two ? __builtin_fabsf(a1) + __builtin_fabsf(a2) : __builtin_fabsf(a1));
       int ahead = 0;
