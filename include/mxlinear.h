@@ -92,9 +92,11 @@ int mxl_mxfp4_gemm(const void* a, const void* sa, int64_t M, const void* w_tiled
                    void* stream);
 
 /* mxl_quantize_mxfp4 then mxl_mxfp4_gemm in one launch: bf16 x [M, K] (row stride ldx, 16-byte
- * aligned, ((M - 1) ldx + K) 2 bytes at most 4 GiB) of few rows, quantized inside the product (the
- * same bits).  Shapes: mxl_mxfp4_quant_gemm_supported (up to 16 rows, fewer of a long K or a
- * wide N), else MXL_EUNSUPPORTED. */
+ * aligned, ((M - 1) ldx + K) 2 bytes at most 4 GiB) of few rows, quantized inside the product: the
+ * same codes, but K may be split over other waves than mxl_mxfp4_gemm splits it, whose fp32 sums then
+ * join in another order (either within K 2^-23 of the products' magnitudes, ahead of the rounding).
+ * Shapes: mxl_mxfp4_quant_gemm_supported (up to 16 rows, fewer of a long K or a wide N), else
+ * MXL_EUNSUPPORTED. */
 int mxl_mxfp4_quant_gemm_supported(int64_t M, int64_t N, int64_t K);
 int mxl_mxfp4_quant_gemm(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, const void* w_tiled,
                          const void* sw_tiled, int64_t N, const void* bias, void* out, int64_t ldc, void* stream);
@@ -102,7 +104,9 @@ int mxl_mxfp4_quant_gemm(const void* x, int64_t M, int64_t K, int64_t ldx, int r
 /* An expert layer's first half in one launch, for few rows an expert: quantized rows of
  * bf16 x [a_rows, K] (gathered as mxl_mxfp4_grouped_gemm does), the gate/up product with
  * W13[e] [2 I, K], and mxl_swiglu_mxfp4 of its rounded result: codes [routed_rows, I/2] and
- * scales [routed_rows, I/32] of the routed rows.  x spans at most 4 GiB.  Shapes:
+ * scales [routed_rows, I/32] of the routed rows.  A K split joins as in mxl_mxfp4_quant_gemm, so a
+ * gate or up next to a rounding border may fall to its other side against the separate launches, and
+ * move a code.  x spans at most 4 GiB.  Shapes:
  * mxl_mxfp4_grouped_swiglu_supported (fewer than 8 rows an expert, I % 32 == 0), else
  * MXL_EUNSUPPORTED. */
 int mxl_mxfp4_grouped_swiglu_supported(int64_t routed_rows, int64_t num_experts, int64_t I, int64_t K);
@@ -126,8 +130,9 @@ int mxl_mxfp4_linear(const void* x, int64_t M, int64_t K, int64_t ldx, int swigl
  * product with w2 [E][H, I], and the combine with fp32 topk_weights [T, topk] into out bf16
  * [T, H].  fuse: the SwiGLU producer in the gate/up product's launch, with few rows an expert
  * the quantization too (mxl_mxfp4_grouped_swiglu; four launches from the ids, without the
- * sort three up to 32 routes, else five): the bits are those of separate launches.
- * H, I multiples of 128; the workspace, 256-byte aligned, holds
+ * sort three up to 32 routes, else five).  The routes of topk_ids give the bits of the same routes
+ * sorted; separate launches (fuse 0) give those of many rows an expert, and for few rows differ
+ * as mxl_mxfp4_grouped_swiglu does.  H, I multiples of 128; the workspace, 256-byte aligned, holds
  * mxl_mxfp4_experts_workspace_bytes (sorted: the routes are given). */
 int64_t mxl_mxfp4_experts_workspace_bytes(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int sorted,
                                           int fuse);

@@ -949,8 +949,9 @@ def _(a, sa, w, sw, n, k, bias=None):
 def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, rule: int = FLOOR_CARRY175,
                  bias: Optional[torch.Tensor] = None, swiglu: bool = False) -> torch.Tensor:
     """bf16 rows x [M, K] quantized to MXFP4 (``quantize_mxfp4``) and multiplied with an MXFP4 weight
-    (``mxfp4_gemm``), the bits of the two; with ``swiglu`` gate/up rows [M, 2K] through ``swiglu_mxfp4``.
-    One launch for few rows, else two."""
+    (``mxfp4_gemm``); with ``swiglu`` gate/up rows [M, 2K] through ``swiglu_mxfp4``.  One launch for few rows, which
+    may split K over other waves than ``mxfp4_gemm`` does and join the fp32 sums in another order, else two with the
+    bits of the two operators."""
     _same_device("mxfp4_linear", x, w, sw, bias)
     if swiglu:
         _fp4_gate_up("mxfp4_linear", x)
@@ -1029,8 +1030,8 @@ def mxfp4_grouped_swiglu(x: torch.Tensor, row_index: Optional[torch.Tensor], row
                          ) -> tuple[torch.Tensor, torch.Tensor]:
     """An expert layer's first half in one launch: ``quantize_mxfp4`` of the gathered bf16 rows x [T, K],
     ``mxfp4_grouped_gemm`` with the gate/up weights [E, 2 I, K] and ``swiglu_mxfp4`` of its rows -> (codes u8
-    [routed_rows, I/2], scales u8 [routed_rows, I/32]).  x is at most 4 GiB.  Rows past expert_offsets[E] are left
-    unwritten."""
+    [routed_rows, I/2], scales u8 [routed_rows, I/32]).  The fp32 sums of a K split may join in another order than
+    those of ``mxfp4_grouped_gemm``.  x is at most 4 GiB.  Rows past expert_offsets[E] are left unwritten."""
     _same_device("mxfp4_grouped_swiglu", x, row_index, expert_offsets, w, sw)
     if x.dtype != torch.bfloat16 or x.ndim != 2:
         raise ValueError("mxfp4_grouped_swiglu needs bf16 rows [T, K]")
@@ -1067,7 +1068,9 @@ def mxfp4_experts(output: torch.Tensor, x: torch.Tensor, topk_ids: Optional[torc
     i32 [T, k] sorted (``moe_route``; or given sorted, as ``moe_route`` and the routers return them), the gate/up
     product of the quantized rows with w13 [e, 2 i, H], ``swiglu_mxfp4``, the product with w2 [e, H, i] and
     ``moe_reduce`` with the fp32 weights [T, k].  ``fuse``: the SwiGLU producer in the gate/up product's launch, with
-    few rows an expert the quantization too (the same bits as separate launches)."""
+    few rows an expert the quantization too.  Ids give the bits of the same routes sorted.  Separate launches give the
+    same bits for many rows an expert; for few they may join a K split's fp32 sums in another order, so that a gate or up
+    next to a rounding border moves a code of the activation."""
     _same_device("mxfp4_experts", x, output, topk_ids, topk_weights, sorted_routes, expert_offsets, inverse, w13, sw13, w2, sw2)
     if x.dtype != torch.bfloat16 or x.ndim != 2:
         raise ValueError("mxfp4_experts needs bf16 x [T, H]")
