@@ -799,3 +799,69 @@ def test_pack_experts_past_64_gib(pkg, dev):
     for x in at:
         one, s = pkg.ops.pack_weight(codes[x], scales[x], pkg.ops.E2M1)
         assert torch.equal(w[x], one) and torch.equal(sw[x], s)
+
+
+def test_rows_past_2_31_values(pkg, dev):
+    """Contiguous activations of more than 2^31 values: the rows around the border and the last."""
+    m, n, k = (1 << 19) + 999, 40, 4096
+    _need(16)
+    g = torch.Generator().manual_seed(m)
+    (w, sw), wv = _weight(pkg, g, n, k)
+    at = torch.cat([torch.arange(300), torch.arange((1 << 19) - 300, (1 << 19) + 300), torch.arange(m - 300, m)])
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=dev)
+    rows = _x(g, len(at), k)
+    x[at.to(dev)] = rows.to(dev)
+    want = ref.quantize(rows)
+    _equal([t[at.to(dev)] for t in pkg.ops.quantize_mxfp4(x)], want)
+    ref.check_product(pkg.ops.mxfp4_linear(x, w, sw, n)[at.to(dev)], ref.dequantize(*want), wv)
+
+
+@pytest.mark.parametrize("m,n,k,split", [(16, 264, 1152, False), (5, 2048, 2048, False), (200, 1032, 384, False),
+                                         (48, 1030, 640, False), (40, 130, 8192, True)])
+def test_rows_do_not_reach_each_other(pkg, dev, m, n, k, split):
+    """An output row is that of its own activations, bit for bit, whatever the others hold, NaN scales among them: few
+    rows, tiles with an odd number of K128 slices (whose last copy ends in the row behind), a K split."""
+    g = torch.Generator().manual_seed(m + n)
+    (w, sw), _ = _weight(pkg, g, n, k)
+    assert (pkg.ops.query("mxl_mxfp4_gemm_workspace_bytes", m, n, k) > 0) == split
+    a, sa = (t.to(dev) for t in ref.random_operand(g, m, k))
+    whole = pkg.ops.mxfp4_gemm(a, sa, w, sw, n, k)
+    for row in sorted({0, 1, m // 2, m - 2, m - 1}):
+        b, sb = (t.to(dev) for t in ref.random_operand(g, m, k, 20))
+        sb[row ^ 1 if row ^ 1 < m else row - 1] = 255
+        b[row], sb[row] = a[row], sa[row]
+        y = pkg.ops.mxfp4_gemm(b, sb, w, sw, n, k)
+        assert torch.equal(y[row], whole[row])
+        assert bool(y[row ^ 1 if row ^ 1 < m else row - 1].isnan().all())
+
+
+def test_vmap_and_forward_mode(pkg, dev):
+    """Under vmap and forward-mode differentiation the operator itself is called: its values are those of plain calls."""
+    g = torch.Generator().manual_seed(2)
+    (w, sw), _ = _weight(pkg, g, 64, 256)
+    x = _x(g, 6, 256).to(dev)
+    lin = lambda v: pkg.ops.mxfp4_linear(v, w, sw, 64)  # noqa: E731
+    want = lin(x)
+    assert torch.equal(torch.func.vmap(lin)(x.view(2, 3, 256)).flatten(0, 1), torch.cat([lin(x[:3]), lin(x[3:])]))
+    assert torch.equal(torch.func.jvp(lin, (x,), (x,))[0], want)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, x)
+        assert torch.equal(torch.autograd.forward_ad.unpack_dual(lin(dual)).primal, want)
+
+
+@pytest.mark.parametrize("t,e,topk", [(1, 8, 2), (20, 3, 2), (90, 3, 2)])
+def test_experts_wider_than_one_launch(pkg, dev, t, e, topk):
+    """Hidden sizes past what a workgroup's waves hold of K: quantizer, product and producer are launches of their own,
+    from ids and from a router's logits alike."""
+    h, i = 7168, 384
+    assert not pkg.ops.mxfp4_grouped_swiglu_supported(t * topk, e, i, h)
+    g = torch.Generator().manual_seed(t)
+    experts, w1, w2, v1, v2 = _experts(pkg, g, e, h, i)
+    x, z = _x(g, t, h), torch.randn(t, e, generator=g).to(dev)
+    p, ids = pkg.select_experts(z, topk)
+    got, routed = experts(x.to(dev), w1, w2, p, ids), torch.empty(t, h, dtype=torch.bfloat16, device=dev)
+    experts.apply_router(routed, x.to(dev), w1, w2, z, topk)
+    assert torch.equal(got, routed)
+    want = _exact_layer(x, p.cpu(), ids.cpu(), v1, v2)
+    # (see test_experts_layer)
+    assert float((got.cpu().double() - want).norm() / want.norm()) <= 2 * 2.0 ** -8 + 2.0 ** -10 * 3
