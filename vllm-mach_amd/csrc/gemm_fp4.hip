@@ -36,8 +36,8 @@ __device__ __forceinline__ v4f mfma_fp4(const uint4& w, const uint4& a, v4f c, u
 // weights are read once whatever its rows.  SWIGLU (an expert's gate/up product): the workgroup's n-tiles are two
 // of gate and the same two of up, and the epilogue quantizes the 32 columns' bf16(bf16(silu(g)) u) in place of
 // storing gate and up.
-// Cold weights: 1 x 2048 x 2048 3.9 us; w13 and w2 of 64 tokens, top 8 of 256 experts (K = 2048, I = 512) 50 and 24 us,
-// 5 TB/s of weights, the rate of a large copy.
+// Cold weights: 1 x 2048 x 2048 3.9 us; w13 and w2 of 64 tokens, top 8 of 256 experts (K = 2048, I = 512) 52 and 24 us,
+// 4.8 and 5.2 TB/s of weights, the rate of a large copy (5.2).
 //
 // kRoutes: a few routes as they come, their experts in row_index and route r's activation row r / row_div: no sort.
 enum Fp4Unit : int { kExperts = 0, kHitExperts = 1, kRoutes = 2 };
@@ -404,8 +404,10 @@ static bool fp4_rows_reach(int64_t rows, int64_t ldx, int64_t K) {
   return rows <= 1 || rows - 1 <= ((int64_t(1) << 31) - K) / ldx;
 }
 
-// A stage of the 2 x 2-wave tiles is 128 bytes of a row, whatever its format, and takes two MFMAs of a K128
-// slice of MXFP4 the time of one of 8-bit activations: the time model of K / 2 bytes holds.
+// A stage of the 2 x 2-wave tiles is 128 bytes of a row, whatever its format, and its two MFMAs of a K128 slice
+// of MXFP4 take the time of one of 8-bit activations, so the plan is the time model's of K / 2 columns.  Its costs (and
+// the hybrid's borders) are fitted to 8-bit stages, not to these: a 128 x 64 stage measures 0.41 us here (512 x 2560 x
+// 9216, 36 stages whole-K in 19.8) and 0.289 there.  Splits end on 1024 columns, two super-tiles.
 static WideConfig fp4_tiles_config(int64_t M, int64_t N, int64_t K) {
   const int64_t KT = (K + kTileK - 1) / kTileK;
   WideConfig c = wide_tiles_config(M, N, (K / 2 + 127) / 128 * 128, false);

@@ -15,8 +15,9 @@
 // Each group has 2^lpg_log of them (the most that fit), each lane successive experts of its group, so that a group's
 // two largest c come from lpg_log exchanges of all groups at once and the lowest lane is the lowest index.
 //
-// Instructions bound it (256 logits are 1 KiB and a thousand operations).  Scores of every expert in binary64 are most
-// of them, so the choice is first made in binary32 (choose_fast):
+// Its instructions and what they wait for bound it (256 logits are 1 KiB and a thousand operations; 16384 tokens read at
+// 0.9 TB/s, with the VALU busy a third of the time, 1.6 wavefronts a SIMD and 41 % of theirs spent in waits).  Scores of
+// every expert in binary64 are most of the instructions, so the choice is first made in binary32 (choose_fast):
 // - the values are 32-bit keys in value order, their lowest log2(NS) bits the slot.  Each lane sorts its own once, by
 //   a network; a round of the choice then is one DPP maximum of the lanes' first keys, and the winner moves up by one.
 // - without a bias the values are the logits themselves.  Logits 2^-20 apart have binary64 scores apart, where none is
@@ -27,7 +28,7 @@
 //   reciprocal are off by 2 u each, so sigmoid is within 4 u.  Softmax's sum takes NS + 5 roundings, so s is within
 //   (NS + 14) u < 46 u of its largest, 1 / sum.  The bias adds u |c|, the key's cut 2 (NS - 1) u |c|.
 // Where every call -- the groups', each expert's against the next -- stands apart by more than the errors of both
-// sides, the choice is the true one; for a token with a closer call (or an infinity or NaN), one in some hundred, the
+// sides, the choice is the true one; for a token with a closer call (or an infinity or NaN, a group's sum among them), one in some hundred, the
 // whole wavefront makes it in binary64 (choose_exact: 64-bit keys, compared by their halves).
 // The weights are of binary64 scores of the k chosen, one a lane.
 //
