@@ -664,9 +664,10 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       return y != y ? (d & 0x0000FFFFu) | 0x7FC00000u : d;
     };
     // BIAS: one is added to the rounded output (MXFP8 2048 x 18432 x 2560 135 us with a pass of its
-    // own, 104 here, 222 through the LDS below), to MXFP4's sums ahead of the rounding.  WIDE (MXFP4, rows of whole 16-byte pieces): of two n-tiles side
-    // by side every other 16 lanes change places, after which a lane holds eight consecutive columns of one
-    // of them: half the stores, of 64 bytes of a row each (4096 x 17408 x 5120 206 -> 198 us).
+    // own, 104 here, 222 through the LDS below), to MXFP4's sums ahead of the rounding.  WIDE (MXFP4, rows of
+    // whole 16-byte pieces): of two n-tiles side by side every other 16 lanes change places, after which a lane holds
+    // eight consecutive columns of one of them: half the stores, of 64 bytes of a row each (4096 x 17408 x 5120
+    // 206 -> 198 us).
     auto store = [&](auto BIAS, auto WIDE) {
       constexpr bool wide = decltype(WIDE)::value;
       u2 bias[NTW];

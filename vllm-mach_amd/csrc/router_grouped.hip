@@ -28,8 +28,8 @@
 //   reciprocal are off by 2 u each, so sigmoid is within 4 u.  Softmax's sum takes NS + 5 roundings, so s is within
 //   (NS + 14) u < 46 u of its largest, 1 / sum.  The bias adds u |c|, the key's cut 2 (NS - 1) u |c|.
 // Where every call -- the groups', each expert's against the next -- stands apart by more than the errors of both
-// sides, the choice is the true one; for a token with a closer call (or an infinity or NaN, a group's sum among them), one in some hundred, the
-// whole wavefront makes it in binary64 (choose_exact: 64-bit keys, compared by their halves).
+// sides, the choice is the true one; for a token with a closer call (or an infinity or NaN, a group's sum among them),
+// one in some hundred, the whole wavefront makes it in binary64 (choose_exact: 64-bit keys, compared by their halves).
 // The weights are of binary64 scores of the k chosen, one a lane.
 //
 // 16384 tokens of 256 experts, 8 of 128 in 4 of 8 groups: 19 us (31.3 with every score in binary64 and a token per

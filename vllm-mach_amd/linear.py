@@ -163,8 +163,8 @@ def _epilogue_bias(bias: Optional[torch.Tensor], x: torch.Tensor, n: int) -> Opt
     """``bias`` if the GEMM's epilogue can add it (the bits of ``y + bias``: the rounded output
     plus the bias, rounded again; MXFP4's adds it to the sum, rounded once), else None: a
     contiguous bf16 [n] tensor on x's device that carries no gradient, tangent or batch dimension
-    into the addition.  Saves the pass over the output and its launch (eager, us a call: W6A8 333 x 5120 x 2688 42.5 -> 36.3, one MXFP8 row 22.7 ->
-    19.8)."""
+    into the addition.  Saves the pass over the output and its launch (eager, us a call: W6A8
+    333 x 5120 x 2688 42.5 -> 36.3, one MXFP8 row 22.7 -> 19.8)."""
     if bias is None or type(bias) not in (torch.Tensor, torch.nn.Parameter):
         return None
     if bias.dtype != torch.bfloat16 or tuple(bias.shape) != (n,) or bias.device != x.device:
