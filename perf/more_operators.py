@@ -274,7 +274,8 @@ def _quantized(fmt, x):
     amax's power of two under the format's largest, doubled from 1.75 of it on; block-FP8: per 128 amax / 448."""
     if fmt == "block":
         b = x.float().view(len(x), -1, 128)
-        s = b.abs().amax(-1, keepdim=True).clamp_min(1e-10) / 448
+        s = b.abs().amax(-1, keepdim=True).clamp_min(1e-10)
+        s = s / torch.full_like(s, 448)  # (by a number torch multiplies with its reciprocal)
         return ((b / s).clamp(-448, 448).to(torch.float8_e4m3fn).float() * s).view(x.shape)
     b = x.float().view(len(x), -1, 32)
     amax = b.abs().amax(-1, keepdim=True)
@@ -397,7 +398,8 @@ def _exact_quantized(fmt, x):
     b = x.double().view(len(x), -1, group)
     amax = b.abs().amax(-1, keepdim=True)
     if top is None:
-        scale = (amax.clamp_min(1e-10).float() / 448).double()  # its scale and quotient are binary32 by definition
+        # its scale and quotient are binary32 by definition, correctly rounded
+        scale = (amax.clamp_min(1e-10).float() / torch.full_like(amax, 448, dtype=torch.float32)).double()
         v = (b.float() / scale.float()).double().clamp(-448, 448)
     else:
         e = torch.frexp(amax.clamp_min(2.0 ** -100))[1].double() - 1
