@@ -559,6 +559,61 @@ int mxl_moe_reduce(const void* routed_output, const float* topk_weights, const i
 int mxl_moe_reduce_add(const void* routed_output, const float* topk_weights, const int32_t* inverse, int64_t T,
                        int64_t topk, int64_t H, const void* addend, void* out, void* stream);
 
+/* ---- beside and behind a layer: adapters, gated blocks, gradients.  No counterpart in the reference. ----
+ *
+ * The input gradient of a frozen layer, dx = dy W: dy bf16 [M, N] (row stride lddy), W [N, K] tiled
+ * with its tiled E8M0 scales, or (block = 1, fmt 0) fp32 scales [ceil(N/128), K/128]; out bf16 [M, K]
+ * (row stride ldo).  The codes' values are exact in bf16 wherever they are normal bf16 numbers; fp32
+ * sums.  N % 8 == 0, K % 128 == 0 (rows of W past an N that is no multiple of 16 are zero).  The
+ * workspace, 16-byte aligned, holds mxl_input_grad_workspace_bytes. */
+int64_t mxl_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int mxl_input_grad(const void* dy, int64_t M, int64_t N, int64_t lddy, const void* w_tiled, const void* sw, int64_t K,
+                   int fmt, int block, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* act(x Wg^T) * (x Wu^T) of a tiled MX weight [2 I, K], gate rows then up rows: x bf16 [M, K] (row
+ * stride ldx) quantized by `rule` (MXFP8; of fmt 4 MXFP4), fp32 products, one rounding to out bf16
+ * [M, I] (row stride ldo).  act 0 = silu, 1 = gelu (tanh form).  mxl_gated_grad: from dh bf16 [M, I]
+ * of that output the products' gradients [dh up act'(gate), dh act(gate)] bf16 [M, 2 I], gate and up
+ * computed again.  I % 16 == 0, K % 128 == 0.  The workspace, 256-byte aligned, holds
+ * mxl_gated_workspace_bytes. */
+int64_t mxl_gated_workspace_bytes(int64_t M, int64_t K, int fmt);
+int mxl_gated_linear(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, const void* w_tiled,
+                     const void* sw_tiled, int64_t I, int fmt, int act, void* out, int64_t ldo, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+int mxl_gated_grad(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, const void* w_tiled,
+                   const void* sw_tiled, int64_t I, int fmt, int act, const void* dh, int64_t lddh, void* out,
+                   int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Low-rank adapters of many requests.  A batch of M tokens sorted by adapter (mxl_moe_route of the ids
+ * as [M, 1], at most 2560 adapters): order i32 [M], offsets i64 [slots + 1], and from them the tiles
+ * i32 [mxl_adapter_tile_count][2] that mxl_adapter_tiles writes.
+ *
+ * mxl_adapter_apply: y[t] += scaling[s] b[s] (a[s] x[t]) for every token t of the batch, s its adapter:
+ * y bf16 [M, N] in place, x bf16 [M, K], a bf16 [slots, parts rank, K], b bf16 [slots, N, rank], N =
+ * cols[parts].  A merged layer's part p is columns [cols[p], cols[p + 1]) (multiples of 16 but for the
+ * last) with rows [p rank, (p + 1) rank) of a; rank a multiple of 8 up to 256, up to 8 parts.  cols is
+ * host memory.  v (fp32, mxl_adapter_v_floats of them) receives scaling a x in the batch's order, in
+ * shares that sum to it; it never passes through bf16.
+ *
+ * mxl_adapter_grad, with that v: db and da (bf16, b's and a's shapes; either may be NULL) and, where dx
+ * is given, dx[t] += a[s]^T (scaling[s] b[s]^T dy[t]).  N % 8 == 0.  An adapter without tokens gets
+ * zeros.  Sums are joined in a fixed order.  The workspace, 256-byte aligned, holds
+ * mxl_adapter_grad_workspace_bytes. */
+int64_t mxl_adapter_tile_count(int64_t M, int64_t slots);
+int mxl_adapter_tiles(const int64_t* offsets, int64_t M, int64_t slots, int32_t* tiles, int64_t num_tiles, void* stream);
+int64_t mxl_adapter_v_floats(int64_t M, int64_t K, int64_t slots, int64_t parts, int64_t rank);
+int mxl_adapter_apply(const void* x, int64_t M, int64_t K, int64_t ldx, const void* a, const void* b,
+                      const float* scaling, int64_t slots, int64_t parts, const int64_t* cols, int64_t rank,
+                      const int32_t* order, const int64_t* offsets, const int32_t* tiles, int64_t num_tiles, float* v,
+                      int64_t v_floats, void* y, int64_t ldy, void* stream);
+int64_t mxl_adapter_grad_workspace_bytes(int64_t M, int64_t K, int64_t slots, int64_t parts, const int64_t* cols,
+                                         int64_t rank);
+int mxl_adapter_grad(const void* x, int64_t M, int64_t K, int64_t ldx, const void* dy, int64_t lddy, const void* a,
+                     const void* b, const float* scaling, int64_t slots, int64_t parts, const int64_t* cols,
+                     int64_t rank, const int32_t* order, const int64_t* offsets, const int32_t* tiles, int64_t num_tiles,
+                     const float* v, int64_t v_floats, void* dx, int64_t lddx, void* da, void* db, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 /* The kernels a dense GEMM call (mxl_mx_gemm_ex, block = 0; mxl_block_fp8_gemm_ex,
  * block = 1) or a grouped GEMM call (mxl_grouped_gemm_ex, prod = 0;
  * mxl_grouped_gemm_quant, prod = 1; mxl_grouped_gemm_swiglu, prod = 2) launches

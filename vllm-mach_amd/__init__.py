@@ -18,11 +18,13 @@ from .linear import (  # noqa: F401
     Mxfp8LinearKernel,
     MxLinearLayerConfig,
     MxLinearMethod,
+    gated_linear,
     is_mi355x_available,
     register_kernels,
     swiglu_mxfp4_down,
     swiglu_mxfp8_down,
 )
+from .adapters import AdapterBatch, LowRankAdapters  # noqa: F401
 from .moe import (  # noqa: F401
     GroupedRouting,
     Mxfp4Experts,

@@ -1,0 +1,211 @@
+"""Low-rank adapters of many requests beside a shared quantized linear layer.
+
+``LowRankAdapters`` holds the adapters of one prepared layer in slots, ``AdapterBatch`` says which slot each token of a
+batch uses; ``MxLinearMethod.apply(layer, x, bias, adapters=, batch=)`` adds them to the layer's output:
+
+    y[t] = layer(x[t]) + scaling[s] * lora_b[s] @ (lora_a[s] @ x[t]),   s the slot of token t
+
+One batch serves every layer of a step.  The adapters see the unquantized bf16 input; their sums are fp32.  Both
+``lora_a`` and ``lora_b``, and the input, have gradients, the layer's own weight stays frozen.  No counterpart in the
+reference.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import ops
+from .linear import _function_bias
+
+
+class AdapterBatch:
+    """The adapter slot of each token of a batch, sorted for the kernels.
+
+    ``ids``: integers [M] on the layers' device; a value outside [0, slots) is a token without an adapter.  ``update``
+    takes the next step's ids into the same memory, for graphs that were captured with it.
+    """
+
+    def __init__(self, ids: torch.Tensor, slots: int):
+        self.slots = int(slots)
+        self.order, self.offsets, self.tiles = ops.adapter_batch(ids, self.slots)
+
+    def __len__(self) -> int:
+        return self.order.shape[0]
+
+    def update(self, ids: torch.Tensor) -> "AdapterBatch":
+        if tuple(ids.shape) != tuple(self.order.shape) or ids.device != self.order.device:
+            raise ValueError(f"update needs ids of {len(self)} tokens on {self.order.device}, got {tuple(ids.shape)} on "
+                             f"{ids.device}")
+        for kept, new in zip((self.order, self.offsets, self.tiles), ops.adapter_batch(ids, self.slots)):
+            kept.copy_(new)
+        return self
+
+
+class LowRankAdapters(torch.nn.Module):
+    """``slots`` adapters of up to ``rank`` (a multiple of 8, at most 256) beside a prepared layer.
+
+    ``lora_a`` bf16 [slots, parts * rank, K]: each merged part of the layer (``layer.logical_widths``) has ``rank`` rows;
+    ``lora_b`` bf16 [slots, N, rank]; ``scaling`` fp32 [slots].  All zero at first, so a slot adds nothing until it is
+    loaded.  Without gradients until ``requires_grad_()``.
+    """
+
+    def __init__(self, layer: torch.nn.Module, slots: int, rank: int, device=None):
+        super().__init__()
+        if not hasattr(layer, "mxl_shape"):
+            raise ValueError("adapters need a layer that process_weights_after_loading has prepared")
+        if not 0 < slots <= 2048:
+            raise ValueError(f"1 to 2048 slots ({slots})")
+        if rank % 8 or not 8 <= rank <= 256:
+            raise ValueError(f"ranks of 8 to 256, multiples of 8 ({rank}): pad smaller ones with zeros")
+        n, k = layer.mxl_shape
+        widths = list(getattr(layer, "logical_widths", None) or [n])
+        if sum(widths) != n or len(widths) > 8 or any(w % 16 for w in widths[:-1]) or (len(widths) > 1 and widths[-1] % 16):
+            raise ValueError(f"up to 8 merged parts of multiples of 16 columns, {n} together ({widths})")
+        device = layer.weight.device if device is None else device
+        self.slots, self.rank, self.widths = int(slots), int(rank), widths
+        self.cols = [sum(widths[:i]) for i in range(len(widths) + 1)]
+        self.lora_a = torch.nn.Parameter(torch.zeros((slots, len(widths) * rank, k), dtype=torch.bfloat16, device=device),
+                                         requires_grad=False)
+        self.lora_b = torch.nn.Parameter(torch.zeros((slots, n, rank), dtype=torch.bfloat16, device=device),
+                                         requires_grad=False)
+        self.register_buffer("scaling", torch.zeros(slots, dtype=torch.float32, device=device))
+
+    def _slot(self, slot: int) -> int:
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"slot {slot} of {self.slots}")
+        return slot
+
+    @torch.no_grad()
+    def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scaling: float, part: Optional[int] = None) -> None:
+        """Put one adapter's a [r, K] and b [columns, r] (r <= rank) into a slot: of the merged part ``part``, or (None) of
+        a layer of one part.  ``scaling`` is the slot's (alpha / r by custom), the same for all of its parts."""
+        if part is None and len(self.widths) > 1:
+            raise ValueError(f"the layer has {len(self.widths)} merged parts: name one")
+        p = 0 if part is None else part
+        if not 0 <= p < len(self.widths):
+            raise ValueError(f"part {p} of {len(self.widths)}")
+        r, k = a.shape[0], self.lora_a.shape[2]
+        if a.ndim != 2 or a.shape[1] != k or tuple(b.shape) != (self.widths[p], r) or not 0 < r <= self.rank:
+            raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} are no adapter of rank <= {self.rank} of "
+                             f"[{self.widths[p]}, {k}]")
+        slot = self._slot(slot)
+        to_a = self.lora_a.data[slot, p * self.rank:(p + 1) * self.rank]
+        to_b = self.lora_b.data[slot, self.cols[p]:self.cols[p + 1]]
+        to_a.zero_()[:r].copy_(a)
+        to_b.zero_()[:, :r].copy_(b)
+        self.scaling[slot] = float(scaling)
+
+    @torch.no_grad()
+    def clear(self, slot: int) -> None:
+        slot = self._slot(slot)
+        for t in (self.lora_a.data, self.lora_b.data, self.scaling):
+            t[slot].zero_()
+
+
+def grad_of(layer: torch.nn.Module) -> tuple:
+    """What ``ops.input_grad`` takes of a prepared layer: (w, sw, n, k, format, block)."""
+    n, k = layer.mxl_shape
+    if hasattr(layer, "mxl_block_scale"):
+        return layer.weight, layer.mxl_block_scale, n, k, ops.E4M3, True
+    return layer.weight, layer.weight_scale, n, k, layer.mxl_format, False
+
+
+class FrozenLinear(torch.autograd.Function):
+    """A prepared layer's product (with a bias in its epilogue) with the gradients of its input and the bias."""
+
+    @staticmethod
+    def forward(x, w, sw, layer, bias):
+        return layer.mxl_kernel.apply_weights(layer, x, bias)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, w, sw, layer, _ = inputs
+        ctx.save_for_backward(w, sw)
+        ctx.meta = grad_of(layer)[2:]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        w, sw = ctx.saved_tensors
+        n, k, fmt, block = ctx.meta
+        dy2 = dy.reshape(-1, n)
+        dx = ops.input_grad(dy2, w, sw, n, k, fmt, block).reshape(*dy.shape[:-1], k) if ctx.needs_input_grad[0] else None
+        return dx, None, None, None, dy2.sum(0) if ctx.needs_input_grad[4] else None
+
+
+class AdapterLinear(torch.autograd.Function):
+    """A prepared layer with its adapters: the gradients of the input and of the adapters."""
+
+    @staticmethod
+    def forward(x, a, b, scaling, order, offsets, tiles, cols, w, sw, layer, bias):
+        y = layer.mxl_kernel.apply_weights(layer, x, bias)
+        v = ops.adapter_apply(y.view(-1, y.shape[-1]), x.reshape(-1, x.shape[-1]), a, b, scaling, order, offsets, tiles, cols)
+        return y, v
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, a, b, scaling, order, offsets, tiles, cols, w, sw, layer, _ = inputs
+        ctx.mark_non_differentiable(output[1])
+        # (a batch updated for the next step before this one's backward is noticed by its tensors' versions)
+        ctx.save_for_backward(x, a, b, scaling, output[1], order, offsets, tiles, w, sw)
+        ctx.meta = (list(cols), *grad_of(layer)[2:])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, _):
+        x, a, b, scaling, v, order, offsets, tiles, w, sw = ctx.saved_tensors
+        cols, n, k, fmt, block = ctx.meta
+        need_x, need_a, need_b = ctx.needs_input_grad[:3]
+        dy2 = dy.reshape(-1, n)
+        dx = ops.input_grad(dy2, w, sw, n, k, fmt, block) if need_x else None
+        da, db = ops.adapter_grad(dx, dy2, x.reshape(-1, k), a, b, scaling, v, order, offsets, tiles, cols, need_a, need_b)
+        return (None if dx is None else dx.reshape(x.shape), da if need_a else None, db if need_b else None, *[None] * 8,
+                dy2.sum(0) if ctx.needs_input_grad[11] else None)
+
+
+class GatedLinear(torch.autograd.Function):
+    """``ops.gated_linear`` with the gradient of its input."""
+
+    @staticmethod
+    def forward(x, w, sw, i, fmt, act, rule):
+        return ops.gated_linear(x.reshape(-1, x.shape[-1]), w, sw, i, fmt, act, rule).reshape(*x.shape[:-1], i)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, w, sw, *ctx.meta = inputs
+        ctx.save_for_backward(x, w, sw)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, w, sw = ctx.saved_tensors
+        i, fmt, act, rule = ctx.meta
+        k = x.shape[-1]
+        both = ops.gated_grad(x.reshape(-1, k), dh.reshape(-1, i), w, sw, i, fmt, act, rule)
+        return ops.input_grad(both, w, sw, 2 * i, k, fmt).reshape(x.shape), *[None] * 6
+
+
+def apply_adapters(layer: torch.nn.Module, x: torch.Tensor, adapters: LowRankAdapters, batch: AdapterBatch,
+                   bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A prepared layer's output with the adapters of a batch's tokens added: x bf16 [..., K] of ``len(batch)`` rows."""
+    n, k = layer.mxl_shape
+    if not isinstance(adapters, LowRankAdapters) or not isinstance(batch, AdapterBatch):
+        raise ValueError("adapters and batch go together: LowRankAdapters and AdapterBatch")
+    if tuple(adapters.lora_b.shape[:2]) != (adapters.slots, n) or adapters.lora_a.shape[2] != k:
+        raise ValueError(f"the adapters are not of this layer, [{n}, {k}]")
+    if batch.slots != adapters.slots:
+        raise ValueError(f"the batch is of {batch.slots} slots, the adapters of {adapters.slots}")
+    if x.dtype != torch.bfloat16 or x.shape[-1] != k or x.numel() != len(batch) * k:
+        raise ValueError(f"adapters need bf16 [..., {k}] of the batch's {len(batch)} rows, got {x.dtype} {tuple(x.shape)}")
+    a, b = adapters.lora_a, adapters.lora_b
+    if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad):
+        w, sw = grad_of(layer)[:2]
+        inner = _function_bias(bias, x, n)
+        y = AdapterLinear.apply(x, a, b, adapters.scaling, batch.order, batch.offsets, batch.tiles, adapters.cols, w, sw,
+                                layer, inner)[0]
+        return y if bias is inner else y + bias
+    y = layer.mxl_kernel.apply_weights(layer, x, bias)
+    ops.adapter_apply(y.view(-1, n), x.reshape(-1, k), a, b, adapters.scaling, batch.order, batch.offsets, batch.tiles,
+                      adapters.cols)
+    return y

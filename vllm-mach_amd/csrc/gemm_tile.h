@@ -38,6 +38,7 @@
 #pragma once
 
 #include "fp4.h"
+#include "gate_act.h"
 #include "gemm_wide.h"
 
 // the copies set M0 (the LDS base of a global->LDS load) themselves
@@ -140,6 +141,31 @@ struct TileShape {
   static constexpr int HALF = CA + CB;                // copies per wave of half a stage (one A and one B unit)
 };
 
+// Stages of the LDS ring.  SHARED: of the workgroups that share a CU (RESIDENT of them); LONE:
+// where the launch has too few for that, four, so that they keep as much in flight.
+template <int MT, int NT>
+struct TileDepth {
+  static constexpr int RESIDENT = MT * NT > 16 ? 1 : MT * NT > 4 ? 2 : 4;
+  static constexpr int SHARED = MT * NT > 32 || MT * NT == 16 || MT * NT == 4 ? 2 : 3;
+  static constexpr int LONE = MT * NT > 16 ? SHARED : 4;
+  // most workgroups per CU that still leave room for LONE stages each
+  static constexpr int LONE_MAX = MT * NT == 4 ? 2 : 1;
+  // of a tile's quarters, in the LDS of the launch
+  static constexpr int QUARTER = 4;
+};
+
+// What a tile's epilogue does with its sums.  All but the first pair columns of a merged gate/up weight (W = gate rows
+// then up rows, I of each): half of a wave's n-tiles are gate columns, half the up columns of the same.
+//   kEpiSwigluFp4  MXFP4 codes and scales of bf16(bf16(silu(gate)) up) (p.mid_codes, p.mid_scales), I % 64 == 0
+//   kEpiGated      act(gate) up, rounded once to bf16 (p.out [M, I]), I % 16 == 0
+//   kEpiGatedGrad  with dh [M, I] of that output, dh up act'(gate) and dh act(gate) (p.out [M, 2 I])
+enum TileEpi : int { kEpiStore = 0, kEpiSwigluFp4 = 1, kEpiGated = 2, kEpiGatedGrad = 3 };
+struct TileGate {
+  int act = 0;                   // kActSilu, kActGeluTanh
+  const uint16_t* dh = nullptr;  // rows of lddh
+  int64_t lddh = 0;
+};
+
 // What a workgroup computes: rows row0 .. row_hi - 1 (at most BM of them stored) by n-block
 // nb, super-tiles kb .. ke - 1.  part: instead of output elements the tile's fp32 partials as
 // one block in MFMA fragment order: fragment f = m-tile * (BN / 16) + n-tile is 64 lanes x 4
@@ -164,11 +190,12 @@ struct TileLds {
   static constexpr int bytes(int depth) { return RING + depth * STAGE; }
 };
 
-// a_row(row): the activation row of output row `row` (rows past the last: any valid one).  SWIGLU (MXFP4, N = 2 I, I %
-// 64 == 0, W = gate rows then up rows): half of a wave's n-tiles are gate columns, half the up columns of the same 32, and the
-// epilogue writes their SwiGLU as MXFP4 (p.mid_codes, p.mid_scales) instead of the product.
-template <int FMT, int MTW, int NTW, bool BLOCK, int DEPTH, bool SWIGLU = false, class Row>
-__device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w, uint8_t* lds, Row&& a_row) {
+// a_row(row): the activation row of output row `row` (rows past the last: any valid one).
+template <int FMT, int MTW, int NTW, bool BLOCK, int DEPTH, int EPI = kEpiStore, class Row>
+__device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w, uint8_t* lds, Row&& a_row,
+                                          const TileGate& gate = TileGate()) {
+  constexpr bool SWIGLU = EPI == kEpiSwigluFp4, GATED = EPI == kEpiGated || EPI == kEpiGatedGrad;
+  static_assert(!GATED || !BLOCK, "gate and up columns have block scales of their own");
   static_assert(!BLOCK || FMT == kE4M3, "block-FP8 weights are E4M3");
   using S = TileShape<MTW, NTW>;
   using L = TileLds<MTW, NTW, BLOCK>;
@@ -190,11 +217,14 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   const int KT = (int)p.KT, ntiles = (int)((p.N + 15) / 16), kb = w.kb, ke = w.ke;
   // stages SPT kb .. te - 1; an odd count runs one more (end), whose weights (past K) are zero
   const int te = SPT * ke < T ? SPT * ke : T, end = (te + 1) & ~1;
-  const int nt_base = w.nb * (S::BN / (SWIGLU ? 32 : 16)), up = ntiles / 2;
+  const int nt_base = w.nb * (S::BN / (EPI != kEpiStore ? 32 : 16)), up = ntiles / 2;
   // n-tile k of half h of wave column c
   auto n_tile = [&](int c, int h, int k) -> int {
     if constexpr (SWIGLU) {
       return nt_base + c * NH + k + h * up;
+    } else if constexpr (GATED) {
+      const int nt = nt_base + c * NH + k;
+      return (nt < up ? nt : up - 1) + h * up;
     } else {
       const int nt = nt_base + c * NTW + h * NH + k;
       return nt < ntiles ? nt : ntiles - 1;
@@ -635,6 +665,53 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    return;
+  }
+  if constexpr (GATED) {
+    // lane: four columns of one row of gate and of up, side by side in its registers
+    const int I = 16 * up, col0 = 16 * (nt_base + wn * NH) + 4 * q;
+    auto rows = [&](auto ACT) {
+#pragma unroll
+      for (int i = 0; i < MTW; ++i) {
+        const int row = w.row0 + (wm * MTW + i) * 16 + r;
+        uint16_t* const out = p.out + (int64_t)row * p.ldc;
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+          const v4f g = values(i, n), u = values(i, NH + n);
+          const int col = col0 + 16 * n;
+          const bool live = row < w.row_hi && col < I;
+          float x[4], y[4];
+          if constexpr (EPI == kEpiGated) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float slope;
+              x[e] = gate_act<decltype(ACT)::value>(g[e], slope) * u[e];
+            }
+          } else {
+            uint2 d = {0, 0};
+            if (live) d = *reinterpret_cast<const uint2*>(gate.dh + (int64_t)row * gate.lddh + col);
+            const float dh[4] = {u2f(d.x << 16), u2f(d.x & 0xFFFF0000u), u2f(d.y << 16), u2f(d.y & 0xFFFF0000u)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float slope;
+              y[e] = dh[e] * gate_act<decltype(ACT)::value>(g[e], slope);
+              x[e] = dh[e] * u[e] * slope;
+            }
+          }
+          auto bits = [](const float* v) {
+            return uint2{f32_to_bf16(v[0]) | (uint32_t)f32_to_bf16(v[1]) << 16,
+                         f32_to_bf16(v[2]) | (uint32_t)f32_to_bf16(v[3]) << 16};
+          };
+          if (live) {
+            *reinterpret_cast<uint2*>(out + col) = bits(x);
+            if constexpr (EPI == kEpiGatedGrad) *reinterpret_cast<uint2*>(out + I + col) = bits(y);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    };
+    if (gate.act == kActSilu) rows(Slice<kActSilu>{});
+    else rows(Slice<kActGeluTanh>{});
     return;
   }
   if (w.part) {

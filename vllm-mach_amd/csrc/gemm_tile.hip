@@ -4,19 +4,6 @@
 
 namespace mxl {
 
-// Stages of the LDS ring.  SHARED: of the workgroups that share a CU (RESIDENT of them); LONE:
-// where the launch has too few for that, four, so that they keep as much in flight.
-template <int MT, int NT>
-struct TileDepth {
-  static constexpr int RESIDENT = MT * NT > 16 ? 1 : MT * NT > 4 ? 2 : 4;
-  static constexpr int SHARED = MT * NT > 32 || MT * NT == 16 || MT * NT == 4 ? 2 : 3;
-  static constexpr int LONE = MT * NT > 16 ? SHARED : 4;
-  // most workgroups per CU that still leave room for LONE stages each
-  static constexpr int LONE_MAX = MT * NT == 4 ? 2 : 1;
-  // of a tile's quarters, in the LDS of the launch
-  static constexpr int QUARTER = 4;
-};
-
 template <int FMT, int MT, int NT, bool BLOCK>
 struct WideKernel<FMT, MT, NT, BLOCK, false, 2> {
   static __device__ __forceinline__ void run(const GemmParams& p, const WideGrid& g) {

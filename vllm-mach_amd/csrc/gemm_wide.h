@@ -61,6 +61,9 @@ __global__ __launch_bounds__(256, (WidePerCu<MT, NT, GROUPED, WM>::value)) void 
   WideKernel<FMT, MT, NT, BLOCK, GROUPED, WM>::run(p, g);
 }
 
+// Tile and grid of the 2 x 2-wave kernels over whole K (N columns, for MXFP4 in its stages of K256), no splits.
+WideConfig wide_tiles_whole(int64_t M, int64_t N, int64_t K, int fmt, WideGrid& g, int64_t& grid);
+
 // The dense 2 x 2-wave launch of `grid` workgroups.
 hipError_t launch_wide_tiles(int fmt, bool block, const WideConfig& c, const GemmParams& p, const WideGrid& g,
                              int64_t grid, hipStream_t s);

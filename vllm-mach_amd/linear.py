@@ -148,6 +148,8 @@ class Mxfp8LinearKernel(_Kernel):
         n, k = layer.mxl_shape
         if x.dtype != torch.bfloat16 or x.shape[-1] != k:
             raise ValueError("MXFP8 requires BF16 activations with matching K")
+        if x.requires_grad and torch.is_grad_enabled():
+            return _with_input_grad(layer, x, bias)
         if x.numel() == 0:
             return x.new_empty((*x.shape[:-1], n))
         x2 = _flatten(x, k).contiguous()
@@ -175,6 +177,21 @@ def _epilogue_bias(bias: Optional[torch.Tensor], x: torch.Tensor, n: int) -> Opt
         if torch.autograd.forward_ad._current_level >= 0 or torch._C._functorch.is_functorch_wrapped_tensor(bias):
             return None
     return bias
+
+
+def _function_bias(bias: Optional[torch.Tensor], x: torch.Tensor, n: int) -> Optional[torch.Tensor]:
+    """``_epilogue_bias`` of a call whose own backward computes the bias' gradient."""
+    with torch.no_grad():
+        return _epilogue_bias(bias, x, n)
+
+
+def _with_input_grad(layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
+    """The layer's output as a function of x that autograd can walk back through: the weight is frozen, the dynamic
+    quantization counts as the identity (``ops.input_grad``)."""
+    from .adapters import FrozenLinear, grad_of
+    inner = _function_bias(bias, x, layer.mxl_shape[0])
+    y = FrozenLinear.apply(x, *grad_of(layer)[:2], layer, inner)
+    return y if bias is inner else y + bias
 
 
 def logical_mxfp6_shape(weight: torch.Tensor) -> tuple[int, int]:
@@ -230,6 +247,8 @@ class Mxfp6LinearKernel(_Kernel):
                              f"{int(x.shape[-1])}, weight K={k}")
         if x.dtype != torch.bfloat16:
             raise ValueError("MXFP6 requires BF16 activations")
+        if x.requires_grad and torch.is_grad_enabled():
+            return _with_input_grad(layer, x, bias)
         if x.numel() == 0:
             return x.new_empty((*x.shape[:-1], n))
         inner = _epilogue_bias(bias, x, n)
@@ -274,6 +293,8 @@ class BlockFp8LinearKernel(_Kernel):
         n, k = layer.mxl_shape
         if x.dtype != torch.bfloat16 or x.shape[-1] != k:
             raise ValueError("block-FP8 requires BF16 activations with matching K")
+        if x.requires_grad and torch.is_grad_enabled():
+            return _with_input_grad(layer, x, bias)
         if x.numel() == 0:
             return x.new_empty((*x.shape[:-1], n))
         inner = _epilogue_bias(bias, x, n)
@@ -321,6 +342,8 @@ class Mxfp4LinearKernel(_Kernel):
         n, k = layer.mxl_shape
         if x.dtype != torch.bfloat16 or x.shape[-1] != k:
             raise ValueError("MXFP4 requires BF16 activations with matching K")
+        if x.requires_grad and torch.is_grad_enabled():
+            return _with_input_grad(layer, x, bias)
         if x.numel() == 0:
             return x.new_empty((*x.shape[:-1], n))
         inner = _epilogue_bias(bias, x, n)
@@ -407,8 +430,40 @@ class MxLinearMethod:
     def process_weights_after_loading(self, layer: torch.nn.Module) -> None:
         self.kernel.process_weights_after_loading(layer)
 
-    def apply(self, layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-        return self.kernel.apply_weights(layer, x, bias)
+    def apply(self, layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor] = None,
+              adapters=None, batch=None) -> torch.Tensor:
+        """y = x W^T (+ bias); with ``adapters`` (``LowRankAdapters`` of this layer) and ``batch`` (``AdapterBatch``) the
+        low-rank adapters of the batch's tokens are added.  Differentiable in x, the adapters and the bias."""
+        if adapters is None and batch is None:
+            return self.kernel.apply_weights(layer, x, bias)
+        from .adapters import apply_adapters
+        return apply_adapters(layer, x, adapters, batch, bias)
+
+
+ACTIVATIONS = {"silu": ops.SILU, "gelu_tanh": ops.GELU_TANH}
+
+
+def gated_linear(x: torch.Tensor, layer: torch.nn.Module, activation: str = "silu") -> torch.Tensor:
+    """act(x Wg^T) * (x Wu^T) for a merged gate/up layer (gate rows, then up rows) prepared by one of the MX kernels: x bf16
+    [..., K] -> bf16 [..., I], gate and up in fp32 up to one rounding (the two-launch path, the layer and then the SwiGLU
+    producer, rounds each to bf16).  ``activation``: ``"silu"`` or ``"gelu_tanh"``.  Differentiable in x."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}: one of {sorted(ACTIVATIONS)}")
+    if not hasattr(layer, "mxl_shape") or not hasattr(layer, "mxl_format"):
+        raise ValueError("gated_linear needs a layer prepared by an MX kernel (MXFP8, MXFP6, MXFP4)")
+    n, k = layer.mxl_shape
+    widths = getattr(layer, "logical_widths", None)
+    if n % 32 or (widths is not None and len(widths) > 1 and list(widths) != [n // 2, n // 2]):
+        raise ValueError(f"gated_linear needs gate and up of the same multiple of 16 columns (N={n}, parts {widths})")
+    if x.dtype != torch.bfloat16 or x.shape[-1] != k:
+        raise ValueError("gated_linear requires BF16 activations with matching K")
+    args = (layer.weight, layer.weight_scale, n // 2, layer.mxl_format, ACTIVATIONS[activation], layer.mxl_kernel.act_rule)
+    if x.requires_grad and torch.is_grad_enabled():
+        from .adapters import GatedLinear
+        return GatedLinear.apply(x, *args)
+    rows = x.ndim == 2
+    y = ops.gated_linear(x if rows else _flatten(x, k), *args)
+    return y if rows else y.reshape(*x.shape[:-1], n // 2)
 
 
 def swiglu_mxfp8_down(gate_up: torch.Tensor, down: torch.nn.Module) -> torch.Tensor:

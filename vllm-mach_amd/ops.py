@@ -1118,6 +1118,252 @@ def _(output, x, topk_ids, topk_weights, sorted_routes, expert_offsets, inverse,
     return None
 
 
+# ------------------------------------------------- frozen layers' input gradient, gated blocks
+#
+# These take a layer's tiled weight as its forward does; scratch is a tensor of the call.
+
+SILU, GELU_TANH = 0, 1  # gated blocks' activations
+_CODE_CHUNKS = {E4M3: 8, E2M3: 6, E3M2: 6, E2M1: 4}  # KiB of a 16 x 512 tile
+
+
+def _tiled_weight(what: str, w: torch.Tensor, sw: torch.Tensor, n: int, k: int, fmt: int, block: bool = False):
+    """The tiled weight's tensors, of the size that (n, k) and the format ask for."""
+    if fmt not in _CODE_CHUNKS or (block and fmt != E4M3):
+        raise ValueError(f"{what}: unknown weight format {fmt}{' of blocks' if block else ''}")
+    if n <= 0 or k <= 0 or k % 128:
+        raise ValueError(f"{what} needs N > 0 and K > 0, K % 128 == 0 (N={n}, K={k})")
+    tiles = ((n + 15) // 16) * ((k + 511) // 512)
+    if w.dtype != torch.uint8 or w.numel() != tiles * _CODE_CHUNKS[fmt] * 1024:
+        raise ValueError(f"{what}: the weight is not [{n}, {k}] of format {fmt} in the tiled layout (pack_weight)")
+    if block:
+        if sw.dtype != torch.float32 or tuple(sw.shape) != ((n + 127) // 128, k // 128):
+            raise ValueError(f"{what}: block scales must be fp32 [{(n + 127) // 128}, {k // 128}]")
+    elif sw.dtype != torch.uint8 or sw.numel() != tiles * 256:
+        raise ValueError(f"{what}: the scales are not [{n}, {k}] in the tiled layout (pack_weight)")
+    return _aligned(w, 16), _aligned(sw, 4)
+
+
+def _bf16_rows(what: str, x: torch.Tensor, k: int, name: str = "x") -> torch.Tensor:
+    if x.dtype != torch.bfloat16 or x.ndim != 2 or x.shape[1] != k:
+        raise ValueError(f"{what}: {name} must be bf16 [M, {k}], got {x.dtype} {tuple(x.shape)}")
+    return _rows16(x)
+
+
+@_operator("input_grad")
+def input_grad(dy: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, k: int, w_fmt: int,
+               block: bool = False) -> torch.Tensor:
+    """The input gradient of a frozen layer, dx = dy W: dy bf16 [M, N], W [N, K] in the tiled layout (``pack_weight``),
+    ``sw`` its tiled E8M0 scales or (``block``) the fp32 block scales; bf16 [M, K].  The codes' values are exact in the
+    product (bf16 products, fp32 sums) wherever a value is a normal bf16; the quantization of the layer's input counts
+    as the identity."""
+    _same_device("input_grad", dy, w, sw)
+    w, sw = _tiled_weight("input_grad", w, sw, n, k, w_fmt, block)
+    dy = _bf16_rows("input_grad", dy, n, "dy")
+    if n % 8:  # (block-FP8 layers of odd widths: the kernel reads eight columns at a time; W's rows past N are zeros)
+        dy = torch.nn.functional.pad(dy, (0, 8 - n % 8))
+    M = dy.shape[0]
+    out = dy.new_empty((M, k))
+    if M:
+        with _on(dy.device):
+            nbytes = query("mxl_input_grad_workspace_bytes", M, dy.shape[1], k)
+            ws = _scratch(nbytes, w)
+            call("mxl_input_grad", ptr(dy), M, dy.shape[1], _row_stride(dy), ptr(w), ptr(sw), k, w_fmt, int(block),
+                 ptr(out), k, ptr(ws), nbytes, stream_handle(dy.device))
+    _count("input_grad")
+    return out
+
+
+@input_grad.register_fake
+def _(dy, w, sw, n, k, w_fmt, block=False):
+    return dy.new_empty((dy.shape[0], k), dtype=torch.bfloat16)
+
+
+def _gated(what: str, x: torch.Tensor, w, sw, i: int, fmt: int, act: int, rule: int, dh: Optional[torch.Tensor]):
+    _same_device(what, x, w, sw, dh)
+    if x.ndim != 2:
+        raise ValueError(f"{what} needs bf16 [M, K]")
+    k = x.shape[1]
+    if i <= 0 or i % 16:
+        raise ValueError(f"{what} needs I > 0, I % 16 == 0 (I={i})")
+    if act not in (SILU, GELU_TANH):
+        raise ValueError(f"{what}: unknown activation {act}")
+    if rule not in ((FLOOR_CARRY175, FLOOR_OCP) if fmt == E2M1 else (FLOOR_CARRY175, CEIL_DIV448, RP_UE8M0)):
+        raise ValueError(f"{what}: unknown rule {rule}")
+    w, sw = _tiled_weight(what, w, sw, 2 * i, k, fmt)
+    x = _bf16_rows(what, x, k)
+    M = x.shape[0]
+    if dh is not None:
+        if dh.shape[0] != M:
+            raise ValueError(f"{what}: dh has {dh.shape[0]} rows, x {M}")
+        dh = _bf16_rows(what, dh, i, "dh")
+    out = x.new_empty((M, i if dh is None else 2 * i))
+    if M:
+        with _on(x.device):
+            nbytes = query("mxl_gated_workspace_bytes", M, k, fmt)
+            ws = _scratch(nbytes, w)
+            args = () if dh is None else (ptr(dh), _row_stride(dh))
+            call("mxl_gated_linear" if dh is None else "mxl_gated_grad", ptr(x), M, k, _row_stride(x), rule, ptr(w), ptr(sw),
+                 i, fmt, act, *args, ptr(out), out.shape[1], ptr(ws), nbytes, stream_handle(x.device))
+    _count(what)
+    return out
+
+
+@_operator("gated_linear")
+def gated_linear(x: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, i: int, w_fmt: int, act: int = SILU,
+                 rule: int = FLOOR_CARRY175) -> torch.Tensor:
+    """act(x Wg^T) * (x Wu^T) of an MX weight [2 I, K] (gate rows, then up rows; tiled layout): bf16 [M, K] quantized as
+    the layer's product does it (MXFP8, of E2M1 weights MXFP4), both products in fp32, one rounding to bf16 [M, I].
+    ``act``: ``SILU`` or ``GELU_TANH``.  The product is one launch, behind the quantizer's."""
+    return _gated("gated_linear", x, w, sw, i, w_fmt, act, rule, None)
+
+
+@gated_linear.register_fake
+def _(x, w, sw, i, w_fmt, act=SILU, rule=FLOOR_CARRY175):
+    return x.new_empty((x.shape[0], i), dtype=torch.bfloat16)
+
+
+@_operator("gated_grad")
+def gated_grad(x: torch.Tensor, dh: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, i: int, w_fmt: int, act: int = SILU,
+               rule: int = FLOOR_CARRY175) -> torch.Tensor:
+    """The gradients of ``gated_linear``'s two products from its output's, dh bf16 [M, I]: [dh up act'(gate), dh act(gate)]
+    bf16 [M, 2 I], gate and up computed again from x (nothing of size [M, 2 I] has to be kept)."""
+    return _gated("gated_grad", x, w, sw, i, w_fmt, act, rule, dh)
+
+
+@gated_grad.register_fake
+def _(x, dh, w, sw, i, w_fmt, act=SILU, rule=FLOOR_CARRY175):
+    return x.new_empty((x.shape[0], 2 * i), dtype=torch.bfloat16)
+
+
+# ----------------------------------------------------------------- low-rank adapters
+
+def adapter_batch(ids: torch.Tensor, slots: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Tokens sorted by adapter: ids integers [M] (outside [0, slots): none) -> order i32 [M] (stable), offsets i64
+    [slots + 1] into it, and the tiles that the adapters' kernels walk, i32 [tiles, 2]."""
+    _check_cuda(ids)
+    if ids.ndim != 1 or ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
+        raise ValueError(f"adapter ids must be integers [M], got {ids.dtype} {tuple(ids.shape)}")
+    if not 0 < slots <= 2048:
+        raise ValueError(f"1 to 2048 adapters ({slots})")
+    M, dev = ids.shape[0], ids.device
+    if M >= 1 << 31:
+        raise ValueError(f"less than 2^31 tokens ({M})")
+    if ids.dtype != torch.int32:  # (values past 32 bits would wrap into range)
+        ids = torch.where((ids >= 0) & (ids < slots), ids, -1).to(torch.int32)
+    ids = ids.contiguous()
+    order = torch.empty(M, dtype=torch.int32, device=dev)
+    offsets = torch.empty(slots + 1, dtype=torch.int64, device=dev)
+    inverse = torch.empty(M, dtype=torch.int32, device=dev)
+    tiles = torch.empty((query("mxl_adapter_tile_count", M, slots), 2), dtype=torch.int32, device=dev)
+    with _on(dev):
+        if M == 0:
+            offsets.zero_()
+        else:
+            nbytes = query("mxl_moe_route_workspace_bytes", M, 1, slots)
+            ws = _scratch(nbytes, order)
+            call("mxl_moe_route", ptr(ids), M, 1, slots, ptr(order), ptr(offsets), ptr(inverse), ptr(ws), nbytes,
+                 stream_handle(dev))
+            call("mxl_adapter_tiles", ptr(offsets), M, slots, ptr(tiles), tiles.shape[0], stream_handle(dev))
+    _count("adapter_batch")
+    return order, offsets, tiles
+
+
+def _adapter_args(what: str, x, a, b, scaling, order, offsets, tiles, cols):
+    """The checked operands of the adapters' kernels: (x, a, b, parts, rank, cols as a C array)."""
+    _same_device(what, x, a, b, scaling, order, offsets, tiles)
+    parts, slots = len(cols) - 1, a.shape[0] if a.ndim == 3 else 0
+    if b.ndim != 3 or a.ndim != 3 or a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: a and b must be bf16 [slots, parts * rank, K] and [slots, N, rank]")
+    rank = b.shape[2]
+    if not 1 <= parts <= 8 or list(cols) != sorted(set(cols)) or cols[0] != 0 or any(c % 16 for c in cols[:-1]):
+        raise ValueError(f"{what}: 1 to 8 parts that start on multiples of 16 columns, from 0 ({list(cols)})")
+    if rank % 8 or not 8 <= rank <= 256:
+        raise ValueError(f"{what}: ranks of 8 to 256, multiples of 8 ({rank})")
+    if tuple(a.shape) != (slots, parts * rank, x.shape[1]) or tuple(b.shape) != (slots, cols[-1], rank):
+        raise ValueError(f"{what}: a {tuple(a.shape)} and b {tuple(b.shape)} do not fit K={x.shape[1]}, N={cols[-1]}, "
+                         f"{parts} parts")
+    if scaling.dtype != torch.float32 or tuple(scaling.shape) != (slots,):
+        raise ValueError(f"{what}: scaling must be fp32 [{slots}]")
+    M = x.shape[0]
+    if (order.dtype != torch.int32 or tuple(order.shape) != (M,) or offsets.dtype != torch.int64
+            or tuple(offsets.shape) != (slots + 1,) or tiles.dtype != torch.int32
+            or tuple(tiles.shape) != (query("mxl_adapter_tile_count", M, slots), 2)
+            or not (order.is_contiguous() and offsets.is_contiguous() and tiles.is_contiguous())):
+        raise ValueError(f"{what}: the batch is not one of {M} tokens and {slots} adapters (adapter_batch)")
+    x = _bf16_rows(what, x, x.shape[1])
+    return x, _aligned(a, 16), _aligned(b, 16), scaling.contiguous(), parts, rank, (ctypes.c_int64 * len(cols))(*cols)
+
+
+@_operator("adapter_apply", mutates_args=("y",))
+def adapter_apply(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
+                  order: torch.Tensor, offsets: torch.Tensor, tiles: torch.Tensor, cols: list[int]) -> torch.Tensor:
+    """y[t] += scaling[s] b[s] (a[s] x[t]) for every token t of a batch (``adapter_batch``), s its adapter: y bf16 [M, N] in
+    place, x bf16 [M, K], a bf16 [slots, parts * rank, K], b bf16 [slots, N, rank], scaling fp32 [slots].  ``cols``: where
+    the layer's merged parts start, and N; a part has ``rank`` rows of a of its own.  Returns v, the scaled a x of the
+    tokens in the batch's order (fp32, in shares that sum to it), which ``adapter_grad`` takes."""
+    if x.ndim != 2:
+        raise ValueError("adapter_apply needs bf16 [M, K]")
+    x, a, b, scaling, parts, rank, c = _adapter_args("adapter_apply", x, a, b, scaling, order, offsets, tiles, cols)
+    (M, K), slots = x.shape, a.shape[0]
+    if (y.dtype != torch.bfloat16 or tuple(y.shape) != (M, cols[-1]) or y.device != x.device or y.stride(1) != 1
+            or (M > 1 and y.stride(0) < y.shape[1])):
+        raise ValueError(f"adapter_apply: y must be bf16 [{M}, {cols[-1]}] of unit column stride on {x.device}")
+    v = x.new_empty(query("mxl_adapter_v_floats", M, K, slots, parts, rank), dtype=torch.float32)
+    if M:
+        with _on(x.device):
+            call("mxl_adapter_apply", ptr(x), M, K, _row_stride(x), ptr(a), ptr(b), ptr(scaling), slots, parts, c, rank,
+                 ptr(order), ptr(offsets), ptr(tiles), tiles.shape[0], ptr(v), v.numel(), ptr(y), _row_stride(y),
+                 stream_handle(x.device))
+    _count("adapter_apply")
+    return v
+
+
+@adapter_apply.register_fake
+def _(y, x, a, b, scaling, order, offsets, tiles, cols):
+    return x.new_empty((torch.library.get_ctx().new_dynamic_size(),), dtype=torch.float32)
+
+
+@_operator("adapter_grad", mutates_args=("dx",))
+def adapter_grad(dx: Optional[torch.Tensor], dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                 scaling: torch.Tensor, v: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, tiles: torch.Tensor,
+                 cols: list[int], need_a: bool = True, need_b: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gradients of ``adapter_apply``'s a and b (bf16, their shapes; empty where not needed) from dy bf16 [M, N], and
+    in place dx[t] += a[s]^T (scaling[s] b[s]^T dy[t]) where dx bf16 [M, K] is given."""
+    if x.ndim != 2:
+        raise ValueError("adapter_grad needs bf16 [M, K]")
+    x, a, b, scaling, parts, rank, c = _adapter_args("adapter_grad", x, a, b, scaling, order, offsets, tiles, cols)
+    _same_device("adapter_grad", x, dy, dx, v)
+    (M, K), slots, N = x.shape, a.shape[0], cols[-1]
+    if N % 8:
+        raise ValueError(f"adapter_grad needs N % 8 == 0 (N={N})")
+    if dy.shape[0] != M:
+        raise ValueError(f"adapter_grad: dy has {dy.shape[0]} rows, x {M}")
+    dy = _bf16_rows("adapter_grad", dy, N, "dy")
+    if dx is not None and (dx.dtype != torch.bfloat16 or tuple(dx.shape) != (M, K) or dx.stride(1) != 1
+                           or (M > 1 and dx.stride(0) < K)):
+        raise ValueError(f"adapter_grad: dx must be bf16 [{M}, {K}] of unit column stride")
+    if v.dtype != torch.float32 or not v.is_contiguous() or v.numel() != query("mxl_adapter_v_floats", M, K, slots, parts, rank):
+        raise ValueError("adapter_grad: v is not adapter_apply's of these operands")
+    make = torch.Tensor.new_empty if M else torch.Tensor.new_zeros
+    da = make(a, a.shape if need_a else (0,))
+    db = make(b, b.shape if need_b else (0,))
+    if M and (need_a or need_b or dx is not None):
+        with _on(x.device):
+            nbytes = query("mxl_adapter_grad_workspace_bytes", M, K, slots, parts, c, rank)
+            ws = _scratch(nbytes, v)
+            call("mxl_adapter_grad", ptr(x), M, K, _row_stride(x), ptr(dy), _row_stride(dy), ptr(a), ptr(b), ptr(scaling),
+                 slots, parts, c, rank, ptr(order), ptr(offsets), ptr(tiles), tiles.shape[0], ptr(v), v.numel(), ptr(dx),
+                 K if dx is None else _row_stride(dx), ptr(da) if need_a else None, ptr(db) if need_b else None, ptr(ws),
+                 nbytes, stream_handle(x.device))
+    _count("adapter_grad")
+    return da, db
+
+
+@adapter_grad.register_fake
+def _(dx, dy, x, a, b, scaling, v, order, offsets, tiles, cols, need_a=True, need_b=True):
+    return a.new_empty(a.shape if need_a else (0,)), b.new_empty(b.shape if need_b else (0,))
+
+
 # ---------------------------------------------------------------------- MoE
 
 @torch.library.custom_op("mach_amd::moe_route", mutates_args=())
