@@ -566,7 +566,7 @@ int mxl_moe_reduce_add(const void* routed_output, const float* topk_weights, con
  * (row stride ldo).  The codes' values are exact in bf16 wherever they are normal bf16 numbers; fp32
  * sums.  N % 8 == 0, K % 128 == 0 (rows of W past an N that is no multiple of 16 are zero).  The
  * workspace, 16-byte aligned, holds mxl_input_grad_workspace_bytes. */
-int64_t mxl_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int64_t mxl_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int block);
 int mxl_input_grad(const void* dy, int64_t M, int64_t N, int64_t lddy, const void* w_tiled, const void* sw, int64_t K,
                    int fmt, int block, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
 
@@ -592,26 +592,41 @@ int mxl_gated_grad(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, c
  * y bf16 [M, N] in place, x bf16 [M, K], a bf16 [slots, parts rank, K], b bf16 [slots, N, rank], N =
  * cols[parts].  A merged layer's part p is columns [cols[p], cols[p + 1]) (multiples of 16 but for the
  * last) with rows [p rank, (p + 1) rank) of a; rank a multiple of 8 up to 256, up to 8 parts.  cols is
- * host memory.  v (fp32, mxl_adapter_v_floats of them) receives scaling a x in the batch's order, in
- * shares that sum to it; it never passes through bf16.
+ * host memory.  v (mxl_adapter_v_elems bf16 values) receives scaling a x of each token with an adapter,
+ * as bf16 values and behind them what those leave of the fp32.
  *
- * mxl_adapter_grad, with that v: db and da (bf16, b's and a's shapes; either may be NULL) and, where dx
- * is given, dx[t] += a[s]^T (scaling[s] b[s]^T dy[t]).  N % 8 == 0.  An adapter without tokens gets
- * zeros.  Sums are joined in a fixed order.  The workspace, 256-byte aligned, holds
- * mxl_adapter_grad_workspace_bytes. */
+ * mxl_adapter_linear: the whole layer -- x quantized by `rule` (block = 1: block-FP8, ldx = K), the
+ * product with w_tiled [N, K] of format fmt, bias (or NULL) as the layer adds it -- with the adapters
+ * added to the product's fp32 sums, ahead of their rounding; ids i32 [M] as sorted.  Shapes:
+ * mxl_adapter_linear_supported (17 rows and more, at least 32 an adapter), else MXL_EUNSUPPORTED.
+ *
+ * mxl_adapter_grad, with that v: dx = dy W (mxl_input_grad) + a[s]^T (scaling[s] b[s]^T dy[t]) bf16
+ * [M, K], da and db bf16 in a's and b's shapes; any of the three may be NULL.  N % 8 == 0.  An adapter
+ * without tokens gets zeros.  Sums are joined in a fixed order.
+ *
+ * Workspaces are 256-byte aligned and of the sizes that the _workspace_bytes functions say. */
 int64_t mxl_adapter_tile_count(int64_t M, int64_t slots);
 int mxl_adapter_tiles(const int64_t* offsets, int64_t M, int64_t slots, int32_t* tiles, int64_t num_tiles, void* stream);
-int64_t mxl_adapter_v_floats(int64_t M, int64_t K, int64_t slots, int64_t parts, int64_t rank);
+int64_t mxl_adapter_v_elems(int64_t M, int64_t parts, int64_t rank);
 int mxl_adapter_apply(const void* x, int64_t M, int64_t K, int64_t ldx, const void* a, const void* b,
                       const float* scaling, int64_t slots, int64_t parts, const int64_t* cols, int64_t rank,
-                      const int32_t* order, const int64_t* offsets, const int32_t* tiles, int64_t num_tiles, float* v,
-                      int64_t v_floats, void* y, int64_t ldy, void* stream);
+                      const int32_t* order, const int64_t* offsets, const int32_t* tiles, int64_t num_tiles, void* v,
+                      int64_t v_elems, void* y, int64_t ldy, void* stream);
+int mxl_adapter_linear_supported(int64_t M, int64_t N, int64_t K, int fmt, int block, int64_t slots, int64_t parts,
+                                 int64_t rank);
+int64_t mxl_adapter_linear_workspace_bytes(int64_t M, int64_t K, int fmt, int block);
+int mxl_adapter_linear(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, const void* w_tiled, const void* sw,
+                       int fmt, int block, const void* bias, const void* a, const void* b, const float* scaling,
+                       int64_t slots, int64_t parts, const int64_t* cols, int64_t rank, const int32_t* ids,
+                       const int32_t* order, const int64_t* offsets, const int32_t* tiles, int64_t num_tiles, void* v,
+                       int64_t v_elems, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t mxl_adapter_grad_workspace_bytes(int64_t M, int64_t K, int64_t slots, int64_t parts, const int64_t* cols,
-                                         int64_t rank);
-int mxl_adapter_grad(const void* x, int64_t M, int64_t K, int64_t ldx, const void* dy, int64_t lddy, const void* a,
-                     const void* b, const float* scaling, int64_t slots, int64_t parts, const int64_t* cols,
-                     int64_t rank, const int32_t* order, const int64_t* offsets, const int32_t* tiles, int64_t num_tiles,
-                     const float* v, int64_t v_floats, void* dx, int64_t lddx, void* da, void* db, void* workspace,
+                                         int64_t rank, int block);
+int mxl_adapter_grad(const void* x, int64_t M, int64_t K, int64_t ldx, const void* dy, int64_t lddy, const void* w_tiled,
+                     const void* sw, int fmt, int block, const void* a, const void* b, const float* scaling,
+                     int64_t slots, int64_t parts, const int64_t* cols, int64_t rank, const int32_t* ids,
+                     const int32_t* order, const int64_t* offsets, const int32_t* tiles, int64_t num_tiles, const void* v,
+                     int64_t v_elems, void* dx, int64_t lddx, void* da, void* db, void* workspace,
                      int64_t workspace_bytes, void* stream);
 
 /* The kernels a dense GEMM call (mxl_mx_gemm_ex, block = 0; mxl_block_fp8_gemm_ex,

@@ -108,11 +108,12 @@ def test_entry_points_refuse(pkg):
     with pytest.raises(err, match="needs dh"):
         call("mxl_gated_grad", 16, 4, 128, 128, 0, 16, 16, 64, 0, 0, None, 64, 16, 128, 256, 1 << 30, None)
     tiles = _lib.query("mxl_adapter_tile_count", 4, 2)
-    v = _lib.query("mxl_adapter_v_floats", 4, 128, 2, 1, 8)
+    v = _lib.query("mxl_adapter_v_elems", 4, 1, 8)
+    assert v == 4 * 2 * 16
     apply = [16, 4, 128, 128, 16, 16, 16, 2, 1, _cols(0, 128), 8, 16, 16, 16, tiles, 16, v, 16, 128, None]
     for at, bad, match in ((7, 0, "slots"), (14, tiles + 1, "tiles"), (8, 9, "parts"), (10, 12, "rank"), (10, 264, "rank"),
                            (2, 100, "K % 8"), (9, _cols(0, 0), "no columns"), (9, _cols(16, 128), "start at column 0"),
-                           (3, 64, "ldx"), (18, 64, "ldy"), (0, 8, "aligned"), (16, v - 1, "floats"), (11, None, "order")):
+                           (3, 64, "ldx"), (18, 64, "ldy"), (0, 8, "aligned"), (16, v - 1, "values"), (11, None, "order")):
         args = list(apply)
         args[at] = bad
         with pytest.raises(err, match=match):
@@ -120,12 +121,31 @@ def test_entry_points_refuse(pkg):
     with pytest.raises(err, match="multiple of 16"):
         call("mxl_adapter_apply", 16, 4, 128, 128, 16, 16, 16, 2, 2, _cols(0, 24, 128), 8, 16, 16, 16, tiles, 16, 1 << 20, 16,
              128, None)
-    with pytest.raises(err, match="N % 8"):
-        call("mxl_adapter_grad", 16, 4, 128, 128, 16, 128, 16, 16, 16, 2, 1, _cols(0, 100), 8, 16, 16, 16, tiles, 16, v, 16,
-             128, 16, 16, 256, 1 << 30, None)
-    with pytest.raises(err, match="workspace"):
-        call("mxl_adapter_grad", 16, 4, 128, 128, 16, 128, 16, 16, 16, 2, 1, _cols(0, 128), 8, 16, 16, 16, tiles, 16, v, 16,
-             128, 16, 16, 256, 100, None)
+    grad = [16, 4, 128, 128, 16, 128, 16, 16, 0, 0, 16, 16, 16, 2, 1, _cols(0, 128), 8, 16, 16, 16, 16, tiles, 16, v, 16, 128,
+            16, 16, 256, 1 << 30, None]
+    for at, bad, match in ((15, _cols(0, 100), "N % 8"), (29, 100, "workspace"), (28, 128, "workspace"), (4, 8, "aligned"),
+                           (5, 64, "lddy"), (17, None, "ids"), (23, 0, "values"), (21, 0, "tiles")):
+        args = list(grad)
+        args[at] = bad
+        with pytest.raises(err, match=match):
+            call("mxl_adapter_grad", *args)
+    many = _lib.query("mxl_adapter_tile_count", 64, 2)
+    layer = [16, 64, 128, 128, 0, 16, 16, 0, 0, None, 16, 16, 16, 2, 1, _cols(0, 128), 8, 16, 16, 16, 16, many, 16, 1 << 20, 16,
+             128, 256, 1 << 30, None]
+    for at, bad, match in ((7, 1, "unknown format"), (3, 100, "ldx"), (25, 64, "ldy"), (17, None, "ids"), (23, 0, "values"),
+                           (27, 64, "workspace"), (5, 8, "aligned"), (8, 1, None)):
+        args = list(layer)
+        args[at] = bad
+        if at == 8:  # block-FP8 rows are contiguous
+            args[3], match = 256, "contiguous"
+        with pytest.raises(err, match=match):
+            call("mxl_adapter_linear", *args)
+    ok = lambda m, slots: _lib.query("mxl_adapter_linear_supported", m, 128, 128, 0, 0, slots, 1, 8)  # noqa: E731
+    assert ok(64, 2) and not ok(16, 1) and not ok(64, 3) and not ok(0, 1)
+    few = _lib.query("mxl_adapter_tile_count", 16, 1)
+    with pytest.raises(err, match="one product"):
+        call("mxl_adapter_linear", 16, 16, 128, 128, 0, 16, 16, 0, 0, None, 16, 16, 16, 1, 1, _cols(0, 128), 8, 16, 16, 16, 16,
+             few, 16, 1 << 20, 16, 128, 256, 1 << 30, None)
 
 
 def test_no_rows_is_no_launch(pkg):
@@ -145,6 +165,12 @@ def test_fakes(pkg):
         assert ns.gated_linear(x, w, w, 64, 0, 0, 0).shape == (5, 64)
         assert ns.gated_grad(x, x, w, w, 64, 0, 0, 0).shape == (5, 128)
         assert ns.input_grad(x, w, w, 256, 384, 0, False).shape == (5, 384)
+        a, b = torch.empty(3, 48, 256, dtype=torch.bfloat16), torch.empty(3, 96, 24, dtype=torch.bfloat16)
+        y, v = ns.adapter_linear(x, w, w, 0, False, 0, None, a, b, w, w, w, w, w, [0, 32, 96])
+        assert y.shape == (5, 96) and v.shape == (5, 128)
+        assert ns.adapter_apply(y, x, a, b, w, w, w, w, w, [0, 32, 96]).shape == (5, 128)
+        dx, da, db = ns.adapter_grad(y, x, w, w, 0, False, a, b, w, v, w, w, w, w, [0, 32, 96], True, False, True)
+        assert dx.shape == (5, 256) and da.shape == (0,) and db.shape == b.shape
 
 
 @pytest.mark.parametrize("fmt", ref.FORMATS)

@@ -49,7 +49,8 @@ def test_against_64_bits(pkg, dev, fmt, m, widths, k, slots, rank):
     ref.check(y, *_want(fmt, x, w, ad, ids))
     assert torch.equal(y, method.apply(layer, x, None, adapters=ad, batch=batch))
     none = ids < 0
-    assert torch.equal(y[none], method.apply(layer, x)[none])  # untouched where there is no adapter
+    if not pkg.ops.adapter_linear_supported(m, sum(widths), k, 0, False, slots, len(widths), rank):
+        assert torch.equal(y[none], method.apply(layer, x)[none])  # untouched where there is no adapter
 
 
 @pytest.mark.parametrize("rank", [8, 40, 104, 256])
@@ -76,14 +77,15 @@ def test_batch_contents(pkg, dev):
             b = pkg.AdapterBatch(kind, slots)
             want = torch.sort(torch.where(ids < 0, slots, ids), stable=True)
             n = int((ids >= 0).sum())
-            assert torch.equal(b.order[:n].long(), want.indices[:n])
-            assert torch.equal(b.offsets, torch.searchsorted(want.values[:n].contiguous(), torch.arange(slots + 1, device=dev)))
-        rows = 16 if m <= 512 else 64
-        tiles = [(s, int(p)) for s in range(slots) for p in range(int(b.offsets[s]), int(b.offsets[s + 1]), rows)]
-        got = [tuple(t) for t in b.tiles.tolist()]
+            _, order, offsets, tiles_ = b.tensors
+            assert torch.equal(order[:n].long(), want.indices[:n])
+            assert torch.equal(offsets, torch.searchsorted(want.values[:n].contiguous(), torch.arange(slots + 1, device=dev)))
+        at = offsets.tolist()
+        tiles = [(s, p) for s in range(slots) for p in range(at[s], at[s + 1], 16)]
+        got = [tuple(t) for t in tiles_.tolist()]
         assert got[:len(tiles)] == tiles and all(t[0] == -1 for t in got[len(tiles):])
     big = pkg.AdapterBatch(torch.tensor([2 ** 32, 1, -2 ** 40, 0], device=dev), 2)
-    assert big.offsets.tolist() == [0, 1, 2] and big.order[:2].tolist() == [3, 1]
+    assert big.tensors[2].tolist() == [0, 1, 2] and big.tensors[1][:2].tolist() == [3, 1]
 
 
 @pytest.mark.parametrize("fmt", ref.FORMATS)
@@ -285,3 +287,96 @@ def test_mlp_with_adapters(pkg, dev):
     assert torch.equal(y.detach(), (x + z).detach()) and torch.equal(da, da2) and torch.equal(db, db2)
     both = pkg.ops.gated_grad(x.detach(), dh, gate_up.weight, gate_up.weight_scale, 512, gate_up.mxl_format)
     assert torch.equal(dx, dy + pkg.ops.input_grad(both, *pkg.adapters.grad_of(gate_up)))
+
+
+@pytest.mark.parametrize("fmt", ref.FORMATS)
+@pytest.mark.parametrize("m,widths,k,slots,rank,runs", [(33, [128], 128, 1, 8, False), (100, [256, 128], 384, 3, 24, False),
+                                                        (300, [1024, 128], 1152, 5, 64, True), (1024, [2560], 256, 2, 16, True),
+                                                        (700, [128, 8320], 384, 4, 104, False)])
+def test_one_product(pkg, dev, fmt, m, widths, k, slots, rank, runs):
+    """The adapters inside the layer's product: one rounding, whichever tile; mixed and whole tiles, with a bias."""
+    n = sum(widths)
+    assert pkg.ops.adapter_linear_supported(m, n, k, 0, False, slots, len(widths), rank)
+    g, method, layer, w, ad, x, ids = _case(pkg, dev, fmt, widths, k, slots, rank, _ids(m, slots, m, runs), m)
+    batch = pkg.AdapterBatch(ids, slots)
+    base, off = ref.product(ref.quantized(fmt, x), w, scaled=True)
+    delta, doff, _ = ref.adapters(x, ad.lora_a, ad.lora_b, ad.scaling, ids, widths, rank)
+    want, bound = base + delta, off + doff + 1e-30
+    y = method.apply(layer, x, None, adapters=ad, batch=batch)
+    ref.check(y, want, ref.U * want.abs() + (1 + ref.U) * bound)
+    assert torch.equal(y, method.apply(layer, x, None, adapters=ad, batch=batch))
+    bias = torch.randn(n, generator=g).bfloat16().to(dev)
+    z = method.apply(layer, x, bias, adapters=ad, batch=batch)
+    if fmt == "mxfp4":  # (joins the sum)
+        ref.check(z, want + bias.double(), ref.U * (want + bias.double()).abs() + (1 + ref.U) * (bound + (want + bias.double()).abs() * 2.0 ** -23))
+    else:
+        assert torch.equal(z, y + bias)
+
+
+def test_one_product_of_odd_columns(pkg, dev):
+    """A last part whose columns end inside an n-tile, and columns that a tile has beyond the layer's."""
+    for fmt, widths in (("mxfp4", [136]), ("mxfp6", [40]), ("block", [32, 99])):
+        n = sum(widths)
+        g = torch.Generator().manual_seed(n)
+        method, layer, w = ref.make_layer(pkg, fmt, [n], 256, dev, g)
+        a = (torch.randn(2, len(widths) * 16, 256, generator=g) / 16).bfloat16().to(dev)
+        b = torch.randn(2, n, 16, generator=g).bfloat16().to(dev)
+        scaling = torch.tensor([0.5, 2.0], device=dev)
+        ids = _ids(80, 2, n).int().to(dev)
+        x = torch.randn(80, 256, generator=g).bfloat16().to(dev)
+        wt, sw, _, k, f, block = pkg.adapters.grad_of(layer)
+        cols = [0, *torch.tensor(widths).cumsum(0).tolist()]
+        batch = pkg.ops.adapter_batch(ids, 2)
+        y, v = pkg.ops.adapter_linear(x, wt, sw, f, block, 0, None, a, b, scaling, *batch, cols)
+        base, off = ref.product(ref.quantized(fmt, x), w, scaled=True)
+        delta, doff, _ = ref.adapters(x, a, b, scaling, ids, widths, 16)
+        ref.check(y, base + delta, ref.U * (base + delta).abs() + (1 + ref.U) * (off + doff))
+        z = method.apply(layer, x)
+        assert torch.equal(pkg.ops.adapter_apply(z, x, a, b, scaling, *batch, cols)[ids >= 0], v[ids >= 0])
+        ref.check(z, base + delta, ref.U * ((base + delta).abs() + base.abs()) + (1 + ref.U) * (2 * off + doff))
+
+
+def test_refusals(pkg, dev):
+    g, method, layer, w, ad, x, ids = _case(pkg, dev, "mxfp8", [128], 256, 3, 8, [0, 1, 2], 1)
+    batch = pkg.AdapterBatch(ids, 3)
+    call = lambda **kw: method.apply(layer, **{"x": x, "adapters": ad, "batch": batch, **kw})  # noqa: E731
+    for kw in (dict(batch=None), dict(adapters=None), dict(batch=ids), dict(adapters=ad.lora_a)):
+        with pytest.raises(ValueError, match="go together"):
+            call(**kw)
+    with pytest.raises(ValueError, match="3 rows"):
+        call(x=x[:2])
+    with pytest.raises(ValueError, match="bf16"):
+        call(x=x.float())
+    with pytest.raises(ValueError, match="slots"):
+        call(batch=pkg.AdapterBatch(ids, 4))
+    _, other, _ = ref.make_layer(pkg, "mxfp8", [256], 256, dev, g)
+    with pytest.raises(ValueError, match="not of this layer"):
+        call(adapters=pkg.LowRankAdapters(other, 3, 8))
+    with pytest.raises(ValueError, match="update needs"):
+        batch.update(ids[:2])
+    for bad in (ids.float(), ids.view(1, 3), ids.bool()):
+        with pytest.raises(ValueError, match="integers"):
+            pkg.AdapterBatch(bad, 3)
+    for slots in (0, 2049):
+        with pytest.raises(ValueError, match="adapters"):
+            pkg.AdapterBatch(ids, slots)
+    o, t, cols = pkg.ops, batch.tensors, [0, 128]
+    y = method.apply(layer, x)
+    args = dict(y=y, x=x, a=ad.lora_a, b=ad.lora_b, scaling=ad.scaling, ids=t[0], order=t[1], offsets=t[2], tiles=t[3], cols=cols)
+    for name, bad, match in (("a", ad.lora_a[:2], "do not fit"), ("b", ad.lora_b.float(), "bf16"), ("cols", [0, 64], "do not fit"),
+                             ("cols", [0, 8, 128], "multiples of 16"), ("scaling", ad.scaling.double(), "scaling"),
+                             ("tiles", t[3][:1], "batch"), ("order", t[1].long(), "batch"), ("y", y[:, ::2], "unit column"),
+                             ("y", y[:2], "y must be"), ("ids", t[0].cpu(), "HIP device|tensors on")):
+        with pytest.raises(ValueError, match=match):
+            o.adapter_apply(**{**args, name: bad})
+    wt, sw, n, k, f, block = pkg.adapters.grad_of(layer)
+    with pytest.raises(ValueError, match="one product"):
+        o.adapter_linear(x, wt, sw, f, block, 0, None, ad.lora_a, ad.lora_b, ad.scaling, *t, cols)
+    v = o.adapter_apply(**args)
+    for dy, vv, match in ((y[:2], v, "rows"), (y.float(), v, "bf16"), (y, v[:, :16], "not adapter_apply's")):
+        with pytest.raises(ValueError, match=match):
+            o.adapter_grad(dy, x, wt, sw, f, block, ad.lora_a, ad.lora_b, ad.scaling, vv, *t, cols)
+    with pytest.raises(ValueError, match="tiled layout"):
+        o.input_grad(y, wt[:-1], sw, n, k, f, block)
+    with pytest.raises(ValueError, match="tiled layout"):
+        o.gated_linear(x, wt, sw[:-1], 64, f)

@@ -46,13 +46,17 @@ SIGNATURES = {
     "mxl_mxfp4_grouped_gemm": (_I, [_P, _P, _I64, _P, _I, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P]),
     "mxl_adapter_tile_count": (_I64, [_I64, _I64]),
     "mxl_adapter_tiles": (_I, [_P, _I64, _I64, _P, _I64, _P]),
-    "mxl_adapter_v_floats": (_I64, [_I64, _I64, _I64, _I64, _I64]),
+    "mxl_adapter_v_elems": (_I64, [_I64, _I64, _I64]),
     "mxl_adapter_apply": (_I, [_P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I64,
                                _P]),
-    "mxl_adapter_grad_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _P, _I64]),
-    "mxl_adapter_grad": (_I, [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64,
-                              _P, _I64, _P, _P, _P, _I64, _P]),
-    "mxl_input_grad_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "mxl_adapter_linear_supported": (_I, [_I64, _I64, _I64, _I, _I, _I64, _I64, _I64]),
+    "mxl_adapter_linear_workspace_bytes": (_I64, [_I64, _I64, _I, _I]),
+    "mxl_adapter_linear": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _I, _I, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _P,
+                                _I64, _P, _I64, _P, _I64, _P, _I64, _P]),
+    "mxl_adapter_grad_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _P, _I64, _I]),
+    "mxl_adapter_grad": (_I, [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _I, _I, _P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _P,
+                              _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P]),
+    "mxl_input_grad_workspace_bytes": (_I64, [_I64, _I64, _I64, _I]),
     "mxl_input_grad": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I, _I, _P, _I64, _P, _I64, _P]),
     "mxl_gated_workspace_bytes": (_I64, [_I64, _I64, _I]),
     "mxl_gated_linear": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _I64, _I, _I, _P, _I64, _P, _I64, _P]),

@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import ops
-from .linear import _function_bias
+from .linear import _epilogue_bias, _function_bias
 
 
 class AdapterBatch:
@@ -28,16 +28,16 @@ class AdapterBatch:
 
     def __init__(self, ids: torch.Tensor, slots: int):
         self.slots = int(slots)
-        self.order, self.offsets, self.tiles = ops.adapter_batch(ids, self.slots)
+        self.tensors = ops.adapter_batch(ids, self.slots)  # ids, order, offsets, tiles
 
     def __len__(self) -> int:
-        return self.order.shape[0]
+        return self.tensors[0].shape[0]
 
     def update(self, ids: torch.Tensor) -> "AdapterBatch":
-        if tuple(ids.shape) != tuple(self.order.shape) or ids.device != self.order.device:
-            raise ValueError(f"update needs ids of {len(self)} tokens on {self.order.device}, got {tuple(ids.shape)} on "
+        if tuple(ids.shape) != (len(self),) or ids.device != self.tensors[0].device:
+            raise ValueError(f"update needs ids of {len(self)} tokens on {self.tensors[0].device}, got {tuple(ids.shape)} on "
                              f"{ids.device}")
-        for kept, new in zip((self.order, self.offsets, self.tiles), ops.adapter_batch(ids, self.slots)):
+        for kept, new in zip(self.tensors, ops.adapter_batch(ids, self.slots)):
             kept.copy_(new)
         return self
 
@@ -135,33 +135,31 @@ class FrozenLinear(torch.autograd.Function):
 
 
 class AdapterLinear(torch.autograd.Function):
-    """A prepared layer with its adapters: the gradients of the input and of the adapters."""
+    """A prepared layer with its adapters: the gradients of the input, the adapters and a bias in the epilogue."""
 
     @staticmethod
-    def forward(x, a, b, scaling, order, offsets, tiles, cols, w, sw, layer, bias):
-        y = layer.mxl_kernel.apply_weights(layer, x, bias)
-        v = ops.adapter_apply(y.view(-1, y.shape[-1]), x.reshape(-1, x.shape[-1]), a, b, scaling, order, offsets, tiles, cols)
-        return y, v
+    def forward(x, a, b, scaling, ids, order, offsets, tiles, cols, w, sw, layer, bias):
+        return _forward(layer, x, bias, a, b, scaling, (ids, order, offsets, tiles), cols)
 
     @staticmethod
     def setup_context(ctx, inputs, output):
-        x, a, b, scaling, order, offsets, tiles, cols, w, sw, layer, _ = inputs
+        x, a, b, scaling, ids, order, offsets, tiles, cols, w, sw, layer, _ = inputs
         ctx.mark_non_differentiable(output[1])
         # (a batch updated for the next step before this one's backward is noticed by its tensors' versions)
-        ctx.save_for_backward(x, a, b, scaling, output[1], order, offsets, tiles, w, sw)
+        ctx.save_for_backward(x, a, b, scaling, output[1], ids, order, offsets, tiles, w, sw)
         ctx.meta = (list(cols), *grad_of(layer)[2:])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, _):
-        x, a, b, scaling, v, order, offsets, tiles, w, sw = ctx.saved_tensors
+        x, a, b, scaling, v, *batch, w, sw = ctx.saved_tensors
         cols, n, k, fmt, block = ctx.meta
         need_x, need_a, need_b = ctx.needs_input_grad[:3]
         dy2 = dy.reshape(-1, n)
-        dx = ops.input_grad(dy2, w, sw, n, k, fmt, block) if need_x else None
-        da, db = ops.adapter_grad(dx, dy2, x.reshape(-1, k), a, b, scaling, v, order, offsets, tiles, cols, need_a, need_b)
-        return (None if dx is None else dx.reshape(x.shape), da if need_a else None, db if need_b else None, *[None] * 8,
-                dy2.sum(0) if ctx.needs_input_grad[11] else None)
+        dx, da, db = ops.adapter_grad(dy2, x.reshape(-1, k), w, sw, fmt, block, a, b, scaling, v, *batch, cols, need_x, need_a,
+                                      need_b)
+        return (dx.reshape(x.shape) if need_x else None, da if need_a else None, db if need_b else None, *[None] * 9,
+                dy2.sum(0) if ctx.needs_input_grad[12] else None)
 
 
 class GatedLinear(torch.autograd.Function):
@@ -186,6 +184,19 @@ class GatedLinear(torch.autograd.Function):
         return ops.input_grad(both, w, sw, 2 * i, k, fmt).reshape(x.shape), *[None] * 6
 
 
+def _forward(layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor], a, b, scaling, batch, cols):
+    """(y, v): in one product where the shape has it, else the layer and then the adapters in place."""
+    w, sw, n, k, fmt, block = grad_of(layer)
+    x2 = x.reshape(-1, k)
+    inner = _epilogue_bias(bias, x, n)
+    if bias is inner and ops.adapter_linear_supported(x2.shape[0], n, k, fmt, block, a.shape[0], len(cols) - 1, b.shape[2]):
+        y, v = ops.adapter_linear(x2, w, sw, fmt, block, getattr(layer.mxl_kernel, "act_rule", 0), inner, a, b, scaling, *batch,
+                                  cols)
+        return y.reshape(*x.shape[:-1], n), v
+    y = layer.mxl_kernel.apply_weights(layer, x, bias)
+    return y, ops.adapter_apply(y.view(-1, n), x2, a, b, scaling, *batch, cols)
+
+
 def apply_adapters(layer: torch.nn.Module, x: torch.Tensor, adapters: LowRankAdapters, batch: AdapterBatch,
                    bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A prepared layer's output with the adapters of a batch's tokens added: x bf16 [..., K] of ``len(batch)`` rows."""
@@ -202,10 +213,6 @@ def apply_adapters(layer: torch.nn.Module, x: torch.Tensor, adapters: LowRankAda
     if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad):
         w, sw = grad_of(layer)[:2]
         inner = _function_bias(bias, x, n)
-        y = AdapterLinear.apply(x, a, b, adapters.scaling, batch.order, batch.offsets, batch.tiles, adapters.cols, w, sw,
-                                layer, inner)[0]
+        y = AdapterLinear.apply(x, a, b, adapters.scaling, *batch.tensors, adapters.cols, w, sw, layer, inner)[0]
         return y if bias is inner else y + bias
-    y = layer.mxl_kernel.apply_weights(layer, x, bias)
-    ops.adapter_apply(y.view(-1, n), x.reshape(-1, k), a, b, adapters.scaling, batch.order, batch.offsets, batch.tiles,
-                      adapters.cols)
-    return y
+    return _forward(layer, x, bias, a, b, adapters.scaling, batch.tensors, adapters.cols)[0]

@@ -1,0 +1,50 @@
+// What the adapters' kernels (adapters.hip) and the products that add them (gemm_tile.h, input_grad.hip) share.
+#pragma once
+
+#include <stdint.h>
+
+namespace mxl {
+
+constexpr int kMaxParts = 8, kMaxRank = 256, kMaxSlots = 4096, kAdapterTile = 16;
+
+// Tokens sorted by adapter: positions [offsets[a], offsets[a + 1]) of order are adapter a's, in tiles of 16 positions:
+// tile i is (adapter, first position), adapter -1 past the last.
+struct AdapterBatch {
+  const int32_t* order;
+  const int64_t* offsets;
+  const int32_t* tiles;
+  int num_tiles;
+  int64_t M;
+};
+
+// v of a token: its parts' ranks, each part padded to groups of 16, as bf16 [2][width]: the values, then what bf16 left of
+// them.  A token without an adapter has none (its v is never written).
+struct LowRank {
+  int parts, rank, groups;  // groups: of 16 ranks of a part
+  int64_t cols[kMaxParts + 1];
+  __host__ __device__ int width() const { return parts * groups * 16; }
+};
+
+// What a product adds of a batch's adapters to its sums, ahead of their rounding: for a row t of adapter ids[t] (outside
+// [0, slots): none) the products of v[t] with mat, B [N, ldm] for y += B v (of a column's part), or A [R, ldm] for
+// dx += A^T dv (of all parts).  slot_stride: of mat's adapters.
+struct RowAdapters {
+  const int32_t* ids = nullptr;
+  int slots = 0;
+  const uint16_t* v = nullptr;
+  const uint16_t* mat = nullptr;
+  int64_t slot_stride = 0, ldm = 0;
+  LowRank l{};
+};
+
+// Whether a product adds the adapters of its rows itself: it walks the adapters of a tile's rows one after the other, so
+// that few rows of many adapters are better added by a launch of their own (adapter_expand_kernel).
+inline bool rows_add(int64_t M, int64_t slots) { return M >= 32 * slots; }
+
+// dx = dy W (input_grad.hip), with `more` the adapters' dx as well.
+int64_t input_grad_bytes(int64_t M, int64_t N, int64_t K, int block);
+int input_grad(const char* who, const void* dy, int64_t M, int64_t N, int64_t lddy, const void* w, const void* sw, int64_t K,
+               int fmt, int block, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, const RowAdapters* more,
+               void* stream);
+
+}  // namespace mxl

@@ -3,78 +3,45 @@
 // Token t of a batch belongs to adapter a(t) (or to none): y[t] += s[a] B[a] (A[a] x[t]), A [R, K] and B [N, r] bf16 of
 // each adapter, R = parts r: a merged layer's part p (columns [cols[p], cols[p + 1])) has the rows [p r, p r + r) of A.
 //
-//   shrink   v[t] = s A x[t]: fp32, by position in the batch sorted by adapter      (also dv = s B^T dy, from B^T)
+//   shrink   v[t] = s A x[t]                                                        (also dv = s B^T dy, from B^T)
 //   expand   y[t] += B v[t], in place                                               (also dx += A^T dv, from A^T)
 //   outer    dB = sum_t dy[t] v[t]^T, dA = sum_t dv[t] x[t]^T over an adapter's tokens
 //
-// v is never rounded to bf16: a product with it takes bf16 v_hi = v and v_lo = v - v_hi side by side along the MFMA's
-// K (16 ranks of each in its 32), which leaves 2^-17 of it and costs nothing, for every one of these kernels waits for
-// memory.  Sums are fp32 in the MFMA, joined in a fixed order.
+// v is never rounded to bf16: it is kept as bf16 v_hi = v and v_lo = v - v_hi, side by side along the MFMA's K (16 ranks
+// of each in its 32), which leaves 2^-16 of it and costs nothing, for every one of these kernels waits for memory.  Sums
+// are fp32 in the MFMA, joined in a fixed order.
 #include <algorithm>
 
-#include "mx_common.h"
+#include "adapters.h"
+#include "fp4.h"
+#include "gemm_wide.h"
 
 namespace mxl {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 
-constexpr int kMaxParts = 8, kMaxRank = 256, kMaxSlots = 4096;
-
-// Tokens sorted by adapter: positions [offsets[a], offsets[a + 1]) of order are adapter a's, in tiles of `rows`
-// positions: tile i is (adapter, first position), adapter -1 past the last.
-struct Batch {
-  const int32_t* order;
-  const int64_t* offsets;
-  const int32_t* tiles;
-  int num_tiles, rows;
-  int64_t M;
-};
-
-struct LowRank {
-  int parts, rank, groups;  // groups: of 16 ranks of a part
-  int64_t cols[kMaxParts + 1];
-  __host__ __device__ int width() const { return parts * groups * 16; }  // of a row of v
-};
-
-// Adapter and positions [lo, hi) of piece i, `rows` positions (a divisor of b.rows); false where there are none.
-__device__ __forceinline__ bool batch_tile(const Batch& b, int rows, int i, int& slot, int64_t& lo, int64_t& hi) {
-  const int pieces = b.rows / rows, tile = i / pieces;
+// The tile's adapter and positions [lo, hi); false past the last tile.
+__device__ __forceinline__ bool batch_tile(const AdapterBatch& b, int tile, int& slot, int64_t& lo, int64_t& hi) {
   slot = b.tiles[2 * tile];
   if (slot < 0) return false;
-  lo = b.tiles[2 * tile + 1] + (i - tile * pieces) * rows;
+  lo = b.tiles[2 * tile + 1];
   const int64_t end = b.offsets[slot + 1];
-  hi = lo + rows < end ? lo + rows : end;
+  hi = lo + kAdapterTile < end ? lo + kAdapterTile : end;
   hi = hi < b.M ? hi : b.M;
   return lo < hi;
 }
 
-__device__ __forceinline__ bf16x8_t as_bf16x8(const uint4& v) { return __builtin_bit_cast(bf16x8_t, v); }
-
-__device__ __forceinline__ uint4 keep(const uint4& v, bool in) {
-  return uint4{in ? v.x : 0u, in ? v.y : 0u, in ? v.z : 0u, in ? v.w : 0u};
-}
-
-// Eight fp32 as bf16: the values, or what they leave of the fp32.
-__device__ __forceinline__ uint4 split8(const float* v, bool rest) {
-  uint32_t d[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    d[i] = cvt_pk_bf16(v[2 * i], v[2 * i + 1]);
-    if (rest) {
-      // (an infinity leaves NaN of itself: its rest is zero)
-      const float h0 = u2f(d[i] << 16), h1 = u2f(d[i] & 0xFFFF0000u);
-      const float r0 = v[2 * i] - h0, r1 = v[2 * i + 1] - h1;
-      d[i] = cvt_pk_bf16(__builtin_isfinite(h0) ? r0 : 0.0f, __builtin_isfinite(h1) ? r1 : 0.0f);
-    }
-  }
-  return uint4{d[0], d[1], d[2], d[3]};
+__device__ __forceinline__ bf16x8_t as_bf16x8(const u32x4& v) { return __builtin_bit_cast(bf16x8_t, v); }
+__device__ __forceinline__ u32x4 keep(const u32x4& v, bool in) {
+  return u32x4{in ? v[0] : 0u, in ? v[1] : 0u, in ? v[2] : 0u, in ? v[3] : 0u};
 }
 
 // ------------------------------------------------------------------ tiles of a batch
 
-__global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offsets, int slots, int rows, int num_tiles,
+__global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offsets, int slots, int num_tiles,
                                                              int32_t* tiles) {
   __shared__ int first[kMaxSlots + 1];  // the first tile of each adapter
   __shared__ int sums[16];
@@ -82,7 +49,7 @@ __global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offs
   int before = 0;
   for (int base = 0; base < slots; base += 1024) {
     const int s = base + t;
-    int n = s < slots ? (int)((offsets[s + 1] - offsets[s] + rows - 1) / rows) : 0, x = n;
+    int n = s < slots ? (int)((offsets[s + 1] - offsets[s] + kAdapterTile - 1) / kAdapterTile) : 0, x = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int y = __shfl_up(x, d, 64);
@@ -110,7 +77,7 @@ __global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offs
         if (first[mid] <= i) lo = mid; else hi = mid;
       }
       slot = lo;
-      pos = (int)offsets[lo] + (i - first[lo]) * rows;
+      pos = (int)offsets[lo] + (i - first[lo]) * kAdapterTile;
     }
     tiles[2 * i] = slot;
     tiles[2 * i + 1] = pos;
@@ -119,171 +86,154 @@ __global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offs
 
 // ------------------------------------------------------------------ shrink
 
-// v[split][position][16 group + j] = s sum_k rows[j][k] x[k] over the split's columns.  BY_PART: part p's rows are [0, r)
-// of the adapter's and its columns [cols[p], cols[p + 1]) (B^T [r, N]); else rows [p r, p r + r) and all columns (A).
-// A workgroup is a tile of 16 TS tokens by RC groups of 16 ranks; its waves share the columns and meet in LDS.  Both
-// operands come straight from memory: the rows' A from L2, where its tiles share it, x once.
-template <int TS, int RC, bool BY_PART>
-__global__ __launch_bounds__(512) void adapter_shrink_kernel(Batch b, LowRank l, const uint16_t* x, int64_t ldx, int64_t cols,
-                                                             const uint16_t* rows, int64_t slot_stride, int64_t ldr,
-                                                             const float* scaling, float* v) {
+// v[t] (adapters.h) of s sum_k rows[j][k] x[t][k].  BY_PART: part p's rows are [0, r) of the adapter's and its columns
+// [cols[p], cols[p + 1]) (B^T [r, N]); else rows [p r, p r + r) and all columns (A).  A workgroup is a tile of 16 tokens
+// by RC groups of 16 ranks; its waves share the columns and meet in LDS.  Both operands come straight from memory: the
+// rows' A from L2, where its tiles share it, x once.
+template <int RC, bool BY_PART>
+__global__ __launch_bounds__(RC == 1 ? 1024 : 512) void adapter_shrink_kernel(AdapterBatch b, LowRank l, const uint16_t* x, int64_t ldx,
+                                                              int64_t cols, const uint16_t* rows, int64_t slot_stride,
+                                                              int64_t ldr, const float* scaling, uint16_t* v) {
   extern __shared__ __attribute__((aligned(16))) float red[];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, q = lane >> 4;
   int slot;
   int64_t lo, hi;
-  if (!batch_tile(b, 16 * TS, blockIdx.x, slot, lo, hi)) return;
+  if (!batch_tile(b, blockIdx.x, slot, lo, hi)) return;
   const int per_part = (l.groups + RC - 1) / RC, part = blockIdx.y / per_part, g0 = (blockIdx.y - part * per_part) * RC;
   const int64_t c0 = BY_PART ? l.cols[part] : 0, c1 = BY_PART ? l.cols[part + 1] : cols;
-  const uint16_t* xr[TS];
-#pragma unroll
-  for (int i = 0; i < TS; ++i) {
-    const int64_t pos = lo + 16 * i + r < hi ? lo + 16 * i + r : hi - 1;
-    xr[i] = x + (int64_t)b.order[pos] * ldx + 8 * q;
-  }
+  const int64_t pos = lo + r < hi ? lo + r : hi - 1;
+  const int token = b.order[pos];
+  const uint16_t* const xr = x + (int64_t)token * ldx + 8 * q;
   const uint16_t* ar[RC];
 #pragma unroll
   for (int g = 0; g < RC; ++g) {
     const int j = 16 * (g0 + g) + r, row = (BY_PART ? 0 : part * l.rank) + (j < l.rank ? j : l.rank - 1);
     ar[g] = rows + slot * slot_stride + row * ldr + 8 * q;
   }
-  v4f acc[TS][RC];
+  v4f acc[RC];
 #pragma unroll
-  for (int i = 0; i < TS; ++i)
-#pragma unroll
-    for (int g = 0; g < RC; ++g) acc[i][g] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int g = 0; g < RC; ++g) acc[g] = v4f{0.f, 0.f, 0.f, 0.f};
   // this wave's columns: 32 an MFMA, U of them loaded together
-  constexpr int U = TS * RC >= 8 ? 2 : 4;
-  const int64_t units = (c1 - c0 + 31) / 32, shares = (int64_t)gridDim.z * waves, per = (units + shares - 1) / shares;
-  const int64_t k0 = c0 + 32 * per * (blockIdx.z * waves + wv), k1 = k0 + 32 * per < c1 ? k0 + 32 * per : c1;
+  constexpr int U = 4;
+  const int64_t units = (c1 - c0 + 31) / 32, per = (units + waves - 1) / waves;
+  const int64_t k0 = c0 + 32 * per * wv, k1 = k0 + 32 * per < c1 ? k0 + 32 * per : c1;
   for (int64_t k = k0; k < k1; k += 32 * U) {
-    uint4 xv[U][TS], av[U][RC];
+    u32x4 xv[U], av[U][RC];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t at = k + 32 * u + 8 * q < k1 ? k + 32 * u : c0 - 8 * q;  // (columns come in eights)
+      xv[u] = *reinterpret_cast<const u32x4*>(xr + at);
 #pragma unroll
-      for (int i = 0; i < TS; ++i) xv[u][i] = *reinterpret_cast<const uint4*>(xr[i] + at);
-#pragma unroll
-      for (int g = 0; g < RC; ++g) av[u][g] = *reinterpret_cast<const uint4*>(ar[g] + at);
+      for (int g = 0; g < RC; ++g) av[u][g] = *reinterpret_cast<const u32x4*>(ar[g] + at);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool in = k + 32 * u + 8 * q < k1;
+      xv[u] = keep(xv[u], in);
 #pragma unroll
-      for (int i = 0; i < TS; ++i) xv[u][i] = keep(xv[u][i], in);
-#pragma unroll
-      for (int g = 0; g < RC; ++g) av[u][g] = keep(av[u][g], in);
-#pragma unroll
-      for (int i = 0; i < TS; ++i)
-#pragma unroll
-        for (int g = 0; g < RC; ++g)
-          acc[i][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(av[u][g]), as_bf16x8(xv[u][i]), acc[i][g], 0, 0, 0);
+      for (int g = 0; g < RC; ++g)
+        acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(keep(av[u][g], in)), as_bf16x8(xv[u]), acc[g], 0, 0, 0);
     }
   }
 #pragma unroll
-  for (int i = 0; i < TS; ++i)
-#pragma unroll
-    for (int g = 0; g < RC; ++g) *reinterpret_cast<v4f*>(red + (((i * RC + g) * waves + wv) * 64 + lane) * 4) = acc[i][g];
+  for (int g = 0; g < RC; ++g) *reinterpret_cast<v4f*>(red + ((g * waves + wv) * 64 + lane) * 4) = acc[g];
   __syncthreads();
   const float s = scaling[slot];
-  for (int f = wv; f < TS * RC; f += waves) {
-    v4f sum = *reinterpret_cast<const v4f*>(red + ((int64_t)f * waves * 64 + lane) * 4);
+  for (int f = wv; f < RC; f += waves) {
+    v4f sum = *reinterpret_cast<const v4f*>(red + (f * waves * 64 + lane) * 4);
     for (int w = 1; w < waves; ++w) {
-      const v4f part_sum = *reinterpret_cast<const v4f*>(red + ((f * waves + w) * 64 + lane) * 4);
+      const v4f one = *reinterpret_cast<const v4f*>(red + ((f * waves + w) * 64 + lane) * 4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += part_sum[e];
+      for (int e = 0; e < 4; ++e) sum[e] += one[e];
     }
-    const int i = f / RC, g = g0 + f % RC;
-    const int64_t pos = lo + 16 * i + r;
-    if (pos < hi && g < l.groups) {
+    const int g = g0 + f;
+    if (lo + r < hi && g < l.groups) {
+      uint32_t hl[2][2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] = 16 * g + 4 * q + e < l.rank ? sum[e] * s : 0.0f;
-      *reinterpret_cast<v4f*>(v + (blockIdx.z * b.M + pos) * l.width() + (part * l.groups + g) * 16 + 4 * q) = sum;
+      for (int e = 0; e < 4; e += 2) {
+        const float v0 = 16 * g + 4 * q + e < l.rank ? sum[e] * s : 0.0f, v1 = 16 * g + 4 * q + e + 1 < l.rank ? sum[e + 1] * s : 0.0f;
+        const uint32_t h = cvt_pk_bf16(v0, v1);
+        const float h0 = u2f(h << 16), h1 = u2f(h & 0xFFFF0000u);
+        hl[0][e / 2] = h;  // (of an infinity nothing is left, where the difference would be NaN)
+        hl[1][e / 2] = cvt_pk_bf16(__builtin_isfinite(h0) ? v0 - h0 : 0.0f, __builtin_isfinite(h1) ? v1 - h1 : 0.0f);
+      }
+      uint16_t* const to = v + (int64_t)token * (2 * l.width()) + (part * l.groups + g) * 16 + 4 * q;
+      *reinterpret_cast<uint2*>(to) = uint2{hl[0][0], hl[0][1]};
+      *reinterpret_cast<uint2*>(to + l.width()) = uint2{hl[1][0], hl[1][1]};
     }
   }
 }
 
 // ------------------------------------------------------------------ expand
 
-// y[t][n] += sum_j mat[n][j] v[t][j], mat [N, ldm] of the tile's adapter, j the ranks of n's part.  A workgroup is a tile
-// of 16 TS tokens by `block` columns of one part (part_block: the first block of each part); v's halves wait in LDS.
-template <int TS>
-__global__ __launch_bounds__(256) void adapter_expand_kernel(Batch b, LowRank l, const float* v, int splits,
+// y[t][n] += sum_j mat[n][j] v[t][j], mat [N, ldm] (j < valid) of the tile's adapter, j the ranks of n's part.  A wave is a
+// tile of 16 tokens by 64 columns of one part: MFMA i's row 4 q + e is column 16 q + 4 i + e, so that after the four a
+// lane holds 16 columns of one token side by side (the rows of y in 32-byte pieces; `wide`: they start on 16 bytes).
+__global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterBatch b, LowRank l, const uint16_t* v,
                                                              const uint16_t* mat, int64_t slot_stride, int64_t ldm,
-                                                             int valid, uint16_t* y, int64_t ldy, int block) {
-  extern __shared__ __attribute__((aligned(16))) uint16_t half[];  // [2][16 TS][stride]
-  const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
+                                                             int valid, uint16_t* y, int64_t ldy, int wide) {
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   int slot;
   int64_t lo, hi;
-  if (!batch_tile(b, 16 * TS, blockIdx.x, slot, lo, hi)) return;
-  int part = 0, blk = blockIdx.y;
-  for (; part + 1 < l.parts; ++part) {
-    const int n = (int)((l.cols[part + 1] - l.cols[part] + block - 1) / block);
+  if (!batch_tile(b, blockIdx.x, slot, lo, hi)) return;
+  int part = 0, blk = 4 * blockIdx.y + wv;  // of 64 columns
+  for (; part < l.parts; ++part) {
+    const int n = (int)((l.cols[part + 1] - l.cols[part] + 63) / 64);
     if (blk < n) break;
     blk -= n;
   }
-  const int64_t c0 = l.cols[part] + (int64_t)blk * block, end = l.cols[part + 1];
-  const int64_t c1 = c0 + block < end ? c0 + block : end;
-  const int ranks = 16 * l.groups, stride = ranks + 8;
-  uint16_t* const rest = half + 16 * TS * stride;
-  for (int at = t; at < 16 * TS * (ranks / 8); at += 256) {
-    const int row = at / (ranks / 8), j = 8 * (at - row * (ranks / 8));
-    const int64_t pos = lo + row < hi ? lo + row : hi - 1;
-    float s[8] = {};
-    for (int k = 0; k < splits; ++k) {
-      const float* src = v + (k * b.M + pos) * l.width() + part * ranks + j;
-      const v4f x0 = *reinterpret_cast<const v4f*>(src), x1 = *reinterpret_cast<const v4f*>(src + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[e] += x0[e];
-        s[4 + e] += x1[e];
-      }
-    }
-    *reinterpret_cast<uint4*>(half + row * stride + j) = split8(s, false);
-    *reinterpret_cast<uint4*>(rest + row * stride + j) = split8(s, true);
+  if (part == l.parts) return;
+  const int64_t c0 = l.cols[part] + (int64_t)blk * 64, c1 = l.cols[part + 1];
+  const bool live = lo + r < hi;
+  const int64_t token = b.order[live ? lo + r : hi - 1];
+  uint16_t* const yr = y + token * ldy + c0 + 16 * q;
+  const bool whole = wide && c0 + 64 <= c1;
+  u32x4 old[2];
+  if (whole) {
+    old[0] = *reinterpret_cast<const u32x4*>(yr);
+    old[1] = *reinterpret_cast<const u32x4*>(yr + 8);
   }
-  __syncthreads();
-  const uint16_t* const vf = (q < 2 ? half : rest) + r * stride + 8 * (q & 1);
-  uint16_t* yr[TS];
-  bool live[TS];
+  const uint16_t* const vr = v + token * (2 * l.width()) + (q >> 1) * l.width() + part * l.groups * 16 + 8 * (q & 1);
+  const uint16_t* mr[4];
 #pragma unroll
-  for (int i = 0; i < TS; ++i) {
-    const int64_t pos = lo + 16 * i + r;
-    live[i] = pos < hi;
-    yr[i] = y + (int64_t)b.order[live[i] ? pos : hi - 1] * ldy;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = c0 + 16 * (r >> 2) + 4 * i + (r & 3);
+    mr[i] = mat + slot * slot_stride + (n < c1 ? n : c1 - 1) * ldm + 8 * (q & 1);
   }
-  const bool wide = ldy % 4 == 0 && ((uintptr_t)y & 7) == 0;
-  for (int64_t n0 = c0 + 16 * wv; n0 < c1; n0 += 64) {
-    const int64_t n = n0 + r < c1 ? n0 + r : c1 - 1, col = n0 + 4 * q;
-    const uint16_t* const mr = mat + slot * slot_stride + n * ldm;
-    v4f acc[TS];
+  v4f acc[4];
 #pragma unroll
-    for (int i = 0; i < TS; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int g = 0; g < l.groups; ++g) {
-      const int j = 16 * g + 8 * (q & 1);
-      uint4 m = {0, 0, 0, 0};
-      if (j < valid) m = *reinterpret_cast<const uint4*>(mr + j);
+  for (int i = 0; i < 4; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int g = 0; g < l.groups; ++g) {
+    const bool in = 16 * g + 8 * (q & 1) < valid;  // (ranks come in eights)
+    const u32x4 h = *reinterpret_cast<const u32x4*>(vr + 16 * g);
+    u32x4 m[4];
 #pragma unroll
-      for (int i = 0; i < TS; ++i) {
-        const uint4 h = *reinterpret_cast<const uint4*>(vf + 16 * i * stride + 16 * g);
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(m), as_bf16x8(h), acc[i], 0, 0, 0);
+    for (int i = 0; i < 4; ++i) m[i] = *reinterpret_cast<const u32x4*>(mr[i] + (in ? 16 * g : -8 * (q & 1)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(keep(m[i], in)), as_bf16x8(h), acc[i], 0, 0, 0);
+  }
+  if (!live) return;
+  if (whole) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4 d;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int i = 2 * h + w / 2, e = 2 * (w & 1);
+        d[w] = f32_to_bf16(u2f(old[h][w] << 16) + acc[i][e]) | (uint32_t)f32_to_bf16(u2f(old[h][w] & 0xFFFF0000u) + acc[i][e + 1]) << 16;
       }
+      *reinterpret_cast<u32x4*>(yr + 8 * h) = d;
     }
+  } else {
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      if (!live[i]) continue;
-      if (wide && col + 4 <= c1) {
-        uint2 d = *reinterpret_cast<const uint2*>(yr[i] + col);
-        const uint16_t h[4] = {f32_to_bf16(u2f(d.x << 16) + acc[i][0]), f32_to_bf16(u2f(d.x & 0xFFFF0000u) + acc[i][1]),
-                               f32_to_bf16(u2f(d.y << 16) + acc[i][2]), f32_to_bf16(u2f(d.y & 0xFFFF0000u) + acc[i][3])};
-        *reinterpret_cast<uint2*>(yr[i] + col) = uint2{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
-      } else {
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < c1) yr[i][col + e] = f32_to_bf16(bf16_to_f32(yr[i][col + e]) + acc[i][e]);
-      }
-    }
+      for (int e = 0; e < 4; ++e)
+        if (c0 + 16 * q + 4 * i + e < c1) yr[4 * i + e] = f32_to_bf16(bf16_to_f32(yr[4 * i + e]) + acc[i][e]);
   }
 }
 
@@ -291,14 +241,15 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(Batch b, LowRank l,
 
 // sum_t big[t][c] v[t][j] over the adapter's positions of split z: to out [N, r] (OF_B: c a column of dy, j the ranks of
 // its part) or out [R, K] (c a column of x, j all ranks).  A workgroup is 128 columns by RC groups; 32 tokens at a time
-// go through LDS, the big matrix's read transposed (each of its bytes is read once), v's stored so.
-constexpr int kOuterCols = 128, kOuterStride = kOuterCols + 16, kOuterTokens = 32, kOuterVStride = kOuterTokens + 8;
+// go through LDS, both operands read from it transposed; the next 32 are on their way.
+constexpr int kOuterCols = 128, kOuterStride = kOuterCols + 16, kOuterTokens = 32;
 template <int RC, bool OF_B>
-__global__ __launch_bounds__(256) void adapter_outer_kernel(Batch b, LowRank l, const uint16_t* big, int64_t ldb,
-                                                            const float* v, int v_splits, int64_t slots, int splits,
+__global__ __launch_bounds__(256) void adapter_outer_kernel(AdapterBatch b, LowRank l, const uint16_t* big, int64_t ldb,
+                                                            const uint16_t* v, int64_t slots, int splits,
                                                             int64_t out_cols, uint16_t* out, float* partial) {
+  constexpr int VS = 16 * RC + 16;  // elements of a token's row of v in LDS, a half
   __shared__ __attribute__((aligned(16))) uint16_t tile[kOuterTokens * kOuterStride];
-  __shared__ __attribute__((aligned(16))) uint16_t vt[2 * RC * 16 * kOuterVStride];  // [half][rank][token]
+  __shared__ __attribute__((aligned(16))) uint16_t vt[2 * kOuterTokens * VS];
   const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int64_t slot = blockIdx.z / splits;
@@ -328,56 +279,55 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(Batch b, LowRank l, 
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int g = 0; g < RC; ++g) acc[i][g] = v4f{0.f, 0.f, 0.f, 0.f};
-  const uint4 zero = {0, 0, 0, 0};
-  for (int64_t p0 = lo; p0 < hi; p0 += kOuterTokens) {
-    uint4 d[2];
+  // pieces of 8: of the big matrix token t / 16 + 16 u, columns 8 (t % 16); of v half, token and ranks
+  constexpr int VP = 2 * kOuterTokens * RC * 2, VU = (VP + 255) / 256;
+  u32x4 d[2], x[VU];
+  auto load = [&](int64_t p0) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {  // piece: token t / 16 + 16 u, columns 8 (t % 16)
+    for (int u = 0; u < 2; ++u) {
       const int64_t pos = p0 + (t >> 4) + 16 * u, c = c0 + 8 * (t & 15);
-      d[u] = zero;
-      if (pos < hi && c < end) d[u] = *reinterpret_cast<const uint4*>(big + (int64_t)b.order[pos] * ldb + c);
+      const bool in = pos < hi && c < end;
+      d[u] = keep(*reinterpret_cast<const u32x4*>(big + (int64_t)b.order[pos < hi ? pos : hi - 1] * ldb + (c < end ? c : c0)), in);
     }
-    float x[RC * 2];
 #pragma unroll
-    for (int u = 0; u < RC * 2; ++u) {  // value: token u_all / (16 RC), rank u_all % (16 RC)
-      const int at = t + 256 * u, tok = at / (16 * RC), j = at - tok * (16 * RC);
+    for (int u = 0; u < VU; ++u) {
+      const int at = t + 256 * u, h = at / (kOuterTokens * RC * 2), tok = at / (RC * 2) % kOuterTokens, j = 8 * (at % (RC * 2));
       const int64_t pos = p0 + tok;
-      x[u] = 0.0f;
-      if (pos < hi && g0 + j / 16 < all)
-        for (int k = 0; k < v_splits; ++k) x[u] += v[(k * b.M + pos) * l.width() + gv * 16 + j];
+      const bool in = pos < hi && g0 + j / 16 < all && at < VP;
+      x[u] = keep(*reinterpret_cast<const u32x4*>(v + (int64_t)b.order[pos < hi ? pos : hi - 1] * (2 * l.width()) +
+                                                  (in ? h * l.width() + gv * 16 + j : 0)), in);
     }
+  };
+  // a transposed fragment: eight tokens 8 q .. of column (of 16) r
+  auto frag = [&](const uint16_t* at, int stride) {
+    const uint16_t* const src = at + (8 * q + (r >> 2)) * stride + 4 * (r & 3);
+    const uint2 y0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src));
+    const uint2 y1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + 4 * stride)));
+    return as_bf16x8(u32x4{y0.x, y0.y, y1.x, y1.y});
+  };
+  if (lo < hi) load(lo);
+  for (int64_t p0 = lo; p0 < hi; p0 += kOuterTokens) {
     __syncthreads();  // the last tokens' reads
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      *reinterpret_cast<uint4*>(tile + ((t >> 4) + 16 * u) * kOuterStride + 8 * (t & 15)) = d[u];
+    for (int u = 0; u < 2; ++u) *reinterpret_cast<u32x4*>(tile + ((t >> 4) + 16 * u) * kOuterStride + 8 * (t & 15)) = d[u];
 #pragma unroll
-    for (int u = 0; u < RC * 2; ++u) {
-      const int at = t + 256 * u, tok = at / (16 * RC), j = at - tok * (16 * RC);
-      const uint32_t h = cvt_pk_bf16(x[u], 0.0f) & 0xFFFFu;
-      const float hf = u2f(h << 16);
-      vt[j * kOuterVStride + tok] = (uint16_t)h;
-      vt[(RC * 16 + j) * kOuterVStride + tok] = (uint16_t)cvt_pk_bf16(__builtin_isfinite(hf) ? x[u] - hf : 0.0f, 0.0f);
+    for (int u = 0; u < VU; ++u) {
+      const int at = t + 256 * u, row = at / (RC * 2), j = 8 * (at % (RC * 2));  // row: half 32 + token
+      if (at < VP) *reinterpret_cast<u32x4*>(vt + row * VS + j) = x[u];
     }
+    if (p0 + kOuterTokens < hi) load(p0 + kOuterTokens);
     __syncthreads();
-    uint4 cf[2];
+    bf16x8_t cf[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {  // columns 32 wv + 16 i + r, tokens 8 q .. + 7
-      const uint16_t* const src = tile + (8 * q + (r >> 2)) * kOuterStride + 32 * wv + 16 * i + 4 * (r & 3);
-      const s16x4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src));
-      const s16x4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + 4 * kOuterStride));
-      const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
-      cf[i] = uint4{y0.x, y0.y, y1.x, y1.y};
-    }
+    for (int i = 0; i < 2; ++i) cf[i] = frag(tile + 32 * wv + 16 * i, kOuterStride);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int g = 0; g < RC; ++g) {
-        const uint4 rf = *reinterpret_cast<const uint4*>(vt + (h * RC * 16 + 16 * g + r) * kOuterVStride + 8 * q);
+        const bf16x8_t rf = frag(vt + h * kOuterTokens * VS + 16 * g, VS);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bf16x8_t a = as_bf16x8(OF_B ? rf : cf[i]), c = as_bf16x8(OF_B ? cf[i] : rf);
-          acc[i][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, c, acc[i][g], 0, 0, 0);
-        }
+        for (int i = 0; i < 2; ++i)
+          acc[i][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(OF_B ? rf : cf[i], OF_B ? cf[i] : rf, acc[i][g], 0, 0, 0);
       }
   }
   // OF_B: lane holds ranks 4 q .. + 3 of column r; else columns 4 q .. + 3 of rank r
@@ -407,6 +357,7 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(const float* partial,
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= count) return;
   v4f s = *reinterpret_cast<const v4f*>(partial + at);
+#pragma unroll 4
   for (int k = 1; k < splits; ++k) {
     const v4f x = *reinterpret_cast<const v4f*>(partial + k * count + at);
 #pragma unroll
@@ -446,21 +397,11 @@ namespace {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Token rows of a tile: 16 while a batch has few, else 64, over which a workgroup's reads of A and B are shared.
-int tile_rows(int64_t M) { return M <= 512 ? 16 : 64; }
-int64_t tile_count(int64_t M, int64_t slots) {
-  const int64_t rows = tile_rows(M);
-  return std::min(M, ceil_div(M, rows) + std::min(slots, M));
-}
+int64_t tile_count(int64_t M, int64_t slots) { return std::min(M, ceil_div(M, kAdapterTile) + std::min(slots, M)); }
 
-// Groups a workgroup of shrink takes, and its shares of the columns: four waves each, until the launch has some 512
-// workgroups or a share is 128 columns a wave.
-int shrink_groups(int groups) { return groups >= 4 ? 4 : groups >= 2 ? 2 : 1; }
-int shrink_splits(int64_t M, int64_t slots, int parts, int groups, int64_t cols) {
-  const int64_t wgs = ceil_div(M, tile_rows(M)) * parts * ceil_div(groups, shrink_groups(groups));
-  int64_t s = std::min<int64_t>(8, ceil_div(512, wgs));
-  return (int)std::max<int64_t>(1, std::min(s, cols / 1024));
-}
+// Groups of 16 ranks a workgroup of shrink takes: up to four, which share the reads of x, once the tiles fill the card
+// without more workgroups; and its waves, over the columns.
+int shrink_groups(int64_t tiles, int groups) { return tiles < 256 || groups < 2 ? 1 : groups < 4 ? 2 : 4; }
 
 int check_batch(const char* who, int64_t M, int64_t slots, const int32_t* order, const int64_t* offsets,
                 const int32_t* tiles, int64_t num_tiles) {
@@ -497,58 +438,67 @@ int launched(const char* who) {
 }
 
 template <bool BY_PART>
-int launch_shrink(const char* who, const Batch& b, const LowRank& l, const uint16_t* x, int64_t ldx, int64_t cols,
-                  const uint16_t* rows, int64_t slot_stride, int64_t ldr, const float* scaling, float* v, int splits,
+int launch_shrink(const char* who, const AdapterBatch& b, const LowRank& l, const uint16_t* x, int64_t ldx, int64_t cols,
+                  const uint16_t* rows, int64_t slot_stride, int64_t ldr, const float* scaling, uint16_t* v,
                   hipStream_t s) {
-  const int rc = shrink_groups(l.groups), waves = b.rows == 16 ? 8 : 4, ts = b.rows / 16;
-  const dim3 grid((unsigned)b.num_tiles, (unsigned)(l.parts * ceil_div(l.groups, rc)), (unsigned)splits);
-  const unsigned lds = (unsigned)(ts * rc * waves * 1024);
-#define MXL_SHRINK(TS_, RC_)                                                                                          \
-  if (ts == TS_ && rc == RC_)                                                                                         \
-    adapter_shrink_kernel<TS_, RC_, BY_PART><<<grid, 64 * waves, lds, s>>>(b, l, x, ldx, cols, rows, slot_stride, ldr, \
-                                                                           scaling, v);
-  MXL_SHRINK(1, 1) MXL_SHRINK(1, 2) MXL_SHRINK(1, 4)
-  MXL_SHRINK(4, 1) MXL_SHRINK(4, 2) MXL_SHRINK(4, 4)
+  const int rc = shrink_groups(b.num_tiles, l.groups);
+  const int64_t chunks = l.parts * ceil_div(l.groups, rc);
+  const int waves = rc == 1 && b.num_tiles * chunks <= 256 ? 16 : 8;
+  const dim3 grid((unsigned)b.num_tiles, (unsigned)chunks);
+  const unsigned lds = (unsigned)(rc * waves * 1024);
+#define MXL_SHRINK(RC_)                                                                                           \
+  if (rc == RC_)                                                                                                  \
+    adapter_shrink_kernel<RC_, BY_PART><<<grid, 64 * waves, lds, s>>>(b, l, x, ldx, cols, rows, slot_stride, ldr, \
+                                                                      scaling, v);
+  MXL_SHRINK(1) MXL_SHRINK(2) MXL_SHRINK(4)
 #undef MXL_SHRINK
   return launched(who);
 }
 
-int launch_expand(const char* who, const Batch& b, const LowRank& l, const float* v, int splits, const uint16_t* mat,
+int launch_expand(const char* who, const AdapterBatch& b, const LowRank& l, const uint16_t* v, const uint16_t* mat,
                   int64_t slot_stride, int64_t ldm, int valid, uint16_t* y, int64_t ldy, hipStream_t s) {
-  // (where the halves of 64 rows pass the LDS, 16 at a time)
-  const int ts = b.rows == 64 && l.groups <= 32 ? 4 : 1;
-  // (64 columns a workgroup where few tiles have to fill the card)
-  const int block = b.num_tiles * ceil_div(l.cols[l.parts], 256) >= 1024 ? 256 : 64;
   int64_t blocks = 0;
-  for (int p = 0; p < l.parts; ++p) blocks += ceil_div(l.cols[p + 1] - l.cols[p], block);
-  MXL_CHECK_ARG(blocks <= 0xFFFF, "%s: too many columns", who);
-  const dim3 grid((unsigned)(b.num_tiles * (b.rows / (16 * ts))), (unsigned)blocks);
-  const unsigned lds = (unsigned)(2 * 16 * ts * (16 * l.groups + 8) * 2);
-  if (ts == 1) adapter_expand_kernel<1><<<grid, 256, lds, s>>>(b, l, v, splits, mat, slot_stride, ldm, valid, y, ldy, block);
-  else adapter_expand_kernel<4><<<grid, 256, lds, s>>>(b, l, v, splits, mat, slot_stride, ldm, valid, y, ldy, block);
+  for (int p = 0; p < l.parts; ++p) blocks += ceil_div(l.cols[p + 1] - l.cols[p], 64);
+  MXL_CHECK_ARG(blocks <= 4 * 0xFFFF, "%s: too many columns", who);
+  const dim3 grid((unsigned)b.num_tiles, (unsigned)ceil_div(blocks, 4));
+  adapter_expand_kernel<<<grid, 256, 0, s>>>(b, l, v, mat, slot_stride, ldm, valid, y, ldy,
+                                             ldy % 8 == 0 && ((uintptr_t)y & 15) == 0);
   return launched(who);
 }
 
-// Shares of an adapter's tokens in the outer products: some 512 tokens each.
-int outer_splits(int64_t M) { return (int)std::min<int64_t>(16, std::max<int64_t>(1, ceil_div(M, 512))); }
+// Shares of an adapter's tokens in the outer products, where columns and groups alone are too few workgroups: at least
+// 64 tokens each.
+int outer_splits(int64_t M, int64_t slots, int64_t wgs) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>({32, ceil_div(768, wgs * slots), M / 64}));
+}
+int64_t outer_blocks(const LowRank& l, int64_t cols, bool of_b) {
+  int64_t blocks = 0;
+  if (!of_b) return ceil_div(cols, kOuterCols);
+  for (int p = 0; p < l.parts; ++p) blocks += ceil_div(l.cols[p + 1] - l.cols[p], kOuterCols);
+  return blocks;
+}
+int outer_groups(const LowRank& l, bool of_b) {
+  const int all = of_b ? l.groups : l.parts * l.groups;
+  return all >= 4 ? 4 : all >= 2 ? 2 : 1;
+}
+int outer_splits(const LowRank& l, int64_t M, int64_t slots, int64_t cols, bool of_b) {
+  const int all = of_b ? l.groups : l.parts * l.groups;
+  return outer_splits(M, slots, outer_blocks(l, cols, of_b) * ceil_div(all, outer_groups(l, of_b)));
+}
 
 template <bool OF_B>
-int launch_outer(const char* who, const Batch& b, const LowRank& l, int64_t slots, const uint16_t* big, int64_t ldb,
-                 int64_t cols, const float* v, int v_splits, uint16_t* out, float* partial, hipStream_t s) {
-  const int splits = outer_splits(b.M), all = OF_B ? l.groups : l.parts * l.groups, rc = shrink_groups(all);
-  int64_t blocks = 0;
-  if (OF_B)
-    for (int p = 0; p < l.parts; ++p) blocks += ceil_div(l.cols[p + 1] - l.cols[p], kOuterCols);
-  else
-    blocks = ceil_div(cols, kOuterCols);
+int launch_outer(const char* who, const AdapterBatch& b, const LowRank& l, int64_t slots, const uint16_t* big, int64_t ldb,
+                 int64_t cols, const uint16_t* v, uint16_t* out, float* partial, hipStream_t s) {
+  const int splits = outer_splits(l, b.M, slots, cols, OF_B), rc = outer_groups(l, OF_B);
   MXL_CHECK_ARG(slots * splits <= 0xFFFF, "%s: too many adapters", who);
-  const dim3 grid((unsigned)blocks, (unsigned)ceil_div(all, rc), (unsigned)(slots * splits));
-#define MXL_OUTER(RC_)                                                                                             \
-  if (rc == RC_)                                                                                                   \
-    adapter_outer_kernel<RC_, OF_B><<<grid, 256, 0, s>>>(b, l, big, ldb, v, v_splits, slots, splits, cols, out, partial);
+  const dim3 grid((unsigned)outer_blocks(l, cols, OF_B), (unsigned)ceil_div(OF_B ? l.groups : l.parts * l.groups, rc),
+                  (unsigned)(slots * splits));
+#define MXL_OUTER(RC_) \
+  if (rc == RC_)       \
+    adapter_outer_kernel<RC_, OF_B><<<grid, 256, 0, s>>>(b, l, big, ldb, v, slots, splits, cols, out, partial);
   MXL_OUTER(1) MXL_OUTER(2) MXL_OUTER(4)
 #undef MXL_OUTER
-  int rc2 = launched(who);
+  const int rc2 = launched(who);
   if (rc2 != MXL_OK || splits == 1) return rc2;
   const int64_t count = slots * cols * l.rank * (OF_B ? 1 : l.parts);
   adapter_join_kernel<<<dim3((unsigned)ceil_div(count, 1024)), 256, 0, s>>>(partial, splits, count, out);
@@ -571,13 +521,13 @@ struct GradScratch {
   int64_t bytes;
 };
 GradScratch grad_scratch(uint8_t* base, int64_t M, int64_t K, int64_t slots, const LowRank& l) {
-  const int64_t N = l.cols[l.parts], out = outer_splits(M) > 1 ? outer_splits(M) : 0;
+  const int64_t N = l.cols[l.parts], nb = outer_splits(l, M, slots, N, true), na = outer_splits(l, M, slots, K, false);
   Pieces p{base};
   GradScratch g;
   g.bt = p.take(slots * l.rank * N * 2);
-  g.at = p.take(slots * K * l.width() * 2);
-  g.dv = p.take(shrink_splits(M, slots, l.parts, l.groups, N / l.parts) * M * l.width() * 4);
-  g.partial = p.take(out * slots * l.rank * std::max(N, l.parts * K) * 4);
+  g.at = p.take(rows_add(M, slots) ? 0 : slots * K * l.width() * 2);
+  g.dv = p.take(M * l.width() * 4);
+  g.partial = p.take(slots * l.rank * 4 * std::max(nb > 1 ? nb * N : 0, na > 1 ? na * l.parts * K : 0));
   g.bytes = p.used;
   return g;
 }
@@ -595,20 +545,18 @@ extern "C" int mxl_adapter_tiles(const int64_t* offsets, int64_t M, int64_t slot
   if (M == 0) return MXL_OK;
   MXL_CHECK_ARG(offsets && tiles && num_tiles == tile_count(M, slots), "%s: needs %lld tiles", who,
                 (long long)tile_count(M, slots));
-  adapter_tiles_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(offsets, (int)slots, tile_rows(M), (int)num_tiles, tiles);
+  adapter_tiles_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(offsets, (int)slots, (int)num_tiles, tiles);
   return launched(who);
 }
 
-extern "C" int64_t mxl_adapter_v_floats(int64_t M, int64_t K, int64_t slots, int64_t parts, int64_t rank) {
-  if (M <= 0 || K <= 0 || slots <= 0 || parts <= 0 || rank <= 0) return 0;
-  const int groups = (int)((rank + 15) / 16);
-  return shrink_splits(M, slots, (int)parts, groups, K) * M * parts * groups * 16;
+extern "C" int64_t mxl_adapter_v_elems(int64_t M, int64_t parts, int64_t rank) {
+  return M <= 0 || parts <= 0 || rank <= 0 ? 0 : M * 2 * parts * ceil_div(rank, 16) * 16;
 }
 
 extern "C" int mxl_adapter_apply(const void* x, int64_t M, int64_t K, int64_t ldx, const void* a, const void* b,
                                  const float* scaling, int64_t slots, int64_t parts, const int64_t* cols, int64_t rank,
                                  const int32_t* order, const int64_t* offsets, const int32_t* tiles, int64_t num_tiles,
-                                 float* v, int64_t v_floats, void* y, int64_t ldy, void* stream) {
+                                 void* v, int64_t v_elems, void* y, int64_t ldy, void* stream) {
   const char* who = "mxl_adapter_apply";
   LowRank l;
   int rc = check_batch(who, M, slots, order, offsets, tiles, num_tiles);
@@ -617,30 +565,113 @@ extern "C" int mxl_adapter_apply(const void* x, int64_t M, int64_t K, int64_t ld
   const int64_t N = l.cols[l.parts];
   MXL_CHECK_ARG(ldx >= K && ldx % 8 == 0 && ldy >= N, "%s: need ldx >= K, a multiple of 8, and ldy >= N", who);
   MXL_CHECK_ARG((((uintptr_t)x | (uintptr_t)a | (uintptr_t)b | (uintptr_t)v) & 15) == 0, "%s: x, a, b and v must be 16-byte aligned", who);
-  MXL_CHECK_ARG(v_floats >= mxl_adapter_v_floats(M, K, slots, parts, rank), "%s: v holds %lld floats, needs %lld", who,
-                (long long)v_floats, (long long)mxl_adapter_v_floats(M, K, slots, parts, rank));
-  const Batch batch{order, offsets, tiles, (int)num_tiles, tile_rows(M), M};
-  const int splits = shrink_splits(M, slots, l.parts, l.groups, K);
+  MXL_CHECK_ARG(v_elems >= mxl_adapter_v_elems(M, parts, rank), "%s: v holds %lld values, needs %lld", who,
+                (long long)v_elems, (long long)mxl_adapter_v_elems(M, parts, rank));
+  const AdapterBatch batch{order, offsets, tiles, (int)num_tiles, M};
   const int64_t R = parts * rank;
-  rc = launch_shrink<false>(who, batch, l, (const uint16_t*)x, ldx, K, (const uint16_t*)a, R * K, K, scaling, v, splits,
+  rc = launch_shrink<false>(who, batch, l, (const uint16_t*)x, ldx, K, (const uint16_t*)a, R * K, K, scaling, (uint16_t*)v,
                             (hipStream_t)stream);
   if (rc != MXL_OK) return rc;
-  return launch_expand(who, batch, l, v, splits, (const uint16_t*)b, N * rank, rank, l.rank, (uint16_t*)y, ldy,
+  return launch_expand(who, batch, l, (const uint16_t*)v, (const uint16_t*)b, N * rank, rank, l.rank, (uint16_t*)y, ldy,
                        (hipStream_t)stream);
 }
 
+// ---- the layer and its adapters in one call
+
+extern "C" int mxl_quantize_mxfp8(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, void* codes, void* scales,
+                                  void* stream);
+extern "C" int mxl_quantize_mxfp4(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, void* codes, void* scales,
+                                  void* stream);
+extern "C" int mxl_quantize_block_fp8(const void* x, int64_t M, int64_t K, void* codes, void* scales, void* stream);
+
+static int64_t code_bytes(int64_t M, int64_t K, int fmt) { return ceil_div(fmt == kE2M1 ? M * (K / 2) : M * K, 256) * 256; }
+
+// The product adds the adapters where it runs in the tiles anyway (from 17 rows) and walks few of them a tile; 32-bit
+// offsets.
+extern "C" int mxl_adapter_linear_supported(int64_t M, int64_t N, int64_t K, int fmt, int block, int64_t slots,
+                                            int64_t parts, int64_t rank) {
+  return M >= 17 && N > 0 && K > 0 && K % 128 == 0 && slots > 0 && parts > 0 && rank > 0 && rows_add(M, slots) &&
+         wide_tiles_eligible(M, N, K, block != 0) && M <= (int64_t(1) << 32) / (4 * parts * ceil_div(rank, 16) * 16) &&
+         N <= (int64_t(1) << 31) / (2 * rank) && (fmt != kE2M1 || !block);
+}
+
+extern "C" int64_t mxl_adapter_linear_workspace_bytes(int64_t M, int64_t K, int fmt, int block) {
+  if (M <= 0 || K <= 0) return 0;
+  return code_bytes(M, K, fmt) + (block ? M * (K / 128) * 4 : M * (K / 32));
+}
+
+extern "C" int mxl_adapter_linear(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, const void* w_tiled,
+                                  const void* sw, int fmt, int block, const void* bias, const void* a, const void* b,
+                                  const float* scaling, int64_t slots, int64_t parts, const int64_t* cols, int64_t rank,
+                                  const int32_t* ids, const int32_t* order, const int64_t* offsets, const int32_t* tiles,
+                                  int64_t num_tiles, void* v, int64_t v_elems, void* y, int64_t ldy, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  const char* who = "mxl_adapter_linear";
+  LowRank l;
+  int rc = check_batch(who, M, slots, order, offsets, tiles, num_tiles);
+  if (rc == MXL_OK) rc = make_low_rank(who, parts, cols, rank, K, l);
+  if (rc != MXL_OK || M == 0) return rc;
+  const int64_t N = l.cols[l.parts], R = parts * rank;
+  MXL_CHECK_ARG(fmt == kE4M3 || fmt == kE2M3 || fmt == kE3M2 || fmt == kE2M1, "%s: unknown format %d", who, fmt);
+  MXL_CHECK_ARG(!block || (fmt == kE4M3 && ldx == K), "%s: block-FP8 takes E4M3 weights and contiguous rows", who);
+  MXL_CHECK_ARG(fmt != kE2M1 || fp4_rule(rule), "%s: unknown rule %d", who, rule);
+  if (!mxl_adapter_linear_supported(M, N, K, fmt, block, slots, parts, rank)) {
+    set_error("%s: %lld rows of %lld adapters do not run in one product (N=%lld K=%lld)", who, (long long)M,
+              (long long)slots, (long long)N, (long long)K);
+    return MXL_EUNSUPPORTED;
+  }
+  MXL_CHECK_ARG(ids && ldx >= K && ldx % 8 == 0 && ldy >= N, "%s: need ids, ldx >= K, a multiple of 8, and ldy >= N", who);
+  MXL_CHECK_ARG((((uintptr_t)x | (uintptr_t)w_tiled | (uintptr_t)a | (uintptr_t)b | (uintptr_t)v) & 15) == 0 &&
+                    ((uintptr_t)sw & 3) == 0 && ((uintptr_t)y & 1) == 0, "%s: x, w, a, b and v must be 16-byte aligned", who);
+  MXL_CHECK_ARG(v_elems >= mxl_adapter_v_elems(M, parts, rank), "%s: v holds %lld values, needs %lld", who,
+                (long long)v_elems, (long long)mxl_adapter_v_elems(M, parts, rank));
+  MXL_CHECK_ARG(workspace && workspace_bytes >= mxl_adapter_linear_workspace_bytes(M, K, fmt, block) &&
+                    ((uintptr_t)workspace & 255) == 0, "%s: needs a 256-byte aligned workspace of %lld bytes (have %lld)", who,
+                (long long)mxl_adapter_linear_workspace_bytes(M, K, fmt, block), (long long)workspace_bytes);
+  hipStream_t s = (hipStream_t)stream;
+  uint8_t* const codes = (uint8_t*)workspace;
+  uint8_t* const scales = codes + code_bytes(M, K, fmt);
+  rc = block          ? mxl_quantize_block_fp8(x, M, K, codes, scales, stream)
+       : fmt == kE2M1 ? mxl_quantize_mxfp4(x, M, K, ldx, rule, codes, scales, stream)
+                      : mxl_quantize_mxfp8(x, M, K, ldx, rule, codes, scales, stream);
+  if (rc != MXL_OK) return rc;
+  const AdapterBatch batch{order, offsets, tiles, (int)num_tiles, M};
+  rc = launch_shrink<false>(who, batch, l, (const uint16_t*)x, ldx, K, (const uint16_t*)a, R * K, K, scaling, (uint16_t*)v, s);
+  if (rc != MXL_OK) return rc;
+  GemmParams p{};
+  p.M = p.a_rows = M; p.N = N; p.K = K; p.KT = ceil_div(K, kTileK);
+  p.a = codes; p.sa = scales; p.lda = fmt == kE2M1 ? K / 2 : K;
+  p.w = (const uint8_t*)w_tiled; p.sw = sw; p.bias = (const uint16_t*)bias; p.out = (uint16_t*)y; p.ldc = ldy;
+  p.row_div = 1; p.S = 1;
+  RowAdapters add;
+  add.ids = ids; add.slots = (int)slots; add.v = (const uint16_t*)v; add.mat = (const uint16_t*)b;
+  add.slot_stride = N * rank; add.ldm = rank; add.l = l;
+  WideGrid g{};
+  int64_t grid;
+  const WideConfig c = wide_tiles_whole(M, N, K, fmt, block != 0, g, grid);
+  const hipError_t e = launch_adapter_tiles(fmt, block != 0, c, p, g, add, grid, s);
+  if (e != hipSuccess) {
+    set_error("%s: launch failed: %s", who, hipGetErrorString(e));
+    return MXL_EHIP;
+  }
+  return MXL_OK;
+}
+
+// ---- gradients
+
 extern "C" int64_t mxl_adapter_grad_workspace_bytes(int64_t M, int64_t K, int64_t slots, int64_t parts,
-                                                    const int64_t* cols, int64_t rank) {
+                                                    const int64_t* cols, int64_t rank, int block) {
   LowRank l;
   if (M <= 0 || slots <= 0 || make_low_rank("mxl_adapter_grad_workspace_bytes", parts, cols, rank, K, l) != MXL_OK) return 0;
-  return grad_scratch(nullptr, M, K, slots, l).bytes;
+  return grad_scratch(nullptr, M, K, slots, l).bytes + input_grad_bytes(M, cols[parts], K, block);
 }
 
 extern "C" int mxl_adapter_grad(const void* x, int64_t M, int64_t K, int64_t ldx, const void* dy, int64_t lddy,
-                                const void* a, const void* b, const float* scaling, int64_t slots, int64_t parts,
-                                const int64_t* cols, int64_t rank, const int32_t* order, const int64_t* offsets,
-                                const int32_t* tiles, int64_t num_tiles, const float* v, int64_t v_floats, void* dx,
-                                int64_t lddx, void* da, void* db, void* workspace, int64_t workspace_bytes, void* stream) {
+                                const void* w_tiled, const void* sw, int fmt, int block, const void* a, const void* b,
+                                const float* scaling, int64_t slots, int64_t parts, const int64_t* cols, int64_t rank,
+                                const int32_t* ids, const int32_t* order, const int64_t* offsets, const int32_t* tiles,
+                                int64_t num_tiles, const void* v, int64_t v_elems, void* dx, int64_t lddx, void* da,
+                                void* db, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* who = "mxl_adapter_grad";
   LowRank l;
   int rc = check_batch(who, M, slots, order, offsets, tiles, num_tiles);
@@ -648,48 +679,54 @@ extern "C" int mxl_adapter_grad(const void* x, int64_t M, int64_t K, int64_t ldx
   if (rc != MXL_OK || M == 0) return rc;
   const int64_t N = l.cols[l.parts], R = parts * rank;
   MXL_CHECK_ARG(N % 8 == 0, "%s: need N %% 8 == 0 (N=%lld)", who, (long long)N);
-  MXL_CHECK_ARG(ldx >= K && ldx % 8 == 0 && lddy >= N && lddy % 8 == 0 && (!dx || lddx >= K),
-                "%s: need ldx >= K, lddy >= N, multiples of 8, and lddx >= K", who);
+  MXL_CHECK_ARG(ldx >= K && ldx % 8 == 0 && lddy >= N && lddy % 8 == 0 && (!dx || (ids && lddx >= K && lddx % 4 == 0)),
+                "%s: need ldx >= K, lddy >= N, multiples of 8, and for dx ids and lddx >= K, a multiple of 4", who);
   MXL_CHECK_ARG((((uintptr_t)x | (uintptr_t)dy | (uintptr_t)a | (uintptr_t)b | (uintptr_t)v | (uintptr_t)da | (uintptr_t)db) & 15) == 0,
                 "%s: operands must be 16-byte aligned", who);
-  MXL_CHECK_ARG(v_floats >= mxl_adapter_v_floats(M, K, slots, parts, rank), "%s: v holds %lld floats", who, (long long)v_floats);
-  const GradScratch g = grad_scratch((uint8_t*)workspace, M, K, slots, l);
-  MXL_CHECK_ARG(workspace && workspace_bytes >= g.bytes && ((uintptr_t)workspace & 255) == 0,
-                "%s: needs a 256-byte aligned workspace of %lld bytes (have %lld)", who, (long long)g.bytes,
+  MXL_CHECK_ARG(!db || v_elems >= mxl_adapter_v_elems(M, parts, rank), "%s: v holds %lld values", who, (long long)v_elems);
+  const int64_t need = mxl_adapter_grad_workspace_bytes(M, K, slots, parts, cols, rank, block);
+  MXL_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0,
+                "%s: needs a 256-byte aligned workspace of %lld bytes (have %lld)", who, (long long)need,
                 (long long)workspace_bytes);
+  const GradScratch g = grad_scratch((uint8_t*)workspace, M, K, slots, l);
   hipStream_t s = (hipStream_t)stream;
-  const Batch batch{order, offsets, tiles, (int)num_tiles, tile_rows(M), M};
-  const int v_splits = shrink_splits(M, slots, l.parts, l.groups, K);
-  const int dv_splits = shrink_splits(M, slots, l.parts, l.groups, N / l.parts);
+  const AdapterBatch batch{order, offsets, tiles, (int)num_tiles, M};
   if (db) {
-    rc = launch_outer<true>(who, batch, l, slots, (const uint16_t*)dy, lddy, N, v, v_splits, (uint16_t*)db,
+    rc = launch_outer<true>(who, batch, l, slots, (const uint16_t*)dy, lddy, N, (const uint16_t*)v, (uint16_t*)db,
                             (float*)g.partial, s);
     if (rc != MXL_OK) return rc;
   }
   if (!da && !dx) return MXL_OK;
   // B [N, r] -> [r, N]
+  MXL_CHECK_ARG(ceil_div(std::max(N, K), 32) <= 0xFFFF && slots <= 0xFFFF, "%s: too large", who);
   adapter_transpose_kernel<<<dim3((unsigned)ceil_div(l.rank, 32), (unsigned)ceil_div(N, 32), (unsigned)slots), 256, 0, s>>>(
       (const uint16_t*)b, N, l.rank, 1, (int)N, (int)N, (uint16_t*)g.bt);
   rc = launched(who);
   if (rc == MXL_OK)
     rc = launch_shrink<true>(who, batch, l, (const uint16_t*)dy, lddy, N, (const uint16_t*)g.bt, l.rank * N, N, scaling,
-                             (float*)g.dv, dv_splits, s);
+                             (uint16_t*)g.dv, s);
   if (rc == MXL_OK && da)
-    rc = launch_outer<false>(who, batch, l, slots, (const uint16_t*)x, ldx, K, (const float*)g.dv, dv_splits,
+    rc = launch_outer<false>(who, batch, l, slots, (const uint16_t*)x, ldx, K, (const uint16_t*)g.dv,
                              (uint16_t*)da, (float*)g.partial, s);
-  if (rc == MXL_OK && dx) {
-    // A [R, K] -> [K, parts 16 groups]
-    adapter_transpose_kernel<<<dim3((unsigned)ceil_div(K, 32), (unsigned)ceil_div(l.width(), 32), (unsigned)slots), 256, 0, s>>>(
-        (const uint16_t*)a, R, K, l.parts, l.rank, l.width(), (uint16_t*)g.at);
-    rc = launched(who);
-    LowRank one = l;  // all ranks at once
-    one.parts = 1;
-    one.groups = l.parts * l.groups;
-    one.rank = one.groups * 16;
-    one.cols[1] = K;
-    if (rc == MXL_OK)
-      rc = launch_expand(who, batch, one, (const float*)g.dv, dv_splits, (const uint16_t*)g.at, K * l.width(), l.width(),
-                         one.rank, (uint16_t*)dx, lddx, s);
-  }
+  if (rc != MXL_OK || !dx) return rc;
+  RowAdapters more;
+  more.ids = ids; more.slots = (int)slots; more.v = (const uint16_t*)g.dv; more.mat = (const uint16_t*)a;
+  more.slot_stride = R * K; more.ldm = K; more.l = l;
+  const bool within = rows_add(M, slots);
+  rc = input_grad(who, dy, M, N, lddy, w_tiled, sw, K, fmt, block, dx, lddx, (uint8_t*)workspace + g.bytes,
+                  workspace_bytes - g.bytes, within ? &more : nullptr, stream);
+  if (rc != MXL_OK || within) return rc;
+  // A [R, K] -> [K, parts 16 groups]
+  adapter_transpose_kernel<<<dim3((unsigned)ceil_div(K, 32), (unsigned)ceil_div(l.width(), 32), (unsigned)slots), 256, 0, s>>>(
+      (const uint16_t*)a, R, K, l.parts, l.rank, l.width(), (uint16_t*)g.at);
+  rc = launched(who);
+  LowRank one = l;  // all ranks at once
+  one.parts = 1;
+  one.groups = l.parts * l.groups;
+  one.rank = one.groups * 16;
+  one.cols[1] = K;
+  if (rc == MXL_OK)
+    rc = launch_expand(who, batch, one, (const uint16_t*)g.dv, (const uint16_t*)g.at, K * l.width(), l.width(), one.rank,
+                       (uint16_t*)dx, lddx, s);
   return rc;
 }

@@ -71,7 +71,7 @@ int run(const char* who, const void* x, int64_t M, int64_t K, int64_t ldx, int r
     gate.lddh = lddh;
     WideGrid g{};
     int64_t grid;
-    const WideConfig c = wide_tiles_whole(p.M, p.N, K, fmt, g, grid);
+    const WideConfig c = wide_tiles_whole(p.M, p.N, K, fmt, false, g, grid);
     const hipError_t e = (dh ? launch_gated_grad_tiles : launch_gated_tiles)(fmt, c, p, g, gate, grid, (hipStream_t)stream);
     if (e != hipSuccess) {
       set_error("%s: launch failed: %s", who, hipGetErrorString(e));

@@ -37,6 +37,7 @@
 // sums share one activation scale.
 #pragma once
 
+#include "adapters.h"
 #include "fp4.h"
 #include "gate_act.h"
 #include "gemm_wide.h"
@@ -191,7 +192,10 @@ struct TileLds {
 };
 
 // a_row(row): the activation row of output row `row` (rows past the last: any valid one).
-template <int FMT, int MTW, int NTW, bool BLOCK, int DEPTH, int EPI = kEpiStore, class Row>
+// ADD (whole K): to the sums of rows with an adapter its low-rank part is added, ahead of any rounding; the kernel's third
+// argument, a RowAdapters behind GemmParams and WideGrid, says what.
+constexpr int kAddOffset = (sizeof(GemmParams) + 7) / 8 * 8 + (sizeof(WideGrid) + 7) / 8 * 8;
+template <int FMT, int MTW, int NTW, bool BLOCK, int DEPTH, int EPI = kEpiStore, bool ADD = false, class Row>
 __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w, uint8_t* lds, Row&& a_row,
                                           const TileGate& gate = TileGate()) {
   constexpr bool SWIGLU = EPI == kEpiSwigluFp4, GATED = EPI == kEpiGated || EPI == kEpiGatedGrad;
@@ -587,9 +591,10 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
     const int one = cur + L::STAGE < ring ? cur + L::STAGE : 0, two = one + L::STAGE < ring ? one + L::STAGE : 0;
     stage(Slice<0>{}, Slice<left>{}, 2 * pr, cur, one);
     stage(Slice<1>{}, Slice<left ? left - 1 : 0>{}, 2 * pr + 1, one, two);
-    // 64 x 64 tiles: the compiler moves the accumulators after the loop, 17 states after the last MFMA whose
-    // result takes 20
-    if constexpr (!BLOCK && MTW * NTW == 4) asm volatile("s_nop 2");
+    // 64 x 64 tiles, gated ones and those with adapters: the compiler moves the accumulators after the loop, 17 states
+    // and more after the last MFMA whose result takes 20
+    if constexpr (!BLOCK && (GATED || ADD)) asm volatile("s_nop 4");
+    else if constexpr (!BLOCK && MTW * NTW == 4) asm volatile("s_nop 2");
     cur = two;
   };
   const int last = end >> 1;  // pairs 2 kb .. last - 1; the copies end in the final one or two
@@ -598,6 +603,112 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   if (DEPTH > 2 && pr + 1 < last) pair(Slice<4>{}, pr++);
   pair(Slice<2>{}, pr);
 
+  if constexpr (ADD) {
+    {
+      // After the last MFMAs' results: 16 ranks an MFMA, v's halves in its two halves of K, zero in the rows of other
+      // adapters than the one at hand (and B in columns of other parts).  Adapters, parts and ranks go one after the
+      // other, the next ranks' operands loaded under the MFMAs.
+      // The arguments are read here (through a pointer that the compiler cannot see through): held in scalar registers
+      // over the main loop they would spill.
+      typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+      typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+      typedef const __attribute__((address_space(4))) uint8_t* kernarg_t;
+      kernarg_t at = (kernarg_t)__builtin_amdgcn_kernarg_segment_ptr() + kAddOffset;
+      asm volatile("" : "+s"(at));
+      const auto* const add = (const __attribute__((address_space(4))) RowAdapters*)at;
+      auto pin = [&] {
+#pragma unroll
+        for (int i = 0; i < MTW; ++i)
+#pragma unroll
+          for (int n = 0; n < NTW; ++n) {
+            if constexpr (BLOCK) asm volatile("" : "+v"(acc[i][n]));
+            else asm volatile("" : "+a"(acc[i][n]));
+          }
+      };
+      if constexpr (!BLOCK) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+      pin();
+      int own[MTW];
+#pragma unroll
+      for (int i = 0; i < MTW; ++i) {
+        const int row = w.row0 + (wm * MTW + i) * 16 + r;
+        const int x = row < w.row_hi ? add->ids[row] : -1;
+        own[i] = (uint32_t)x < (uint32_t)add->slots ? x : 0x7FFFFFFF;
+      }
+      // the part of a column
+      auto part_of = [&](int col) {
+        int of = 0;
+        for (int k = 1; k < add->l.parts; ++k) of += col >= (int)add->l.cols[k] ? 1 : 0;
+        return of;
+      };
+      // the smallest adapter past `last` of the wave's rows
+      auto next = [&](int last) {
+        int a = 0x7FFFFFFF;
+#pragma unroll
+        for (int i = 0; i < MTW; ++i) a = own[i] > last && own[i] < a ? own[i] : a;
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+          const int b = __shfl_xor(a, d, 64);
+          a = b < a ? b : a;
+        }
+        return __builtin_amdgcn_readfirstlane(a);
+      };
+      const int first = part_of(16 * n_tile(wn, 0, 0)), end = part_of(16 * n_tile(wn, 1, NH - 1));
+      int a = next(-1), part = first, g = 0;
+      while (a != 0x7FFFFFFF) {  // (one loop: nested ones would move the accumulators)
+        asm volatile("" : "+s"(at));
+        const auto* const o = (const __attribute__((address_space(4))) RowAdapters*)at;
+        const int parts = o->l.parts, rank = o->l.rank, groups = o->l.groups, width = 16 * groups * parts;
+        const int lo = (int)o->l.cols[part], hi = part + 1 < parts ? (int)o->l.cols[part + 1] : (int)p.N;
+        const uint8_t* const mat = reinterpret_cast<const uint8_t*>(o->mat + a * o->slot_stride) + 32 * g;
+        const uint8_t* const v = reinterpret_cast<const uint8_t*>(o->v) + 32 * (part * groups + g);
+        const bool in = 16 * g + 8 * (q & 1) < rank;  // (ranks come in eights)
+        // every lane loads, from a valid place; what does not count becomes zero
+        u32x4 xv[MTW], xb[NTW];
+        const uint32_t vrow = (uint32_t)(w.row0 + wm * MTW * 16 + r) * (uint32_t)(4 * width) + (q >> 1) * 2 * width + 16 * (q & 1);
+#pragma unroll
+        for (int i = 0; i < MTW; ++i)
+          xv[i] = *reinterpret_cast<const u32x4*>(v + (own[i] == a ? vrow + (uint32_t)(64 * i) * (uint32_t)width : 0u));
+#pragma unroll
+        for (int n = 0; n < NTW; ++n) {
+          const int col = 16 * n_tile(wn, n / NH, n % NH) + r, from = col < lo ? lo : col < hi ? col : hi - 1;
+          xb[n] = *reinterpret_cast<const u32x4*>(mat + ((uint32_t)from * (uint32_t)(2 * o->ldm) + (in ? 16 * (q & 1) : 0)));
+        }
+#pragma unroll
+        for (int i = 0; i < MTW; ++i) {
+          const uint32_t m = own[i] == a ? 0xFFFFFFFFu : 0u;
+          xv[i] &= u32x4{m, m, m, m};
+          asm volatile("" : "+v"(xv[i]));
+        }
+#pragma unroll
+        for (int n = 0; n < NTW; ++n) {
+          const int col = 16 * n_tile(wn, n / NH, n % NH) + r;
+          const uint32_t m = in && col >= lo && col < hi ? 0xFFFFFFFFu : 0u;
+          xb[n] &= u32x4{m, m, m, m};
+          asm volatile("" : "+v"(xb[n]));
+        }
+        if (++g == groups) {
+          g = 0;
+          if (++part > end) {
+            part = first;
+            a = next(a);
+          }
+        }
+        if constexpr (!BLOCK) asm volatile("s_nop 1");
+#pragma unroll
+        for (int n = 0; n < NTW; ++n)
+#pragma unroll
+          for (int i = 0; i < MTW; ++i) {
+            if constexpr (BLOCK)
+              acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xb[n]),
+                                                                 __builtin_bit_cast(bf16x8, xv[i]), acc[i][n], 0, 0, 0);
+            else
+              asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[i][n]) : "v"(xb[n]), "v"(xv[i]));
+          }
+        if constexpr (!BLOCK) asm volatile("s_nop 15");  // (the next ranks' sums start from these results)
+      }
+      pin();
+    }
+  }
   auto values = [&](int i, int n) -> v4f {
     if constexpr (BLOCK) return acc[i][n];
     else return tile_values(acc[i][n]);

@@ -2,6 +2,7 @@
 // gemm_wide.hip and the 2 x 2-wave tiles of gemm_tile.hip.
 #pragma once
 
+#include "adapters.h"
 #include "gemm_common.h"
 
 namespace mxl {
@@ -62,11 +63,15 @@ __global__ __launch_bounds__(256, (WidePerCu<MT, NT, GROUPED, WM>::value)) void 
 }
 
 // Tile and grid of the 2 x 2-wave kernels over whole K (N columns, for MXFP4 in its stages of K256), no splits.
-WideConfig wide_tiles_whole(int64_t M, int64_t N, int64_t K, int fmt, WideGrid& g, int64_t& grid);
+WideConfig wide_tiles_whole(int64_t M, int64_t N, int64_t K, int fmt, bool block, WideGrid& g, int64_t& grid);
 
 // The dense 2 x 2-wave launch of `grid` workgroups.
 hipError_t launch_wide_tiles(int fmt, bool block, const WideConfig& c, const GemmParams& p, const WideGrid& g,
                              int64_t grid, hipStream_t s);
+
+// The same with the adapters of the rows (gemm_tile_adapters.hip).
+hipError_t launch_adapter_tiles(int fmt, bool block, const WideConfig& c, const GemmParams& p, const WideGrid& g,
+                                const RowAdapters& add, int64_t grid, hipStream_t s);
 
 // The grouped (MoE) launch of `grid` persistent workgroups (gemm_tile_grouped.hip).
 hipError_t launch_wide_grouped(int fmt, const WideConfig& c, const GemmParams& p, const WideGrid& g, int64_t grid,

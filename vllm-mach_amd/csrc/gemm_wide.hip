@@ -867,13 +867,14 @@ WideConfig wide_tiles_config(int64_t M, int64_t N, int64_t K, bool block) {
   return best;
 }
 
-WideConfig wide_tiles_whole(int64_t M, int64_t N, int64_t K, int fmt, WideGrid& g, int64_t& grid) {
+WideConfig wide_tiles_whole(int64_t M, int64_t N, int64_t K, int fmt, bool block, WideGrid& g, int64_t& grid) {
   const int64_t T = fmt == kE2M1 ? (K + 255) / 256 : K / 128, cus = cu_count();
   WideConfig best{2, 1, (K + kTileK - 1) / kTileK};
   double best_us = 1e300;
   for (const TileCost& t : kTileCosts) {
     const int64_t mblocks = (M + 16 * t.MT - 1) / (16 * t.MT), nblocks = (N + 64 * t.NT - 1) / (64 * t.NT);
     const int64_t tiles = mblocks * nblocks, tail = wide_tail(t, tiles, cus), n = (tiles + cus - 1) / cus;
+    if (block && t.NT == 4) continue;  // (not instantiated)
     auto work = [&](int64_t k) { return k * T * t.stage + ((k + t.resident - 1) / t.resident - 1) * kTileGap; };
     const double us = t.fixed + (tail ? work(n - 1) + (4 * tail + cus - 1) / cus * T * t.quarter + kTileGap : work(n));
     if (us >= best_us) continue;

@@ -10,7 +10,10 @@
 // and the MFMA's operand, eight rows of one column a lane, comes out of LDS transposed (ds_read_b64_tr_b16).  W takes the
 // A operand, so a lane holds four consecutive columns of a row of dx.
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
+#include "adapters.h"
 #include "gemm_wide.h"
 
 namespace mxl {
@@ -19,10 +22,21 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x32_t __attribute__((ext_vector_type(32)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef unsigned int v6u_t __attribute__((ext_vector_type(6)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 
 constexpr int kGradStage = 64;  // rows of W
+
+// f of 0 .. N - 1 as constants (register arrays are indexed by nothing else)
+template <int N, class F>
+__device__ __forceinline__ void for_n(F&& f) {
+  if constexpr (N > 0) {
+    for_n<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
 
 struct GradParams {
   const uint16_t* dy;
@@ -30,26 +44,31 @@ struct GradParams {
   const void* sw;  // tiled E8M0, or fp32 [ceil(N / 128), K / 128]
   uint16_t* out;
   float* partial;  // [S, M, K] when split
-  int64_t M, N, K, KT, lddy, ldo;
-  int S;
+  int64_t M, N, K, KT, lddy, ldo;  // (N in whole pairs of stages)
+  int S, strips;   // of 16 rows of W
   int64_t per;     // stages of a split, an even number
   uint32_t mblocks, kblocks, group_m;
+  RowAdapters more;  // (ids null: none)
 };
 
-template <int FMT, int TK>
-struct GradW {
-  static constexpr int SL = TK / 128;  // 128-column slices of a wave's strip
+// The pieces of a stage that a thread moves from memory to LDS: NA 16-byte pieces of dy, and of its wave's strip of W
+// (16 rows) the lane's codes of SL 128-column slices.
+template <int FMT, int TM, int TK>
+struct GradPieces {
+  static constexpr int NA = TM / 32, SL = TK / 128;
   static constexpr int NC = FMT == kE4M3 ? 2 * SL : FMT == kE2M1 ? SL : SL == 2 ? 3 : 2;  // 16-byte pieces a lane
-  uint4 c[NC];
+  static constexpr int UNITS = FMT == kE4M3 ? 2 * SL : SL;                              // decoded one by one
+  u32x4 a[NA], c[NC];
   uint32_t s[2];
 };
 
 template <int FMT, int TM, int TK, bool BLOCK>
-__global__ __launch_bounds__(256) void input_grad_kernel(GradParams p) {
-  constexpr int MI = TM / 64, KI = TK / 64, SL = TK / 128;  // 32 x 32 tiles of a wave; slices
-  constexpr int RS = TK + 32;                              // elements of a row of W in LDS
+__global__ __launch_bounds__(256, (TM * TK > 128 * 128 ? 1 : 2)) void input_grad_kernel(GradParams p) {
+  using Pieces = GradPieces<FMT, TM, TK>;
+  constexpr int MI = TM / 64, KI = TK / 64, SL = Pieces::SL;  // 32 x 32 tiles of a wave; slices
+  constexpr int RS = TK + 32;                                // elements of a row of W in LDS
   constexpr int A_BYTES = TM * 128, W_BYTES = kGradStage * RS * 2;
-  constexpr int NA = TM / 32;                              // 16-byte pieces of dy a thread
+  constexpr int NA = Pieces::NA, NC = Pieces::NC;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [2] dy, [2] W
   const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wm = wv >> 1, wk = wv & 1, r = lane & 15, q = lane >> 4;
@@ -59,101 +78,83 @@ __global__ __launch_bounds__(256) void input_grad_kernel(GradParams p) {
   uint32_t mb, kb;
   wide_coords(unit - split * tiles, p.mblocks, p.kblocks, p.group_m, mb, kb);
   const int64_t row0 = (int64_t)mb * TM;
-  const int stages = (int)((p.N + kGradStage - 1) / kGradStage);
-  const int s0 = (int)(split * p.per), s1 = s0 + (int)p.per < stages ? s0 + (int)p.per : stages;
-  const int ntiles = (int)((p.N + 15) / 16), j0 = (int)(kb * SL) & 3;  // the first slice's place in its super-tile
+  // the split's stages, an even number (dy has columns for all of them, zeros past W's last row)
+  const int stages = (int)(p.N / kGradStage), s0 = (int)(split * p.per);
+  const int s1 = s0 + (int)p.per < stages ? s0 + (int)p.per : stages;
+  const int j0 = (int)(kb * SL) & 3;  // the first slice's place in its super-tile
   const int64_t kt = (int64_t)kb * SL >> 2;
 
-  // dy: piece u of a thread is row t / 8 + 32 u, columns 8 (t % 8) of the stage
-  const uint16_t* const a_base = p.dy + row0 * p.lddy;
-  uint32_t a_off[NA];
-#pragma unroll
-  for (int u = 0; u < NA; ++u) {
-    const int64_t row = row0 + (t >> 3) + 32 * u < p.M ? (t >> 3) + 32 * u : p.M - 1 - row0;
-    a_off[u] = (uint32_t)(row * p.lddy) + 8 * (t & 7);
-  }
-  uint4 av[NA];
-  GradW<FMT, TK> wr;
-  auto load = [&](int s) {
-    const int64_t n0 = (int64_t)s * kGradStage;
-    const bool in = n0 + 8 * (t & 7) < p.N;  // (N comes in eights)
-#pragma unroll
-    for (int u = 0; u < NA; ++u) {
-      av[u] = *reinterpret_cast<const uint4*>(a_base + (in ? n0 : -8 * (t & 7)) + a_off[u]);
-      if (!in) av[u] = uint4{0, 0, 0, 0};
-    }
-    const int nt = s * 4 + wv < ntiles ? s * 4 + wv : ntiles - 1;  // (of strips past the last, zeros below)
+  // dy: piece u of a thread is row t / 8 + 32 u, columns 8 (t % 8) of the stage; rows past M are the last again
+  const uint8_t* const a_base = reinterpret_cast<const uint8_t*>(p.dy + row0 * p.lddy);
+  const uint32_t ld = (uint32_t)p.lddy * 2, a_rows = (uint32_t)(p.M - row0 < TM ? p.M - row0 : TM);
+  const uint32_t a_at = (uint32_t)(t >> 3) * ld + 16 * (t & 7), a_max = (a_rows - 1) * ld + 16 * (t & 7);
+  Pieces x;
+  auto load_a = [&](auto u, int s) {
+    const uint32_t off = __builtin_elementwise_min(a_at + (uint32_t)(32 * u) * ld, a_max);
+    x.a[u] = *reinterpret_cast<const u32x4*>(a_base + (int64_t)s * (2 * kGradStage) + off);
+  };
+  auto load_w = [&](int s) {  // (strips past the last: the last again, times zeros)
+    const int nt = 4 * s + wv < p.strips ? 4 * s + wv : p.strips - 1;
     const int64_t tile = (int64_t)nt * p.KT + kt;
     const uint8_t* const w = p.w + tile * (FmtTraits<FMT>::CH * 1024) + lane * 16;
     const int c0 = FMT == kE4M3 ? 2 * j0 : FMT == kE2M1 ? j0 : (3 * j0) >> 1;
 #pragma unroll
-    for (int c = 0; c < GradW<FMT, TK>::NC; ++c) wr.c[c] = *reinterpret_cast<const uint4*>(w + (c0 + c) * 1024);
+    for (int c = 0; c < NC; ++c) x.c[c] = *reinterpret_cast<const u32x4*>(w + (c0 + c) * 1024);
     if constexpr (!BLOCK) {
       const uint8_t* const sw = static_cast<const uint8_t*>(p.sw) + tile * 256;
       if constexpr (FMT == kE4M3) {  // pieces of 16 columns: half a block each, of lane groups q / 2 and 2 + q / 2
-        wr.s[0] = *reinterpret_cast<const uint32_t*>(sw + (16 * (q >> 1) + r) * 4) >> (8 * j0);
-        wr.s[1] = *reinterpret_cast<const uint32_t*>(sw + (16 * (2 + (q >> 1)) + r) * 4) >> (8 * j0);
+        x.s[0] = *reinterpret_cast<const uint32_t*>(sw + (16 * (q >> 1) + r) * 4);
+        x.s[1] = *reinterpret_cast<const uint32_t*>(sw + (16 * (2 + (q >> 1)) + r) * 4);
       } else {
-        wr.s[0] = *reinterpret_cast<const uint32_t*>(sw + lane * 4) >> (8 * j0);
+        x.s[0] = *reinterpret_cast<const uint32_t*>(sw + lane * 4);
       }
-    }
-    if (s * 4 + wv >= ntiles) {
-#pragma unroll
-      for (int c = 0; c < GradW<FMT, TK>::NC; ++c) wr.c[c] = uint4{0, 0, 0, 0};
-      wr.s[0] = wr.s[1] = 0x7F7F7F7Fu;
     }
   };
-  // dy: piece p of row x sits at 16 (p ^ x % 8) of its 128 bytes
-  const uint32_t a_to = (t >> 3) * 128 + 16 * ((t & 7) ^ ((t >> 3) & 7));
-  auto store = [&](int buf) {
-    uint8_t* const a = lds + buf * A_BYTES;
+  // dy: piece i of row y sits at 16 (i ^ y / 2 % 8) of its 128 bytes: sixteen rows' same piece in all 64 banks
+  uint8_t* const a_to = lds + (t >> 3) * 128 + 16 * ((t & 7) ^ ((t >> 4) & 7));
+  auto store_a = [&](auto u, int buf) { *reinterpret_cast<u32x4*>(a_to + buf * A_BYTES + u * 4096) = x.a[u]; };
+  // W: rows 64 bytes past a multiple of 256 apart, and of each 64 bytes of row y the pieces change places by y / 4 % 4:
+  // sixteen rows' same piece, and four rows' 64 bytes, in all 64 banks.  A unit of the strip's row r: 16 (E4M3) or 32 columns
+  uint8_t* const w_to = lds + 2 * A_BYTES + (16 * wv + r) * (RS * 2);
+  const int w_swz = r >> 2;
+  auto store_w = [&](auto U, int buf) {
+    constexpr int un = decltype(U)::value, sl = FMT == kE4M3 ? un / 2 : un, h = FMT == kE4M3 ? un & 1 : 0;
+    const float f = u2f(BLOCK ? 127u << 23 : __builtin_amdgcn_ubfe(x.s[h], 8 * (j0 + sl), 8) << 23);
+    uint8_t* const base = w_to + buf * W_BYTES + (128 * sl + (FMT == kE4M3 ? 64 * h + 32 * (q >> 1) : 32 * q)) * 2;
+    auto dst = [&](int i) -> u32x4& {  // piece i of the unit
+      return *reinterpret_cast<u32x4*>(base + 16 * ((FMT == kE4M3 ? 2 * (q & 1) + i : i) ^ w_swz));
+    };
+    auto bits = [](auto v) { return __builtin_bit_cast(uint32_t, v); };
+    if constexpr (FMT == kE4M3) {
+      const u32x4 c = x.c[un];
+      const uint32_t d[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-    for (int u = 0; u < NA; ++u) *reinterpret_cast<uint4*>(a + a_to + u * 4096) = av[u];
-    uint8_t* const w = lds + 2 * A_BYTES + buf * W_BYTES + (16 * wv + r) * (RS * 2);
-    auto scale = [&](int i, int sl) { return u2f(BLOCK ? 127u << 23 : ((wr.s[i] >> (8 * sl)) & 0xFFu) << 23); };
+      for (int i = 0; i < 2; ++i)
+        dst(i) = u32x4{bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d[2 * i], f, false)),
+                       bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d[2 * i], f, true)),
+                       bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d[2 * i + 1], f, false)),
+                       bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d[2 * i + 1], f, true))};
+    } else if constexpr (FMT == kE2M1) {
+      const uint32_t d[4] = {x.c[un].x, x.c[un].y, x.c[un].z, x.c[un].w};
 #pragma unroll
-    for (int sl = 0; sl < SL; ++sl) {
-      if constexpr (FMT == kE4M3) {
+      for (int i = 0; i < 4; ++i)
+        dst(i) = u32x4{bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d[i], f, 0)),
+                       bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d[i], f, 1)),
+                       bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d[i], f, 2)),
+                       bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d[i], f, 3))};
+    } else {
+      v6u_t d;  // six dwords, of an odd first slice from the first piece's middle
+      const u32x4 y = x.c[un], z = x.c[un + 1];
+      const bool odd = SL == 2 ? un == 1 : (j0 & 1) != 0;
+      d[0] = odd ? y.z : y.x; d[1] = odd ? y.w : y.y; d[2] = odd ? z.x : y.z;
+      d[3] = odd ? z.y : y.w; d[4] = odd ? z.z : z.x; d[5] = odd ? z.w : z.y;
+      bf16x32_t v;
+      if constexpr (FMT == kE2M3) v = __builtin_amdgcn_cvt_scalef32_pk32_bf16_fp6(d, f);
+      else v = __builtin_amdgcn_cvt_scalef32_pk32_bf16_bf6(d, f);
+      struct Q { u32x4 x[4]; };
+      const Q o = __builtin_bit_cast(Q, v);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // columns 64 h + 16 q of the slice
-          const uint4 c = wr.c[2 * sl + h];
-          const uint32_t d[4] = {c.x, c.y, c.z, c.w};
-          uint32_t o[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d[i], scale(h, sl), false));
-            o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d[i], scale(h, sl), true));
-          }
-          uint4* const to = reinterpret_cast<uint4*>(w + (128 * sl + 64 * h + 16 * q) * 2);
-          to[0] = uint4{o[0], o[1], o[2], o[3]};
-          to[1] = uint4{o[4], o[5], o[6], o[7]};
-        }
-      } else {  // columns 32 q of the slice
-        uint4* const to = reinterpret_cast<uint4*>(w + (128 * sl + 32 * q) * 2);
-        if constexpr (FMT == kE2M1) {
-          const uint32_t d[4] = {wr.c[sl].x, wr.c[sl].y, wr.c[sl].z, wr.c[sl].w};
-          const float f = scale(0, sl);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            to[i] = uint4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d[i], f, 0)),
-                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d[i], f, 1)),
-                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d[i], f, 2)),
-                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d[i], f, 3))};
-        } else {
-          v6u_t d;  // six dwords, of an odd first slice from the first piece's middle
-          const uint4 x = wr.c[sl], y = wr.c[sl + 1];
-          const bool odd = SL == 2 ? sl == 1 : (j0 & 1) != 0;
-          d[0] = odd ? x.z : x.x; d[1] = odd ? x.w : x.y; d[2] = odd ? y.x : x.z;
-          d[3] = odd ? y.y : x.w; d[4] = odd ? y.z : y.x; d[5] = odd ? y.w : y.y;
-          bf16x32_t v;
-          if constexpr (FMT == kE2M3) v = __builtin_amdgcn_cvt_scalef32_pk32_bf16_fp6(d, scale(0, sl));
-          else v = __builtin_amdgcn_cvt_scalef32_pk32_bf16_bf6(d, scale(0, sl));
-          struct Q { uint4 x[4]; };
-          const Q o = __builtin_bit_cast(Q, v);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) to[i] = o.x[i];
-        }
-      }
+      for (int i = 0; i < 4; ++i) dst(i) = o.x[i];
     }
   };
 
@@ -170,85 +171,199 @@ __global__ __launch_bounds__(256) void input_grad_kernel(GradParams p) {
 #pragma unroll
       for (int c = 0; c < KI; ++c) raw[m][c] = acc[m][c];
   }
-  // fragments: dy row lane % 32 and columns 16 kk + 8 (lane / 32); W column lane % 32 and those rows
-  const int ah = lane >> 5, ax = lane & 7;
-  const uint32_t a_from = (wm * (TM / 2) + (lane & 31)) * 128;
-  const uint32_t w_from = (8 * (q >> 1) + (r >> 2)) * (RS * 2) + (wk * (TK / 2) + 16 * (q & 1) + 4 * (r & 3)) * 2;
-  auto compute = [&](int buf) {
-    const uint8_t* const a = lds + buf * A_BYTES + a_from;
-    const uint8_t* const w = lds + 2 * A_BYTES + buf * W_BYTES + w_from;
+  // fragments of a slice of 16 rows of W: dy row lane % 32 and columns 8 (lane / 32), W column lane % 32 and those rows
+  const int ah = lane >> 5;
+  const uint8_t* const a_from = lds + (wm * (TM / 2) + (lane & 31)) * 128;
+  const uint8_t* w_from[2];  // rows 0 .. 3 and 4 .. 7 of the lane's eight
 #pragma unroll
-    for (int kk = 0; kk < kGradStage / 16; ++kk) {
-      uint4 af[MI], wf[KI];
-#pragma unroll
-      for (int m = 0; m < MI; ++m) af[m] = *reinterpret_cast<const uint4*>(a + m * 4096 + 16 * ((2 * kk + ah) ^ ax));
-#pragma unroll
-      for (int c = 0; c < KI; ++c) {
-        const s16x4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(w + 16 * kk * (RS * 2) + c * 64));
-        const s16x4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(w + (16 * kk + 4) * (RS * 2) + c * 64));
-        const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
-        wf[c] = uint4{y0.x, y0.y, y1.x, y1.y};
-      }
+  for (int h = 0; h < 2; ++h)
+    w_from[h] = lds + 2 * A_BYTES + (8 * (q >> 1) + 4 * h + (r >> 2)) * (RS * 2) + wk * TK +
+                (16 * ((2 * (q & 1) + ((r & 3) >> 1)) ^ (2 * (q >> 1) + h)) + 8 * (r & 1));
+  u32x4 af[2][MI];
+  u32x2 wf[2][KI][2];
+  constexpr int READS = MI + 2 * KI;
+  auto read = [&](auto I, auto KK, int buf) {  // read I of slice KK
+    constexpr int i = decltype(I)::value, kk = decltype(KK)::value;
+    if constexpr (i < 2 * KI) {
+      const uint8_t* const src = w_from[i & 1] + buf * W_BYTES + 16 * kk * (RS * 2) + (i >> 1) * 64;
+      wf[kk & 1][i >> 1][i & 1] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src));
+    } else {
+      af[kk & 1][i - 2 * KI] = *reinterpret_cast<const u32x4*>(a_from + buf * A_BYTES + (i - 2 * KI) * 4096 + 16 * ((2 * kk) ^ ah ^ ((lane >> 1) & 7)));
+    }
+  };
+  auto mfma = [&](auto I, auto KK) {
+    constexpr int i = decltype(I)::value, kk = decltype(KK)::value, m = i / KI, c = i % KI;
+    v16f& sum = BLOCK ? raw[BLOCK ? m : 0][BLOCK ? c : 0] : acc[m][c];
+    const u32x2 lo = wf[kk & 1][c][0], hi = wf[kk & 1][c][1];
+    sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, u32x4{lo.x, lo.y, hi.x, hi.y}),
+                                                 __builtin_bit_cast(bf16x8_t, af[kk & 1][m]), sum, 0, 0, 0);
+  };
+  auto fold = [&](int block_row) {  // 128 rows of W end: their sums by their block's scale
+    if constexpr (BLOCK) {
+      const int64_t col = (int64_t)kb * SL + (SL == 2 ? wk : 0);
+      const float f = static_cast<const float*>(p.sw)[block_row * (p.K / 128) + (col < p.K / 128 ? col : p.K / 128 - 1)];
 #pragma unroll
       for (int m = 0; m < MI; ++m)
 #pragma unroll
-        for (int c = 0; c < KI; ++c) {
-          v16f& to = BLOCK ? raw[BLOCK ? m : 0][BLOCK ? c : 0] : acc[m][c];
-          to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, wf[c]),
-                                                       __builtin_bit_cast(bf16x8_t, af[m]), to, 0, 0, 0);
-        }
+        for (int c = 0; c < KI; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            acc[m][c][e] = __builtin_fmaf(raw[m][c][e], f, acc[m][c][e]);
+            raw[m][c][e] = 0.0f;
+          }
     }
   };
+  // this wave's LDS reads and writes are done, then the barrier (loads stay in flight)
+  auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
   if (s0 < s1) {
-    load(s0);
-    store(0);
-    if (s0 + 1 < s1) load(s0 + 1);
-    __syncthreads();
-    for (int s = s0; s < s1; ++s) {
-      const int buf = (s - s0) & 1;
-      if (s + 1 < s1) store(buf ^ 1);
-      if (s + 2 < s1) load(s + 2);
-      compute(buf);
-      if constexpr (BLOCK) {
-        if ((s & 1) || s + 1 == s1) {  // a block of 128 rows ends
-          const float f = static_cast<const float*>(p.sw)[(int64_t)(s >> 1) * (p.K / 128) +
-                                                          std::min<int64_t>(kb * SL + (SL == 2 ? wk : 0), p.K / 128 - 1)];
-#pragma unroll
-          for (int m = 0; m < MI; ++m)
-#pragma unroll
-            for (int c = 0; c < KI; ++c)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                acc[m][c][e] = __builtin_fmaf(raw[m][c][e], f, acc[m][c][e]);
-                raw[m][c][e] = 0.0f;
+    // Stage s of four slices, MI KI MFMAs each.  Under them the next slice's fragments are read, the next stage's pieces
+    // go from registers to LDS (slices 0 to 2) and those of the stage after it are requested.  Before the last slice
+    // all waves meet: the next stage lies in LDS whole, and this one's fragments are all in registers, so the last
+    // slice reads the next stage's first fragments and its buffer is free for the stage after.
+    constexpr int S = MI * KI;
+    auto stage = [&](auto BUF, int s) {
+      constexpr int buf = decltype(BUF)::value;
+      const int next = s + 2 < s1 ? s + 2 : s1 - 1;
+      auto slice = [&](auto KK) {
+        constexpr int kk = decltype(KK)::value, rk = (kk + 1) & 3, rb = kk == 3 ? buf ^ 1 : buf;
+        if constexpr (kk == 3) meet();
+        auto step = [&](auto I) {
+          constexpr int i = decltype(I)::value;
+          mfma(I, KK);
+          // (the last quarter of a slice's steps reads nothing: its reads have landed when the next begins)
+          constexpr int over = S - S / 4, first = i < over ? i * READS / over : READS, end = i < over ? (i + 1) * READS / over : READS;
+          for_n<end - first>([&](auto n) {
+            read(std::integral_constant<int, first + decltype(n)::value>{}, std::integral_constant<int, rk>{}, rb);
+          });
+          if constexpr (kk < 3) {
+            // pieces to LDS: the strip's units, then dy's NA
+            constexpr int ALL = NA + Pieces::UNITS, over = 3 * S - S / 2, at = kk * S + i;
+            constexpr int lo = at < over ? at * ALL / over : ALL, hi = at < over ? (at + 1) * ALL / over : ALL;
+            if constexpr (hi > lo) {
+              static_assert(hi - lo == 1, "a piece a step");
+              if constexpr (lo < Pieces::UNITS) {
+                store_w(std::integral_constant<int, lo>{}, buf ^ 1);
+                if constexpr (lo == Pieces::UNITS - 1) load_w(next);
+              } else {
+                store_a(std::integral_constant<int, lo - Pieces::UNITS>{}, buf ^ 1);
+                load_a(std::integral_constant<int, lo - Pieces::UNITS>{}, next);
               }
-        }
-      }
-      __syncthreads();
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        for_n<S>(step);
+      };
+      for_n<4>(slice);
+      if constexpr (BLOCK && buf == 1) fold(s >> 1);
+    };
+    for_n<NA>([&](auto u) { load_a(u, s0); });
+    load_w(s0);
+    for_n<NA>([&](auto u) { store_a(u, 0); });
+    for_n<Pieces::UNITS>([&](auto u) { store_w(u, 0); });
+    for_n<NA>([&](auto u) { load_a(u, s0 + 1); });
+    load_w(s0 + 1);
+    meet();
+    for_n<READS>([&](auto i) { read(i, std::integral_constant<int, 0>{}, 0); });
+    for (int s = s0; s < s1; s += 2) {
+      stage(std::integral_constant<int, 0>{}, s);
+      stage(std::integral_constant<int, 1>{}, s + 1);
     }
   }
 
-  // lane: row lane % 32, columns 8 g + 4 (lane / 32) .. + 3 of a 32 x 32 tile in registers 4 g ..
+  if (p.more.ids && split == 0) {
+    // The adapters of the tile's rows, in turn, 16 ranks at a time: A's rows take the place of W's (as they are), dv's
+    // halves that of dy, zero in other adapters' rows.
+    const RowAdapters& o = p.more;
+    int own[MI], all[TM / 64];  // of the lane's row of each m-tile; of rows lane + 64 i of the tile
+    auto id = [&](int64_t row) {
+      const int x = row < p.M ? o.ids[row] : -1;
+      return (uint32_t)x < (uint32_t)o.slots ? x : 0x7FFFFFFF;
+    };
+    for_n<MI>([&](auto m) { own[m] = id(row0 + wm * (TM / 2) + 32 * m + (lane & 31)); });
+    for_n<TM / 64>([&](auto i) { all[i] = id(row0 + lane + 64 * i); });
+    const int width = o.l.width(), groups = o.l.parts * o.l.groups;
+    for (int last = -1;;) {
+      int a = 0x7FFFFFFF;
+      for_n<TM / 64>([&](auto i) { a = all[i] > last && all[i] < a ? all[i] : a; });
 #pragma unroll
-  for (int m = 0; m < MI; ++m) {
-    const int64_t row = row0 + wm * (TM / 2) + 32 * m + (lane & 31);
-    if (row >= p.M) continue;
-#pragma unroll
-    for (int c = 0; c < KI; ++c)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int64_t col = (int64_t)kb * TK + wk * (TK / 2) + 32 * c + 8 * g + 4 * ah;
-        if (col >= p.K) continue;
-        const v4f v = {acc[m][c][4 * g], acc[m][c][4 * g + 1], acc[m][c][4 * g + 2], acc[m][c][4 * g + 3]};
-        if (p.S > 1) {
-          *reinterpret_cast<v4f*>(p.partial + (split * p.M + row) * p.K + col) = v;
-        } else {
-          const uint32_t h[4] = {f32_to_bf16(v[0]), f32_to_bf16(v[1]), f32_to_bf16(v[2]), f32_to_bf16(v[3])};
-          *reinterpret_cast<uint2*>(p.out + row * p.ldo + col) = uint2{h[0] | h[1] << 16, h[2] | h[3] << 16};
-        }
+      for (int d = 1; d < 64; d <<= 1) {
+        const int b = __shfl_xor(a, d, 64);
+        a = b < a ? b : a;
       }
+      a = last = __builtin_amdgcn_readfirstlane(a);
+      if (a == 0x7FFFFFFF) break;
+      for (int g = 0; g < groups; ++g) {
+        const int part = g / o.l.groups, j0r = 16 * (g - part * o.l.groups);
+        const uint16_t* const rows = o.mat + a * o.slot_stride + (int64_t)(part * o.l.rank + j0r) * o.ldm + (int64_t)kb * TK;
+        u32x4 piece[TK / 128];
+        for_n<TK / 128>([&](auto u) {  // row, columns 8 c ..
+          const int at = t + 256 * u, y = at / (TK / 8), c = at % (TK / 8);
+          piece[u] = u32x4{0, 0, 0, 0};
+          if (j0r + y < o.l.rank && (int64_t)kb * TK + 8 * c < p.K) piece[u] = *reinterpret_cast<const u32x4*>(rows + y * o.ldm + 8 * c);
+        });
+        u32x4 vf[2][MI];
+        for_n<MI>([&](auto m) {
+          const int64_t row = row0 + wm * (TM / 2) + 32 * m + (lane & 31);
+          const uint16_t* const v = o.v + (own[m] == a ? row : 0) * (2 * width) + 16 * g + 8 * ah;
+          for_n<2>([&](auto h) {
+            vf[h][m] = u32x4{0, 0, 0, 0};
+            if (own[m] == a) vf[h][m] = *reinterpret_cast<const u32x4*>(v + h * width);
+          });
+        });
+        meet();  // (the last reads of W's buffer)
+        for_n<TK / 128>([&](auto u) {
+          const int at = t + 256 * u, y = at / (TK / 8), c = at % (TK / 8);
+          *reinterpret_cast<u32x4*>(lds + 2 * A_BYTES + y * (RS * 2) + 16 * (c ^ (y >> 2))) = piece[u];
+        });
+        meet();
+        for_n<2 * KI>([&](auto i) { read(i, std::integral_constant<int, 0>{}, 0); });
+        for_n<2>([&](auto h) {
+          for_n<MI * KI>([&](auto i) {
+            constexpr int m = decltype(i)::value / KI, c = decltype(i)::value % KI;
+            const u32x2 x0 = wf[0][c][0], x1 = wf[0][c][1];
+            acc[m][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, u32x4{x0.x, x0.y, x1.x, x1.y}),
+                                                               __builtin_bit_cast(bf16x8_t, vf[h][m]), acc[m][c], 0, 0, 0);
+          });
+        });
+      }
+    }
   }
+
+  // (with all 256 accumulators live the compiler would first copy them to vector registers, more than there are)
+  auto value = [&](auto m, auto c, auto e) -> float {
+    if constexpr (MI * KI < 16) {
+      return acc[m][c][decltype(e)::value];
+    } else {
+      float x;
+      asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x) : "a"(acc[m][c][decltype(e)::value]));
+      return x;
+    }
+  };
+  // lane: row lane % 32, columns 8 g + 4 (lane / 32) .. + 3 of a 32 x 32 tile in registers 4 g ..
+  for_n<MI>([&](auto m) {
+    const int64_t row = row0 + wm * (TM / 2) + 32 * m + (lane & 31);
+    for_n<KI>([&](auto c) {
+      for_n<4>([&](auto g) {
+        const int64_t col = (int64_t)kb * TK + wk * (TK / 2) + 32 * c + 8 * g + 4 * ah;
+        v4f v;
+        for_n<4>([&](auto e) {
+          constexpr int i = decltype(e)::value;
+          v[i] = value(m, c, std::integral_constant<int, 4 * decltype(g)::value + i>{});
+        });
+        if (row < p.M && col < p.K) {
+          if (p.S > 1) {
+            *reinterpret_cast<v4f*>(p.partial + (split * p.M + row) * p.K + col) = v;
+          } else {
+            const uint32_t h[4] = {f32_to_bf16(v[0]), f32_to_bf16(v[1]), f32_to_bf16(v[2]), f32_to_bf16(v[3])};
+            *reinterpret_cast<u32x2*>(p.out + row * p.ldo + col) = u32x2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    });
+  });
 }
 
 // out = the sum of the splits' partials [S, M, K], rounded; four columns a thread.
@@ -267,6 +382,16 @@ __global__ __launch_bounds__(256) void input_grad_join_kernel(const float* parti
   *reinterpret_cast<uint2*>(out + row * ldo + col) = uint2{h[0] | h[1] << 16, h[2] | h[3] << 16};
 }
 
+// dst [M, wide] = src [M, N] with zeros behind it; N and wide in eights.
+__global__ __launch_bounds__(256) void input_grad_pad_kernel(const uint16_t* src, int64_t M, int64_t N, int64_t lds,
+                                                             int64_t wide, uint16_t* dst) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / (wide / 8), col = 8 * (at - row * (wide / 8));
+  if (row >= M) return;
+  uint4 v = {0, 0, 0, 0};
+  if (col < N) v = *reinterpret_cast<const uint4*>(src + row * lds + col);
+  *reinterpret_cast<uint4*>(dst + row * wide + col) = v;
+}
+
 }  // namespace mxl
 
 // ------------------------------------------------------------------- C ABI
@@ -282,13 +407,35 @@ struct GradPlan {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
-  GradPlan g{128, 128, 1, 0};
-  const int64_t tiles = ceil_div(M, g.TM) * ceil_div(K, g.TK), pairs = ceil_div(N, 2 * kGradStage);
-  g.S = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)cu_count() / tiles, pairs / 4, 16}));
-  g.per = ceil_div(pairs, g.S) * 2;
-  g.S = (int)ceil_div(2 * pairs, g.per);
-  return g;
+// Tile and split by a time model: us of a stage on a CU (of two workgroups where `resident`, and of one alone), in full
+// launches at the clock that the power limit leaves; a split's partials make a round trip.
+struct GradCost {
+  int TM, TK, resident;
+  double stage, alone;
+};
+constexpr GradCost kGradCosts[] = {{256, 256, 1, 1.73, 1.73}, {256, 128, 1, 0.92, 0.92}, {128, 256, 1, 1.06, 1.06},
+                                   {128, 128, 2, 1.03, 0.62}};
+constexpr double kGradFixed = 5.0, kGradJoin = 4.0, kGradBytesPerUs = 5.0e6;
+
+GradPlan grad_plan(int64_t M, int64_t N, int64_t K, bool block) {
+  const int64_t pairs = ceil_div(N, 2 * kGradStage), cus = cu_count();
+  GradPlan best{};
+  double best_us = 1e300;
+  for (const GradCost& c : kGradCosts) {
+    if (block ? c.TM != 128 : c.TM == 128 && c.TK == 256) continue;
+    const int64_t tiles = ceil_div(M, c.TM) * ceil_div(K, c.TK);
+    for (int64_t s = 1; s <= 16 && s <= pairs; ++s) {
+      const int64_t per = ceil_div(pairs, s);
+      if (ceil_div(pairs, per) != s) continue;
+      const int64_t n = ceil_div(tiles * s, cus);  // workgroups of the fullest CU
+      double us = kGradFixed + 2 * per * (n / c.resident * c.stage + n % c.resident * c.alone);
+      if (s > 1) us += kGradJoin + (8.0 * s + 2.0) * M * K / kGradBytesPerUs;
+      if (us >= best_us) continue;
+      best_us = us;
+      best = GradPlan{c.TM, c.TK, (int)s, 2 * per};
+    }
+  }
+  return best;
 }
 
 template <int FMT, bool BLOCK>
@@ -301,6 +448,12 @@ hipError_t launch_grad(const GradPlan& g, const GradParams& p, hipStream_t s) {
     input_grad_kernel<FMT, TM_, TK_, BLOCK><<<grid, 256, lds, s>>>(p);                                 \
     return hipGetLastError();                                                                          \
   }
+  if constexpr (!BLOCK) {
+    MXL_GRAD(256, 256)
+    MXL_GRAD(256, 128)
+  } else {
+    MXL_GRAD(128, 256)
+  }
   MXL_GRAD(128, 128)
 #undef MXL_GRAD
   return hipErrorInvalidValue;
@@ -308,16 +461,21 @@ hipError_t launch_grad(const GradPlan& g, const GradParams& p, hipStream_t s) {
 
 }  // namespace
 
-extern "C" int64_t mxl_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const GradPlan g = grad_plan(M, N, K);
-  return g.S > 1 ? g.S * M * K * 4 : 0;
+// A dy whose columns end inside a pair of stages is copied with zeros behind them, ahead of the partials.
+static int64_t pad_bytes(int64_t M, int64_t N) {
+  const int64_t wide = ceil_div(N, 2 * kGradStage) * 2 * kGradStage;
+  return wide == N ? 0 : ceil_div(M * wide * 2, 256) * 256;
 }
 
-extern "C" int mxl_input_grad(const void* dy, int64_t M, int64_t N, int64_t lddy, const void* w_tiled, const void* sw,
-                              int64_t K, int fmt, int block, void* out, int64_t ldo, void* workspace,
-                              int64_t workspace_bytes, void* stream) {
-  const char* who = "mxl_input_grad";
+int64_t mxl::input_grad_bytes(int64_t M, int64_t N, int64_t K, int block) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const GradPlan g = grad_plan(M, N, K, block);
+  return pad_bytes(M, N) + (g.S > 1 ? g.S * M * K * 4 : 0);
+}
+
+int mxl::input_grad(const char* who, const void* dy, int64_t M, int64_t N, int64_t lddy, const void* w, const void* sw,
+                    int64_t K, int fmt, int block, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes,
+                    const RowAdapters* more, void* stream) {
   MXL_CHECK_ARG(fmt == kE4M3 || fmt == kE2M3 || fmt == kE3M2 || fmt == kE2M1, "%s: unknown format %d", who, fmt);
   MXL_CHECK_ARG(!block || fmt == kE4M3, "%s: block-FP8 weights are E4M3", who);
   MXL_CHECK_ARG(M >= 0 && N > 0 && N % 8 == 0 && K > 0 && K % 128 == 0 && N <= (1 << 22) && K <= (1 << 22) && M <= 0x7FFFFFFF,
@@ -325,22 +483,31 @@ extern "C" int mxl_input_grad(const void* dy, int64_t M, int64_t N, int64_t lddy
                 (long long)M, (long long)N, (long long)K);
   MXL_CHECK_ARG(lddy >= N && lddy % 8 == 0 && lddy <= (1 << 22) && ldo >= K && ldo % 4 == 0,
                 "%s: need lddy >= N, a multiple of 8 up to 2^22, and ldo >= K, a multiple of 4", who);
-  MXL_CHECK_ARG((((uintptr_t)dy | (uintptr_t)w_tiled) & 15) == 0 && ((uintptr_t)sw & 3) == 0 && ((uintptr_t)out & 7) == 0,
+  MXL_CHECK_ARG((((uintptr_t)dy | (uintptr_t)w) & 15) == 0 && ((uintptr_t)sw & 3) == 0 && ((uintptr_t)out & 7) == 0,
                 "%s: misaligned operands", who);
   if (M == 0) return MXL_OK;
-  const GradPlan g = grad_plan(M, N, K);
-  const int64_t need = mxl_input_grad_workspace_bytes(M, N, K);
+  const GradPlan g = grad_plan(M, N, K, block);
+  const int64_t need = input_grad_bytes(M, N, K, block);
   MXL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                 "%s: needs a 16-byte aligned workspace of %lld bytes (have %lld)", who, (long long)need,
                 (long long)workspace_bytes);
   GradParams p{};
-  p.dy = (const uint16_t*)dy; p.w = (const uint8_t*)w_tiled; p.sw = sw; p.out = (uint16_t*)out; p.partial = (float*)workspace;
-  p.M = M; p.N = N; p.K = K; p.KT = ceil_div(K, kTileK); p.lddy = lddy; p.ldo = ldo; p.S = g.S; p.per = g.per;
+  p.dy = (const uint16_t*)dy; p.w = (const uint8_t*)w; p.sw = sw; p.out = (uint16_t*)out;
+  p.M = M; p.N = ceil_div(N, 2 * kGradStage) * 2 * kGradStage; p.K = K; p.KT = ceil_div(K, kTileK);
+  p.lddy = lddy; p.ldo = ldo; p.S = g.S; p.per = g.per; p.strips = (int)ceil_div(N, 16);
+  p.partial = (float*)((uint8_t*)workspace + pad_bytes(M, N));
+  if (more) p.more = *more;
   MXL_CHECK_ARG(ceil_div(M, g.TM) * ceil_div(K, g.TK) * g.S <= 0x7FFFFFFF, "%s: too large", who);
   p.mblocks = (uint32_t)ceil_div(M, g.TM);
   p.kblocks = (uint32_t)ceil_div(K, g.TK);
   p.group_m = std::min<uint32_t>(p.mblocks, 1024 / g.TM);
   hipStream_t s = (hipStream_t)stream;
+  if (p.N != N) {
+    input_grad_pad_kernel<<<dim3((unsigned)ceil_div(M * p.N / 8, 256)), 256, 0, s>>>(p.dy, M, N, lddy, p.N, (uint16_t*)workspace);
+    MXL_CHECK_LAUNCH(who);
+    p.dy = (const uint16_t*)workspace;
+    p.lddy = p.N;
+  }
   const hipError_t e = block          ? launch_grad<kE4M3, true>(g, p, s)
                        : fmt == kE4M3 ? launch_grad<kE4M3, false>(g, p, s)
                        : fmt == kE2M3 ? launch_grad<kE2M3, false>(g, p, s)
@@ -355,4 +522,15 @@ extern "C" int mxl_input_grad(const void* dy, int64_t M, int64_t N, int64_t lddy
     MXL_CHECK_LAUNCH(who);
   }
   return MXL_OK;
+}
+
+extern "C" int64_t mxl_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int block) {
+  return input_grad_bytes(M, N, K, block);
+}
+
+extern "C" int mxl_input_grad(const void* dy, int64_t M, int64_t N, int64_t lddy, const void* w_tiled, const void* sw,
+                              int64_t K, int fmt, int block, void* out, int64_t ldo, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+  return input_grad("mxl_input_grad", dy, M, N, lddy, w_tiled, sw, K, fmt, block, out, ldo, workspace, workspace_bytes,
+                    nullptr, stream);
 }

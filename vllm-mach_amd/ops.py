@@ -1165,7 +1165,7 @@ def input_grad(dy: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, k: i
     out = dy.new_empty((M, k))
     if M:
         with _on(dy.device):
-            nbytes = query("mxl_input_grad_workspace_bytes", M, dy.shape[1], k)
+            nbytes = query("mxl_input_grad_workspace_bytes", M, dy.shape[1], k, int(block))
             ws = _scratch(nbytes, w)
             call("mxl_input_grad", ptr(dy), M, dy.shape[1], _row_stride(dy), ptr(w), ptr(sw), k, w_fmt, int(block),
                  ptr(out), k, ptr(ws), nbytes, stream_handle(dy.device))
@@ -1237,9 +1237,9 @@ def _(x, dh, w, sw, i, w_fmt, act=SILU, rule=FLOOR_CARRY175):
 
 # ----------------------------------------------------------------- low-rank adapters
 
-def adapter_batch(ids: torch.Tensor, slots: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Tokens sorted by adapter: ids integers [M] (outside [0, slots): none) -> order i32 [M] (stable), offsets i64
-    [slots + 1] into it, and the tiles that the adapters' kernels walk, i32 [tiles, 2]."""
+def adapter_batch(ids: torch.Tensor, slots: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Tokens sorted by adapter: ids integers [M] (outside [0, slots): none) -> the ids as i32 [M], order i32 [M] (stable),
+    offsets i64 [slots + 1] into it, and the tiles that the adapters' kernels walk, i32 [tiles, 2]."""
     _check_cuda(ids)
     if ids.ndim != 1 or ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
         raise ValueError(f"adapter ids must be integers [M], got {ids.dtype} {tuple(ids.shape)}")
@@ -1248,9 +1248,10 @@ def adapter_batch(ids: torch.Tensor, slots: int) -> tuple[torch.Tensor, torch.Te
     M, dev = ids.shape[0], ids.device
     if M >= 1 << 31:
         raise ValueError(f"less than 2^31 tokens ({M})")
-    if ids.dtype != torch.int32:  # (values past 32 bits would wrap into range)
-        ids = torch.where((ids >= 0) & (ids < slots), ids, -1).to(torch.int32)
-    ids = ids.contiguous()
+    if ids.dtype == torch.int32:  # (a copy: the caller may write its own for the next step)
+        ids = ids.clone(memory_format=torch.contiguous_format)
+    else:  # (values past 32 bits would wrap into range)
+        ids = torch.where((ids >= 0) & (ids < slots), ids, -1).to(torch.int32).contiguous()
     order = torch.empty(M, dtype=torch.int32, device=dev)
     offsets = torch.empty(slots + 1, dtype=torch.int64, device=dev)
     inverse = torch.empty(M, dtype=torch.int32, device=dev)
@@ -1265,12 +1266,14 @@ def adapter_batch(ids: torch.Tensor, slots: int) -> tuple[torch.Tensor, torch.Te
                  stream_handle(dev))
             call("mxl_adapter_tiles", ptr(offsets), M, slots, ptr(tiles), tiles.shape[0], stream_handle(dev))
     _count("adapter_batch")
-    return order, offsets, tiles
+    return ids, order, offsets, tiles
 
 
-def _adapter_args(what: str, x, a, b, scaling, order, offsets, tiles, cols):
-    """The checked operands of the adapters' kernels: (x, a, b, parts, rank, cols as a C array)."""
-    _same_device(what, x, a, b, scaling, order, offsets, tiles)
+def _adapter_args(what: str, x, a, b, scaling, ids, order, offsets, tiles, cols):
+    """The checked operands of the adapters' kernels: (x, a, b, scaling, parts, rank, cols as a C array)."""
+    _same_device(what, x, a, b, scaling, ids, order, offsets, tiles)
+    if x.ndim != 2:
+        raise ValueError(f"{what} needs bf16 [M, K]")
     parts, slots = len(cols) - 1, a.shape[0] if a.ndim == 3 else 0
     if b.ndim != 3 or a.ndim != 3 or a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
         raise ValueError(f"{what}: a and b must be bf16 [slots, parts * rank, K] and [slots, N, rank]")
@@ -1285,30 +1288,33 @@ def _adapter_args(what: str, x, a, b, scaling, order, offsets, tiles, cols):
     if scaling.dtype != torch.float32 or tuple(scaling.shape) != (slots,):
         raise ValueError(f"{what}: scaling must be fp32 [{slots}]")
     M = x.shape[0]
-    if (order.dtype != torch.int32 or tuple(order.shape) != (M,) or offsets.dtype != torch.int64
-            or tuple(offsets.shape) != (slots + 1,) or tiles.dtype != torch.int32
+    if (ids.dtype != torch.int32 or tuple(ids.shape) != (M,) or order.dtype != torch.int32 or tuple(order.shape) != (M,)
+            or offsets.dtype != torch.int64 or tuple(offsets.shape) != (slots + 1,) or tiles.dtype != torch.int32
             or tuple(tiles.shape) != (query("mxl_adapter_tile_count", M, slots), 2)
-            or not (order.is_contiguous() and offsets.is_contiguous() and tiles.is_contiguous())):
+            or not (ids.is_contiguous() and order.is_contiguous() and offsets.is_contiguous() and tiles.is_contiguous())):
         raise ValueError(f"{what}: the batch is not one of {M} tokens and {slots} adapters (adapter_batch)")
     x = _bf16_rows(what, x, x.shape[1])
     return x, _aligned(a, 16), _aligned(b, 16), scaling.contiguous(), parts, rank, (ctypes.c_int64 * len(cols))(*cols)
 
 
+def _v_shape(m: int, parts: int, rank: int) -> tuple[int, int]:
+    return m, 2 * parts * ((rank + 15) // 16) * 16
+
+
 @_operator("adapter_apply", mutates_args=("y",))
 def adapter_apply(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
-                  order: torch.Tensor, offsets: torch.Tensor, tiles: torch.Tensor, cols: list[int]) -> torch.Tensor:
+                  ids: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, tiles: torch.Tensor,
+                  cols: list[int]) -> torch.Tensor:
     """y[t] += scaling[s] b[s] (a[s] x[t]) for every token t of a batch (``adapter_batch``), s its adapter: y bf16 [M, N] in
     place, x bf16 [M, K], a bf16 [slots, parts * rank, K], b bf16 [slots, N, rank], scaling fp32 [slots].  ``cols``: where
-    the layer's merged parts start, and N; a part has ``rank`` rows of a of its own.  Returns v, the scaled a x of the
-    tokens in the batch's order (fp32, in shares that sum to it), which ``adapter_grad`` takes."""
-    if x.ndim != 2:
-        raise ValueError("adapter_apply needs bf16 [M, K]")
-    x, a, b, scaling, parts, rank, c = _adapter_args("adapter_apply", x, a, b, scaling, order, offsets, tiles, cols)
+    the layer's merged parts start, and N; a part has ``rank`` rows of a of its own.  Returns v for ``adapter_grad``: the
+    scaled a x of each token with an adapter, as bf16 values and what those leave of the fp32."""
+    x, a, b, scaling, parts, rank, c = _adapter_args("adapter_apply", x, a, b, scaling, ids, order, offsets, tiles, cols)
     (M, K), slots = x.shape, a.shape[0]
     if (y.dtype != torch.bfloat16 or tuple(y.shape) != (M, cols[-1]) or y.device != x.device or y.stride(1) != 1
             or (M > 1 and y.stride(0) < y.shape[1])):
         raise ValueError(f"adapter_apply: y must be bf16 [{M}, {cols[-1]}] of unit column stride on {x.device}")
-    v = x.new_empty(query("mxl_adapter_v_floats", M, K, slots, parts, rank), dtype=torch.float32)
+    v = x.new_empty(_v_shape(M, parts, rank))
     if M:
         with _on(x.device):
             call("mxl_adapter_apply", ptr(x), M, K, _row_stride(x), ptr(a), ptr(b), ptr(scaling), slots, parts, c, rank,
@@ -1319,49 +1325,88 @@ def adapter_apply(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Te
 
 
 @adapter_apply.register_fake
-def _(y, x, a, b, scaling, order, offsets, tiles, cols):
-    return x.new_empty((torch.library.get_ctx().new_dynamic_size(),), dtype=torch.float32)
+def _(y, x, a, b, scaling, ids, order, offsets, tiles, cols):
+    return x.new_empty(_v_shape(x.shape[0], len(cols) - 1, b.shape[2]))
 
 
-@_operator("adapter_grad", mutates_args=("dx",))
-def adapter_grad(dx: Optional[torch.Tensor], dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
-                 scaling: torch.Tensor, v: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, tiles: torch.Tensor,
-                 cols: list[int], need_a: bool = True, need_b: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
-    """The gradients of ``adapter_apply``'s a and b (bf16, their shapes; empty where not needed) from dy bf16 [M, N], and
-    in place dx[t] += a[s]^T (scaling[s] b[s]^T dy[t]) where dx bf16 [M, K] is given."""
-    if x.ndim != 2:
-        raise ValueError("adapter_grad needs bf16 [M, K]")
-    x, a, b, scaling, parts, rank, c = _adapter_args("adapter_grad", x, a, b, scaling, order, offsets, tiles, cols)
-    _same_device("adapter_grad", x, dy, dx, v)
+def adapter_linear_supported(m: int, n: int, k: int, w_fmt: int, block: bool, slots: int, parts: int, rank: int) -> bool:
+    """Shapes whose product adds the adapters itself (``adapter_linear``): from 17 rows, at least 32 an adapter."""
+    return bool(query("mxl_adapter_linear_supported", m, n, k, w_fmt, int(block), slots, parts, rank))
+
+
+@_operator("adapter_linear")
+def adapter_linear(x: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, w_fmt: int, block: bool, rule: int,
+                   bias: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
+                   ids: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, tiles: torch.Tensor,
+                   cols: list[int]) -> tuple[torch.Tensor, torch.Tensor]:
+    """A quantized layer's product of x bf16 [M, K] (quantized by ``rule``; ``block``: block-FP8) with the adapters of
+    ``adapter_apply`` added to its fp32 sums, ahead of their one rounding -> (y bf16 [M, N], v).  Shapes:
+    ``adapter_linear_supported``."""
+    x, a, b, scaling, parts, rank, c = _adapter_args("adapter_linear", x, a, b, scaling, ids, order, offsets, tiles, cols)
     (M, K), slots, N = x.shape, a.shape[0], cols[-1]
+    _same_device("adapter_linear", x, w, sw, bias)
+    w, sw = _tiled_weight("adapter_linear", w, sw, N, K, w_fmt, block)
+    bias = _fp4_bias("adapter_linear", bias, N)
+    if M and not adapter_linear_supported(M, N, K, w_fmt, block, slots, parts, rank):
+        raise ValueError(f"adapter_linear: {M} rows of {slots} adapters do not run in one product (N={N}, K={K})")
+    if block:
+        x = x.contiguous()
+    y, v = x.new_empty((M, N)), x.new_empty(_v_shape(M, parts, rank))
+    if M:
+        with _on(x.device):
+            nbytes = query("mxl_adapter_linear_workspace_bytes", M, K, w_fmt, int(block))
+            ws = _scratch(nbytes, w)
+            call("mxl_adapter_linear", ptr(x), M, K, _row_stride(x), rule, ptr(w), ptr(sw), w_fmt, int(block), ptr(bias),
+                 ptr(a), ptr(b), ptr(scaling), slots, parts, c, rank, ptr(ids), ptr(order), ptr(offsets), ptr(tiles),
+                 tiles.shape[0], ptr(v), v.numel(), ptr(y), N, ptr(ws), nbytes, stream_handle(x.device))
+    _count("adapter_linear")
+    return y, v
+
+
+@adapter_linear.register_fake
+def _(x, w, sw, w_fmt, block, rule, bias, a, b, scaling, ids, order, offsets, tiles, cols):
+    return x.new_empty((x.shape[0], cols[-1])), x.new_empty(_v_shape(x.shape[0], len(cols) - 1, b.shape[2]))
+
+
+@_operator("adapter_grad")
+def adapter_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, w_fmt: int, block: bool,
+                 a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor, v: torch.Tensor, ids: torch.Tensor,
+                 order: torch.Tensor, offsets: torch.Tensor, tiles: torch.Tensor, cols: list[int], need_x: bool = True,
+                 need_a: bool = True, need_b: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The gradients of a frozen layer with adapters from dy bf16 [M, N]: (dx, da, db) bf16 in the shapes of x, a and b, empty
+    where not needed.  dx[t] = dy[t] W (``input_grad``) + a[s]^T (scaling[s] b[s]^T dy[t]); an adapter without tokens gets
+    zeros."""
+    x, a, b, scaling, parts, rank, c = _adapter_args("adapter_grad", x, a, b, scaling, ids, order, offsets, tiles, cols)
+    _same_device("adapter_grad", x, dy, w, sw, v)
+    (M, K), slots, N = x.shape, a.shape[0], cols[-1]
+    w, sw = _tiled_weight("adapter_grad", w, sw, N, K, w_fmt, block)
     if N % 8:
         raise ValueError(f"adapter_grad needs N % 8 == 0 (N={N})")
     if dy.shape[0] != M:
         raise ValueError(f"adapter_grad: dy has {dy.shape[0]} rows, x {M}")
     dy = _bf16_rows("adapter_grad", dy, N, "dy")
-    if dx is not None and (dx.dtype != torch.bfloat16 or tuple(dx.shape) != (M, K) or dx.stride(1) != 1
-                           or (M > 1 and dx.stride(0) < K)):
-        raise ValueError(f"adapter_grad: dx must be bf16 [{M}, {K}] of unit column stride")
-    if v.dtype != torch.float32 or not v.is_contiguous() or v.numel() != query("mxl_adapter_v_floats", M, K, slots, parts, rank):
+    if v.dtype != torch.bfloat16 or not v.is_contiguous() or tuple(v.shape) != _v_shape(M, parts, rank):
         raise ValueError("adapter_grad: v is not adapter_apply's of these operands")
     make = torch.Tensor.new_empty if M else torch.Tensor.new_zeros
+    dx = x.new_empty((M, K) if need_x else (0,))
     da = make(a, a.shape if need_a else (0,))
     db = make(b, b.shape if need_b else (0,))
-    if M and (need_a or need_b or dx is not None):
+    if M and (need_a or need_b or need_x):
         with _on(x.device):
-            nbytes = query("mxl_adapter_grad_workspace_bytes", M, K, slots, parts, c, rank)
+            nbytes = query("mxl_adapter_grad_workspace_bytes", M, K, slots, parts, c, rank, int(block))
             ws = _scratch(nbytes, v)
-            call("mxl_adapter_grad", ptr(x), M, K, _row_stride(x), ptr(dy), _row_stride(dy), ptr(a), ptr(b), ptr(scaling),
-                 slots, parts, c, rank, ptr(order), ptr(offsets), ptr(tiles), tiles.shape[0], ptr(v), v.numel(), ptr(dx),
-                 K if dx is None else _row_stride(dx), ptr(da) if need_a else None, ptr(db) if need_b else None, ptr(ws),
-                 nbytes, stream_handle(x.device))
+            call("mxl_adapter_grad", ptr(x), M, K, _row_stride(x), ptr(dy), _row_stride(dy), ptr(w), ptr(sw), w_fmt, int(block),
+                 ptr(a), ptr(b), ptr(scaling), slots, parts, c, rank, ptr(ids), ptr(order), ptr(offsets), ptr(tiles),
+                 tiles.shape[0], ptr(v), v.numel(), ptr(dx) if need_x else None, K, ptr(da) if need_a else None,
+                 ptr(db) if need_b else None, ptr(ws), nbytes, stream_handle(x.device))
     _count("adapter_grad")
-    return da, db
+    return dx, da, db
 
 
 @adapter_grad.register_fake
-def _(dx, dy, x, a, b, scaling, v, order, offsets, tiles, cols, need_a=True, need_b=True):
-    return a.new_empty(a.shape if need_a else (0,)), b.new_empty(b.shape if need_b else (0,))
+def _(dy, x, w, sw, w_fmt, block, a, b, scaling, v, ids, order, offsets, tiles, cols, need_x=True, need_a=True, need_b=True):
+    return (x.new_empty(x.shape if need_x else (0,)), a.new_empty(a.shape if need_a else (0,)),
+            b.new_empty(b.shape if need_b else (0,)))
 
 
 # ---------------------------------------------------------------------- MoE
