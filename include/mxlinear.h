@@ -586,7 +586,7 @@ int mxl_gated_grad(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, c
 
 /* Low-rank adapters of many requests.  A batch of M tokens sorted by adapter (mxl_moe_route of the ids
  * as [M, 1], at most 2560 adapters): order i32 [M], offsets i64 [slots + 1], and from them the tiles
- * i32 [mxl_adapter_tile_count][2] that mxl_adapter_tiles writes.
+ * i32 [mxl_adapter_tile_count][4] (16-byte aligned) that mxl_adapter_tiles writes.
  *
  * mxl_adapter_apply: y[t] += scaling[s] b[s] (a[s] x[t]) for every token t of the batch, s its adapter:
  * y bf16 [M, N] in place, x bf16 [M, K], a bf16 [slots, parts rank, K], b bf16 [slots, N, rank], N =
@@ -608,10 +608,11 @@ int mxl_gated_grad(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, c
 int64_t mxl_adapter_tile_count(int64_t M, int64_t slots);
 int mxl_adapter_tiles(const int64_t* offsets, int64_t M, int64_t slots, int32_t* tiles, int64_t num_tiles, void* stream);
 int64_t mxl_adapter_v_elems(int64_t M, int64_t parts, int64_t rank);
+int64_t mxl_adapter_apply_workspace_bytes(int64_t M, int64_t K, int64_t slots, int64_t parts, int64_t rank);
 int mxl_adapter_apply(const void* x, int64_t M, int64_t K, int64_t ldx, const void* a, const void* b,
                       const float* scaling, int64_t slots, int64_t parts, const int64_t* cols, int64_t rank,
                       const int32_t* order, const int64_t* offsets, const int32_t* tiles, int64_t num_tiles, void* v,
-                      int64_t v_elems, void* y, int64_t ldy, void* stream);
+                      int64_t v_elems, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream);
 int mxl_adapter_linear_supported(int64_t M, int64_t N, int64_t K, int fmt, int block, int64_t slots, int64_t parts,
                                  int64_t rank);
 int64_t mxl_adapter_linear_workspace_bytes(int64_t M, int64_t K, int fmt, int block);

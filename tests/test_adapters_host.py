@@ -110,7 +110,7 @@ def test_entry_points_refuse(pkg):
     tiles = _lib.query("mxl_adapter_tile_count", 4, 2)
     v = _lib.query("mxl_adapter_v_elems", 4, 1, 8)
     assert v == 4 * 2 * 16
-    apply = [16, 4, 128, 128, 16, 16, 16, 2, 1, _cols(0, 128), 8, 16, 16, 16, tiles, 16, v, 16, 128, None]
+    apply = [16, 4, 128, 128, 16, 16, 16, 2, 1, _cols(0, 128), 8, 16, 16, 16, tiles, 16, v, 16, 128, 16, 1 << 20, None]
     for at, bad, match in ((7, 0, "slots"), (14, tiles + 1, "tiles"), (8, 9, "parts"), (10, 12, "rank"), (10, 264, "rank"),
                            (2, 100, "K % 8"), (9, _cols(0, 0), "no columns"), (9, _cols(16, 128), "start at column 0"),
                            (3, 64, "ldx"), (18, 64, "ldy"), (0, 8, "aligned"), (16, v - 1, "values"), (11, None, "order")):
@@ -120,7 +120,7 @@ def test_entry_points_refuse(pkg):
             call("mxl_adapter_apply", *args)
     with pytest.raises(err, match="multiple of 16"):
         call("mxl_adapter_apply", 16, 4, 128, 128, 16, 16, 16, 2, 2, _cols(0, 24, 128), 8, 16, 16, 16, tiles, 16, 1 << 20, 16,
-             128, None)
+             128, 16, 1 << 20, None)
     grad = [16, 4, 128, 128, 16, 128, 16, 16, 0, 0, 16, 16, 16, 2, 1, _cols(0, 128), 8, 16, 16, 16, 16, tiles, 16, v, 16, 128,
             16, 16, 256, 1 << 30, None]
     for at, bad, match in ((15, _cols(0, 100), "N % 8"), (29, 100, "workspace"), (28, 128, "workspace"), (4, 8, "aligned"),
@@ -154,7 +154,7 @@ def test_no_rows_is_no_launch(pkg):
     _lib.call("mxl_gated_linear", 16, 0, 128, 128, 0, 16, 16, 64, 0, 0, 16, 64, None, 0, None)
     _lib.call("mxl_gated_grad", 16, 0, 128, 128, 0, 16, 16, 64, 0, 0, None, 64, 16, 128, None, 0, None)
     _lib.call("mxl_adapter_apply", 16, 0, 128, 128, 16, 16, 16, 2, 1, _cols(0, 128), 8, None, None, None, 0, 16, 0, 16, 128,
-              None)
+              None, 0, None)
 
 
 def test_fakes(pkg):

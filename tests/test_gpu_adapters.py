@@ -81,7 +81,7 @@ def test_batch_contents(pkg, dev):
             assert torch.equal(order[:n].long(), want.indices[:n])
             assert torch.equal(offsets, torch.searchsorted(want.values[:n].contiguous(), torch.arange(slots + 1, device=dev)))
         at = offsets.tolist()
-        tiles = [(s, p) for s in range(slots) for p in range(at[s], at[s + 1], 16)]
+        tiles = [(s, p, min(p + 16, at[s + 1]), 0) for s in range(slots) for p in range(at[s], at[s + 1], 16)]
         got = [tuple(t) for t in tiles_.tolist()]
         assert got[:len(tiles)] == tiles and all(t[0] == -1 for t in got[len(tiles):])
     big = pkg.AdapterBatch(torch.tensor([2 ** 32, 1, -2 ** 40, 0], device=dev), 2)

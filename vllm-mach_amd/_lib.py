@@ -47,8 +47,9 @@ SIGNATURES = {
     "mxl_adapter_tile_count": (_I64, [_I64, _I64]),
     "mxl_adapter_tiles": (_I, [_P, _I64, _I64, _P, _I64, _P]),
     "mxl_adapter_v_elems": (_I64, [_I64, _I64, _I64]),
+    "mxl_adapter_apply_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "mxl_adapter_apply": (_I, [_P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I64,
-                               _P]),
+                               _P, _I64, _P]),
     "mxl_adapter_linear_supported": (_I, [_I64, _I64, _I64, _I, _I, _I64, _I64, _I64]),
     "mxl_adapter_linear_workspace_bytes": (_I64, [_I64, _I64, _I, _I]),
     "mxl_adapter_linear": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _I, _I, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _P,

@@ -27,7 +27,7 @@ class AdapterBatch:
     """
 
     def __init__(self, ids: torch.Tensor, slots: int):
-        self.slots = int(slots)
+        self.slots, self.updates = int(slots), 0
         self.tensors = ops.adapter_batch(ids, self.slots)  # ids, order, offsets, tiles
 
     def __len__(self) -> int:
@@ -39,6 +39,7 @@ class AdapterBatch:
                              f"{ids.device}")
         for kept, new in zip(self.tensors, ops.adapter_batch(ids, self.slots)):
             kept.copy_(new)
+        self.updates += 1
         return self
 
 
@@ -115,70 +116,59 @@ class FrozenLinear(torch.autograd.Function):
     """A prepared layer's product (with a bias in its epilogue) with the gradients of its input and the bias."""
 
     @staticmethod
-    def forward(x, w, sw, layer, bias):
+    def forward(ctx, x, bias, layer):
+        ctx.layer = grad_of(layer)
         return layer.mxl_kernel.apply_weights(layer, x, bias)
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        _, w, sw, layer, _ = inputs
-        ctx.save_for_backward(w, sw)
-        ctx.meta = grad_of(layer)[2:]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        w, sw = ctx.saved_tensors
-        n, k, fmt, block = ctx.meta
+        w, sw, n, k, fmt, block = ctx.layer
         dy2 = dy.reshape(-1, n)
         dx = ops.input_grad(dy2, w, sw, n, k, fmt, block).reshape(*dy.shape[:-1], k) if ctx.needs_input_grad[0] else None
-        return dx, None, None, None, dy2.sum(0) if ctx.needs_input_grad[4] else None
+        return dx, dy2.sum(0) if ctx.needs_input_grad[1] else None, None
 
 
 class AdapterLinear(torch.autograd.Function):
     """A prepared layer with its adapters: the gradients of the input, the adapters and a bias in the epilogue."""
 
     @staticmethod
-    def forward(x, a, b, scaling, ids, order, offsets, tiles, cols, w, sw, layer, bias):
-        return _forward(layer, x, bias, a, b, scaling, (ids, order, offsets, tiles), cols)
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        x, a, b, scaling, ids, order, offsets, tiles, cols, w, sw, layer, _ = inputs
-        ctx.mark_non_differentiable(output[1])
-        # (a batch updated for the next step before this one's backward is noticed by its tensors' versions)
-        ctx.save_for_backward(x, a, b, scaling, output[1], ids, order, offsets, tiles, w, sw)
-        ctx.meta = (list(cols), *grad_of(layer)[2:])
+    def forward(ctx, x, a, b, bias, layer, adapters, batch):
+        y, v = _forward(layer, x, bias, a, b, adapters.scaling, batch.tensors, adapters.cols)
+        ctx.save_for_backward(x, a, b)
+        ctx.held = (v, grad_of(layer), adapters.scaling, adapters.scaling._version, batch, batch.updates, adapters.cols)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, _):
-        x, a, b, scaling, v, *batch, w, sw = ctx.saved_tensors
-        cols, n, k, fmt, block = ctx.meta
-        need_x, need_a, need_b = ctx.needs_input_grad[:3]
+    def backward(ctx, dy):
+        x, a, b = ctx.saved_tensors
+        v, (w, sw, n, k, fmt, block), scaling, version, batch, updates, cols = ctx.held
+        if batch.updates != updates or scaling._version != version:
+            raise RuntimeError("the batch or the adapters' scaling has been modified by an inplace operation between this "
+                               "layer's forward and its backward")
+        need_x, need_a, need_b, need_bias = ctx.needs_input_grad[:4]
         dy2 = dy.reshape(-1, n)
-        dx, da, db = ops.adapter_grad(dy2, x.reshape(-1, k), w, sw, fmt, block, a, b, scaling, v, *batch, cols, need_x, need_a,
-                                      need_b)
-        return (dx.reshape(x.shape) if need_x else None, da if need_a else None, db if need_b else None, *[None] * 9,
-                dy2.sum(0) if ctx.needs_input_grad[12] else None)
+        dx, da, db = ops.adapter_grad(dy2, x.reshape(-1, k), w, sw, fmt, block, a, b, scaling, v, *batch.tensors, cols, need_x,
+                                      need_a, need_b)
+        return (dx.reshape(x.shape) if need_x else None, da if need_a else None, db if need_b else None,
+                dy2.sum(0) if need_bias else None, None, None, None)
 
 
 class GatedLinear(torch.autograd.Function):
     """``ops.gated_linear`` with the gradient of its input."""
 
     @staticmethod
-    def forward(x, w, sw, i, fmt, act, rule):
-        return ops.gated_linear(x.reshape(-1, x.shape[-1]), w, sw, i, fmt, act, rule).reshape(*x.shape[:-1], i)
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        x, w, sw, *ctx.meta = inputs
-        ctx.save_for_backward(x, w, sw)
+    def forward(ctx, x, *args):
+        ctx.save_for_backward(x)
+        ctx.args = args
+        return ops.gated_linear(x.reshape(-1, x.shape[-1]), *args).reshape(*x.shape[:-1], args[2])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        x, w, sw = ctx.saved_tensors
-        i, fmt, act, rule = ctx.meta
+        x, = ctx.saved_tensors
+        w, sw, i, fmt, act, rule = ctx.args
         k = x.shape[-1]
         both = ops.gated_grad(x.reshape(-1, k), dh.reshape(-1, i), w, sw, i, fmt, act, rule)
         return ops.input_grad(both, w, sw, 2 * i, k, fmt).reshape(x.shape), *[None] * 6
@@ -211,8 +201,7 @@ def apply_adapters(layer: torch.nn.Module, x: torch.Tensor, adapters: LowRankAda
         raise ValueError(f"adapters need bf16 [..., {k}] of the batch's {len(batch)} rows, got {x.dtype} {tuple(x.shape)}")
     a, b = adapters.lora_a, adapters.lora_b
     if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad):
-        w, sw = grad_of(layer)[:2]
         inner = _function_bias(bias, x, n)
-        y = AdapterLinear.apply(x, a, b, adapters.scaling, *batch.tensors, adapters.cols, w, sw, layer, inner)[0]
+        y = AdapterLinear.apply(x, a, b, inner, layer, adapters, batch)
         return y if bias is inner else y + bias
     return _forward(layer, x, bias, a, b, adapters.scaling, batch.tensors, adapters.cols)[0]

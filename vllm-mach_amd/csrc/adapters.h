@@ -8,7 +8,7 @@ namespace mxl {
 constexpr int kMaxParts = 8, kMaxRank = 256, kMaxSlots = 4096, kAdapterTile = 16;
 
 // Tokens sorted by adapter: positions [offsets[a], offsets[a + 1]) of order are adapter a's, in tiles of 16 positions:
-// tile i is (adapter, first position), adapter -1 past the last.
+// tile i is (adapter, first position, end, 0), adapter -1 past the last.
 struct AdapterBatch {
   const int32_t* order;
   const int64_t* offsets;

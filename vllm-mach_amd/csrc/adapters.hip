@@ -25,18 +25,31 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 
 // The tile's adapter and positions [lo, hi); false past the last tile.
 __device__ __forceinline__ bool batch_tile(const AdapterBatch& b, int tile, int& slot, int64_t& lo, int64_t& hi) {
-  slot = b.tiles[2 * tile];
-  if (slot < 0) return false;
-  lo = b.tiles[2 * tile + 1];
-  const int64_t end = b.offsets[slot + 1];
-  hi = lo + kAdapterTile < end ? lo + kAdapterTile : end;
-  hi = hi < b.M ? hi : b.M;
-  return lo < hi;
+  const int4 t = reinterpret_cast<const int4*>(b.tiles)[tile];
+  slot = t.x;
+  lo = t.y;
+  hi = t.z;
+  return slot >= 0;
 }
 
 __device__ __forceinline__ bf16x8_t as_bf16x8(const u32x4& v) { return __builtin_bit_cast(bf16x8_t, v); }
 __device__ __forceinline__ u32x4 keep(const u32x4& v, bool in) {
   return u32x4{in ? v[0] : 0u, in ? v[1] : 0u, in ? v[2] : 0u, in ? v[3] : 0u};
+}
+
+constexpr int kMaxShares = 8;  // of a column sum (the shrink kernel's)
+
+// The wave's own writes to LDS are there for its other lanes.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// What the bf16 pair h leaves of (a, b), as bf16.  (Of an infinity nothing, where the difference would be NaN.)
+__device__ __forceinline__ uint32_t rest_of(float a, float b, uint32_t h) {
+  const float h0 = u2f(h << 16), h1 = u2f(h & 0xFFFF0000u);
+  return cvt_pk_bf16(__builtin_isfinite(h0) ? a - h0 : 0.0f, __builtin_isfinite(h1) ? b - h1 : 0.0f);
 }
 
 // ------------------------------------------------------------------ tiles of a batch
@@ -69,7 +82,7 @@ __global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offs
   if (t == 0) first[slots] = before;
   __syncthreads();
   for (int i = t; i < num_tiles; i += 1024) {
-    int slot = -1, pos = 0;
+    int slot = -1, pos = 0, to = 0;
     if (i < before) {
       int lo = 0, hi = slots;  // the last adapter whose first tile is not past i
       while (hi - lo > 1) {
@@ -78,9 +91,9 @@ __global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offs
       }
       slot = lo;
       pos = (int)offsets[lo] + (i - first[lo]) * kAdapterTile;
+      to = pos + kAdapterTile < (int)offsets[lo + 1] ? pos + kAdapterTile : (int)offsets[lo + 1];
     }
-    tiles[2 * i] = slot;
-    tiles[2 * i + 1] = pos;
+    reinterpret_cast<int4*>(tiles)[i] = int4{slot, pos, to, 0};
   }
 }
 
@@ -89,11 +102,14 @@ __global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offs
 // v[t] (adapters.h) of s sum_k rows[j][k] x[t][k].  BY_PART: part p's rows are [0, r) of the adapter's and its columns
 // [cols[p], cols[p + 1]) (B^T [r, N]); else rows [p r, p r + r) and all columns (A).  A workgroup is a tile of 16 tokens
 // by RC groups of 16 ranks; its waves share the columns and meet in LDS.  Both operands come straight from memory: the
-// rows' A from L2, where its tiles share it, x once.
-template <int RC, bool BY_PART>
+// rows' A from L2, where its tiles share it, x once.  SHARES: few tiles fill the card by splitting the columns over
+// workgroups, whose fp32 sums [blockIdx.z][token][width] the expand kernel joins (48 tokens of 32 adapters, K = 5120, both
+// kernels: 20.0 us whole, 14.3 in shares).
+template <int RC, bool BY_PART, bool SHARES>
 __global__ __launch_bounds__(RC == 1 ? 1024 : 512) void adapter_shrink_kernel(AdapterBatch b, LowRank l, const uint16_t* x, int64_t ldx,
                                                               int64_t cols, const uint16_t* rows, int64_t slot_stride,
-                                                              int64_t ldr, const float* scaling, uint16_t* v) {
+                                                              int64_t ldr, const float* scaling, uint16_t* v,
+                                                              float* shares) {
   extern __shared__ __attribute__((aligned(16))) float red[];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, q = lane >> 4;
@@ -114,21 +130,25 @@ __global__ __launch_bounds__(RC == 1 ? 1024 : 512) void adapter_shrink_kernel(Ad
   v4f acc[RC];
 #pragma unroll
   for (int g = 0; g < RC; ++g) acc[g] = v4f{0.f, 0.f, 0.f, 0.f};
-  // this wave's columns: 32 an MFMA, U of them loaded together
-  constexpr int U = 4;
-  const int64_t units = (c1 - c0 + 31) / 32, per = (units + waves - 1) / waves;
-  const int64_t k0 = c0 + 32 * per * wv, k1 = k0 + 32 * per < c1 ? k0 + 32 * per : c1;
-  for (int64_t k = k0; k < k1; k += 32 * U) {
+  // This wave's columns: 32 an MFMA, up to U of them loaded together; the waves' shares of a pass lie side by side.
+  constexpr int U = RC == 1 ? 8 : 4;
+  const int all = waves * (SHARES ? (int)gridDim.z : 1), who = (SHARES ? (int)blockIdx.z * waves : 0) + wv;
+  const int units = (int)((c1 - c0 + 31) / 32), each = (units + all - 1) / all, passes = (each + U - 1) / U;
+  const int step = (each + passes - 1) / passes;
+  for (int u0 = who * step; u0 < units; u0 += all * step) {
+    const int64_t k = c0 + 32 * (int64_t)u0, k1 = k + 32 * step < c1 ? k + 32 * step : c1;
     u32x4 xv[U], av[U][RC];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (u >= step) break;
       const int64_t at = k + 32 * u + 8 * q < k1 ? k + 32 * u : c0 - 8 * q;  // (columns come in eights)
-      xv[u] = *reinterpret_cast<const u32x4*>(xr + at);
 #pragma unroll
       for (int g = 0; g < RC; ++g) av[u][g] = *reinterpret_cast<const u32x4*>(ar[g] + at);
+      xv[u] = *reinterpret_cast<const u32x4*>(xr + at);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (u >= step) break;
       const bool in = k + 32 * u + 8 * q < k1;
       xv[u] = keep(xv[u], in);
 #pragma unroll
@@ -142,21 +162,25 @@ __global__ __launch_bounds__(RC == 1 ? 1024 : 512) void adapter_shrink_kernel(Ad
   const float s = scaling[slot];
   for (int f = wv; f < RC; f += waves) {
     v4f sum = *reinterpret_cast<const v4f*>(red + (f * waves * 64 + lane) * 4);
+#pragma unroll 4
     for (int w = 1; w < waves; ++w) {
       const v4f one = *reinterpret_cast<const v4f*>(red + ((f * waves + w) * 64 + lane) * 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[e] += one[e];
     }
     const int g = g0 + f;
-    if (lo + r < hi && g < l.groups) {
+    if constexpr (SHARES) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = 16 * g + 4 * q + e < l.rank ? sum[e] * s : 0.0f;
+      if (lo + r < hi && g < l.groups)
+        *reinterpret_cast<v4f*>(shares + (blockIdx.z * b.M + token) * l.width() + (part * l.groups + g) * 16 + 4 * q) = sum;
+    } else if (lo + r < hi && g < l.groups) {
       uint32_t hl[2][2];
 #pragma unroll
       for (int e = 0; e < 4; e += 2) {
         const float v0 = 16 * g + 4 * q + e < l.rank ? sum[e] * s : 0.0f, v1 = 16 * g + 4 * q + e + 1 < l.rank ? sum[e + 1] * s : 0.0f;
-        const uint32_t h = cvt_pk_bf16(v0, v1);
-        const float h0 = u2f(h << 16), h1 = u2f(h & 0xFFFF0000u);
-        hl[0][e / 2] = h;  // (of an infinity nothing is left, where the difference would be NaN)
-        hl[1][e / 2] = cvt_pk_bf16(__builtin_isfinite(h0) ? v0 - h0 : 0.0f, __builtin_isfinite(h1) ? v1 - h1 : 0.0f);
+        hl[0][e / 2] = cvt_pk_bf16(v0, v1);
+        hl[1][e / 2] = rest_of(v0, v1, hl[0][e / 2]);
       }
       uint16_t* const to = v + (int64_t)token * (2 * l.width()) + (part * l.groups + g) * 16 + 4 * q;
       *reinterpret_cast<uint2*>(to) = uint2{hl[0][0], hl[0][1]};
@@ -170,8 +194,10 @@ __global__ __launch_bounds__(RC == 1 ? 1024 : 512) void adapter_shrink_kernel(Ad
 // y[t][n] += sum_j mat[n][j] v[t][j], mat [N, ldm] (j < valid) of the tile's adapter, j the ranks of n's part.  A wave is a
 // tile of 16 tokens by 64 columns of one part: MFMA i's row 4 q + e is column 16 q + 4 i + e, so that after the four a
 // lane holds 16 columns of one token side by side (the rows of y in 32-byte pieces; `wide`: they start on 16 bytes).
-__global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterBatch b, LowRank l, const uint16_t* v,
-                                                             const uint16_t* mat, int64_t slot_stride, int64_t ldm,
+// SHARES: v comes as the shrink kernel's shares, and the first columns' workgroup writes it down.
+template <bool SHARES>
+__global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterBatch b, LowRank l, uint16_t* v, const float* shares,
+                                                             int num_shares, const uint16_t* mat, int64_t slot_stride, int64_t ldm,
                                                              int valid, uint16_t* y, int64_t ldy, int wide) {
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
@@ -202,16 +228,50 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterBatch b, Low
     const int64_t n = c0 + 16 * (r >> 2) + 4 * i + (r & 3);
     mr[i] = mat + slot * slot_stride + (n < c1 ? n : c1 - 1) * ldm + 8 * (q & 1);
   }
+  extern __shared__ __attribute__((aligned(16))) float red[];
+  // SHARES: the wave's rows of v, halves side by side, a row's 16-byte pieces exchanged by its number
+  const int pieces = 4 * l.groups;
+  u32x4* const joined = reinterpret_cast<u32x4*>(red) + wv * 16 * pieces;
+  if constexpr (SHARES) {
+    for (int i = lane; i < (int)(hi - lo) * pieces; i += 64) {  // four values
+      const int row = i / pieces, c = i - row * pieces;
+      const int64_t at = b.order[lo + row];
+      const float* const src = shares + at * l.width() + part * l.groups * 16 + 4 * c;
+      v4f one[kMaxShares];
+#pragma unroll
+      for (int z = 0; z < kMaxShares; ++z)
+        one[z] = *reinterpret_cast<const v4f*>(src + (z < num_shares ? z : 0) * (b.M * l.width()));
+      v4f sum = one[0];
+#pragma unroll
+      for (int z = 1; z < kMaxShares; ++z)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += z < num_shares ? one[z][e] : 0.0f;
+      const uint32_t h0 = cvt_pk_bf16(sum[0], sum[1]), h1 = cvt_pk_bf16(sum[2], sum[3]);
+      const uint2 big{h0, h1}, rest{rest_of(sum[0], sum[1], h0), rest_of(sum[2], sum[3], h1)};
+      uint2* const to = reinterpret_cast<uint2*>(joined + row * pieces);
+      to[2 * ((c >> 1) ^ (row & 3)) + (c & 1)] = big;
+      to[2 * ((2 * l.groups + (c >> 1)) ^ (row & 3)) + (c & 1)] = rest;
+      if (blk == 0) {
+        uint16_t* const out = v + at * (2 * l.width()) + part * l.groups * 16 + 4 * c;
+        *reinterpret_cast<uint2*>(out) = big;
+        *reinterpret_cast<uint2*>(out + l.width()) = rest;
+      }
+    }
+    wave_lds_fence();
+  }
   v4f acc[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
   for (int g = 0; g < l.groups; ++g) {
     const bool in = 16 * g + 8 * (q & 1) < valid;  // (ranks come in eights)
-    const u32x4 h = *reinterpret_cast<const u32x4*>(vr + 16 * g);
-    u32x4 m[4];
+    u32x4 m[4], h;
 #pragma unroll
     for (int i = 0; i < 4; ++i) m[i] = *reinterpret_cast<const u32x4*>(mr[i] + (in ? 16 * g : -8 * (q & 1)));
+    if constexpr (SHARES)
+      h = joined[r * pieces + ((2 * l.groups * (q >> 1) + 2 * g + (q & 1)) ^ (r & 3))];
+    else
+      h = *reinterpret_cast<const u32x4*>(vr + 16 * g);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(keep(m[i], in)), as_bf16x8(h), acc[i], 0, 0, 0);
@@ -409,7 +469,8 @@ int check_batch(const char* who, int64_t M, int64_t slots, const int32_t* order,
                 who, kMaxSlots, (long long)M, (long long)slots);
   MXL_CHECK_ARG(num_tiles == tile_count(M, slots), "%s: %lld tiles for M=%lld slots=%lld, need %lld", who,
                 (long long)num_tiles, (long long)M, (long long)slots, (long long)tile_count(M, slots));
-  MXL_CHECK_ARG(M == 0 || (order && offsets && tiles), "%s: needs the batch's order, offsets and tiles", who);
+  MXL_CHECK_ARG(M == 0 || (order && offsets && tiles && ((uintptr_t)tiles & 15) == 0),
+                "%s: needs the batch's order, offsets and tiles (16-byte aligned)", who);
   return MXL_OK;
 }
 
@@ -437,39 +498,50 @@ int launched(const char* who) {
   return MXL_EHIP;
 }
 
+// Shares of the columns where the expand kernel follows: until some 256 workgroups run, or a wave has 32 columns.
+int shrink_shares(int64_t tiles, const LowRank& l, int64_t cols) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>({kMaxShares, 256 / (tiles * l.parts * l.groups), cols / 256}));
+}
+
 template <bool BY_PART>
 int launch_shrink(const char* who, const AdapterBatch& b, const LowRank& l, const uint16_t* x, int64_t ldx, int64_t cols,
                   const uint16_t* rows, int64_t slot_stride, int64_t ldr, const float* scaling, uint16_t* v,
-                  hipStream_t s) {
-  const int rc = shrink_groups(b.num_tiles, l.groups);
+                  float* shares, int num_shares, hipStream_t s) {
+  const int rc = num_shares > 1 ? 1 : shrink_groups(b.num_tiles, l.groups);
   const int64_t chunks = l.parts * ceil_div(l.groups, rc);
-  const int waves = rc == 1 && b.num_tiles * chunks <= 256 ? 16 : 8;
-  const dim3 grid((unsigned)b.num_tiles, (unsigned)chunks);
+  const int waves = rc == 1 && num_shares == 1 && b.num_tiles * chunks <= 256 ? 16 : 8;
+  const dim3 grid((unsigned)b.num_tiles, (unsigned)chunks, (unsigned)num_shares);
   const unsigned lds = (unsigned)(rc * waves * 1024);
-#define MXL_SHRINK(RC_)                                                                                           \
-  if (rc == RC_)                                                                                                  \
-    adapter_shrink_kernel<RC_, BY_PART><<<grid, 64 * waves, lds, s>>>(b, l, x, ldx, cols, rows, slot_stride, ldr, \
-                                                                      scaling, v);
-  MXL_SHRINK(1) MXL_SHRINK(2) MXL_SHRINK(4)
+#define MXL_SHRINK(RC_, SHARES_)                                                                                          \
+  if (rc == RC_ && (num_shares > 1) == SHARES_)                                                                           \
+    adapter_shrink_kernel<RC_, BY_PART, SHARES_><<<grid, 64 * waves, lds, s>>>(b, l, x, ldx, cols, rows, slot_stride, ldr, \
+                                                                               scaling, v, shares);
+  MXL_SHRINK(1, false) MXL_SHRINK(2, false) MXL_SHRINK(4, false)
+  if constexpr (!BY_PART) MXL_SHRINK(1, true)
 #undef MXL_SHRINK
   return launched(who);
 }
 
-int launch_expand(const char* who, const AdapterBatch& b, const LowRank& l, const uint16_t* v, const uint16_t* mat,
-                  int64_t slot_stride, int64_t ldm, int valid, uint16_t* y, int64_t ldy, hipStream_t s) {
+int launch_expand(const char* who, const AdapterBatch& b, const LowRank& l, uint16_t* v, const float* shares,
+                  int num_shares, const uint16_t* mat, int64_t slot_stride, int64_t ldm, int valid, uint16_t* y,
+                  int64_t ldy, hipStream_t s) {
   int64_t blocks = 0;
   for (int p = 0; p < l.parts; ++p) blocks += ceil_div(l.cols[p + 1] - l.cols[p], 64);
   MXL_CHECK_ARG(blocks <= 4 * 0xFFFF, "%s: too many columns", who);
   const dim3 grid((unsigned)b.num_tiles, (unsigned)ceil_div(blocks, 4));
-  adapter_expand_kernel<<<grid, 256, 0, s>>>(b, l, v, mat, slot_stride, ldm, valid, y, ldy,
-                                             ldy % 8 == 0 && ((uintptr_t)y & 15) == 0);
+  const int wide = ldy % 8 == 0 && ((uintptr_t)y & 15) == 0;
+  if (num_shares > 1)
+    adapter_expand_kernel<true><<<grid, 256, (unsigned)(4096 * l.groups), s>>>(b, l, v, shares, num_shares, mat, slot_stride, ldm, valid, y, ldy, wide);
+  else
+    adapter_expand_kernel<false><<<grid, 256, 0, s>>>(b, l, v, shares, num_shares, mat, slot_stride, ldm, valid, y, ldy, wide);
   return launched(who);
 }
 
-// Shares of an adapter's tokens in the outer products, where columns and groups alone are too few workgroups: at least
-// 64 tokens each.
+// Shares of an adapter's tokens in the outer products, where columns and groups alone are too few workgroups: some 128
+// tokens each (of adapters with as many), and none while an adapter has fewer than 256: a share costs the join's launch.
 int outer_splits(int64_t M, int64_t slots, int64_t wgs) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>({32, ceil_div(768, wgs * slots), M / 64}));
+  const int64_t each = M / slots;
+  return each < 256 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({32, ceil_div(768, wgs * slots), each / 128}));
 }
 int64_t outer_blocks(const LowRank& l, int64_t cols, bool of_b) {
   int64_t blocks = 0;
@@ -543,7 +615,7 @@ extern "C" int mxl_adapter_tiles(const int64_t* offsets, int64_t M, int64_t slot
   const char* who = "mxl_adapter_tiles";
   MXL_CHECK_ARG(M >= 0 && M <= 0x7FFFFFFF && slots > 0 && slots <= kMaxSlots, "%s: need 0 <= M < 2^31 and 0 < slots <= %d", who, kMaxSlots);
   if (M == 0) return MXL_OK;
-  MXL_CHECK_ARG(offsets && tiles && num_tiles == tile_count(M, slots), "%s: needs %lld tiles", who,
+  MXL_CHECK_ARG(offsets && tiles && ((uintptr_t)tiles & 15) == 0 && num_tiles == tile_count(M, slots), "%s: needs %lld tiles", who,
                 (long long)tile_count(M, slots));
   adapter_tiles_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(offsets, (int)slots, (int)num_tiles, tiles);
   return launched(who);
@@ -553,10 +625,20 @@ extern "C" int64_t mxl_adapter_v_elems(int64_t M, int64_t parts, int64_t rank) {
   return M <= 0 || parts <= 0 || rank <= 0 ? 0 : M * 2 * parts * ceil_div(rank, 16) * 16;
 }
 
+extern "C" int64_t mxl_adapter_apply_workspace_bytes(int64_t M, int64_t K, int64_t slots, int64_t parts, int64_t rank) {
+  if (M <= 0 || K <= 0 || slots <= 0 || parts <= 0 || rank <= 0) return 0;
+  LowRank l{};
+  l.parts = (int)parts;
+  l.groups = (int)ceil_div(rank, 16);
+  const int shares = shrink_shares(tile_count(M, slots), l, K);
+  return shares > 1 ? shares * M * l.width() * 4 : 0;
+}
+
 extern "C" int mxl_adapter_apply(const void* x, int64_t M, int64_t K, int64_t ldx, const void* a, const void* b,
                                  const float* scaling, int64_t slots, int64_t parts, const int64_t* cols, int64_t rank,
                                  const int32_t* order, const int64_t* offsets, const int32_t* tiles, int64_t num_tiles,
-                                 void* v, int64_t v_elems, void* y, int64_t ldy, void* stream) {
+                                 void* v, int64_t v_elems, void* y, int64_t ldy, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
   const char* who = "mxl_adapter_apply";
   LowRank l;
   int rc = check_batch(who, M, slots, order, offsets, tiles, num_tiles);
@@ -567,13 +649,18 @@ extern "C" int mxl_adapter_apply(const void* x, int64_t M, int64_t K, int64_t ld
   MXL_CHECK_ARG((((uintptr_t)x | (uintptr_t)a | (uintptr_t)b | (uintptr_t)v) & 15) == 0, "%s: x, a, b and v must be 16-byte aligned", who);
   MXL_CHECK_ARG(v_elems >= mxl_adapter_v_elems(M, parts, rank), "%s: v holds %lld values, needs %lld", who,
                 (long long)v_elems, (long long)mxl_adapter_v_elems(M, parts, rank));
+  const int64_t need = mxl_adapter_apply_workspace_bytes(M, K, slots, parts, rank);
+  MXL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+                "%s: needs a 16-byte aligned workspace of %lld bytes (have %lld)", who, (long long)need,
+                (long long)workspace_bytes);
   const AdapterBatch batch{order, offsets, tiles, (int)num_tiles, M};
   const int64_t R = parts * rank;
+  const int shares = shrink_shares(num_tiles, l, K);
   rc = launch_shrink<false>(who, batch, l, (const uint16_t*)x, ldx, K, (const uint16_t*)a, R * K, K, scaling, (uint16_t*)v,
-                            (hipStream_t)stream);
+                            (float*)workspace, shares, (hipStream_t)stream);
   if (rc != MXL_OK) return rc;
-  return launch_expand(who, batch, l, (const uint16_t*)v, (const uint16_t*)b, N * rank, rank, l.rank, (uint16_t*)y, ldy,
-                       (hipStream_t)stream);
+  return launch_expand(who, batch, l, (uint16_t*)v, (const float*)workspace, shares, (const uint16_t*)b, N * rank, rank,
+                       l.rank, (uint16_t*)y, ldy, (hipStream_t)stream);
 }
 
 // ---- the layer and its adapters in one call
@@ -636,7 +723,8 @@ extern "C" int mxl_adapter_linear(const void* x, int64_t M, int64_t K, int64_t l
                       : mxl_quantize_mxfp8(x, M, K, ldx, rule, codes, scales, stream);
   if (rc != MXL_OK) return rc;
   const AdapterBatch batch{order, offsets, tiles, (int)num_tiles, M};
-  rc = launch_shrink<false>(who, batch, l, (const uint16_t*)x, ldx, K, (const uint16_t*)a, R * K, K, scaling, (uint16_t*)v, s);
+  rc = launch_shrink<false>(who, batch, l, (const uint16_t*)x, ldx, K, (const uint16_t*)a, R * K, K, scaling, (uint16_t*)v,
+                            nullptr, 1, s);
   if (rc != MXL_OK) return rc;
   GemmParams p{};
   p.M = p.a_rows = M; p.N = N; p.K = K; p.KT = ceil_div(K, kTileK);
@@ -704,7 +792,7 @@ extern "C" int mxl_adapter_grad(const void* x, int64_t M, int64_t K, int64_t ldx
   rc = launched(who);
   if (rc == MXL_OK)
     rc = launch_shrink<true>(who, batch, l, (const uint16_t*)dy, lddy, N, (const uint16_t*)g.bt, l.rank * N, N, scaling,
-                             (uint16_t*)g.dv, s);
+                             (uint16_t*)g.dv, nullptr, 1, s);
   if (rc == MXL_OK && da)
     rc = launch_outer<false>(who, batch, l, slots, (const uint16_t*)x, ldx, K, (const uint16_t*)g.dv,
                              (uint16_t*)da, (float*)g.partial, s);
@@ -726,7 +814,7 @@ extern "C" int mxl_adapter_grad(const void* x, int64_t M, int64_t K, int64_t ldx
   one.rank = one.groups * 16;
   one.cols[1] = K;
   if (rc == MXL_OK)
-    rc = launch_expand(who, batch, one, (const uint16_t*)g.dv, (const uint16_t*)g.at, K * l.width(), l.width(), one.rank,
+    rc = launch_expand(who, batch, one, (uint16_t*)g.dv, nullptr, 1, (const uint16_t*)g.at, K * l.width(), l.width(), one.rank,
                        (uint16_t*)dx, lddx, s);
   return rc;
 }

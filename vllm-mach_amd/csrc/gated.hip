@@ -44,10 +44,10 @@ int run(const char* who, const void* x, int64_t M, int64_t K, int64_t ldx, int r
                 (long long)I, (long long)K);
   MXL_CHECK_ARG(2 * I / 16 * ((K + kTileK - 1) / kTileK) < (1 << 24), "%s: too large (I=%lld K=%lld)", who, (long long)I,
                 (long long)K);
-  MXL_CHECK_ARG(ldx >= K && ldx % 8 == 0 && ldo >= wide && ldo % 4 == 0 && (!dh || (lddh >= I && lddh % 4 == 0)),
+  MXL_CHECK_ARG(ldx >= K && ldx % 8 == 0 && ldo >= wide && ldo % 8 == 0 && (!dh || (lddh >= I && lddh % 4 == 0)),
                 "%s: bad row stride (ldx=%lld ldo=%lld lddh=%lld)", who, (long long)ldx, (long long)ldo, (long long)lddh);
   MXL_CHECK_ARG((((uintptr_t)x | (uintptr_t)w) & 15) == 0 && ((uintptr_t)sw & 3) == 0 &&
-                    (((uintptr_t)out | (uintptr_t)dh) & 7) == 0, "%s: misaligned operands", who);
+                    ((uintptr_t)out & 15) == 0 && ((uintptr_t)dh & 7) == 0, "%s: misaligned operands", who);
   if (M == 0) return MXL_OK;
   MXL_CHECK_ARG(workspace && bytes >= workspace_bytes(M, K, fmt) && ((uintptr_t)workspace & 255) == 0,
                 "%s: needs a 256-byte aligned workspace of %lld bytes (have %lld)", who,

@@ -532,6 +532,14 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
     }
   };
 
+  typedef const __attribute__((address_space(4))) uint8_t* kernarg_t;
+  if constexpr (ADD) {  // the rows' adapters, behind the ring, for the end
+    const kernarg_t at = (kernarg_t)__builtin_amdgcn_kernarg_segment_ptr() + kAddOffset;
+    const int32_t* const ids = ((const __attribute__((address_space(4))) RowAdapters*)at)->ids;
+    const int wr = 64 * (wv % (S::BM / 64));
+    tile_copy4(reinterpret_cast<const uint8_t*>(ids + w.row0), 4 * (uint32_t)(a_row(w.row0 + wr + lane) - w.row0),
+               tile_lds(lds + L::bytes(DEPTH)) + 4 * wr);
+  }
   copy_scales(kb, Slice<1>{});
   if (FP4 && kb + 1 < ke) copy_scales(kb + 1, Slice<0>{});
   const int count = end - tb;  // stages: an even number
@@ -612,7 +620,6 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       // over the main loop they would spill.
       typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
       typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-      typedef const __attribute__((address_space(4))) uint8_t* kernarg_t;
       kernarg_t at = (kernarg_t)__builtin_amdgcn_kernarg_segment_ptr() + kAddOffset;
       asm volatile("" : "+s"(at));
       const auto* const add = (const __attribute__((address_space(4))) RowAdapters*)at;
@@ -630,9 +637,9 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       int own[MTW];
 #pragma unroll
       for (int i = 0; i < MTW; ++i) {
-        const int row = w.row0 + (wm * MTW + i) * 16 + r;
-        const int x = row < w.row_hi ? add->ids[row] : -1;
-        own[i] = (uint32_t)x < (uint32_t)add->slots ? x : 0x7FFFFFFF;
+        const int row = (wm * MTW + i) * 16 + r;
+        const int x = *reinterpret_cast<const int32_t*>(lds + L::bytes(DEPTH) + 4 * row);
+        own[i] = w.row0 + row < w.row_hi && (uint32_t)x < (uint32_t)add->slots ? x : 0x7FFFFFFF;
       }
       // the part of a column
       auto part_of = [&](int col) {
@@ -779,43 +786,69 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
     return;
   }
   if constexpr (GATED) {
-    // lane: four columns of one row of gate and of up, side by side in its registers
-    const int I = 16 * up, col0 = 16 * (nt_base + wn * NH) + 4 * q;
+    // Lane: four columns of one row of gate and of up, side by side in its registers.  Of two n-tiles every other 16
+    // lanes change places, after which a lane stores eight columns of one of them (as the wide stores below).  dh's rows
+    // are loaded a row of n-tiles ahead.
+    typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+    const int I = 16 * up, col0 = 16 * (nt_base + wn * NH);
     auto rows = [&](auto ACT) {
+      uint2 dh[2][EPI == kEpiGatedGrad ? NH : 1];
+      auto load = [&](int i) {
+        if constexpr (EPI == kEpiGatedGrad) {
+          const int row = w.row0 + (wm * MTW + i) * 16 + r;
+          const uint16_t* const src = gate.dh + (int64_t)(row < w.row_hi ? row : w.row_hi - 1) * gate.lddh;
+#pragma unroll
+          for (int n = 0; n < NH; ++n)
+            dh[i & 1][n] = *reinterpret_cast<const uint2*>(src + (col0 + 16 * n < I ? col0 + 16 * n + 4 * q : 0));
+        }
+      };
+      load(0);
 #pragma unroll
       for (int i = 0; i < MTW; ++i) {
         const int row = w.row0 + (wm * MTW + i) * 16 + r;
         uint16_t* const out = p.out + (int64_t)row * p.ldc;
+        if (i + 1 < MTW) load(i + 1);
+        uint32_t even[2][2];
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
           const v4f g = values(i, n), u = values(i, NH + n);
-          const int col = col0 + 16 * n;
-          const bool live = row < w.row_hi && col < I;
-          float x[4], y[4];
-          if constexpr (EPI == kEpiGated) {
+          float x[2][4];  // the output, or the gradients of gate and of up
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float slope;
-              x[e] = gate_act<decltype(ACT)::value>(g[e], slope) * u[e];
-            }
-          } else {
-            uint2 d = {0, 0};
-            if (live) d = *reinterpret_cast<const uint2*>(gate.dh + (int64_t)row * gate.lddh + col);
-            const float dh[4] = {u2f(d.x << 16), u2f(d.x & 0xFFFF0000u), u2f(d.y << 16), u2f(d.y & 0xFFFF0000u)};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float slope;
-              y[e] = dh[e] * gate_act<decltype(ACT)::value>(g[e], slope);
-              x[e] = dh[e] * u[e] * slope;
+          for (int e = 0; e < 4; ++e) {
+            float slope;
+            const float act = gate_act<decltype(ACT)::value>(g[e], slope);
+            if constexpr (EPI == kEpiGated) {
+              x[0][e] = act * u[e];
+            } else {
+              const uint2 d2 = dh[i & 1][n];
+              const uint32_t pair = e < 2 ? d2.x : d2.y;
+              const float d = u2f(e & 1 ? pair & 0xFFFF0000u : pair << 16);
+              x[0][e] = d * u[e] * slope;
+              x[1][e] = d * act;
             }
           }
-          auto bits = [](const float* v) {
-            return uint2{f32_to_bf16(v[0]) | (uint32_t)f32_to_bf16(v[1]) << 16,
-                         f32_to_bf16(v[2]) | (uint32_t)f32_to_bf16(v[3]) << 16};
-          };
-          if (live) {
-            *reinterpret_cast<uint2*>(out + col) = bits(x);
-            if constexpr (EPI == kEpiGatedGrad) *reinterpret_cast<uint2*>(out + I + col) = bits(y);
+#pragma unroll
+          for (int h = 0; h < (EPI == kEpiGated ? 1 : 2); ++h) {
+            uint32_t b[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) b[k] = f32_to_bf16(x[h][2 * k]) | (uint32_t)f32_to_bf16(x[h][2 * k + 1]) << 16;
+            if constexpr (NH == 1) {
+              const int col = col0 + 4 * q;
+              if (row < w.row_hi && col < I) *reinterpret_cast<uint2*>(out + h * I + col) = uint2{b[0], b[1]};
+            } else if (n & 1) {
+              u4 o;
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const auto y = __builtin_amdgcn_permlane16_swap(even[h][k], b[k], false, false);
+                o[k] = y[0];
+                o[2 + k] = y[1];
+              }
+              const int col = col0 + 16 * (n - 1) + 16 * (q & 1) + 8 * (q >> 1);
+              if (row < w.row_hi && col < I) *reinterpret_cast<u4*>(out + h * I + col) = o;
+            } else {
+              even[h][0] = b[0];
+              even[h][1] = b[1];
+            }
           }
           __builtin_amdgcn_sched_barrier(0);
         }

@@ -46,9 +46,10 @@ static hipError_t launch_adapter_fmt(const WideConfig& c, const GemmParams& p, c
   if (c.MT == MT_ && c.NT == NT_) {                                                                            \
     using D = TileDepth<MT_, NT_>;                                                                             \
     using L = TileLds<MT_ / 2, 2 * NT_, BLOCK>;                                                                \
+    static_assert(L::bytes(D::LONE) + 1024 <= 160 * 1024 && L::bytes(D::SHARED) + 1024 <= 160 * 1024, "LDS"); \
     g.depth = grid <= (int64_t)D::LONE_MAX * cu_count() ? D::LONE : D::SHARED;                                 \
     hipLaunchKernelGGL((adapter_tile_kernel<FMT, MT_, NT_, BLOCK>), dim3((unsigned)grid), dim3(256),           \
-                       (unsigned)L::bytes(g.depth), s, p, g, add);                                             \
+                       (unsigned)L::bytes(g.depth) + 1024, s, p, g, add); /* (the rows' ids) */                \
     return hipGetLastError();                                                                                  \
   }
   if constexpr (!BLOCK) {

@@ -188,9 +188,9 @@ def _function_bias(bias: Optional[torch.Tensor], x: torch.Tensor, n: int) -> Opt
 def _with_input_grad(layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
     """The layer's output as a function of x that autograd can walk back through: the weight is frozen, the dynamic
     quantization counts as the identity (``ops.input_grad``)."""
-    from .adapters import FrozenLinear, grad_of
+    from .adapters import FrozenLinear
     inner = _function_bias(bias, x, layer.mxl_shape[0])
-    y = FrozenLinear.apply(x, *grad_of(layer)[:2], layer, inner)
+    y = FrozenLinear.apply(x, inner, layer)
     return y if bias is inner else y + bias
 
 

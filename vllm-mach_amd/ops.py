@@ -1239,7 +1239,7 @@ def _(x, dh, w, sw, i, w_fmt, act=SILU, rule=FLOOR_CARRY175):
 
 def adapter_batch(ids: torch.Tensor, slots: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """Tokens sorted by adapter: ids integers [M] (outside [0, slots): none) -> the ids as i32 [M], order i32 [M] (stable),
-    offsets i64 [slots + 1] into it, and the tiles that the adapters' kernels walk, i32 [tiles, 2]."""
+    offsets i64 [slots + 1] into it, and the tiles that the adapters' kernels walk, i32 [tiles, 4]."""
     _check_cuda(ids)
     if ids.ndim != 1 or ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
         raise ValueError(f"adapter ids must be integers [M], got {ids.dtype} {tuple(ids.shape)}")
@@ -1255,7 +1255,7 @@ def adapter_batch(ids: torch.Tensor, slots: int) -> tuple[torch.Tensor, torch.Te
     order = torch.empty(M, dtype=torch.int32, device=dev)
     offsets = torch.empty(slots + 1, dtype=torch.int64, device=dev)
     inverse = torch.empty(M, dtype=torch.int32, device=dev)
-    tiles = torch.empty((query("mxl_adapter_tile_count", M, slots), 2), dtype=torch.int32, device=dev)
+    tiles = torch.empty((query("mxl_adapter_tile_count", M, slots), 4), dtype=torch.int32, device=dev)
     with _on(dev):
         if M == 0:
             offsets.zero_()
@@ -1290,7 +1290,7 @@ def _adapter_args(what: str, x, a, b, scaling, ids, order, offsets, tiles, cols)
     M = x.shape[0]
     if (ids.dtype != torch.int32 or tuple(ids.shape) != (M,) or order.dtype != torch.int32 or tuple(order.shape) != (M,)
             or offsets.dtype != torch.int64 or tuple(offsets.shape) != (slots + 1,) or tiles.dtype != torch.int32
-            or tuple(tiles.shape) != (query("mxl_adapter_tile_count", M, slots), 2)
+            or tuple(tiles.shape) != (query("mxl_adapter_tile_count", M, slots), 4)
             or not (ids.is_contiguous() and order.is_contiguous() and offsets.is_contiguous() and tiles.is_contiguous())):
         raise ValueError(f"{what}: the batch is not one of {M} tokens and {slots} adapters (adapter_batch)")
     x = _bf16_rows(what, x, x.shape[1])
@@ -1317,9 +1317,11 @@ def adapter_apply(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Te
     v = x.new_empty(_v_shape(M, parts, rank))
     if M:
         with _on(x.device):
+            nbytes = query("mxl_adapter_apply_workspace_bytes", M, K, slots, parts, rank)
+            ws = _scratch(nbytes, v)
             call("mxl_adapter_apply", ptr(x), M, K, _row_stride(x), ptr(a), ptr(b), ptr(scaling), slots, parts, c, rank,
-                 ptr(order), ptr(offsets), ptr(tiles), tiles.shape[0], ptr(v), v.numel(), ptr(y), _row_stride(y),
-                 stream_handle(x.device))
+                 ptr(order), ptr(offsets), ptr(tiles), tiles.shape[0], ptr(v), v.numel(), ptr(y), _row_stride(y), ptr(ws),
+                 nbytes, stream_handle(x.device))
     _count("adapter_apply")
     return v
 
