@@ -106,7 +106,7 @@ __global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offs
 // workgroups, whose fp32 sums [blockIdx.z][token][width] the expand kernel joins (48 tokens of 32 adapters, K = 5120, both
 // kernels: 20.0 us whole, 14.3 in shares).
 template <int RC, bool BY_PART, bool SHARES>
-__global__ __launch_bounds__(RC == 1 ? 1024 : 512) void adapter_shrink_kernel(AdapterBatch b, LowRank l, const uint16_t* x, int64_t ldx,
+__global__ __launch_bounds__(RC < 4 ? 1024 : 512) void adapter_shrink_kernel(AdapterBatch b, LowRank l, const uint16_t* x, int64_t ldx,
                                                               int64_t cols, const uint16_t* rows, int64_t slot_stride,
                                                               int64_t ldr, const float* scaling, uint16_t* v,
                                                               float* shares) {
@@ -118,14 +118,17 @@ __global__ __launch_bounds__(RC == 1 ? 1024 : 512) void adapter_shrink_kernel(Ad
   if (!batch_tile(b, blockIdx.x, slot, lo, hi)) return;
   const int per_part = (l.groups + RC - 1) / RC, part = blockIdx.y / per_part, g0 = (blockIdx.y - part * per_part) * RC;
   const int64_t c0 = BY_PART ? l.cols[part] : 0, c1 = BY_PART ? l.cols[part + 1] : cols;
-  const int64_t pos = lo + r < hi ? lo + r : hi - 1;
-  const int token = b.order[pos];
-  const uint16_t* const xr = x + (int64_t)token * ldx + 8 * q;
+  // Loads: lane 4 i + j has 16 bytes of row i, so that four lanes read a row's 64; the piece is j ^ (i >> 2), and through
+  // the wave's own LDS, written as the lanes stand and read by row r and piece q, no two of sixteen lanes share a bank.
+  const int i = lane >> 2, piece = (lane & 3) ^ (lane >> 4), from = 4 * r + (q ^ (r >> 2));
+  const uint16_t* const xr = x + (int64_t)b.order[lo + i < hi ? lo + i : hi - 1] * ldx + 8 * piece;
+  const int token = b.order[lo + r < hi ? lo + r : hi - 1];
+  u32x4* const turn = reinterpret_cast<u32x4*>(red) + wv * (1 + RC) * 64;
   const uint16_t* ar[RC];
 #pragma unroll
   for (int g = 0; g < RC; ++g) {
-    const int j = 16 * (g0 + g) + r, row = (BY_PART ? 0 : part * l.rank) + (j < l.rank ? j : l.rank - 1);
-    ar[g] = rows + slot * slot_stride + row * ldr + 8 * q;
+    const int j = 16 * (g0 + g) + i, row = (BY_PART ? 0 : part * l.rank) + (j < l.rank ? j : l.rank - 1);
+    ar[g] = rows + slot * slot_stride + row * ldr + 8 * piece;
   }
   v4f acc[RC];
 #pragma unroll
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(RC == 1 ? 1024 : 512) void adapter_shrink_kernel(Ad
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (u >= step) break;
-      const int64_t at = k + 32 * u + 8 * q < k1 ? k + 32 * u : c0 - 8 * q;  // (columns come in eights)
+      const int64_t at = k + 32 * u + 8 * piece < k1 ? k + 32 * u : c0 - 8 * piece;  // (columns come in eights)
 #pragma unroll
       for (int g = 0; g < RC; ++g) av[u][g] = *reinterpret_cast<const u32x4*>(ar[g] + at);
       xv[u] = *reinterpret_cast<const u32x4*>(xr + at);
@@ -150,12 +153,18 @@ __global__ __launch_bounds__(RC == 1 ? 1024 : 512) void adapter_shrink_kernel(Ad
     for (int u = 0; u < U; ++u) {
       if (u >= step) break;
       const bool in = k + 32 * u + 8 * q < k1;
-      xv[u] = keep(xv[u], in);
+#pragma unroll
+      for (int g = 0; g < RC; ++g) turn[64 * g + lane] = av[u][g];
+      turn[64 * RC + lane] = xv[u];
+      wave_lds_fence();
+      const bf16x8_t xs = as_bf16x8(keep(turn[64 * RC + from], in));
 #pragma unroll
       for (int g = 0; g < RC; ++g)
-        acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(keep(av[u][g], in)), as_bf16x8(xv[u]), acc[g], 0, 0, 0);
+        acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(keep(turn[64 * g + from], in)), xs, acc[g], 0, 0, 0);
+      wave_lds_fence();
     }
   }
+  __syncthreads();  // the sums take the same LDS
 #pragma unroll
   for (int g = 0; g < RC; ++g) *reinterpret_cast<v4f*>(red + ((g * waves + wv) * 64 + lane) * 4) = acc[g];
   __syncthreads();
@@ -509,9 +518,9 @@ int launch_shrink(const char* who, const AdapterBatch& b, const LowRank& l, cons
                   float* shares, int num_shares, hipStream_t s) {
   const int rc = num_shares > 1 ? 1 : shrink_groups(b.num_tiles, l.groups);
   const int64_t chunks = l.parts * ceil_div(l.groups, rc);
-  const int waves = rc == 1 && num_shares == 1 && b.num_tiles * chunks <= 256 ? 16 : 8;
+  const int waves = num_shares == 1 && rc < 4 && b.num_tiles * chunks <= 512 ? 16 : 8;
   const dim3 grid((unsigned)b.num_tiles, (unsigned)chunks, (unsigned)num_shares);
-  const unsigned lds = (unsigned)(rc * waves * 1024);
+  const unsigned lds = (unsigned)((1 + rc) * waves * 1024);
 #define MXL_SHRINK(RC_, SHARES_)                                                                                          \
   if (rc == RC_ && (num_shares > 1) == SHARES_)                                                                           \
     adapter_shrink_kernel<RC_, BY_PART, SHARES_><<<grid, 64 * waves, lds, s>>>(b, l, x, ldx, cols, rows, slot_stride, ldr, \
