@@ -210,6 +210,51 @@ def test_batch_updated_before_backward(pkg, dev):
         y.float().sum().backward()
 
 
+@pytest.mark.parametrize("which", ["scaling", "weight", "scales"])
+def test_changed_before_backward(pkg, dev, which):
+    """What a backward reads again has to be what its forward read."""
+    g, method, layer, w, ad, x, ids = _case(pkg, dev, "mxfp6", [128], 256, 3, 8, [0, 2, 2, -1, 0], 2, True)
+    y = method.apply(layer, x, None, adapters=ad, batch=pkg.AdapterBatch(ids, 3))
+    with torch.no_grad():
+        {"scaling": ad.scaling, "weight": layer.weight, "scales": layer.weight_scale}[which][:1].zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.float().sum().backward()
+
+
+@pytest.mark.parametrize("m", [5, 80])
+def test_gradient_of_the_bias_alone(pkg, dev, m):
+    """Nothing but the bias is trained: in one product (80 rows) and apart (5)."""
+    g, method, layer, w, ad, x, ids = _case(pkg, dev, "mxfp4", [128], 256, 2, 8, _ids(m, 2, 1), 2)
+    bias, dy = torch.randn(128, generator=g).bfloat16().to(dev), torch.randn(m, 128, generator=g).bfloat16().to(dev)
+    batch = pkg.AdapterBatch(ids, 2)
+    want = method.apply(layer, x, bias, adapters=ad, batch=batch)
+    bias.requires_grad_()
+    y = method.apply(layer, x, bias, adapters=ad, batch=batch)
+    assert torch.equal(y, want)
+    db, = torch.autograd.grad(y, bias, dy)
+    ref.check(db, dy.double().sum(0), ref.U * dy.double().sum(0).abs() + m * 2.0 ** -24 * dy.double().abs().sum(0))
+
+
+def test_apply_counts_as_a_write(pkg, dev):
+    """``adapter_apply`` into a tensor that a backward needs is found out."""
+    g, method, layer, w, ad, x, ids = _case(pkg, dev, "mxfp8", [128], 256, 2, 8, [0, 1, 1], 2)
+    z = torch.randn(3, 128, generator=g).bfloat16().to(dev).requires_grad_()
+    y = z.exp()  # (keeps its result)
+    with torch.no_grad():
+        pkg.ops.adapter_apply(y, x, ad.lora_a, ad.lora_b, ad.scaling, *pkg.AdapterBatch(ids, 2).tensors, ad.cols)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.float().sum().backward()
+
+
+@pytest.mark.parametrize("m,widths,k,slots,rank", [(48, [192, 64], 2560, 32, 24), (2, [128], 5120, 3, 256),
+                                                   (16, [64] * 8, 1024, 1, 8), (31, [256], 2176, 2, 40)])
+def test_few_rows_of_many_columns(pkg, dev, m, widths, k, slots, rank):
+    """The columns in shares over workgroups, joined by the product with b."""
+    g, method, layer, w, ad, x, ids = _case(pkg, dev, "mxfp8", widths, k, slots, rank, _ids(m, slots, 3), m)
+    y = method.apply(layer, x, None, adapters=ad, batch=pkg.AdapterBatch(ids, slots))
+    ref.check(y, *_want("mxfp8", x, w, ad, ids))
+
+
 @pytest.mark.parametrize("m,fmt", [(1, "mxfp8"), (40, "mxfp4"), (600, "mxfp6")])
 def test_captured(pkg, dev, m, fmt):
     """A captured step, replayed with other inputs and another batch in the same memory; two graphs in turns."""

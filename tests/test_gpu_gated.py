@@ -80,6 +80,17 @@ def test_gradients(pkg, dev, fmt, act, m, i, k):
     ref.check(dx, want, ref.U * want.abs() + (1 + ref.U) * off)
 
 
+def test_weight_changed_before_backward(pkg, dev):
+    g = torch.Generator().manual_seed(2)
+    method, layer, w = ref.make_layer(pkg, "mxfp8", [64, 64], 256, dev, g)
+    x = torch.randn(3, 256, generator=g).bfloat16().to(dev).requires_grad_()
+    for loss in (pkg.gated_linear(x, layer).sum(), method.apply(layer, x).sum()):
+        with torch.no_grad():
+            layer.weight[:1].zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
 def test_extremes(pkg, dev):
     """Gates far out: 0 and the gate itself, with finite slopes; a NaN or infinite row stays a row."""
     n, k = 64, 128

@@ -112,18 +112,29 @@ def grad_of(layer: torch.nn.Module) -> tuple:
     return layer.weight, layer.weight_scale, n, k, layer.mxl_format, False
 
 
+def _versions(*tensors: torch.Tensor) -> tuple:
+    return tuple(None if t.is_inference() else t._version for t in tensors)
+
+
+def _check_versions(what: str, versions: tuple, *tensors: torch.Tensor) -> None:
+    if _versions(*tensors) != versions:
+        raise RuntimeError(f"{what} has been modified by an inplace operation between this layer's forward and its backward")
+
+
 class FrozenLinear(torch.autograd.Function):
     """A prepared layer's product (with a bias in its epilogue) with the gradients of its input and the bias."""
 
     @staticmethod
     def forward(ctx, x, bias, layer):
         ctx.layer = grad_of(layer)
+        ctx.versions = _versions(*ctx.layer[:2])
         return layer.mxl_kernel.apply_weights(layer, x, bias)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         w, sw, n, k, fmt, block = ctx.layer
+        _check_versions("the layer's weight", ctx.versions, w, sw)
         dy2 = dy.reshape(-1, n)
         dx = ops.input_grad(dy2, w, sw, n, k, fmt, block).reshape(*dy.shape[:-1], k) if ctx.needs_input_grad[0] else None
         return dx, dy2.sum(0) if ctx.needs_input_grad[1] else None, None
@@ -136,17 +147,20 @@ class AdapterLinear(torch.autograd.Function):
     def forward(ctx, x, a, b, bias, layer, adapters, batch):
         y, v = _forward(layer, x, bias, a, b, adapters.scaling, batch.tensors, adapters.cols)
         ctx.save_for_backward(x, a, b)
-        ctx.held = (v, grad_of(layer), adapters.scaling, adapters.scaling._version, batch, batch.updates, adapters.cols)
+        of = grad_of(layer)
+        ctx.held = v, of, adapters.scaling, batch, batch.updates, adapters.cols
+        ctx.versions = _versions(adapters.scaling, *of[:2])
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, a, b = ctx.saved_tensors
-        v, (w, sw, n, k, fmt, block), scaling, version, batch, updates, cols = ctx.held
-        if batch.updates != updates or scaling._version != version:
-            raise RuntimeError("the batch or the adapters' scaling has been modified by an inplace operation between this "
-                               "layer's forward and its backward")
+        v, (w, sw, n, k, fmt, block), scaling, batch, updates, cols = ctx.held
+        if batch.updates != updates:
+            raise RuntimeError("the batch has been modified by an inplace operation (update) between this layer's forward and "
+                               "its backward")
+        _check_versions("the adapters' scaling or the layer's weight", ctx.versions, scaling, w, sw)
         need_x, need_a, need_b, need_bias = ctx.needs_input_grad[:4]
         dy2 = dy.reshape(-1, n)
         dx, da, db = ops.adapter_grad(dy2, x.reshape(-1, k), w, sw, fmt, block, a, b, scaling, v, *batch.tensors, cols, need_x,
@@ -161,7 +175,7 @@ class GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, *args):
         ctx.save_for_backward(x)
-        ctx.args = args
+        ctx.args, ctx.versions = args, _versions(*args[:2])
         return ops.gated_linear(x.reshape(-1, x.shape[-1]), *args).reshape(*x.shape[:-1], args[2])
 
     @staticmethod
@@ -169,6 +183,7 @@ class GatedLinear(torch.autograd.Function):
     def backward(ctx, dh):
         x, = ctx.saved_tensors
         w, sw, i, fmt, act, rule = ctx.args
+        _check_versions("the layer's weight", ctx.versions, w, sw)
         k = x.shape[-1]
         both = ops.gated_grad(x.reshape(-1, k), dh.reshape(-1, i), w, sw, i, fmt, act, rule)
         return ops.input_grad(both, w, sw, 2 * i, k, fmt).reshape(x.shape), *[None] * 6
@@ -200,7 +215,7 @@ def apply_adapters(layer: torch.nn.Module, x: torch.Tensor, adapters: LowRankAda
     if x.dtype != torch.bfloat16 or x.shape[-1] != k or x.numel() != len(batch) * k:
         raise ValueError(f"adapters need bf16 [..., {k}] of the batch's {len(batch)} rows, got {x.dtype} {tuple(x.shape)}")
     a, b = adapters.lora_a, adapters.lora_b
-    if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, a, b, bias)):
         inner = _function_bias(bias, x, n)
         y = AdapterLinear.apply(x, a, b, inner, layer, adapters, batch)
         return y if bias is inner else y + bias

@@ -1322,6 +1322,8 @@ def adapter_apply(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Te
             call("mxl_adapter_apply", ptr(x), M, K, _row_stride(x), ptr(a), ptr(b), ptr(scaling), slots, parts, c, rank,
                  ptr(order), ptr(offsets), ptr(tiles), tiles.shape[0], ptr(v), v.numel(), ptr(y), _row_stride(y), ptr(ws),
                  nbytes, stream_handle(x.device))
+        if not y.is_inference():
+            torch.autograd.graph.increment_version(y)
     _count("adapter_apply")
     return v
 
