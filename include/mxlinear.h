@@ -598,7 +598,7 @@ int mxl_gated_grad(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, c
  * mxl_adapter_linear: the whole layer -- x quantized by `rule` (block = 1: block-FP8, ldx = K), the
  * product with w_tiled [N, K] of format fmt, bias (or NULL) as the layer adds it -- with the adapters
  * added to the product's fp32 sums, ahead of their rounding; ids i32 [M] as sorted.  Shapes:
- * mxl_adapter_linear_supported (17 rows and more, at least 32 an adapter), else MXL_EUNSUPPORTED.
+ * mxl_adapter_linear_supported (17 rows and more, at least 32 an adapter, up to 16 adapters), else MXL_EUNSUPPORTED.
  *
  * mxl_adapter_grad, with that v: dx = dy W (mxl_input_grad) + a[s]^T (scaling[s] b[s]^T dy[t]) bf16
  * [M, K], da and db bf16 in a's and b's shapes; any of the three may be NULL.  N % 8 == 0.  An adapter

@@ -142,6 +142,7 @@ def test_entry_points_refuse(pkg):
             call("mxl_adapter_linear", *args)
     ok = lambda m, slots: _lib.query("mxl_adapter_linear_supported", m, 128, 128, 0, 0, slots, 1, 8)  # noqa: E731
     assert ok(64, 2) and not ok(16, 1) and not ok(64, 3) and not ok(0, 1)
+    assert ok(512, 16) and not ok(1 << 20, 17)  # (a tile walks its rows' adapters in turn)
     few = _lib.query("mxl_adapter_tile_count", 16, 1)
     with pytest.raises(err, match="one product"):
         call("mxl_adapter_linear", 16, 16, 128, 128, 0, 16, 16, 0, 0, None, 16, 16, 16, 1, 1, _cols(0, 128), 8, 16, 16, 16, 16,

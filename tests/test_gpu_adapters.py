@@ -174,7 +174,7 @@ def test_gradients(pkg, dev, fmt, m, widths, k, slots, rank):
 
 
 @pytest.mark.parametrize("m,widths,slots,rank,runs", [(1300, [256, 256], 1, 16, True), (777, [128, 384, 128], 6, 64, True),
-                                                      (520, [256], 2, 256, False), (40, [128, 128, 128], 2, 104, False)])
+                                                      (700, [256, 128], 20, 24, False), (520, [256], 2, 256, False), (40, [128, 128, 128], 2, 104, False)])
 def test_gradients_of_larger_batches(pkg, dev, m, widths, slots, rank, runs):
     case = _case(pkg, dev, "mxfp8", widths, 384, slots, rank, _ids(m, slots, m, runs), m, True)
     _check_gradients(pkg, "mxfp8", *case)

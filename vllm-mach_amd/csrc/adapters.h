@@ -37,9 +37,13 @@ struct RowAdapters {
   LowRank l{};
 };
 
-// Whether a product adds the adapters of its rows itself: it walks the adapters of a tile's rows one after the other, so
-// that few rows of many adapters are better added by a launch of their own (adapter_expand_kernel).
-inline bool rows_add(int64_t M, int64_t slots) { return M >= 32 * slots; }
+// Whether a product adds the adapters of its rows itself: it walks the adapters of a tile's rows one after the other (some
+// 4 us each on the largest tile, waits for memory), so that few rows an adapter, and rows of many adapters, are better added
+// by a launch of their own (adapter_expand_kernel).  MXFP8 layers with ranks of 16 or (17408 x 5120, 8 adapters) 64, us in
+// one product / apart, tokens in runs of an adapter and, the worst case, mixed at random:
+//   256 x 5120 x 2560, 8 adapters: 23 / 25, mixed 28 / 26       2048 x 17408 x 5120, 8 adapters: 207 / 276, mixed 296 / 288
+//   1024 x 5120 x 2560, 32: 36 / 40, mixed 56 / 42              2048 x 17408 x 5120, 64: 194 / 210, mixed 374 / 215
+inline bool rows_add(int64_t M, int64_t slots) { return slots <= 16 && M >= 32 * slots; }
 
 // dx = dy W (input_grad.hip), with `more` the adapters' dx as well.
 int64_t input_grad_bytes(int64_t M, int64_t N, int64_t K, int block);

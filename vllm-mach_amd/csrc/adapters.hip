@@ -101,8 +101,10 @@ __global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offs
 
 // v[t] (adapters.h) of s sum_k rows[j][k] x[t][k].  BY_PART: part p's rows are [0, r) of the adapter's and its columns
 // [cols[p], cols[p + 1]) (B^T [r, N]); else rows [p r, p r + r) and all columns (A).  A workgroup is a tile of 16 tokens
-// by RC groups of 16 ranks; its waves share the columns and meet in LDS.  Both operands come straight from memory: the
-// rows' A from L2, where its tiles share it, x once.  SHARES: few tiles fill the card by splitting the columns over
+// by RC groups of 16 ranks; its waves share the columns and meet in LDS.  x is read once, the rows' A from L2, where its
+// tiles share it.  Bound: memory (dy 2048 x 18432 to 2 x 16 ranks: 17.5 us, 4.3 TB/s); of many ranks A's loads (4096 x 5120
+// to 64 ranks: 24 us, of which x alone is 8).  Loads by rows of the MFMA's operand put sixteen lines into every sixteen
+// lanes, 64 cycles an instruction: 37.0 and 34 us where the loads are turned in LDS now.  SHARES: few tiles fill the card by splitting the columns over
 // workgroups, whose fp32 sums [blockIdx.z][token][width] the expand kernel joins (48 tokens of 32 adapters, K = 5120, both
 // kernels: 20.0 us whole, 14.3 in shares).
 template <int RC, bool BY_PART, bool SHARES>
@@ -203,7 +205,8 @@ __global__ __launch_bounds__(RC < 4 ? 1024 : 512) void adapter_shrink_kernel(Ada
 // y[t][n] += sum_j mat[n][j] v[t][j], mat [N, ldm] (j < valid) of the tile's adapter, j the ranks of n's part.  A wave is a
 // tile of 16 tokens by 64 columns of one part: MFMA i's row 4 q + e is column 16 q + 4 i + e, so that after the four a
 // lane holds 16 columns of one token side by side (the rows of y in 32-byte pieces; `wide`: they start on 16 bytes).
-// SHARES: v comes as the shrink kernel's shares, and the first columns' workgroup writes it down.
+// SHARES: v comes as the shrink kernel's shares, and the first columns' workgroup writes it down.  Bound: B's bytes and two
+// dependent round trips to memory (48 tokens of 32 adapters, rank 16, N = 17408: 9.0 us, 2.3 TB/s).
 template <bool SHARES>
 __global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterBatch b, LowRank l, uint16_t* v, const float* shares,
                                                              int num_shares, const uint16_t* mat, int64_t slot_stride, int64_t ldm,
@@ -310,7 +313,8 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterBatch b, Low
 
 // sum_t big[t][c] v[t][j] over the adapter's positions of split z: to out [N, r] (OF_B: c a column of dy, j the ranks of
 // its part) or out [R, K] (c a column of x, j all ranks).  A workgroup is 128 columns by RC groups; 32 tokens at a time
-// go through LDS, both operands read from it transposed; the next 32 are on their way.
+// go through LDS, both operands read from it transposed; the next 32 are on their way.  Bound: the big matrix' bytes where
+// the shares fill the card (2048 x 18432 of dy 24.7 us, 3.1 TB/s), else a token tile's latency.
 constexpr int kOuterCols = 128, kOuterStride = kOuterCols + 16, kOuterTokens = 32;
 template <int RC, bool OF_B>
 __global__ __launch_bounds__(256) void adapter_outer_kernel(AdapterBatch b, LowRank l, const uint16_t* big, int64_t ldb,
@@ -469,7 +473,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t tile_count(int64_t M, int64_t slots) { return std::min(M, ceil_div(M, kAdapterTile) + std::min(slots, M)); }
 
 // Groups of 16 ranks a workgroup of shrink takes: up to four, which share the reads of x, once the tiles fill the card
-// without more workgroups; and its waves, over the columns.
+// without more workgroups (4096 x 5120 to 64 ranks: one group 33.0 us, two 25.9, four 24.4).
 int shrink_groups(int64_t tiles, int groups) { return tiles < 256 || groups < 2 ? 1 : groups < 4 ? 2 : 4; }
 
 int check_batch(const char* who, int64_t M, int64_t slots, const int32_t* order, const int64_t* offsets,
@@ -507,7 +511,8 @@ int launched(const char* who) {
   return MXL_EHIP;
 }
 
-// Shares of the columns where the expand kernel follows: until some 256 workgroups run, or a wave has 32 columns.
+// Shares of the columns where the expand kernel follows: until some 256 workgroups run, or a wave has 32 columns.  (48
+// tokens of 32 adapters of rank 16, K = 5120, N = 17408, us of both kernels: one share 20.0, two 15.2, five 14.0.)
 int shrink_shares(int64_t tiles, const LowRank& l, int64_t cols) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({kMaxShares, 256 / (tiles * l.parts * l.groups), cols / 256}));
 }
@@ -548,6 +553,9 @@ int launch_expand(const char* who, const AdapterBatch& b, const LowRank& l, uint
 
 // Shares of an adapter's tokens in the outer products, where columns and groups alone are too few workgroups: some 128
 // tokens each (of adapters with as many), and none while an adapter has fewer than 256: a share costs the join's launch.
+// (2048 tokens of one adapter, rank 16, us with the join: of N = 18432 one share 69.4, four 35.2, here 29.5; of K = 2560
+// 70.3, 26.7, 14.4.  333 tokens of three, N = 5120, K = 2688: one share 10.3 and 10.8, four 9.5 and 8.2 and two launches
+// more, which the host pays for.)
 int outer_splits(int64_t M, int64_t slots, int64_t wgs) {
   const int64_t each = M / slots;
   return each < 256 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({32, ceil_div(768, wgs * slots), each / 128}));

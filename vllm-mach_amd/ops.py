@@ -1334,7 +1334,7 @@ def _(y, x, a, b, scaling, ids, order, offsets, tiles, cols):
 
 
 def adapter_linear_supported(m: int, n: int, k: int, w_fmt: int, block: bool, slots: int, parts: int, rank: int) -> bool:
-    """Shapes whose product adds the adapters itself (``adapter_linear``): from 17 rows, at least 32 an adapter."""
+    """Shapes whose product adds the adapters itself (``adapter_linear``): 17 rows or more, 32 an adapter, up to 16 adapters."""
     return bool(query("mxl_adapter_linear_supported", m, n, k, w_fmt, int(block), slots, parts, rank))
 
 
