@@ -615,7 +615,8 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
     {
       // After the last MFMAs' results: 16 ranks an MFMA, v's halves in its two halves of K, zero in the rows of other
       // adapters than the one at hand (and B in columns of other parts).  Adapters, parts and ranks go one after the
-      // other, the next ranks' operands loaded under the MFMAs.
+      // other; what it costs is the wait for each one's first bytes (some 4 us on a 256 x 256 tile), not the loads: laid out
+      // so that every load met whole lines, 2048 x 18432 x 2560 took 119 us against 112.
       // The arguments are read here (through a pointer that the compiler cannot see through): held in scalar registers
       // over the main loop they would spill.
       typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
