@@ -90,6 +90,18 @@ def test_autograd_of_a_layer(pkg, dev, fmt):
             ref.check(dx.view(-1, 384), *_want(dy.view(-1, 256), w))
 
 
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4", "block"])
+def test_compiled(pkg, dev, fmt):
+    """One graph of a layer whose input takes a gradient."""
+    g = torch.Generator().manual_seed(9)
+    method, layer, w = ref.make_layer(pkg, fmt, [128], 256, dev, g)
+    x = torch.randn(40, 256, generator=g).bfloat16().to(dev).requires_grad_()
+    dy = torch.randn(40, 128, generator=g).bfloat16().to(dev)
+    y, want = torch.compile(lambda t: method.apply(layer, t), fullgraph=True, backend="eager")(x), method.apply(layer, x)
+    assert torch.equal(y, want)
+    assert torch.equal(torch.autograd.grad(y, x, dy)[0], torch.autograd.grad(want, x, dy)[0])
+
+
 def test_gradient_of_an_expanded_output(pkg, dev):
     """A gradient that autograd hands over expanded (of a sum) or transposed."""
     g = torch.Generator().manual_seed(3)

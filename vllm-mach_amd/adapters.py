@@ -112,12 +112,15 @@ def grad_of(layer: torch.nn.Module) -> tuple:
     return layer.weight, layer.weight_scale, n, k, layer.mxl_format, False
 
 
-def _versions(*tensors: torch.Tensor) -> tuple:
-    return tuple(None if t.is_inference() else t._version for t in tensors)
+def _versions(*tensors: torch.Tensor) -> Optional[tuple]:
+    """The tensors' writes so far (inference tensors count none; traced code has no versions)."""
+    if torch.compiler.is_compiling():
+        return None
+    return tuple([None if t.is_inference() else t._version for t in tensors])
 
 
-def _check_versions(what: str, versions: tuple, *tensors: torch.Tensor) -> None:
-    if _versions(*tensors) != versions:
+def _check_versions(what: str, versions: Optional[tuple], *tensors: torch.Tensor) -> None:
+    if versions is not None and _versions(*tensors) != versions:
         raise RuntimeError(f"{what} has been modified by an inplace operation between this layer's forward and its backward")
 
 
