@@ -193,10 +193,11 @@ struct TileLds {
 
 // a_row(row): the activation row of output row `row` (rows past the last: any valid one).
 // ADD (whole K): to the sums of rows with an adapter its low-rank part is added, ahead of any rounding; the kernel's third
-// argument, a RowAdapters behind GemmParams and WideGrid, says what.
+// argument, a RowAdapters behind GemmParams and WideGrid, says what.  Returns whether the wave left out values that are not
+// finite (add_odd adds them).
 constexpr int kAddOffset = (sizeof(GemmParams) + 7) / 8 * 8 + (sizeof(WideGrid) + 7) / 8 * 8;
 template <int FMT, int MTW, int NTW, bool BLOCK, int DEPTH, int EPI = kEpiStore, bool ADD = false, class Row>
-__device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w, uint8_t* lds, Row&& a_row,
+__device__ __forceinline__ bool tile_gemm(const GemmParams& p, const TileWork& w, uint8_t* lds, Row&& a_row,
                                           const TileGate& gate = TileGate()) {
   constexpr bool SWIGLU = EPI == kEpiSwigluFp4, GATED = EPI == kEpiGated || EPI == kEpiGatedGrad;
   static_assert(!GATED || !BLOCK, "gate and up columns have block scales of their own");
@@ -611,6 +612,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
   if (DEPTH > 2 && pr + 1 < last) pair(Slice<4>{}, pr++);
   pair(Slice<2>{}, pr);
 
+  bool odd = false;
   if constexpr (ADD) {
     {
       // After the last MFMAs' results: 16 ranks an MFMA, v's halves in its two halves of K, zero in the rows of other
@@ -693,6 +695,26 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
           const uint32_t m = in && col >= lo && col < hi ? 0xFFFFFFFFu : 0u;
           xb[n] &= u32x4{m, m, m, m};
           asm volatile("" : "+v"(xb[n]));
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < MTW; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = adapter_top(top, xv[i][e]);
+#pragma unroll
+        for (int n = 0; n < NTW; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = adapter_top(top, xb[n][e]);
+        if (__builtin_amdgcn_ballot_w64(adapter_odd(top)) != 0) {
+          odd = true;
+#pragma unroll
+          for (int i = 0; i < MTW; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) xv[i][e] = adapter_finite(xv[i][e]);
+#pragma unroll
+          for (int n = 0; n < NTW; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) xb[n][e] = adapter_finite(xb[n][e]);
         }
         if (++g == groups) {
           g = 0;
@@ -784,7 +806,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    return;
+    return odd;
   }
   if constexpr (GATED) {
     // Lane: four columns of one row of gate and of up, side by side in its registers.  Of two n-tiles every other 16
@@ -857,7 +879,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
     };
     if (gate.act == kActSilu) rows(Slice<kActSilu>{});
     else rows(Slice<kActGeluTanh>{});
-    return;
+    return odd;
   }
   if (w.part) {
 #pragma unroll
@@ -948,7 +970,7 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
       if (p.N % 8 == 0 && p.ldc % 8 == 0 && ((uintptr_t)p.out & 15) == 0) {
         if (p.bias) store(Slice<1>{}, Slice<1>{});
         else store(Slice<0>{}, Slice<1>{});
-        return;
+        return odd;
       }
     }
     if (p.bias) store(Slice<1>{}, Slice<0>{});
@@ -972,6 +994,50 @@ __device__ __forceinline__ void tile_gemm(const GemmParams& p, const TileWork& w
         if (row < w.row_hi && col < p.N) p.out[row * p.ldc + col] = FP4 ? out_bits_fp4(v, p.bias, col) : out_bits(p, v, col);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  }
+  return odd;
+}
+
+// What a wave of an ADD tile left out: the terms with a value of B or v that is not finite, added to its outputs as they are
+// stored (with such a term an output is an infinity or NaN, whatever its rounding).  It reads the kernel's arguments anew:
+// kept in scalar registers over the tile they would spill.
+template <int MTW, int NTW>
+__device__ __forceinline__ void add_odd(int row0, int nb) {
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+  auto at = (const __attribute__((address_space(4))) uint8_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  const auto& p = *(const __attribute__((address_space(4))) GemmParams*)at;
+  const auto& add = *(const __attribute__((address_space(4))) RowAdapters*)(at + kAddOffset);
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rank = add.l.rank, groups = add.l.groups, parts = add.l.parts, width = parts * groups * 16;
+  const int M = (int)p.M, N = (int)p.N;
+  __threadfence();  // the wave's stores, before it loads them
+#pragma unroll 1
+  for (int c = lane; c < 16 * NTW; c += 64) {
+    const int col = nb * (32 * NTW) + (wv & 1) * 16 * NTW + c;
+    if (col >= N) continue;
+    int part = 0;
+    for (int k = 1; k < parts; ++k) part += col >= (int)add.l.cols[k] ? 1 : 0;
+#pragma unroll 1
+    for (int i = 0; i < 16 * MTW; ++i) {
+      const int row = row0 + (wv >> 1) * 16 * MTW + i;
+      if (row >= M) break;
+      const int a = add.ids[row];
+      if ((uint32_t)a >= (uint32_t)add.slots) continue;
+      const uint16_t* const b = add.mat + a * add.slot_stride + (int64_t)col * add.ldm;
+      const uint16_t* const v = add.v + (int64_t)row * (2 * width) + part * groups * 16;
+      float sum = 0.0f;
+      bool odd = false;
+#pragma unroll 2
+      for (int j = 0; j < rank; j += 8) {
+        const u16x8 x = *reinterpret_cast<const u16x8*>(b + j), y = *reinterpret_cast<const u16x8*>(v + j),
+                    z = *reinterpret_cast<const u16x8*>(v + width + j);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += adapter_odd_term(x[e], y[e], z[e], odd);
+      }
+      uint16_t& y = p.out[(int64_t)row * p.ldc + col];
+      if (odd) y = f32_to_bf16(bf16_to_f32(y) + sum);
     }
   }
 }

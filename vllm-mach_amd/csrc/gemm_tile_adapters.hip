@@ -30,15 +30,18 @@ __global__ __launch_bounds__(256, (WidePerCu<MT, NT, false, 2>::value)) void ada
       const int row0 = (int)(mb * BM + (unit & 1) * (BM / 2)), qn = (int)(2 * nb + (unit >> 1 & 1));
       if (row0 >= M || (int64_t)qn * (TW / 2) >= p.N) return;
       const TileWork w{row0, M, qn, 0, KT, p.w, sw, nullptr};
-      tile_gemm<FMT, MTW / 2, NTW / 2, BLOCK, TileDepth<MT, NT>::QUARTER, kEpiStore, true>(p, w, lds, a_row);
+      if (tile_gemm<FMT, MTW / 2, NTW / 2, BLOCK, TileDepth<MT, NT>::QUARTER, kEpiStore, true>(p, w, lds, a_row))
+        add_odd<MTW / 2, NTW / 2>(row0, qn);
       return;
     }
   }
   wide_coords(wide_logical(L, tail0), mblocks, nblocks, group_m, mb, nb);
   const TileWork w{(int)(mb * BM), M, (int)nb, 0, KT, p.w, sw, nullptr};
   using D = TileDepth<MT, NT>;
-  if (D::LONE != D::SHARED && g.depth == D::LONE) tile_gemm<FMT, MTW, NTW, BLOCK, D::LONE, kEpiStore, true>(p, w, lds, a_row);
-  else tile_gemm<FMT, MTW, NTW, BLOCK, D::SHARED, kEpiStore, true>(p, w, lds, a_row);
+  const bool odd = D::LONE != D::SHARED && g.depth == D::LONE
+                       ? tile_gemm<FMT, MTW, NTW, BLOCK, D::LONE, kEpiStore, true>(p, w, lds, a_row)
+                       : tile_gemm<FMT, MTW, NTW, BLOCK, D::SHARED, kEpiStore, true>(p, w, lds, a_row);
+  if (odd) add_odd<MTW, NTW>(w.row0, w.nb);
 }
 
 template <int FMT, bool BLOCK>

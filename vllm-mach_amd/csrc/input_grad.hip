@@ -276,6 +276,7 @@ __global__ __launch_bounds__(256, (TM * TK > 128 * 128 ? 1 : 2)) void input_grad
     }
   }
 
+  bool odd = false;  // the wave left out values that are not finite
   if (p.more.ids && split == 0) {
     // The adapters of the tile's rows, in turn, 16 ranks at a time: A's rows take the place of W's (as they are), dv's
     // halves that of dy, zero in other adapters' rows.
@@ -323,6 +324,12 @@ __global__ __launch_bounds__(256, (TM * TK > 128 * 128 ? 1 : 2)) void input_grad
         });
         meet();
         for_n<2 * KI>([&](auto i) { read(i, std::integral_constant<int, 0>{}, 0); });
+        uint32_t top = 0;
+        for_n<4 * KI>([&](auto i) { top = adapter_top(top, wf[0][i / 4][i / 2 % 2][i % 2]); });
+        if (__builtin_amdgcn_ballot_w64(adapter_odd(top)) != 0) {
+          odd = true;
+          for_n<4 * KI>([&](auto i) { wf[0][i / 4][i / 2 % 2][i % 2] = adapter_finite(wf[0][i / 4][i / 2 % 2][i % 2]); });
+        }
         for_n<2>([&](auto h) {
           for_n<MI * KI>([&](auto i) {
             constexpr int m = decltype(i)::value / KI, c = decltype(i)::value % KI;
@@ -368,6 +375,44 @@ __global__ __launch_bounds__(256, (TM * TK > 128 * 128 ? 1 : 2)) void input_grad
       });
     });
   });
+  if (!odd) return;
+  // The terms left out, with a value of A that is not finite: added to what the wave has stored.
+  const RowAdapters& o = p.more;
+  const int width = o.l.width();
+  __threadfence();  // the wave's stores, before it loads them
+#pragma unroll 1
+  for (int c = lane; c < TK / 2; c += 64) {
+    const int64_t col = (int64_t)kb * TK + wk * (TK / 2) + c;
+    if (col >= p.K) continue;
+    int seen = -1;  // an adapter of which the column's values are known to be finite
+#pragma unroll 1
+    for (int i = 0; i < TM / 2; ++i) {
+      const int64_t row = row0 + wm * (TM / 2) + i;
+      if (row >= p.M) break;
+      const int a = o.ids[row];
+      if ((uint32_t)a >= (uint32_t)o.slots || a == seen) continue;
+      float sum = 0.0f;
+      bool found = false;
+#pragma unroll 1
+      for (int part = 0; part < o.l.parts; ++part) {
+        const uint16_t* const rows = o.mat + a * o.slot_stride + (int64_t)part * o.l.rank * o.ldm + col;
+        const uint16_t* const v = o.v + row * (2 * width) + part * o.l.groups * 16;
+#pragma unroll 8
+        for (int j = 0; j < o.l.rank; ++j) {
+          const uint16_t x = rows[j * o.ldm];
+          if ((x & 0x7FFF) >= 0x7F80) sum += adapter_odd_term(x, v[j], v[width + j], found);
+        }
+      }
+      if (!found) {
+        seen = a;
+      } else if (p.S > 1) {
+        p.partial[row * p.K + col] += sum;
+      } else {
+        uint16_t& y = p.out[row * p.ldo + col];
+        y = f32_to_bf16(bf16_to_f32(y) + sum);
+      }
+    }
+  }
 }
 
 // out = the sum of the splits' partials [S, M, K], rounded; four columns a thread.
