@@ -570,6 +570,10 @@ int64_t mxl_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int bloc
 int mxl_input_grad(const void* dy, int64_t M, int64_t N, int64_t lddy, const void* w_tiled, const void* sw, int64_t K,
                    int fmt, int block, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The bias' gradient, the column sums of dy bf16 [M, N] (row stride lddy) to out bf16 [N]:
+ * fp32 sums in a fixed order, one rounding. */
+int mxl_bias_grad(const void* dy, int64_t M, int64_t N, int64_t lddy, void* out, void* stream);
+
 /* act(x Wg^T) * (x Wu^T) of a tiled MX weight [2 I, K], gate rows then up rows: x bf16 [M, K] (row
  * stride ldx) quantized by `rule` (MXFP8; of fmt 4 MXFP4), fp32 products, one rounding to out bf16
  * [M, I] (row stride ldo).  act 0 = silu, 1 = gelu (tanh form).  mxl_gated_grad: from dh bf16 [M, I]

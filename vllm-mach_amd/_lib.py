@@ -59,6 +59,7 @@ SIGNATURES = {
                               _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P]),
     "mxl_input_grad_workspace_bytes": (_I64, [_I64, _I64, _I64, _I]),
     "mxl_input_grad": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I, _I, _P, _I64, _P, _I64, _P]),
+    "mxl_bias_grad": (_I, [_P, _I64, _I64, _I64, _P, _P]),
     "mxl_gated_workspace_bytes": (_I64, [_I64, _I64, _I]),
     "mxl_gated_linear": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _I64, _I, _I, _P, _I64, _P, _I64, _P]),
     "mxl_gated_grad": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _I64, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P]),

@@ -140,7 +140,7 @@ class FrozenLinear(torch.autograd.Function):
         _check_versions("the layer's weight", ctx.versions, w, sw)
         dy2 = dy.reshape(-1, n)
         dx = ops.input_grad(dy2, w, sw, n, k, fmt, block).reshape(*dy.shape[:-1], k) if ctx.needs_input_grad[0] else None
-        return dx, dy2.sum(0) if ctx.needs_input_grad[1] else None, None
+        return dx, ops.bias_grad(dy2) if ctx.needs_input_grad[1] else None, None
 
 
 class AdapterLinear(torch.autograd.Function):
@@ -169,7 +169,7 @@ class AdapterLinear(torch.autograd.Function):
         dx, da, db = ops.adapter_grad(dy2, x.reshape(-1, k), w, sw, fmt, block, a, b, scaling, v, *batch.tensors, cols, need_x,
                                       need_a, need_b)
         return (dx.reshape(x.shape) if need_x else None, da if need_a else None, db if need_b else None,
-                dy2.sum(0) if need_bias else None, None, None, None)
+                ops.bias_grad(dy2) if need_bias else None, None, None, None)
 
 
 class GatedLinear(torch.autograd.Function):

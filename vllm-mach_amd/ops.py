@@ -1178,6 +1178,27 @@ def _(dy, w, sw, n, k, w_fmt, block=False):
     return dy.new_empty((dy.shape[0], k), dtype=torch.bfloat16)
 
 
+@_operator("bias_grad")
+def bias_grad(dy: torch.Tensor) -> torch.Tensor:
+    """The gradient of a layer's bias, the column sums of dy bf16 [M, N]: bf16 [N], fp32 sums in a fixed order, one rounding.
+    One launch without scratch, so a backward with it may be captured."""
+    _check_cuda(dy)
+    if dy.ndim != 2 or dy.shape[1] == 0 or dy.dtype != torch.bfloat16:
+        raise ValueError(f"bias_grad needs bf16 [M, N], N > 0, got {dy.dtype} {tuple(dy.shape)}")
+    if (dy.stride(1) != 1 and dy.shape[1] > 1) or _row_stride(dy) < dy.shape[1]:
+        dy = dy.contiguous()
+    out = dy.new_empty(dy.shape[1])
+    with _on(dy.device):
+        call("mxl_bias_grad", ptr(dy), dy.shape[0], dy.shape[1], _row_stride(dy), ptr(out), stream_handle(dy.device))
+    _count("bias_grad")
+    return out
+
+
+@bias_grad.register_fake
+def _(dy):
+    return dy.new_empty(dy.shape[1])
+
+
 def _gated(what: str, x: torch.Tensor, w, sw, i: int, fmt: int, act: int, rule: int, dh: Optional[torch.Tensor]):
     _same_device(what, x, w, sw, dh)
     if x.ndim != 2:
