@@ -5,7 +5,7 @@ import torch
 
 def test_bias_grad_refuses(pkg):
     from vllm_mach_amd import _lib
-    for args, match in (((2, 4, 0, 8, 2, None), "N > 0"), ((2, -1, 8, 8, 2, None), "M >= 0"), ((2, 4, 8, 7, 2, None), "lddy"),
+    for args, match in (((2, 4, 0, 8, 2, None), "0 < N"), ((2, -1, 8, 8, 2, None), "M >= 0"), ((2, 4, 8, 7, 2, None), "lddy"),
                         ((3, 4, 8, 8, 2, None), "lddy")):
         with pytest.raises(_lib.MxlError, match=match):
             _lib.call("mxl_bias_grad", *args)
