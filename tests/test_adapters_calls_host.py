@@ -17,3 +17,14 @@ def test_bias_grad_shape(pkg):
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():
         assert torch.ops.mach_amd.bias_grad(torch.empty(5, 24, dtype=torch.bfloat16)).shape == (24,)
+
+
+def test_gated_refuses_two_limbs(pkg):
+    layer = torch.nn.Module()
+    layer.mxl_shape, layer.mxl_format, layer.mxl_kernel = (128, 256), 0, pkg.Mxfp8LinearKernel(dual_m=(2, 32))
+    layer.weight = layer.weight_scale = torch.zeros(1)
+    for shape in ((2, 256), (4, 8, 256)):
+        with pytest.raises(ValueError, match="one limb"):
+            pkg.gated_linear(torch.zeros(*shape).bfloat16(), layer)
+    with pytest.raises(ValueError, match="HIP device"):
+        pkg.gated_linear(torch.zeros(3, 256).bfloat16(), layer)

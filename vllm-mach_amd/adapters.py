@@ -197,7 +197,8 @@ def _forward(layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tenso
     w, sw, n, k, fmt, block = grad_of(layer)
     x2 = x.reshape(-1, k)
     inner = _epilogue_bias(bias, x, n)
-    if bias is inner and ops.adapter_linear_supported(x2.shape[0], n, k, fmt, block, a.shape[0], len(cols) - 1, b.shape[2]):
+    two_limbs = x2.shape[0] in getattr(layer.mxl_kernel, "dual_m", ())  # (the product with adapters has one)
+    if bias is inner and not two_limbs and ops.adapter_linear_supported(x2.shape[0], n, k, fmt, block, a.shape[0], len(cols) - 1, b.shape[2]):
         y, v = ops.adapter_linear(x2, w, sw, fmt, block, getattr(layer.mxl_kernel, "act_rule", 0), inner, a, b, scaling, *batch,
                                   cols)
         return y.reshape(*x.shape[:-1], n), v

@@ -446,7 +446,8 @@ ACTIVATIONS = {"silu": ops.SILU, "gelu_tanh": ops.GELU_TANH}
 def gated_linear(x: torch.Tensor, layer: torch.nn.Module, activation: str = "silu") -> torch.Tensor:
     """act(x Wg^T) * (x Wu^T) for a merged gate/up layer (gate rows, then up rows) prepared by one of the MX kernels: x bf16
     [..., K] -> bf16 [..., I], gate and up in fp32 up to one rounding (the two-launch path, the layer and then the SwiGLU
-    producer, rounds each to bf16).  ``activation``: ``"silu"`` or ``"gelu_tanh"``.  Differentiable in x."""
+    producer, rounds each to bf16).  ``activation``: ``"silu"`` or ``"gelu_tanh"``.  Differentiable in x.  x is quantized to one
+    limb: row counts that the layer's kernel serves with two (``dual_m``) are refused."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(ACTIVATIONS)}")
     if not hasattr(layer, "mxl_shape") or not hasattr(layer, "mxl_format"):
@@ -457,6 +458,10 @@ def gated_linear(x: torch.Tensor, layer: torch.nn.Module, activation: str = "sil
         raise ValueError(f"gated_linear needs gate and up of the same multiple of 16 columns (N={n}, parts {widths})")
     if x.dtype != torch.bfloat16 or x.shape[-1] != k:
         raise ValueError("gated_linear requires BF16 activations with matching K")
+    dual_m = getattr(layer.mxl_kernel, "dual_m", ())
+    if dual_m and x.numel() // k in dual_m:
+        raise ValueError(f"gated_linear quantizes x to one limb, but the layer's kernel serves {x.numel() // k} rows with two "
+                         "(dual_m): apply the layer, then the activation")
     args = (layer.weight, layer.weight_scale, n // 2, layer.mxl_format, ACTIVATIONS[activation], layer.mxl_kernel.act_rule)
     if x.requires_grad and torch.is_grad_enabled():
         from .adapters import GatedLinear

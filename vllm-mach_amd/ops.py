@@ -1233,7 +1233,7 @@ def _gated(what: str, x: torch.Tensor, w, sw, i: int, fmt: int, act: int, rule: 
 def gated_linear(x: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, i: int, w_fmt: int, act: int = SILU,
                  rule: int = FLOOR_CARRY175) -> torch.Tensor:
     """act(x Wg^T) * (x Wu^T) of an MX weight [2 I, K] (gate rows, then up rows; tiled layout): bf16 [M, K] quantized as
-    the layer's product does it (MXFP8, of E2M1 weights MXFP4), both products in fp32, one rounding to bf16 [M, I].
+    the layer's one-limb product does it (MXFP8, of E2M1 weights MXFP4), both products in fp32, one rounding to bf16 [M, I].
     ``act``: ``SILU`` or ``GELU_TANH``.  The product is one launch, behind the quantizer's."""
     return _gated("gated_linear", x, w, sw, i, w_fmt, act, rule, None)
 
