@@ -28,3 +28,47 @@ def test_gated_refuses_two_limbs(pkg):
             pkg.gated_linear(torch.zeros(*shape).bfloat16(), layer)
     with pytest.raises(ValueError, match="HIP device"):
         pkg.gated_linear(torch.zeros(3, 256).bfloat16(), layer)
+
+
+def test_supported_shapes_agree(pkg):
+    """The Python rule is the library's, also next to its borders."""
+    from vllm_mach_amd import _lib
+    ask = lambda *a: bool(_lib.query("mxl_adapter_linear_supported", *a))  # noqa: E731
+    rows = [0, 1, 16, 17, 31, 32, 63, 64, 511, 512, 513, 4096, 1 << 20, (1 << 22) - 1, 1 << 22, 1 << 25]
+    for m in rows:
+        for n, k in ((128, 128), (17408, 5120), (0, 128), (128, 100), (128, 32768), (128, 32896), (1 << 22, 128), (128, 1 << 12)):
+            for fmt, block in ((0, 0), (0, 1), (4, 0), (4, 1)):
+                for slots, parts, rank in ((1, 1, 8), (2, 8, 256), (16, 1, 24), (17, 1, 8), (0, 1, 8)):
+                    args = (m, n, k, fmt, block, slots, parts, rank)
+                    assert pkg.ops.adapter_linear_supported(*args) == ask(*args), args
+    assert pkg.ops.adapter_linear_supported(64, 128, 128, 0, False, 2, 1, 8)
+
+
+@pytest.mark.parametrize("m,slots", [(200, 1), (200, 30), (7, 1), (1, 2)])
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_layer_with_adapters_traces(pkg, m, slots, grad):
+    """One graph, without running it."""
+    from vllm_mach_amd import _lib
+    n, k = 128, 256
+    layer = torch.nn.Module()
+    layer.mxl_shape, layer.mxl_format, layer.mxl_kernel = (n, k), 0, pkg.Mxfp8LinearKernel()
+    layer.weight = torch.nn.Parameter(torch.zeros(8 * 8192, dtype=torch.uint8), requires_grad=False)
+    layer.weight_scale = torch.nn.Parameter(torch.zeros(8 * 256, dtype=torch.uint8), requires_grad=False)
+    ad = pkg.LowRankAdapters(layer, slots, 8).requires_grad_(grad)
+    batch = object.__new__(pkg.AdapterBatch)
+    batch.slots, batch.updates = slots, 0
+    tiles = _lib.query("mxl_adapter_tile_count", m, slots)
+    batch.tensors = (torch.zeros(m, dtype=torch.int32), torch.zeros(m, dtype=torch.int32),
+                     torch.zeros(slots + 1, dtype=torch.int64), torch.zeros(tiles, 4, dtype=torch.int32))
+    graphs = []
+
+    def backend(gm, example_inputs):
+        graphs.append(gm)
+        return lambda *args: (torch.zeros(m, n),)
+
+    torch._dynamo.reset()
+    method = pkg.MxLinearMethod()
+    call = torch.compile(lambda x: method.apply(layer, x, None, adapters=ad, batch=batch), fullgraph=True, backend=backend)
+    assert call(torch.zeros(m, k).bfloat16()).shape == (m, n) and len(graphs) == 1
+    text = graphs[0].print_readable(print_output=False)
+    assert ("adapter_linear" if m == 200 and slots == 1 else "adapter_apply") in text and ("adapter_grad" in text) == grad

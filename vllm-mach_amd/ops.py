@@ -473,6 +473,11 @@ def _(a, sa, w, sw, n, k, w_fmt, bias=None):
     return a.new_empty((a.shape[0], n), dtype=torch.bfloat16)
 
 
+@torch.compiler.assume_constant_result  # (tracing evaluates it)
+def _producer_supported(kind: int, m: int, k: int, rule: int, w_fmt: int) -> bool:
+    return bool(query("mxl_producer_gemm_supported", kind, m, k, rule, w_fmt))
+
+
 def swiglu_row_fusable(m: int, k: int, rule: int, w_fmt: int = E4M3) -> bool:
     """Shapes ``mxl_swiglu_mx_gemm`` runs in one launch (M <= 16 rows; rules ceil_div448 and
     rp_ue8m0; the weight-streaming GEMM's K range, see ``mxl_producer_gemm_supported``)."""
@@ -489,7 +494,7 @@ def quant_rows_inreg(m: int, k: int, rule: int, w_fmt: int = E4M3) -> bool:
     """Shapes whose MXFP8 quantization ``mxl_quant_mx_gemm`` runs inside the GEMM's own
     wavefronts (one row; or up to 16 rows at K <= 6144), the one-launch scheme that measured
     faster than the quantizer and GEMM as two launches."""
-    return 1 <= m <= 16 and bool(query("mxl_producer_gemm_supported", 3, m, k, rule, w_fmt))
+    return 1 <= m <= 16 and _producer_supported(3, m, k, rule, w_fmt)
 
 
 def block_row_fusable(m: int, k: int) -> bool:
@@ -501,7 +506,7 @@ def block_row_inreg(m: int, k: int) -> bool:
     """Shapes whose block-FP8 quantization ``mxl_block_fp8_quant_gemm`` runs inside the
     GEMM's own wavefronts (one row), the one-launch scheme that measured faster than the
     quantizer and GEMM as two launches."""
-    return m == 1 and bool(query("mxl_producer_gemm_supported", 4, m, k, 0, E4M3))
+    return m == 1 and _producer_supported(4, m, k, 0, E4M3)
 
 
 @torch.library.custom_op("mach_amd::quant_mx_gemm", mutates_args=())
@@ -1354,9 +1359,16 @@ def _(y, x, a, b, scaling, ids, order, offsets, tiles, cols):
     return x.new_empty(_v_shape(x.shape[0], len(cols) - 1, b.shape[2]))
 
 
+_BLOCK_STAGES = 256  # 128-column scales of a block-FP8 tile (kWideBlockStages)
+
+
 def adapter_linear_supported(m: int, n: int, k: int, w_fmt: int, block: bool, slots: int, parts: int, rank: int) -> bool:
-    """Shapes whose product adds the adapters itself (``adapter_linear``): 17 rows or more, 32 an adapter, up to 16 adapters."""
-    return bool(query("mxl_adapter_linear_supported", m, n, k, w_fmt, int(block), slots, parts, rank))
+    """Shapes whose product adds the adapters itself (``adapter_linear``): 17 rows or more, 32 an adapter, up to 16 adapters,
+    and offsets of 32 bits.  ``mxl_adapter_linear_supported``, in Python for tracing to see through."""
+    return (m >= 17 and n > 0 and k > 0 and k % 128 == 0 and 0 < slots <= 16 and m >= 32 * slots and parts > 0 and rank > 0
+            and not (block and w_fmt == E2M1) and m * k < 1 << 32 and ((n + 15) // 16) * ((k + 511) // 512) < 1 << 24
+            and (not block or k <= 128 * _BLOCK_STAGES) and m <= (1 << 32) // (64 * parts * ((rank + 15) // 16))
+            and n <= (1 << 31) // (2 * rank))
 
 
 @_operator("adapter_linear")
