@@ -193,13 +193,13 @@ class GatedLinear(torch.autograd.Function):
 
 
 def _forward(layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor], a, b, scaling, batch, cols):
-    """(y, v): in one product where the shape has it, else the layer and then the adapters in place."""
+    """(y, v): in one product where the shape has it, else the layer and then the adapters in place.  ``bias``: one that the
+    product's epilogue adds, or None."""
     w, sw, n, k, fmt, block = grad_of(layer)
     x2 = x.reshape(-1, k)
-    inner = _epilogue_bias(bias, x, n)
     two_limbs = x2.shape[0] in getattr(layer.mxl_kernel, "dual_m", ())  # (the product with adapters has one)
-    if bias is inner and not two_limbs and ops.adapter_linear_supported(x2.shape[0], n, k, fmt, block, a.shape[0], len(cols) - 1, b.shape[2]):
-        y, v = ops.adapter_linear(x2, w, sw, fmt, block, getattr(layer.mxl_kernel, "act_rule", 0), inner, a, b, scaling, *batch,
+    if not two_limbs and ops.adapter_linear_supported(x2.shape[0], n, k, fmt, block, a.shape[0], len(cols) - 1, b.shape[2]):
+        y, v = ops.adapter_linear(x2, w, sw, fmt, block, getattr(layer.mxl_kernel, "act_rule", 0), bias, a, b, scaling, *batch,
                                   cols)
         return y.reshape(*x.shape[:-1], n), v
     y = layer.mxl_kernel.apply_weights(layer, x, bias)
@@ -223,4 +223,6 @@ def apply_adapters(layer: torch.nn.Module, x: torch.Tensor, adapters: LowRankAda
         inner = _function_bias(bias, x, n)
         y = AdapterLinear.apply(x, a, b, inner, layer, adapters, batch)
         return y if bias is inner else y + bias
-    return _forward(layer, x, bias, a, b, adapters.scaling, batch.tensors, adapters.cols)[0]
+    inner = _epilogue_bias(bias, x, n)  # (any other joins the output, as a layer without adapters has it)
+    y = _forward(layer, x, inner, a, b, adapters.scaling, batch.tensors, adapters.cols)[0]
+    return y if bias is inner else y + bias
