@@ -1417,13 +1417,15 @@ def adapter_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, sw: torch.T
     _same_device("adapter_grad", x, dy, w, sw, v)
     (M, K), slots, N = x.shape, a.shape[0], cols[-1]
     w, sw = _tiled_weight("adapter_grad", w, sw, N, K, w_fmt, block)
-    if N % 8:
-        raise ValueError(f"adapter_grad needs N % 8 == 0 (N={N})")
     if dy.shape[0] != M:
         raise ValueError(f"adapter_grad: dy has {dy.shape[0]} rows, x {M}")
     dy = _bf16_rows("adapter_grad", dy, N, "dy")
     if v.dtype != torch.bfloat16 or not v.is_contiguous() or tuple(v.shape) != _v_shape(M, parts, rank):
         raise ValueError("adapter_grad: v is not adapter_apply's of these operands")
+    pad = -N % 8
+    if pad:  # (block-FP8 layers of odd widths: the kernels read eight columns at a time; W's rows past N are zeros)
+        dy, b = torch.nn.functional.pad(dy, (0, pad)), torch.nn.functional.pad(b, (0, 0, 0, pad))
+        c[len(cols) - 1] = N + pad
     make = torch.Tensor.new_empty if M else torch.Tensor.new_zeros
     dx = x.new_empty((M, K) if need_x else (0,))
     da = make(a, a.shape if need_a else (0,))
@@ -1437,7 +1439,7 @@ def adapter_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, sw: torch.T
                  tiles.shape[0], ptr(v), v.numel(), ptr(dx) if need_x else None, K, ptr(da) if need_a else None,
                  ptr(db) if need_b else None, ptr(ws), nbytes, stream_handle(x.device))
     _count("adapter_grad")
-    return dx, da, db
+    return dx, da, db[:, :N].contiguous() if pad and need_b else db
 
 
 @adapter_grad.register_fake
