@@ -1154,6 +1154,12 @@ def _bf16_rows(what: str, x: torch.Tensor, k: int, name: str = "x") -> torch.Ten
     return _rows16(x)
 
 
+def _grad_rows(what: str, dy: torch.Tensor, n: int) -> torch.Tensor:
+    """dy as the input gradient's kernel reads it, rows up to 2^22 values apart (32-bit offsets within a tile)."""
+    dy = _bf16_rows(what, dy, n, "dy")
+    return dy.contiguous() if _row_stride(dy) > 1 << 22 else dy
+
+
 @_operator("input_grad")
 def input_grad(dy: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, k: int, w_fmt: int,
                block: bool = False) -> torch.Tensor:
@@ -1163,7 +1169,7 @@ def input_grad(dy: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, n: int, k: i
     as the identity."""
     _same_device("input_grad", dy, w, sw)
     w, sw = _tiled_weight("input_grad", w, sw, n, k, w_fmt, block)
-    dy = _bf16_rows("input_grad", dy, n, "dy")
+    dy = _grad_rows("input_grad", dy, n)
     if n % 8:  # (block-FP8 layers of odd widths: the kernel reads eight columns at a time; W's rows past N are zeros)
         dy = torch.nn.functional.pad(dy, (0, 8 - n % 8))
     M = dy.shape[0]
@@ -1419,7 +1425,7 @@ def adapter_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, sw: torch.T
     w, sw = _tiled_weight("adapter_grad", w, sw, N, K, w_fmt, block)
     if dy.shape[0] != M:
         raise ValueError(f"adapter_grad: dy has {dy.shape[0]} rows, x {M}")
-    dy = _bf16_rows("adapter_grad", dy, N, "dy")
+    dy = _grad_rows("adapter_grad", dy, N)
     if v.dtype != torch.bfloat16 or not v.is_contiguous() or tuple(v.shape) != _v_shape(M, parts, rank):
         raise ValueError("adapter_grad: v is not adapter_apply's of these operands")
     pad = -N % 8
