@@ -149,17 +149,17 @@ class AdapterLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, a, b, bias, layer, adapters, batch):
         y, v = _forward(layer, x, bias, a, b, adapters.scaling, batch.tensors, adapters.cols)
-        ctx.save_for_backward(x, a, b)
+        ctx.save_for_backward(x, a, b, v)
         of = grad_of(layer)
-        ctx.held = v, of, adapters.scaling, batch, batch.updates, adapters.cols
+        ctx.held = of, adapters.scaling, batch, batch.updates, adapters.cols
         ctx.versions = _versions(adapters.scaling, *of[:2])
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, a, b = ctx.saved_tensors
-        v, (w, sw, n, k, fmt, block), scaling, batch, updates, cols = ctx.held
+        x, a, b, v = ctx.saved_tensors
+        (w, sw, n, k, fmt, block), scaling, batch, updates, cols = ctx.held
         if batch.updates != updates:
             raise RuntimeError("the batch has been modified by an inplace operation (update) between this layer's forward and "
                                "its backward")
