@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import ops
-from .linear import _epilogue_bias, _function_bias
+from .linear import _epilogue_bias, _function_bias, _gated_args
 
 
 class AdapterBatch:
@@ -124,14 +124,33 @@ def _check_versions(what: str, versions: Optional[tuple], *tensors: torch.Tensor
         raise RuntimeError(f"{what} has been modified by an inplace operation between this layer's forward and its backward")
 
 
+# Each of the functions below has a second form whose context is set up apart, which torch.func's transforms ask for and which
+# costs a call some 50 us: ``_apply`` takes it under a transform.
+
+def _saved(ctx):
+    if torch.compiler.is_compiling():
+        return ctx.saved_tensors
+    return [torch._C._functorch.unwrap_if_dead(t) for t in ctx.saved_tensors]  # (of a transform that has ended)
+
+
+def _apply(function, *args):
+    if not torch.compiler.is_compiling() and torch._C._functorch.peek_interpreter_stack() is not None:
+        return function.transformed.apply(*args)
+    return function.apply(*args)
+
+
 class FrozenLinear(torch.autograd.Function):
     """A prepared layer's product (with a bias in its epilogue) with the gradients of its input and the bias."""
 
     @staticmethod
     def forward(ctx, x, bias, layer):
+        FrozenLinear.hold(ctx, layer)
+        return layer.mxl_kernel.apply_weights(layer, x, bias)
+
+    @staticmethod
+    def hold(ctx, layer):
         ctx.layer = grad_of(layer)
         ctx.versions = _versions(*ctx.layer[:2])
-        return layer.mxl_kernel.apply_weights(layer, x, bias)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -143,22 +162,47 @@ class FrozenLinear(torch.autograd.Function):
         return dx, ops.bias_grad(dy2) if ctx.needs_input_grad[1] else None, None
 
 
+class _FrozenLinear(torch.autograd.Function):
+    """``FrozenLinear`` under torch.func's transforms; a batch of inputs is so many rows more."""
+
+    @staticmethod
+    def forward(x, bias, layer):
+        return layer.mxl_kernel.apply_weights(layer, x, bias)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        FrozenLinear.hold(ctx, inputs[2])
+
+    @staticmethod
+    def vmap(info, in_dims, x, bias, layer):
+        return _FrozenLinear.apply(x.movedim(in_dims[0], 0), bias, layer), 0
+
+    backward = FrozenLinear.backward
+
+
+FrozenLinear.transformed = _FrozenLinear
+
+
 class AdapterLinear(torch.autograd.Function):
     """A prepared layer with its adapters: the gradients of the input, the adapters and a bias in the epilogue."""
 
     @staticmethod
     def forward(ctx, x, a, b, bias, layer, adapters, batch):
         y, v = _forward(layer, x, bias, a, b, adapters.scaling, batch.tensors, adapters.cols)
+        AdapterLinear.hold(ctx, x, a, b, v, layer, adapters, batch)
+        return y
+
+    @staticmethod
+    def hold(ctx, x, a, b, v, layer, adapters, batch):
         ctx.save_for_backward(x, a, b, v)
         of = grad_of(layer)
         ctx.held = of, adapters.scaling, batch, batch.updates, adapters.cols
         ctx.versions = _versions(adapters.scaling, *of[:2])
-        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, a, b, v = ctx.saved_tensors
+    def backward(ctx, dy, *_):
+        x, a, b, v = _saved(ctx)
         (w, sw, n, k, fmt, block), scaling, batch, updates, cols = ctx.held
         if batch.updates != updates:
             raise RuntimeError("the batch has been modified by an inplace operation (update) between this layer's forward and "
@@ -172,24 +216,74 @@ class AdapterLinear(torch.autograd.Function):
                 ops.bias_grad(dy2) if need_bias else None, None, None, None)
 
 
+class _AdapterLinear(torch.autograd.Function):
+    """``AdapterLinear`` under torch.func's transforms -> (y, v): a context set up apart keeps inputs and outputs only."""
+
+    @staticmethod
+    def forward(x, a, b, bias, layer, adapters, batch):
+        return _forward(layer, x, bias, a, b, adapters.scaling, batch.tensors, adapters.cols)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, a, b, _, layer, adapters, batch = inputs
+        ctx.mark_non_differentiable(output[1])
+        AdapterLinear.hold(ctx, x, a, b, output[1], layer, adapters, batch)
+
+    backward = AdapterLinear.backward
+
+
+AdapterLinear.transformed = _AdapterLinear
+
+
 class GatedLinear(torch.autograd.Function):
     """``ops.gated_linear`` with the gradient of its input."""
 
     @staticmethod
-    def forward(ctx, x, *args):
-        ctx.save_for_backward(x)
-        ctx.args, ctx.versions = args, _versions(*args[:2])
+    def forward(ctx, x, layer, act):
+        GatedLinear.hold(ctx, x, layer, act)
+        return GatedLinear.product(x, layer, act)
+
+    @staticmethod
+    def product(x, layer, act):
+        args = _gated_args(layer, act)
         return ops.gated_linear(x.reshape(-1, x.shape[-1]), *args).reshape(*x.shape[:-1], args[2])
+
+    @staticmethod
+    def hold(ctx, x, layer, act):
+        ctx.save_for_backward(x)
+        ctx.args = _gated_args(layer, act)
+        ctx.versions = _versions(*ctx.args[:2])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        x, = ctx.saved_tensors
+        x, = _saved(ctx)
         w, sw, i, fmt, act, rule = ctx.args
         _check_versions("the layer's weight", ctx.versions, w, sw)
         k = x.shape[-1]
         both = ops.gated_grad(x.reshape(-1, k), dh.reshape(-1, i), w, sw, i, fmt, act, rule)
-        return ops.input_grad(both, w, sw, 2 * i, k, fmt).reshape(x.shape), *[None] * 6
+        return ops.input_grad(both, w, sw, 2 * i, k, fmt).reshape(x.shape), None, None
+
+
+class _GatedLinear(torch.autograd.Function):
+    """``GatedLinear`` under torch.func's transforms."""
+
+    @staticmethod
+    def forward(x, layer, act):
+        return GatedLinear.product(x, layer, act)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        GatedLinear.hold(ctx, *inputs)
+
+    @staticmethod
+    def vmap(info, in_dims, x, layer, act):
+        return _GatedLinear.apply(x.movedim(in_dims[0], 0), layer, act), 0
+
+    backward = GatedLinear.backward
+
+
+GatedLinear.transformed = _GatedLinear
 
 
 def _forward(layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor], a, b, scaling, batch, cols):
@@ -221,7 +315,8 @@ def apply_adapters(layer: torch.nn.Module, x: torch.Tensor, adapters: LowRankAda
     a, b = adapters.lora_a, adapters.lora_b
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, a, b, bias)):
         inner = _function_bias(bias, x, n)
-        y = AdapterLinear.apply(x, a, b, inner, layer, adapters, batch)
+        y = _apply(AdapterLinear, x, a, b, inner, layer, adapters, batch)
+        y = y[0] if isinstance(y, tuple) else y
         return y if bias is inner else y + bias
     inner = _epilogue_bias(bias, x, n)  # (any other joins the output, as a layer without adapters has it)
     y = _forward(layer, x, inner, a, b, adapters.scaling, batch.tensors, adapters.cols)[0]

@@ -188,9 +188,9 @@ def _function_bias(bias: Optional[torch.Tensor], x: torch.Tensor, n: int) -> Opt
 def _with_input_grad(layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
     """The layer's output as a function of x that autograd can walk back through: the weight is frozen, the dynamic
     quantization counts as the identity (``ops.input_grad``)."""
-    from .adapters import FrozenLinear
+    from .adapters import FrozenLinear, _apply
     inner = _function_bias(bias, x, layer.mxl_shape[0])
-    y = FrozenLinear.apply(x, inner, layer)
+    y = _apply(FrozenLinear, x, inner, layer)
     return y if bias is inner else y + bias
 
 
@@ -443,6 +443,11 @@ class MxLinearMethod:
 ACTIVATIONS = {"silu": ops.SILU, "gelu_tanh": ops.GELU_TANH}
 
 
+def _gated_args(layer: torch.nn.Module, act: int) -> tuple:
+    """What ``ops.gated_linear`` takes of a prepared layer: (w, sw, I, format, activation, rule)."""
+    return layer.weight, layer.weight_scale, layer.mxl_shape[0] // 2, layer.mxl_format, act, layer.mxl_kernel.act_rule
+
+
 def gated_linear(x: torch.Tensor, layer: torch.nn.Module, activation: str = "silu") -> torch.Tensor:
     """act(x Wg^T) * (x Wu^T) for a merged gate/up layer (gate rows, then up rows) prepared by one of the MX kernels: x bf16
     [..., K] -> bf16 [..., I], gate and up in fp32 up to one rounding (the two-launch path, the layer and then the SwiGLU
@@ -462,12 +467,11 @@ def gated_linear(x: torch.Tensor, layer: torch.nn.Module, activation: str = "sil
     if dual_m and x.numel() // k in dual_m:
         raise ValueError(f"gated_linear quantizes x to one limb, but the layer's kernel serves {x.numel() // k} rows with two "
                          "(dual_m): apply the layer, then the activation")
-    args = (layer.weight, layer.weight_scale, n // 2, layer.mxl_format, ACTIVATIONS[activation], layer.mxl_kernel.act_rule)
     if x.requires_grad and torch.is_grad_enabled():
-        from .adapters import GatedLinear
-        return GatedLinear.apply(x, *args)
+        from .adapters import GatedLinear, _apply
+        return _apply(GatedLinear, x, layer, ACTIVATIONS[activation])
     rows = x.ndim == 2
-    y = ops.gated_linear(x if rows else _flatten(x, k), *args)
+    y = ops.gated_linear(x if rows else _flatten(x, k), *_gated_args(layer, ACTIVATIONS[activation]))
     return y if rows else y.reshape(*x.shape[:-1], n // 2)
 
 
