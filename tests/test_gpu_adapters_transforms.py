@@ -79,3 +79,19 @@ def test_adapters(pkg, dev, m):
     values = {name: p.detach() for name, p in block.named_parameters()}
     got = torch.func.grad(lambda v: (torch.func.functional_call(block, v, (x.detach(),)).float() * dy.float()).sum())(values)
     assert torch.equal(got["adapters.lora_a"], want[1]) and torch.equal(got["adapters.lora_b"], want[2])
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("fmt", ref.FORMATS)
+@pytest.mark.parametrize("m", [1, 40])
+def test_recorded_layers_save(pkg, dev, fmt, m):
+    """A layer recorded with an input that takes a gradient holds operators only, as one without does."""
+    import io
+    g = torch.Generator().manual_seed(m)
+    method, layer, _ = ref.make_layer(pkg, fmt, [128], 256, dev, g)
+    x = torch.randn(m, 256, generator=g).bfloat16().to(dev)
+    want, file = method.apply(layer, x), io.BytesIO()
+    torch.jit.save(torch.jit.trace(lambda t: method.apply(layer, t), x.clone().requires_grad_(), check_trace=False), file)
+    file.seek(0)
+    with torch.no_grad():
+        assert torch.equal(torch.jit.load(file)(x), want)
