@@ -72,3 +72,29 @@ def test_a_layer_with_adapters_traces(pkg, m, slots, grad):
     assert call(torch.zeros(m, k).bfloat16()).shape == (m, n) and len(graphs) == 1
     text = graphs[0].print_readable(print_output=False)
     assert ("adapter_linear" if m == 200 and slots == 1 else "adapter_apply") in text and ("adapter_grad" in text) == grad
+
+
+def _adapters(pkg, slots=3, rank=16, widths=None):
+    layer = torch.nn.Module()
+    layer.mxl_shape, layer.mxl_format = (128, 256), 0
+    layer.weight = torch.nn.Parameter(torch.zeros(1), requires_grad=False)
+    if widths:
+        layer.logical_widths = widths
+    return pkg.LowRankAdapters(layer, slots, rank)
+
+
+def test_load_of_own_values(pkg):
+    """A slot's own values, whole or cut to a smaller rank, and another slot's."""
+    ad = _adapters(pkg)
+    g = torch.Generator().manual_seed(1)
+    a, b = torch.randn(16, 256, generator=g).bfloat16(), torch.randn(128, 16, generator=g).bfloat16()
+    ad.load(1, a, b, 0.5)
+    ad.load(1, ad.lora_a[1], ad.lora_b[1], 2.0)
+    assert torch.equal(ad.lora_a[1], a) and torch.equal(ad.lora_b[1], b) and float(ad.scaling[1]) == 2.0
+    ad.load(1, ad.lora_a[1, 4:12], ad.lora_b[1, :, 4:12], 2.0)
+    assert torch.equal(ad.lora_a[1, :8], a[4:12]) and torch.equal(ad.lora_b[1, :, :8], b[:, 4:12])
+    assert not bool(ad.lora_a[1, 8:].any()) and not bool(ad.lora_b[1, :, 8:].any())
+    ad.load(0, ad.lora_a[1], ad.lora_b[1], 1.0)
+    assert torch.equal(ad.lora_a[0], ad.lora_a[1]) and torch.equal(ad.lora_b[0], ad.lora_b[1])
+    with pytest.raises(ValueError, match="no adapter"):
+        ad.load(0, torch.tensor(1.0), b, 1.0)

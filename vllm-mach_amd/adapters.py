@@ -86,15 +86,17 @@ class LowRankAdapters(torch.nn.Module):
         p = 0 if part is None else part
         if not 0 <= p < len(self.widths):
             raise ValueError(f"part {p} of {len(self.widths)}")
-        r, k = a.shape[0], self.lora_a.shape[2]
+        r, k = a.shape[0] if a.ndim else 0, self.lora_a.shape[2]
         if a.ndim != 2 or a.shape[1] != k or tuple(b.shape) != (self.widths[p], r) or not 0 < r <= self.rank:
             raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} are no adapter of rank <= {self.rank} of "
                              f"[{self.widths[p]}, {k}]")
         slot = self._slot(slot)
         to_a = self.lora_a.data[slot, p * self.rank:(p + 1) * self.rank]
         to_b = self.lora_b.data[slot, self.cols[p]:self.cols[p + 1]]
-        to_a.zero_()[:r].copy_(a)
-        to_b.zero_()[:, :r].copy_(b)
+        to_a[:r].copy_(a.clone())  # (the slot's own values may come back, or others of this set)
+        to_b[:, :r].copy_(b.clone())
+        to_a[r:].zero_()
+        to_b[:, r:].zero_()
         self.scaling[slot] = float(scaling)
 
     @torch.no_grad()
