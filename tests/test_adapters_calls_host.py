@@ -37,8 +37,8 @@ def test_supported_shapes_agree(pkg):
     rows = [0, 1, 16, 17, 31, 32, 63, 64, 511, 512, 513, 4096, 1 << 20, (1 << 22) - 1, 1 << 22, 1 << 25]
     for m in rows:
         for n, k in ((128, 128), (17408, 5120), (0, 128), (128, 100), (128, 32768), (128, 32896), (1 << 22, 128), (128, 1 << 12)):
-            for fmt, block in ((0, 0), (0, 1), (4, 0), (4, 1)):
-                for slots, parts, rank in ((1, 1, 8), (2, 8, 256), (16, 1, 24), (17, 1, 8), (0, 1, 8)):
+            for fmt, block in ((0, 0), (0, 1), (4, 0), (4, 1), (1, 0), (2, 1), (5, 0)):
+                for slots, parts, rank in ((1, 1, 8), (2, 8, 256), (16, 1, 24), (17, 1, 8), (0, 1, 8), (1, 9, 8), (1, 1, 12), (1, 1, 264)):
                     args = (m, n, k, fmt, block, slots, parts, rank)
                     assert pkg.ops.adapter_linear_supported(*args) == ask(*args), args
     assert pkg.ops.adapter_linear_supported(64, 128, 128, 0, False, 2, 1, 8)
@@ -98,3 +98,40 @@ def test_load_of_own_values(pkg):
     assert torch.equal(ad.lora_a[0], ad.lora_a[1]) and torch.equal(ad.lora_b[0], ad.lora_b[1])
     with pytest.raises(ValueError, match="no adapter"):
         ad.load(0, torch.tensor(1.0), b, 1.0)
+
+
+_QUERIES = '''
+import sys
+sys.path.insert(0, {root!r})
+import __graft_entry__
+__graft_entry__.load_package()
+from vllm_mach_amd import _lib
+huge = [0, -1, 3, 2 ** 31, 2 ** 32, 2 ** 36, 2 ** 62, 2 ** 63 - 1]
+for name, good in (("mxl_adapter_tile_count", [4, 2]), ("mxl_adapter_v_elems", [4, 1, 8]),
+                   ("mxl_adapter_apply_workspace_bytes", [4, 128, 2, 1, 8]),
+                   ("mxl_adapter_linear_supported", [64, 128, 128, 0, 0, 1, 1, 8]),
+                   ("mxl_adapter_linear_workspace_bytes", [64, 128, 0, 0]),
+                   ("mxl_input_grad_workspace_bytes", [64, 120, 128, 0]), ("mxl_gated_workspace_bytes", [64, 128, 0])):
+    flags = {{"mxl_adapter_linear_supported": (3, 4), "mxl_adapter_linear_workspace_bytes": (2, 3),
+             "mxl_input_grad_workspace_bytes": (3,), "mxl_gated_workspace_bytes": (2,)}}.get(name, ())
+    sizes = [i for i in range(len(good)) if i not in flags]
+    for i in sizes:
+        for j in sizes:
+            for x in huge:
+                args = list(good)
+                args[i] = args[j] = x
+                assert _lib.query(name, *args) >= 0, (name, args)
+    if name != "mxl_adapter_apply_workspace_bytes":
+        assert _lib.query(name, *good) > 0, name
+print("answered")
+'''
+
+
+def test_queries_of_any_size_answer():
+    """In a process of its own: a query that divides by zero would end this one."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = str(Path(__file__).resolve().parents[1])
+    out = subprocess.run([sys.executable, "-c", _QUERIES.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip().endswith("answered"), (out.returncode, out.stderr[-500:])

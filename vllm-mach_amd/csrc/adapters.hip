@@ -476,6 +476,12 @@ int64_t tile_count(int64_t M, int64_t slots) { return std::min(M, ceil_div(M, kA
 // without more workgroups (4096 x 5120 to 64 ranks: one group 33.0 us, two 25.9, four 24.4).
 int shrink_groups(int64_t tiles, int groups) { return tiles < 256 || groups < 2 ? 1 : groups < 4 ? 2 : 4; }
 
+// The sizes that a call takes; queries of others say 0.
+bool batch_ok(int64_t M, int64_t slots) { return M > 0 && M <= 0x7FFFFFFF && slots > 0 && slots <= kMaxSlots; }
+bool low_rank_ok(int64_t parts, int64_t rank) {
+  return parts >= 1 && parts <= kMaxParts && rank > 0 && rank <= kMaxRank && rank % 8 == 0;
+}
+
 int check_batch(const char* who, int64_t M, int64_t slots, const int32_t* order, const int64_t* offsets,
                 const int32_t* tiles, int64_t num_tiles) {
   MXL_CHECK_ARG(M >= 0 && M <= 0x7FFFFFFF && slots > 0 && slots <= kMaxSlots, "%s: need 0 <= M < 2^31 and 0 < slots <= %d (M=%lld slots=%lld)",
@@ -624,7 +630,7 @@ GradScratch grad_scratch(uint8_t* base, int64_t M, int64_t K, int64_t slots, con
 }  // namespace
 
 extern "C" int64_t mxl_adapter_tile_count(int64_t M, int64_t slots) {
-  return M <= 0 || slots <= 0 ? 0 : tile_count(M, slots);
+  return batch_ok(M, slots) ? tile_count(M, slots) : 0;
 }
 
 extern "C" int mxl_adapter_tiles(const int64_t* offsets, int64_t M, int64_t slots, int32_t* tiles, int64_t num_tiles,
@@ -639,11 +645,11 @@ extern "C" int mxl_adapter_tiles(const int64_t* offsets, int64_t M, int64_t slot
 }
 
 extern "C" int64_t mxl_adapter_v_elems(int64_t M, int64_t parts, int64_t rank) {
-  return M <= 0 || parts <= 0 || rank <= 0 ? 0 : M * 2 * parts * ceil_div(rank, 16) * 16;
+  return batch_ok(M, 1) && low_rank_ok(parts, rank) ? M * 2 * parts * ceil_div(rank, 16) * 16 : 0;
 }
 
 extern "C" int64_t mxl_adapter_apply_workspace_bytes(int64_t M, int64_t K, int64_t slots, int64_t parts, int64_t rank) {
-  if (M <= 0 || K <= 0 || slots <= 0 || parts <= 0 || rank <= 0) return 0;
+  if (!batch_ok(M, slots) || !low_rank_ok(parts, rank) || K <= 0) return 0;
   LowRank l{};
   l.parts = (int)parts;
   l.groups = (int)ceil_div(rank, 16);
@@ -694,13 +700,15 @@ static int64_t code_bytes(int64_t M, int64_t K, int fmt) { return ceil_div(fmt =
 // offsets.
 extern "C" int mxl_adapter_linear_supported(int64_t M, int64_t N, int64_t K, int fmt, int block, int64_t slots,
                                             int64_t parts, int64_t rank) {
-  return M >= 17 && N > 0 && K > 0 && K % 128 == 0 && slots > 0 && parts > 0 && rank > 0 && rows_add(M, slots) &&
+  if (!batch_ok(M, slots) || !low_rank_ok(parts, rank) || N <= 0 || N > 0x7FFFFFFF || K <= 0 || K > 0x7FFFFFFF) return 0;
+  if (fmt != kE4M3 && fmt != kE2M3 && fmt != kE3M2 && fmt != kE2M1) return 0;
+  return M >= 17 && K % 128 == 0 && rows_add(M, slots) &&
          wide_tiles_eligible(M, N, K, block != 0) && M <= (int64_t(1) << 32) / (4 * parts * ceil_div(rank, 16) * 16) &&
-         N <= (int64_t(1) << 31) / (2 * rank) && (fmt != kE2M1 || !block);
+         N <= (int64_t(1) << 31) / (2 * rank) && (fmt == kE4M3 || !block);
 }
 
 extern "C" int64_t mxl_adapter_linear_workspace_bytes(int64_t M, int64_t K, int fmt, int block) {
-  if (M <= 0 || K <= 0) return 0;
+  if (M <= 0 || M > 0x7FFFFFFF || K <= 0 || K > 0x7FFFFFFF) return 0;
   return code_bytes(M, K, fmt) + (block ? M * (K / 128) * 4 : M * (K / 32));
 }
 
@@ -767,7 +775,7 @@ extern "C" int mxl_adapter_linear(const void* x, int64_t M, int64_t K, int64_t l
 extern "C" int64_t mxl_adapter_grad_workspace_bytes(int64_t M, int64_t K, int64_t slots, int64_t parts,
                                                     const int64_t* cols, int64_t rank, int block) {
   LowRank l;
-  if (M <= 0 || slots <= 0 || make_low_rank("mxl_adapter_grad_workspace_bytes", parts, cols, rank, K, l) != MXL_OK) return 0;
+  if (!batch_ok(M, slots) || make_low_rank("mxl_adapter_grad_workspace_bytes", parts, cols, rank, K, l) != MXL_OK) return 0;
   return grad_scratch(nullptr, M, K, slots, l).bytes + input_grad_bytes(M, cols[parts], K, block);
 }
 

@@ -84,7 +84,7 @@ int run(const char* who, const void* x, int64_t M, int64_t K, int64_t ldx, int r
 }  // namespace
 
 extern "C" int64_t mxl_gated_workspace_bytes(int64_t M, int64_t K, int fmt) {
-  return M <= 0 || K <= 0 ? 0 : workspace_bytes(M, K, fmt);
+  return M <= 0 || M > 0x7FFFFFFF || K <= 0 || K > (1 << 22) ? 0 : workspace_bytes(M, K, fmt);
 }
 
 extern "C" int mxl_gated_linear(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, const void* w_tiled,

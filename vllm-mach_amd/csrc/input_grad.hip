@@ -568,7 +568,7 @@ static int64_t pad_bytes(int64_t M, int64_t N) {
 }
 
 int64_t mxl::input_grad_bytes(int64_t M, int64_t N, int64_t K, int block) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || M > 0x7FFFFFFF || N <= 0 || N > (1 << 22) || K <= 0 || K > (1 << 22)) return 0;
   const GradPlan g = grad_plan(M, N, K, block);
   return pad_bytes(M, N) + (g.S > 1 ? g.S * M * K * 4 : 0);
 }

@@ -1371,8 +1371,8 @@ _BLOCK_STAGES = 256  # 128-column scales of a block-FP8 tile (kWideBlockStages)
 def adapter_linear_supported(m: int, n: int, k: int, w_fmt: int, block: bool, slots: int, parts: int, rank: int) -> bool:
     """Shapes whose product adds the adapters itself (``adapter_linear``): 17 rows or more, 32 an adapter, up to 16 adapters,
     and offsets of 32 bits.  ``mxl_adapter_linear_supported``, in Python for tracing to see through."""
-    return (m >= 17 and n > 0 and k > 0 and k % 128 == 0 and 0 < slots <= 16 and m >= 32 * slots and parts > 0 and rank > 0
-            and not (block and w_fmt == E2M1) and m * k < 1 << 32 and ((n + 15) // 16) * ((k + 511) // 512) < 1 << 24
+    return (w_fmt in (_CODE_CHUNKS if not block else (E4M3,)) and m >= 17 and n > 0 and k > 0 and k % 128 == 0 and 0 < slots <= 16
+            and m >= 32 * slots and 1 <= parts <= 8 and 8 <= rank <= 256 and rank % 8 == 0 and m * k < 1 << 32 and ((n + 15) // 16) * ((k + 511) // 512) < 1 << 24
             and (not block or k <= 128 * _BLOCK_STAGES) and m <= (1 << 32) // (64 * parts * ((rank + 15) // 16))
             and n <= (1 << 31) // (2 * rank))
 
