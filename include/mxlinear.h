@@ -589,7 +589,7 @@ int mxl_gated_grad(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, c
                    int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Low-rank adapters of many requests.  A batch of M tokens sorted by adapter (mxl_moe_route of the ids
- * as [M, 1], at most 2560 adapters): order i32 [M], offsets i64 [slots + 1], and from them the tiles
+ * as [M, 1], at most 2048 adapters): order i32 [M], offsets i64 [slots + 1], and from them the tiles
  * i32 [mxl_adapter_tile_count][4] (16-byte aligned) that mxl_adapter_tiles writes.
  *
  * mxl_adapter_apply: y[t] += scaling[s] b[s] (a[s] x[t]) for every token t of the batch, s its adapter:

@@ -135,3 +135,14 @@ def test_queries_of_any_size_answer():
     root = str(Path(__file__).resolve().parents[1])
     out = subprocess.run([sys.executable, "-c", _QUERIES.format(root=root)], capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and out.stdout.strip().endswith("answered"), (out.returncode, out.stderr[-500:])
+
+
+def test_one_limit_of_slots(pkg):
+    """2048, wherever it is asked."""
+    from vllm_mach_amd import _lib
+    assert _lib.query("mxl_adapter_tile_count", 4, 2048) == 4 and _lib.query("mxl_adapter_tile_count", 4, 2049) == 0
+    with pytest.raises(_lib.MxlError, match="slots <= 2048"):
+        _lib.call("mxl_adapter_tiles", 16, 4, 2049, 16, 4, None)
+    with pytest.raises(ValueError, match="slots"):
+        _adapters(pkg, 2049, 8)
+    assert _adapters(pkg, 2048, 8).slots == 2048

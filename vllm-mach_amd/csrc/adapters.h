@@ -5,7 +5,7 @@
 
 namespace mxl {
 
-constexpr int kMaxParts = 8, kMaxRank = 256, kMaxSlots = 4096, kAdapterTile = 16;
+constexpr int kMaxParts = 8, kMaxRank = 256, kMaxSlots = 2048, kAdapterTile = 16;
 
 // Tokens sorted by adapter: positions [offsets[a], offsets[a + 1]) of order are adapter a's, in tiles of 16 positions:
 // tile i is (adapter, first position, end, 0), adapter -1 past the last.
