@@ -645,6 +645,12 @@ int mxl_gemm_plan_name(int64_t M, int64_t N, int64_t K, int w_fmt, int block, co
                        char* buf, int64_t len);
 int mxl_grouped_plan_name(int64_t routed_rows, int64_t num_experts, int64_t K, int w_fmt, int prod, int rule,
                           const mxl_gemm_options* options, char* buf, int64_t len);
+/* The same of mxl_gated_linear (grad = 1: mxl_gated_grad), mxl_adapter_linear and mxl_input_grad (mxl_adapter_grad's
+ * dx); the first two with the stages of the tiles' ring, and whether the last tiles run in quarters:
+ * "gated_tile_kernel<0,16,4,2> (depth 2, quarters)". */
+int mxl_gated_plan_name(int64_t M, int64_t I, int64_t K, int fmt, int grad, char* buf, int64_t len);
+int mxl_adapter_linear_plan_name(int64_t M, int64_t N, int64_t K, int fmt, int block, char* buf, int64_t len);
+int mxl_input_grad_plan_name(int64_t M, int64_t N, int64_t K, int fmt, int block, char* buf, int64_t len);
 
 #ifdef __cplusplus
 }

@@ -146,3 +146,15 @@ def test_one_limit_of_slots(pkg):
     with pytest.raises(ValueError, match="slots"):
         _adapters(pkg, 2049, 8)
     assert _adapters(pkg, 2048, 8).slots == 2048
+
+
+def test_plan_names(pkg):
+    from vllm_mach_amd import _lib
+    name = _lib.tile_plan_name
+    assert name("mxl_gated_plan_name", 1, 64, 128, 0, 0) == "gated_tile_kernel<0,4,1,2> (depth 4)"
+    assert name("mxl_adapter_linear_plan_name", 35, 64, 128, 0, 1) == "adapter_tile_kernel<0,4,1,true> (depth 4)"
+    assert name("mxl_input_grad_plan_name", 1, 640, 128, 4, 0) == "input_grad_kernel<4,128,128,false> + input_grad_join_kernel"
+    for fn, *args in (("mxl_gated_plan_name", 0, 64, 128, 0, 0), ("mxl_gated_plan_name", 4, 24, 128, 0, 0),
+                      ("mxl_adapter_linear_plan_name", 16, 64, 128, 0, 0), ("mxl_input_grad_plan_name", 4, 64, 64, 0, 0)):
+        with pytest.raises(_lib.MxlError, match="bad shape"):
+            name(fn, *args)

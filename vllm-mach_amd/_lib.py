@@ -113,6 +113,9 @@ SIGNATURES = {
     "mxl_moe_router_grouped": (_I, [_P, _I, _P, _I64, _I64, _I64, _I, _I64, _I64, _I, _F, _P, _P, _P, _P, _P, _P, _I64,
                                     _P]),
     "mxl_gemm_plan_name": (_I, [_I64, _I64, _I64, _I, _I, _P, ctypes.c_char_p, _I64]),
+    "mxl_gated_plan_name": (_I, [_I64, _I64, _I64, _I, _I, ctypes.c_char_p, _I64]),
+    "mxl_adapter_linear_plan_name": (_I, [_I64, _I64, _I64, _I, _I, ctypes.c_char_p, _I64]),
+    "mxl_input_grad_plan_name": (_I, [_I64, _I64, _I64, _I, _I, ctypes.c_char_p, _I64]),
     "mxl_grouped_plan_name": (_I, [_I64, _I64, _I64, _I, _I, _I, _P, ctypes.c_char_p, _I64]),
 }
 
@@ -184,6 +187,13 @@ def plan_name(fn: str, *args, options: "GemmOptions | None" = None) -> str:
     """The kernels ``mxl_gemm_plan_name`` / ``mxl_grouped_plan_name`` report for a call."""
     buf = ctypes.create_string_buffer(512)
     call(fn, *args, options_ptr(options), buf, len(buf))
+    return buf.value.decode()
+
+
+def tile_plan_name(fn: str, *args) -> str:
+    """The same of the entry points without options (gated, adapters, input gradient)."""
+    buf = ctypes.create_string_buffer(512)
+    call(fn, *args, buf, len(buf))
     return buf.value.decode()
 
 

@@ -87,6 +87,15 @@ extern "C" int64_t mxl_gated_workspace_bytes(int64_t M, int64_t K, int fmt) {
   return M <= 0 || M > 0x7FFFFFFF || K <= 0 || K > (1 << 22) ? 0 : workspace_bytes(M, K, fmt);
 }
 
+extern "C" int mxl_gated_plan_name(int64_t M, int64_t I, int64_t K, int fmt, int grad, char* buf, int64_t len) {
+  MXL_CHECK_ARG(M > 0 && M <= 0x7FFFFFFF && I > 0 && I <= (1 << 22) && I % 16 == 0 && K > 0 && K <= (1 << 22) && K % 128 == 0 && buf,
+                "mxl_gated_plan_name: bad shape");
+  WideGrid g{};
+  int64_t grid;
+  const WideConfig c = wide_tiles_whole(slab_rows(M, K, fmt), 2 * I, K, fmt, false, g, grid);
+  return tile_plan_name("gated_tile_kernel", grad ? "3" : "2", c, g, grid, fmt, buf, len);
+}
+
 extern "C" int mxl_gated_linear(const void* x, int64_t M, int64_t K, int64_t ldx, int rule, const void* w_tiled,
                                 const void* sw_tiled, int64_t I, int fmt, int act, void* out, int64_t ldo,
                                 void* workspace, int64_t workspace_bytes, void* stream) {

@@ -37,6 +37,8 @@
 // sums share one activation scale.
 #pragma once
 
+#include <stdio.h>
+
 #include "adapters.h"
 #include "fp4.h"
 #include "gate_act.h"
@@ -154,6 +156,23 @@ struct TileDepth {
   // of a tile's quarters, in the LDS of the launch
   static constexpr int QUARTER = 4;
 };
+
+// Of a launch of `grid` workgroups on `cus` CUs: the stages of its ring, and " (depth D)" or " (depth D, quarters)" for the
+// name of its plan.
+inline int tile_depth(const WideConfig& c, int64_t grid, int64_t cus) {
+#define MXL_DEPTH(MT_, NT_) \
+  if (c.MT == MT_ && c.NT == NT_) return grid <= TileDepth<MT_, NT_>::LONE_MAX * cus ? TileDepth<MT_, NT_>::LONE : TileDepth<MT_, NT_>::SHARED;
+  MXL_DEPTH(16, 4) MXL_DEPTH(8, 4) MXL_DEPTH(8, 2) MXL_DEPTH(8, 1) MXL_DEPTH(4, 2) MXL_DEPTH(4, 1)
+#undef MXL_DEPTH
+  return 0;
+}
+inline int tile_plan_name(const char* kernel, const char* last, const WideConfig& c, const WideGrid& g, int64_t grid, int fmt,
+                          char* buf, int64_t len) {
+  const int n = snprintf(buf, len > 0 ? (size_t)len : 0, "%s<%d,%d,%d,%s> (depth %d%s)", kernel, fmt, c.MT, c.NT, last,
+                         tile_depth(c, grid, cu_count()), grid > g.tail0 ? ", quarters" : "");
+  MXL_CHECK_ARG(n < len, "plan name needs %d bytes", n + 1);
+  return MXL_OK;
+}
 
 // What a tile's epilogue does with its sums.  All but the first pair columns of a merged gate/up weight (W = gate rows
 // then up rows, I of each): half of a wave's n-tiles are gate columns, half the up columns of the same.

@@ -82,3 +82,16 @@ hipError_t launch_adapter_tiles(int fmt, bool block, const WideConfig& c, const 
 }
 
 }  // namespace mxl
+
+using namespace mxl;
+
+extern "C" int mxl_adapter_linear_supported(int64_t M, int64_t N, int64_t K, int fmt, int block, int64_t slots,
+                                            int64_t parts, int64_t rank);
+
+extern "C" int mxl_adapter_linear_plan_name(int64_t M, int64_t N, int64_t K, int fmt, int block, char* buf, int64_t len) {
+  MXL_CHECK_ARG(buf && mxl_adapter_linear_supported(M, N, K, fmt, block, 1, 1, 8), "mxl_adapter_linear_plan_name: bad shape");
+  WideGrid g{};
+  int64_t grid;
+  const WideConfig c = wide_tiles_whole(M, N, K, fmt, block != 0, g, grid);
+  return tile_plan_name("adapter_tile_kernel", block ? "true" : "false", c, g, grid, fmt, buf, len);
+}

@@ -13,6 +13,8 @@
 // Bound: the MFMAs at the clock that the power limit leaves, busy 65 % of the time (the rest: the stage's barrier and LDS
 // issue).  2048 x 18432 x 2560 in 256 x 256 tiles: 184 us, 1.05 PFLOP/s, and 13 us for the join of the splits (as a library
 // bf16 product of decoded weights 250 us).  Each workgroup decodes its strip of W anew: 256 rows share a decode.
+#include <stdio.h>
+
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -638,6 +640,16 @@ extern "C" int mxl_bias_grad(const void* dy, int64_t M, int64_t N, int64_t lddy,
 
 extern "C" int64_t mxl_input_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int block) {
   return input_grad_bytes(M, N, K, block);
+}
+
+extern "C" int mxl_input_grad_plan_name(int64_t M, int64_t N, int64_t K, int fmt, int block, char* buf, int64_t len) {
+  MXL_CHECK_ARG(M > 0 && M <= 0x7FFFFFFF && N > 0 && N <= (1 << 22) && K > 0 && K <= (1 << 22) && K % 128 == 0 && buf,
+                "mxl_input_grad_plan_name: bad shape");
+  const GradPlan g = grad_plan(M, N, K, block != 0);
+  const int n = snprintf(buf, len > 0 ? (size_t)len : 0, "input_grad_kernel<%d,%d,%d,%s>%s", fmt, g.TM, g.TK,
+                         block ? "true" : "false", g.S > 1 ? " + input_grad_join_kernel" : "");
+  MXL_CHECK_ARG(n < len, "plan name needs %d bytes", n + 1);
+  return MXL_OK;
 }
 
 extern "C" int mxl_input_grad(const void* dy, int64_t M, int64_t N, int64_t lddy, const void* w_tiled, const void* sw,
