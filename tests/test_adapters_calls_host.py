@@ -158,3 +158,29 @@ def test_plan_names(pkg):
                       ("mxl_adapter_linear_plan_name", 16, 64, 128, 0, 0), ("mxl_input_grad_plan_name", 4, 64, 64, 0, 0)):
         with pytest.raises(_lib.MxlError, match="bad shape"):
             name(fn, *args)
+
+
+def test_every_compiled_tile_is_reached():
+    """What the build compiled of the tiles is what the GPU tests reach by their plans."""
+    import json
+    import re
+    from pathlib import Path
+    import test_gpu_tile_plans as plans
+    report = Path(__file__).resolve().parents[1] / "vllm-mach_amd" / "_build" / "kernel_resources.json"
+    if not report.exists():
+        pytest.skip("no build report (run __graft_entry__.build() first)")
+    built = {"gated": set(), "adapter": set(), "input_grad": set()}
+    for kernel in re.findall(r'"(_ZN3mxl[^"]*)"', report.read_text()):
+        m = re.match(r"_ZN3mxl\d+(gated_tile|adapter_tile|input_grad)_kernelI((?:L[ib]\d+E)+)E", kernel)
+        if m:
+            built[m[1].removesuffix("_tile")].add(tuple(int(v) for v in re.findall(r"L[ib](\d+)E", m[2])))
+    code = plans.CODES
+    gated = {(code[f], *c[0], epi) for f, cases in (("mxfp8", plans.GATED_8), ("mxfp6", plans.GATED_8),
+                                                    ("mxfp6_e3m2", plans.GATED_8), ("mxfp4", plans.GATED_4))
+             for c in cases for epi in (2, 3)}
+    adapter = {(code[f], *c[0], int(f == "block"))
+               for f, cases in (("mxfp8", plans.ADD_8), ("mxfp6", plans.ADD_8), ("mxfp6_e3m2", plans.ADD_8),
+                                ("mxfp4", plans.ADD_4), ("block", plans.ADD_BLOCK)) for c in cases}
+    grad = {(code[f], *c[0], int(f == "block")) for f in code for c in (plans.GRAD_BLOCK if f == "block" else plans.GRAD)}
+    assert built == {"gated": gated, "adapter": adapter, "input_grad": grad}
+    assert len(json.loads(report.read_text())) > 0
