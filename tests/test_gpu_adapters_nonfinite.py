@@ -26,6 +26,7 @@ def _case(pkg, dev, fmt, widths, k, slots, rank, m):
         y = method.apply(layer, x, None, adapters=ad, batch=batch)
         return (y.detach(), *torch.autograd.grad(y, [x, ad.lora_a, ad.lora_b], dy))
 
+    step.x, step.dy = x, dy
     return ad, ids, step
 
 
@@ -92,3 +93,34 @@ def test_a_token_stays_in_its_row(pkg, dev, m):
     keep = torch.ones(m, dtype=torch.bool, device=dev)
     keep[2:4] = False
     assert torch.equal(y[keep], clean[keep]) and not bool(y[2:4].isfinite().any())
+
+
+@pytest.mark.parametrize("m,slots", [(4, 2), (50, 2), (200, 3), (800, 20), (1500, 1)])
+def test_an_infinity_is_an_infinity(pkg, dev, m, slots):
+    """Of B, x and dy: with the sign that the product has in 64 bits."""
+    k, n, rank = 256, 128, 16
+    ad, ids, step = _case(pkg, dev, "mxfp8", [n], k, slots, rank, m)
+    mine = (ids == 0).nonzero().squeeze(-1)
+    x, dy = step.x, step.dy
+    ad.lora_b.data[0, 5, 3] = 0.5
+    scale = ad.scaling[0].double()
+    v = scale * (x[mine].double() @ ad.lora_a[0].double().t())
+    dv = scale * (dy[mine].double() @ ad.lora_b[0].double())
+    for bad in (float("inf"), float("-inf")):
+        ad.lora_b.data[0, 5, 3] = bad
+        z = step()[0]
+        ad.lora_b.data[0, 5, 3] = 0.5
+        assert torch.equal(z[mine, 5].double(), bad * v[:, 3].sign())
+        kept = ad.lora_a.data[0, 2, 7].clone()
+        ad.lora_a.data[0, 2, 7] = bad
+        assert torch.equal(step()[1][mine, 7].double(), bad * dv[:, 2].sign())
+        ad.lora_a.data[0, 2, 7] = kept
+        t = int(mine[-1])
+        kept = x.data[t, 9].clone()
+        x.data[t, 9] = bad
+        assert torch.equal(step()[2][0, :, 9].double(), bad * dv[-1].sign())
+        x.data[t, 9] = kept
+        kept = dy[t, 6].clone()
+        dy[t, 6] = bad
+        assert torch.equal(step()[3][0, 6].double(), bad * v[-1].sign())
+        dy[t, 6] = kept
