@@ -43,6 +43,8 @@ struct RowAdapters {
 // one product / apart, tokens in runs of an adapter and, the worst case, mixed at random:
 //   256 x 5120 x 2560, 8 adapters: 23 / 25, mixed 28 / 26       2048 x 17408 x 5120, 8 adapters: 207 / 276, mixed 296 / 288
 //   1024 x 5120 x 2560, 32: 36 / 40, mixed 56 / 42              2048 x 17408 x 5120, 64: 194 / 210, mixed 374 / 215
+// The rule has no N or K in it, and few tiles of a long K lose by that, one adapter each 32 rows or more: 64 x 2560 x 17408, 2
+// adapters, 64 / 28; 256 x 2560 x 17408, 8: 68 / 39; 64 x 512 x 5120, 2: 23 / 17; even at 64 x 17408 x 5120, 2: 32 / 30.
 inline bool rows_add(int64_t M, int64_t slots) { return slots <= 16 && M >= 32 * slots; }
 
 // A product multiplies an adapter's values with zeros too, in rows of other adapters and columns of other parts, where an

@@ -111,7 +111,7 @@ __global__ __launch_bounds__(1024) void adapter_tiles_kernel(const int64_t* offs
 // to 64 ranks: 24 us, of which x alone is 8).  Loads by rows of the MFMA's operand put sixteen lines into every sixteen
 // lanes, 64 cycles an instruction: 37.0 and 34 us where the loads are turned in LDS now.  SHARES: few tiles fill the card by splitting the columns over
 // workgroups, whose fp32 sums [blockIdx.z][token][width] the expand kernel joins (48 tokens of 32 adapters, K = 5120, both
-// kernels: 20.0 us whole, 14.3 in shares).
+// kernels: 20.0 us whole, 14.1 in shares).
 template <int RC, bool BY_PART, bool SHARES>
 __global__ __launch_bounds__(RC < 4 ? 1024 : 512) void adapter_shrink_kernel(AdapterBatch b, LowRank l, const uint16_t* x, int64_t ldx,
                                                               int64_t cols, const uint16_t* rows, int64_t slot_stride,
@@ -210,8 +210,10 @@ __global__ __launch_bounds__(RC < 4 ? 1024 : 512) void adapter_shrink_kernel(Ada
 // y[t][n] += sum_j mat[n][j] v[t][j], mat [N, ldm] (j < valid) of the tile's adapter, j the ranks of n's part.  A wave is a
 // tile of 16 tokens by 64 columns of one part: MFMA i's row 4 q + e is column 16 q + 4 i + e, so that after the four a
 // lane holds 16 columns of one token side by side (the rows of y in 32-byte pieces; `wide`: they start on 16 bytes).
-// SHARES: v comes as the shrink kernel's shares, and the first columns' workgroup writes it down.  Bound: B's bytes and two
-// dependent round trips to memory (48 tokens of 32 adapters, rank 16, N = 17408: 9.0 us, 2.3 TB/s).
+// SHARES: v comes as the shrink kernel's shares, and the first columns' workgroup writes it down.  y is the layer's output,
+// rounded to bf16 by its launch, and is rounded again here: the layers' kernels write bf16, and an fp32 y between the two
+// launches would be twice its bytes (against 64 bits, relative: 0.0022 instead of the one rounding's 0.0017).  Bound: B's bytes
+// and two dependent round trips to memory (48 tokens of 32 adapters, rank 16, N = 17408: 9.2 us, 2.3 TB/s).
 template <bool SHARES>
 __global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterBatch b, LowRank l, uint16_t* v, const float* shares,
                                                              int num_shares, const uint16_t* mat, int64_t slot_stride, int64_t ldm,
@@ -334,7 +336,7 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterBatch b, Low
 // sum_t big[t][c] v[t][j] over the adapter's positions of split z: to out [N, r] (OF_B: c a column of dy, j the ranks of
 // its part) or out [R, K] (c a column of x, j all ranks).  A workgroup is 128 columns by RC groups; 32 tokens at a time
 // go through LDS, both operands read from it transposed; the next 32 are on their way.  Bound: the big matrix' bytes where
-// the shares fill the card (2048 x 18432 of dy 24.7 us, 3.1 TB/s), else a token tile's latency.
+// the shares fill the card (2048 x 18432 of dy 25.5 us, 3.0 TB/s), else a token tile's latency.
 constexpr int kOuterCols = 128, kOuterStride = kOuterCols + 16, kOuterTokens = 32;
 template <int RC, bool OF_B>
 __global__ __launch_bounds__(256) void adapter_outer_kernel(AdapterBatch b, LowRank l, const uint16_t* big, int64_t ldb,
@@ -561,7 +563,7 @@ int launched(const char* who) {
 }
 
 // Shares of the columns where the expand kernel follows: until some 256 workgroups run, or a wave has 32 columns.  (48
-// tokens of 32 adapters of rank 16, K = 5120, N = 17408, us of both kernels: one share 20.0, two 15.2, five 14.0.)
+// tokens of 32 adapters of rank 16, K = 5120, N = 17408, us of both kernels: one share 20.0, two 15.2, five 14.1.)
 int shrink_shares(int64_t tiles, const LowRank& l, int64_t cols) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({kMaxShares, 256 / (tiles * l.parts * l.groups), cols / 256}));
 }

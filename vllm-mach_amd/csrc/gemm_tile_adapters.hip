@@ -2,7 +2,7 @@
 // (gemm_tile.h, ADD), the activations' quantization, and the adapters' first half (adapters.hip) ahead of them.
 //
 // Bound: the product, and some 4 us a tile and adapter in waits for v's and B's first bytes.  2048 x 18432 x 2560 MXFP8, rank
-// 16: 109 us at its best, the product alone 95; 4096 x 17408 x 5120, 8 adapters of rank 64: 342 at its best, alone 300.
+// 16: 108 us at its best, the product alone 95; 4096 x 17408 x 5120, 8 adapters of rank 64: 351 at its best, alone 300.
 #include <algorithm>
 
 #include "gemm_tile.h"
@@ -10,7 +10,8 @@
 namespace mxl {
 
 // Whole tiles and, past them, quarters (the gated kernels' grid; a K split's workgroups beside the adapters' operands
-// would run out of scalar registers, and few rows of a long K have the launches apart).
+// would run out of scalar registers).  So few tiles of a long K, where the layer's own product splits K, are slower here than
+// apart (figures at rows_add, adapters.h).
 template <int FMT, int MT, int NT, bool BLOCK>
 __global__ __launch_bounds__(256, (WidePerCu<MT, NT, false, 2>::value)) void adapter_tile_kernel(GemmParams p, WideGrid g,
                                                                                                 RowAdapters add) {

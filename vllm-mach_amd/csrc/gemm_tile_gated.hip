@@ -3,9 +3,10 @@
 //
 // A tile's columns are half gate, half the up columns of the same, so both sums of an output meet in one lane's
 // registers, and neither is written nor rounded.  What bounds the launch is the product (gemm_tile.h); the epilogue's
-// exponentials run in the last round only.  4096 x 18432 x 2560 MXFP8 172 us (2.25 PFLOP/s); 2048 x 18432 x 2560 MXFP4 71 us,
-// with the gradient's epilogue 90 (101 with 4-byte stores and dh loaded where it is used).  1 x 18432 x 2560 MXFP8 10.5 us,
-// 4.6 TB/s of weights.
+// exponentials run in the last round only.  The products' gradients are rounded to bf16 on their way to the input gradient,
+// whose MFMA takes no more (against 64 bits dx is off by 0.0023, relative, with fp32 there by 0.0017).  4096 x 18432 x 2560
+// MXFP8 172 us (2.25 PFLOP/s); 2048 x 18432 x 2560 MXFP4 67 us, with the gradient's epilogue 87 (14 more with 4-byte stores and
+// dh loaded where it is used).  1 x 18432 x 2560 MXFP8 10.5 us, 4.6 TB/s of weights.
 #include <algorithm>
 
 #include "gemm_tile.h"
