@@ -1282,7 +1282,8 @@ def adapter_batch(ids: torch.Tensor, slots: int) -> tuple[torch.Tensor, torch.Te
         raise ValueError(f"less than 2^31 tokens ({M})")
     if ids.dtype == torch.int32:  # (a copy: the caller may write its own for the next step)
         ids = ids.clone(memory_format=torch.contiguous_format)
-    else:  # (values past 32 bits would wrap into range)
+    else:  # (values past 32 bits would wrap into range; unsigned types have no comparisons)
+        ids = ids.long()
         ids = torch.where((ids >= 0) & (ids < slots), ids, -1).to(torch.int32).contiguous()
     order = torch.empty(M, dtype=torch.int32, device=dev)
     offsets = torch.empty(slots + 1, dtype=torch.int64, device=dev)
