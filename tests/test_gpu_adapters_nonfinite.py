@@ -124,3 +124,19 @@ def test_an_infinity_is_an_infinity(pkg, dev, m, slots):
         dy[t, 6] = bad
         assert torch.equal(step()[3][0, 6].double(), bad * v[-1].sign())
         dy[t, 6] = kept
+
+
+@pytest.mark.parametrize("n,m", [(131, 200), (77, 100), (260, 700)])
+def test_odd_widths(pkg, dev, n, m):
+    """Columns that do not end on a store's: the product's other way out."""
+    ad, ids, step = _case(pkg, dev, "block", [n], 256, 3, 24, m)
+    y, dx, da, db = step()
+    mine, cols = ids == BAD, torch.arange(n, device=dev)
+    for col in (0, n // 2, n - 1):
+        kept = ad.lora_b.data[BAD, col, 5].clone()
+        ad.lora_b.data[BAD, col, 5] = float("inf")
+        y2, dx2, da2, db2 = step()
+        ad.lora_b.data[BAD, col, 5] = kept
+        assert torch.equal(y2[~mine], y[~mine]) and torch.equal(y2[:, cols != col], y[:, cols != col])
+        assert not bool(y2[mine, col].isfinite().any())
+        assert torch.equal(dx2[~mine], dx[~mine]) and torch.equal(db2, db)

@@ -148,7 +148,7 @@ class Mxfp8LinearKernel(_Kernel):
         n, k = layer.mxl_shape
         if x.dtype != torch.bfloat16 or x.shape[-1] != k:
             raise ValueError("MXFP8 requires BF16 activations with matching K")
-        if _differentiated(x):
+        if x.requires_grad and _differentiated():
             return _with_input_grad(layer, x, bias)
         if x.numel() == 0:
             return x.new_empty((*x.shape[:-1], n))
@@ -185,10 +185,10 @@ def _function_bias(bias: Optional[torch.Tensor], x: torch.Tensor, n: int) -> Opt
         return _epilogue_bias(bias, x, n)
 
 
-def _differentiated(x: torch.Tensor) -> bool:
-    """Whether a gradient of x may be asked for.  (A recorded trace holds operators, without gradients: a Python function in it
-    could not be saved.)"""
-    return x.requires_grad and torch.is_grad_enabled() and (torch.compiler.is_compiling() or torch._C._get_tracing_state() is None)
+def _differentiated() -> bool:
+    """Whether the gradient of an input that takes one may be asked for.  (A recorded trace holds operators, without gradients: a
+    Python function in it could not be saved.)"""
+    return torch.is_grad_enabled() and (torch.compiler.is_compiling() or torch._C._get_tracing_state() is None)
 
 
 def _with_input_grad(layer: torch.nn.Module, x: torch.Tensor, bias: Optional[torch.Tensor]) -> torch.Tensor:
@@ -253,7 +253,7 @@ class Mxfp6LinearKernel(_Kernel):
                              f"{int(x.shape[-1])}, weight K={k}")
         if x.dtype != torch.bfloat16:
             raise ValueError("MXFP6 requires BF16 activations")
-        if _differentiated(x):
+        if x.requires_grad and _differentiated():
             return _with_input_grad(layer, x, bias)
         if x.numel() == 0:
             return x.new_empty((*x.shape[:-1], n))
@@ -299,7 +299,7 @@ class BlockFp8LinearKernel(_Kernel):
         n, k = layer.mxl_shape
         if x.dtype != torch.bfloat16 or x.shape[-1] != k:
             raise ValueError("block-FP8 requires BF16 activations with matching K")
-        if _differentiated(x):
+        if x.requires_grad and _differentiated():
             return _with_input_grad(layer, x, bias)
         if x.numel() == 0:
             return x.new_empty((*x.shape[:-1], n))
@@ -348,7 +348,7 @@ class Mxfp4LinearKernel(_Kernel):
         n, k = layer.mxl_shape
         if x.dtype != torch.bfloat16 or x.shape[-1] != k:
             raise ValueError("MXFP4 requires BF16 activations with matching K")
-        if _differentiated(x):
+        if x.requires_grad and _differentiated():
             return _with_input_grad(layer, x, bias)
         if x.numel() == 0:
             return x.new_empty((*x.shape[:-1], n))
